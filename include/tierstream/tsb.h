@@ -352,6 +352,165 @@ SS_API ss_status tsb_peer_store_migrate(tsb_peer_store* dst, const int32_t* old_
  * release its old stores once all ranks returned from this call. */
 SS_API ss_status tsb_dg_peer_retier(ss_ctx* c, const tsb_peer_tier* peer);
 
+/* ---- Operators beside the streamed units (no reference counterpart: the reference leaves routing and products to the
+ * engine) ----
+ * What an engine runs on the units this library brings: the router's selection (its ids feed ss_dg_enqueue_export), the
+ * gated feed-forward block of the routed units in their slots, and the matrix product with its epilogue (the router's
+ * logits, a streamed dense layer), each with its backward pass. All matrices are row-major, ld* in elements between
+ * rows. Every call enqueues kernels on `stream` of the current device and returns; it allocates nothing, waits for
+ * nothing, and may be captured into a graph. Scratch comes from the caller: *_workspace gives its bytes (0: none is
+ * needed; on a refused argument 0 too, and the call itself names the refusal), a 256-byte aligned device area that
+ * belongs to the call until the stream has passed it (two calls that may run at the same time, or two graphs, need one
+ * each). No result depends on the order in which anything ran: the same inputs give the same bits. Outputs must not
+ * overlap inputs, except that y may be the residual. Sums are held in 32 bits; what is 16 bits wide between two
+ * products of a call is said at each. */
+#define TSB_BF16 0
+#define TSB_F16 1
+#define TSB_F32 2 /* router logits only */
+#define TSB_ACT_NONE 0
+#define TSB_ACT_SILU 1
+#define TSB_ACT_GELU 2      /* z Phi(z) */
+#define TSB_ACT_GELU_TANH 3 /* its tanh form */
+#define TSB_ACT_RELU 4
+
+/* z = x w^T + bias, y = act(z) + residual: x [rows][k], w [n][k], bias [n], residual and y [rows][n], all of `dtype`
+ * (TSB_BF16 or TSB_F16). pre: z, rounded to dtype, for the backward pass. bias, residual and pre may be NULL.
+ * rows = 0 does nothing; n and k are at least 1. Rows that start on 16 bytes (x and w, so k and the lds multiples of 8)
+ * take the fast kernels; every other alignment is served too. */
+typedef struct tsb_linear_args {
+  uint32_t struct_size, dtype, act, reserved0;
+  uint64_t rows, n, k;
+  const void* x;
+  uint64_t ldx;
+  const void* w;
+  uint64_t ldw;
+  const void* bias;
+  const void* residual;
+  uint64_t ldr;
+  void* y;
+  uint64_t ldy;
+  void* pre;
+  uint64_t ldp;
+  void* workspace;
+  uint64_t workspace_bytes;
+  void* stream;
+} tsb_linear_args;
+SS_API uint64_t tsb_linear_workspace(const tsb_linear_args* a);
+SS_API ss_status tsb_linear(const tsb_linear_args* a);
+
+/* The gradients of tsb_linear from dy [rows][n]: dz = dy act'(pre) (rounded to dtype for the products), dx = dz w,
+ * dw = dz^T x, db = the sums of dz over the rows before that rounding. (The residual's gradient is dy itself.) dx, dw
+ * and db may each be NULL; pre is read unless act is TSB_ACT_NONE. rows = 0 zeroes dw and db. */
+typedef struct tsb_linear_grad_args {
+  uint32_t struct_size, dtype, act, reserved0;
+  uint64_t rows, n, k;
+  const void* dy;
+  uint64_t lddy;
+  const void* x;
+  uint64_t ldx;
+  const void* w;
+  uint64_t ldw;
+  const void* pre;
+  uint64_t ldp;
+  void* dx;
+  uint64_t lddx;
+  void* dw;
+  uint64_t lddw;
+  void* db;
+  void* workspace;
+  uint64_t workspace_bytes;
+  void* stream;
+} tsb_linear_grad_args;
+SS_API uint64_t tsb_linear_backward_workspace(const tsb_linear_grad_args* a);
+SS_API ss_status tsb_linear_backward(const tsb_linear_grad_args* a);
+
+/* The router's selection: per row of logits [rows][experts] (dtype any of the three, experts at most 1024) the `top`
+ * (at most 32, at most experts) largest, largest first, the lowest expert first among equal ones, as ids [rows][top];
+ * weights [rows][top] is the softmax over the row's chosen logits (norm != 0) or the chosen ones' share of the softmax
+ * over the whole row (norm = 0). A logit of -inf or NaN is never chosen and has no share (a masked expert); +inf counts
+ * as the largest finite value. A row with fewer than `top` experts left ends in ids -1 with weight 0: the feed-forward
+ * block skips them. */
+SS_API ss_status tsb_route(uint32_t dtype, const void* logits, uint64_t ld, uint64_t rows, uint32_t experts,
+                           uint32_t top, int norm, int32_t* ids, float* weights, void* stream);
+/* dlogits [rows][experts] (logits' dtype) from dweights [rows][top] (dw_dtype) and what tsb_route gave: ids distinct in
+ * a row, weights. With norm != 0 the logits are not read (may be NULL). */
+SS_API ss_status tsb_route_backward(uint32_t dtype, uint32_t dw_dtype, const void* dweights, const void* logits,
+                                    uint64_t ld, const int32_t* ids, const float* weights, uint64_t rows,
+                                    uint32_t experts, uint32_t top, int norm, void* dlogits, uint64_t ldd,
+                                    void* stream);
+
+/* Where a layer's units live. Matrix p of unit u (0 gate [ffn][hidden], 1 up [ffn][hidden], 2 down [hidden][ffn]) is at
+ * part[p] + slot x stride[p] bytes, slot = slot_of[*unit_base + u] (device memory, read when the kernels run; slot_of
+ * NULL: slot = u; unit_base NULL: 0), or, with `table` (device array of n_units addresses, a host-mode
+ * ss_layer_view.table_dev), at table[u] + stride[p] bytes. A slot outside [0, n_slots) or a zero address is a unit that
+ * is not there: its rows contribute nothing and *absent_err (may be NULL) is set to 1; while *abort (may be NULL) is
+ * non-zero no unit is there. */
+typedef struct tsb_units {
+  uint32_t struct_size, n_units, n_slots, reserved0;
+  const int32_t* slot_of;
+  const uint32_t* unit_base;
+  const uint64_t* table;
+  const uint32_t* abort;
+  uint32_t* absent_err;
+  const void* part[3];
+  uint64_t stride[3];
+} tsb_units;
+/* Gated layer g (n_units units) of a device-gated context whose first three parts are gate, up and down, each at least
+ * matrix_bytes. The ids given to ss_dg_enqueue_export(g) are the units' ids; use after ss_dg_enqueue_wait(g). */
+SS_API ss_status tsb_units_from_view(const ss_dg_device_view* v, uint32_t g, uint32_t n_units, uint64_t matrix_bytes,
+                                     tsb_units* out);
+
+/* The gated feed-forward block of the routed units: y[t] = residual[t] + sum over k of weights[t][k] x
+ * Wd_e (act(Wg_e x[t]) * (Wu_e x[t])), e = ids[t][k]; x and y [rows][hidden], ids and weights [rows][top] (device
+ * memory). An id outside [0, n_units) contributes nothing (a padded row's -1); a row with none gives its residual, or
+ * zeros. The same unit twice in a row counts twice. act(..) * (..) is rounded to dtype between the products; the
+ * choices' sums are added in 32 bits. residual may be NULL. top is at most 64, rows x top at most 2^28. */
+typedef struct tsb_ffn_args {
+  uint32_t struct_size, dtype, act, top;
+  uint64_t rows, hidden, ffn;
+  const void* x;
+  uint64_t ldx;
+  const int32_t* ids;
+  const float* weights;
+  const tsb_units* units;
+  const void* residual;
+  uint64_t ldr;
+  void* y;
+  uint64_t ldy;
+  void* workspace;
+  uint64_t workspace_bytes;
+  void* stream;
+} tsb_ffn_args;
+SS_API uint64_t tsb_ffn_workspace(const tsb_ffn_args* a);
+SS_API ss_status tsb_ffn(const tsb_ffn_args* a);
+
+/* Its gradients from dy [rows][hidden], with the gate and up products computed again: dx [rows][hidden], dweights
+ * [rows][top], and for training the units dgate, dup [n_units][ffn][hidden] and ddown [n_units][hidden][ffn], by unit
+ * (not by slot; zeros for a unit without rows), all of dtype, all three or none. dx, dweights and the three may be NULL.
+ * The gradients of the gate and up products, and weights x act(..) * (..), are rounded to dtype between the products. */
+typedef struct tsb_ffn_grad_args {
+  uint32_t struct_size, dtype, act, top;
+  uint64_t rows, hidden, ffn;
+  const void* dy;
+  uint64_t lddy;
+  const void* x;
+  uint64_t ldx;
+  const int32_t* ids;
+  const float* weights;
+  const tsb_units* units;
+  void* dx;
+  uint64_t lddx;
+  void* dweights;
+  void* dgate;
+  void* dup;
+  void* ddown;
+  void* workspace;
+  uint64_t workspace_bytes;
+  void* stream;
+} tsb_ffn_grad_args;
+SS_API uint64_t tsb_ffn_backward_workspace(const tsb_ffn_grad_args* a);
+SS_API ss_status tsb_ffn_backward(const tsb_ffn_grad_args* a);
+
 #ifdef __cplusplus
 }
 #endif

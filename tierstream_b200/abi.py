@@ -127,6 +127,44 @@ _DG_STATS_U64_1 = ["tokens", "lookups", "misses", "covered", "fetched", "prefetc
                    "round_units", "round_bytes", "round_ns", "round_cancelled"]
 
 
+# the operators (tsb.h)
+TSB_BF16, TSB_F16, TSB_F32 = range(3)
+TSB_ACT_NONE, TSB_ACT_SILU, TSB_ACT_GELU, TSB_ACT_GELU_TANH, TSB_ACT_RELU = range(5)
+
+
+class tsb_linear_args(C.Structure):
+    _fields_ = [("struct_size", u32), ("dtype", u32), ("act", u32), ("reserved0", u32), ("rows", u64), ("n", u64),
+                ("k", u64), ("x", vp), ("ldx", u64), ("w", vp), ("ldw", u64), ("bias", vp), ("residual", vp),
+                ("ldr", u64), ("y", vp), ("ldy", u64), ("pre", vp), ("ldp", u64), ("workspace", vp),
+                ("workspace_bytes", u64), ("stream", vp)]
+
+
+class tsb_linear_grad_args(C.Structure):
+    _fields_ = [("struct_size", u32), ("dtype", u32), ("act", u32), ("reserved0", u32), ("rows", u64), ("n", u64),
+                ("k", u64), ("dy", vp), ("lddy", u64), ("x", vp), ("ldx", u64), ("w", vp), ("ldw", u64), ("pre", vp),
+                ("ldp", u64), ("dx", vp), ("lddx", u64), ("dw", vp), ("lddw", u64), ("db", vp), ("workspace", vp),
+                ("workspace_bytes", u64), ("stream", vp)]
+
+
+class tsb_units(C.Structure):
+    _fields_ = [("struct_size", u32), ("n_units", u32), ("n_slots", u32), ("reserved0", u32), ("slot_of", vp),
+                ("unit_base", vp), ("table", vp), ("abort", vp), ("absent_err", vp), ("part", vp * 3),
+                ("stride", u64 * 3)]
+
+
+class tsb_ffn_args(C.Structure):
+    _fields_ = [("struct_size", u32), ("dtype", u32), ("act", u32), ("top", u32), ("rows", u64), ("hidden", u64),
+                ("ffn", u64), ("x", vp), ("ldx", u64), ("ids", vp), ("weights", vp), ("units", vp), ("residual", vp),
+                ("ldr", u64), ("y", vp), ("ldy", u64), ("workspace", vp), ("workspace_bytes", u64), ("stream", vp)]
+
+
+class tsb_ffn_grad_args(C.Structure):
+    _fields_ = [("struct_size", u32), ("dtype", u32), ("act", u32), ("top", u32), ("rows", u64), ("hidden", u64),
+                ("ffn", u64), ("dy", vp), ("lddy", u64), ("x", vp), ("ldx", u64), ("ids", vp), ("weights", vp),
+                ("units", vp), ("dx", vp), ("lddx", u64), ("dweights", vp), ("dgate", vp), ("dup", vp), ("ddown", vp),
+                ("workspace", vp), ("workspace_bytes", u64), ("stream", vp)]
+
+
 class ss_dg_stats(C.Structure):
     """The leading fields of ss_dg_stats (a versioned struct: the library writes min(size, its own) bytes)."""
     _fields_ = [("struct_size", u32), ("reserved0", u32)] + [(n, u64) for n in _DG_STATS_U64_1]
@@ -300,6 +338,20 @@ _ENGINE_PROTOS = {
     "tse_host_forward": (C.c_int, [vp, vp, vp, u32, vp, vp, vp, u32, C.c_int, vp]),
     "tse_expect_sums": (C.c_int, [u64, vp, u32, u64, C.c_int, vp, u32, vp]),
 }
+
+_PROTOS.update({
+    "tsb_linear_workspace": (u64, [vp]),
+    "tsb_linear": (C.c_int, [vp]),
+    "tsb_linear_backward_workspace": (u64, [vp]),
+    "tsb_linear_backward": (C.c_int, [vp]),
+    "tsb_route": (C.c_int, [u32, vp, u64, u64, u32, u32, C.c_int, vp, vp, vp]),
+    "tsb_route_backward": (C.c_int, [u32, u32, vp, vp, u64, vp, vp, u64, u32, u32, C.c_int, vp, u64, vp]),
+    "tsb_units_from_view": (C.c_int, [vp, u32, u32, u64, vp]),
+    "tsb_ffn_workspace": (u64, [vp]),
+    "tsb_ffn": (C.c_int, [vp]),
+    "tsb_ffn_backward_workspace": (u64, [vp]),
+    "tsb_ffn_backward": (C.c_int, [vp]),
+})
 
 _lib = None
 _engine = None

@@ -1,0 +1,184 @@
+// The operators an engine runs beside the streamed units: the matrix product with its epilogue, the router's selection
+// and the gated feed-forward block of the units in their slots. Internal types shared by the entry points (ops_api.cu)
+// and the kernels: ops_plan.cu (grouping, joins, routing), ops_tile.cu (every size and alignment), ops_stream.cu (few
+// rows: the weights' bytes bound it) and ops_tc.cu (many rows: the tensor cores bound it).
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+#include "tierstream/tsb.h"
+
+namespace tsb {
+namespace ops {
+
+// Where the units' matrices live: part p of unit u at base[p] + slot x stride[p] (slot_of[first + u], or u), or at
+// table[u] + offset[p]. part 0 gate [ffn][hidden], 1 up [ffn][hidden], 2 down [hidden][ffn], rows back to back.
+struct Units {
+  const int32_t* slot_of;
+  const uint32_t* unit_base;  // device word added to the unit's index in slot_of (NULL: 0)
+  const uint64_t* table;
+  const uint32_t* abort;
+  uint32_t* absent;
+  uint32_t n_units, n_slots;
+  const char* part[3];
+  uint64_t stride[3];
+};
+
+// The (row, choice) pairs grouped by unit, built on the device by launch_plan: unit e's pairs, in ascending order, are
+// rows [off[e], off[e] + cnt[e]) of every grouped buffer; rows up to the next multiple of `pad` have no pair (-1).
+struct Plan {
+  int32_t* head;  // [0] tiles, [1] grouped rows (padding included)
+  int32_t* cnt;
+  int32_t* off;
+  int32_t* slot;
+  int32_t* pair_of_row;
+  int32_t* row_of_pair;
+  int32_t* tile_unit;  // tiles of `bm` rows, group by group
+  int32_t* tile_m0;    // the tile's first row inside its group
+  uint32_t units, pairs, max_rows, max_tiles, pad, bm;
+};
+
+__host__ __device__ inline uint64_t ceil_div(uint64_t a, uint64_t b) { return (a + b - 1) / b; }
+
+#ifdef __CUDACC__
+__device__ __forceinline__ const char* unit_part(const Units& u, int p, int32_t e, int32_t slot) {
+  return u.table ? reinterpret_cast<const char*>(u.table[e]) + u.stride[p] : u.part[p] + uint64_t(slot) * u.stride[p];
+}
+
+// Activations and their slopes in 32 bits, by the accurate library functions: their cost hides behind the products.
+template <int ACT>
+__device__ __forceinline__ float act_of(float z) {
+  if constexpr (ACT == TSB_ACT_SILU) return z / (1.f + expf(-z));
+  if constexpr (ACT == TSB_ACT_GELU) return 0.5f * z * (1.f + erff(z * 0.70710678118654752f));
+  if constexpr (ACT == TSB_ACT_GELU_TANH)
+    return 0.5f * z * (1.f + tanhf(0.79788456080286536f * (z + 0.044715f * z * z * z)));
+  if constexpr (ACT == TSB_ACT_RELU) return z < 0.f ? 0.f : z;  // (a NaN stays one)
+  return z;
+}
+template <int ACT>
+__device__ __forceinline__ float slope_of(float z) {
+  if constexpr (ACT == TSB_ACT_SILU) {
+    const float p = 1.f / (1.f + expf(-z));
+    return p * (1.f + z * (1.f - p));
+  }
+  if constexpr (ACT == TSB_ACT_GELU)
+    return 0.5f * (1.f + erff(z * 0.70710678118654752f)) + z * expf(-0.5f * z * z) * 0.39894228040143268f;
+  if constexpr (ACT == TSB_ACT_GELU_TANH) {
+    const float p = tanhf(0.79788456080286536f * (z + 0.044715f * z * z * z));
+    return 0.5f * (1.f + p) + 0.5f * z * (1.f - p * p) * 0.79788456080286536f * (1.f + 0.134145f * z * z);
+  }
+  if constexpr (ACT == TSB_ACT_RELU) return z > 0.f ? 1.f : 0.f;
+  return 1.f;
+}
+__device__ __forceinline__ float act_rt(int act, float z) {
+  switch (act) {
+    case TSB_ACT_SILU: return act_of<TSB_ACT_SILU>(z);
+    case TSB_ACT_GELU: return act_of<TSB_ACT_GELU>(z);
+    case TSB_ACT_GELU_TANH: return act_of<TSB_ACT_GELU_TANH>(z);
+    case TSB_ACT_RELU: return act_of<TSB_ACT_RELU>(z);
+  }
+  return z;
+}
+__device__ __forceinline__ float slope_rt(int act, float z) {
+  switch (act) {
+    case TSB_ACT_SILU: return slope_of<TSB_ACT_SILU>(z);
+    case TSB_ACT_GELU: return slope_of<TSB_ACT_GELU>(z);
+    case TSB_ACT_GELU_TANH: return slope_of<TSB_ACT_GELU_TANH>(z);
+    case TSB_ACT_RELU: return slope_of<TSB_ACT_RELU>(z);
+  }
+  return 1.f;
+}
+
+template <class T>
+__device__ __forceinline__ float to_f(T v);
+template <>
+__device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <>
+__device__ __forceinline__ float to_f(__half v) { return __half2float(v); }
+template <>
+__device__ __forceinline__ float to_f(float v) { return v; }
+template <class T>
+__device__ __forceinline__ T from_f(float v);
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f(float v) { return __float2bfloat16_rn(v); }
+template <>
+__device__ __forceinline__ __half from_f(float v) { return __float2half_rn(v); }
+template <>
+__device__ __forceinline__ float from_f(float v) { return v; }
+#endif
+
+// What a product writes. Sums are held in 32 bits up to here; each store below rounds once.
+enum Epi {
+  kEpiLinear,   // z = acc + bias; pre = z; out = act(z) + residual
+  kEpiStore,    // out = acc (a gradient), per unit at out + e x out_unit
+  kEpiRows32,   // rows32[row][n] = acc in 32 bits (joined later)
+  kEpiUp,       // out[row][n] = act(acc0) x acc1
+  kEpiUpBack,   // from g = acc0, u = acc1, dh = acc2 and the pair's weight w: dg, du, hw = w x h, and per row the sum
+                // of dh x h over this tile's columns into dwp[row][tile]
+};
+
+// One operand of a product: element (i, k) at p + i x s_i + k x s_k elements. map: rows are gathered, row r of the
+// grouped buffer being row map[r] / div of p (-1: zeros); the gathered index is i, or k with map_k.
+struct Operand {
+  const void* p;
+  int64_t s_i, s_k;
+  const int32_t* map;
+  int32_t div, map_k;
+  int32_t part;  // >= 0: p is part `part` of the group's unit
+};
+
+struct Product {
+  Operand a[3], b[3];
+  int32_t acc[3];  // which accumulator segment s adds to
+  int32_t segs;
+  // m runs over the rows of a group (grouped) or over `m` (a matrix per unit, or one matrix); n over `n`; k over `k`, or
+  // over the group's rows (k_rows)
+  int64_t m, n, k;
+  int32_t grouped, per_unit, k_rows;
+  Epi epi;
+  int32_t act;
+  void* out;
+  int64_t ldo, out_unit;
+  const void* bias;
+  const void* residual;
+  int64_t ldr;
+  void* pre;
+  int64_t ldp;
+  float* rows32;
+  void* dg;
+  void* du;
+  void* hw;
+  float* dwp;
+  int64_t ld_dwp;
+  const float* weights;
+};
+
+// ops_plan.cu
+uint64_t plan_bytes(uint32_t units, uint64_t pairs, uint32_t pad, uint32_t bm);
+Plan plan_at(void* ws, uint32_t units, uint64_t pairs, uint32_t pad, uint32_t bm);
+int launch_plan(const Plan& p, const Units& u, const int32_t* ids, cudaStream_t s);
+// y[t] = residual[t] + sum over k, then over the splits, of w[t][k] x rows32[split][row_of_pair[t top + k]]
+int launch_join(int dtype, const Plan& p, const float* rows32, uint32_t splits, const float* weights, uint32_t top,
+                uint64_t rows, uint64_t n, const void* residual, uint64_t ldr, void* y, uint64_t ldy, cudaStream_t s);
+// dweights[pair] = sum over tiles of dwp[row][tile]
+int launch_join_dw(int dtype, const Plan& p, const float* dwp, uint32_t tiles, void* dw, cudaStream_t s);
+int launch_route(int dtype, const void* logits, uint64_t ld, uint64_t rows, uint32_t experts, uint32_t top, int norm,
+                 int32_t* ids, float* weights, cudaStream_t s);
+int launch_route_back(int dtype, int dw_dtype, const void* dw, const void* logits, uint64_t ld, const int32_t* ids,
+                      const float* weights, uint64_t rows, uint32_t experts, uint32_t top, int norm, void* dlogits,
+                      uint64_t ldd, cudaStream_t s);
+// dz = dy x act'(pre) (act none: not written) and, with db, its column sums; part: [chunks][n] floats
+uint32_t dz_chunks(uint64_t rows, uint64_t n);
+int launch_dz(int dtype, int act, const void* dy, uint64_t ldy, const void* pre, uint64_t ldp, void* dz, uint64_t ldz,
+              uint64_t rows, uint64_t n, void* db, float* part, cudaStream_t s);
+
+// ops_tile.cu: any product at any size, stride and alignment
+constexpr uint32_t kTileM = 64, kTileN = 64;
+int launch_tile(int dtype, const Product& p, const Plan* plan, const Units* units, cudaStream_t s);
+
+}  // namespace ops
+}  // namespace tsb

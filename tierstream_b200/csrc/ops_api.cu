@@ -1,0 +1,464 @@
+// The entry points of the operators (include/tierstream/tsb.h): argument checks, the workspace's layout and the choice
+// of kernels.
+#include <cstring>
+#include <string>
+
+#include "errors.hpp"
+#include "ops.hpp"
+
+namespace tsb {
+const char* set_error(const std::string& msg);
+}
+
+namespace {
+
+using namespace tsb::ops;
+
+template <class F>
+ss_status run(F&& f) {
+  try {
+    f();
+    return SS_OK;
+  } catch (const tsb::Error& e) {
+    tsb::set_error(e.what());
+    return e.status();
+  } catch (const std::exception& e) {
+    tsb::set_error(e.what());
+    return SS_E_BACKEND;
+  }
+}
+void need(bool ok, const char* fn, const char* what) {
+  if (!ok) tsb::fail(SS_E_INVALID, std::string(fn) + ": " + what);
+}
+void ck(int e, const char* fn, const char* what) {
+  if (e == 0) return;
+  (void)cudaGetLastError();
+  tsb::fail(SS_E_BACKEND, std::string(fn) + ": " + what + ": " + cudaGetErrorString(cudaError_t(e)));
+}
+
+constexpr uint64_t kMaxDim = uint64_t(1) << 22, kMaxRows = uint64_t(1) << 28;
+
+// The workspace handed out front to back, every piece on 256 bytes.
+struct Arena {
+  char* base;
+  uint64_t used = 0;
+  void* take(uint64_t bytes) {
+    char* p = base ? base + used : nullptr;
+    used += (bytes + 255) / 256 * 256;
+    return p;
+  }
+};
+void need_workspace(const char* fn, const void* ws, uint64_t have, uint64_t want) {
+  need(!want || (ws && have >= want), fn, "the workspace is smaller than the call's _workspace says");
+  need(!want || (reinterpret_cast<uintptr_t>(ws) & 255u) == 0, fn, "the workspace must be 256-byte aligned");
+}
+
+Operand dense(const void* p, int64_t s_i, int64_t s_k, int map_k = 0) { return {p, s_i, s_k, nullptr, 1, map_k, -1}; }
+Operand gathered(const void* p, int64_t s_i, int64_t s_k, const Plan& plan, uint32_t top, int map_k = 0) {
+  return {p, s_i, s_k, plan.pair_of_row, int32_t(top), map_k, -1};
+}
+Operand of_unit(int part, int64_t s_i, int64_t s_k) { return {nullptr, s_i, s_k, nullptr, 1, 0, part}; }
+
+// ---- linear ----
+void check_linear(const tsb_linear_args* a) {
+  const char* fn = "tsb_linear";
+  need(a && a->struct_size >= sizeof *a, fn, "null or short argument struct");
+  need(a->dtype == TSB_BF16 || a->dtype == TSB_F16, fn, "dtype must be TSB_BF16 or TSB_F16");
+  need(a->act <= TSB_ACT_RELU, fn, "unknown activation");
+  need(a->n >= 1 && a->k >= 1 && a->n < kMaxDim && a->k < kMaxDim, fn, "n and k must be in [1, 2^22)");
+  need(a->rows < kMaxRows, fn, "rows must be below 2^28");
+  if (!a->rows) return;
+  need(a->x && a->w && a->y, fn, "null argument");
+  need(a->ldx >= a->k && a->ldw >= a->k && a->ldy >= a->n && (!a->residual || a->ldr >= a->n) &&
+           (!a->pre || a->ldp >= a->n),
+       fn, "a leading dimension is shorter than its row");
+}
+
+void linear(const tsb_linear_args* a) {
+  const char* fn = "tsb_linear";
+  check_linear(a);
+  if (!a->rows) return;
+  cudaStream_t s = static_cast<cudaStream_t>(a->stream);
+  Product p{};
+  p.segs = 1;
+  p.a[0] = dense(a->x, int64_t(a->ldx), 1);
+  p.b[0] = dense(a->w, int64_t(a->ldw), 1);
+  p.m = int64_t(a->rows), p.n = int64_t(a->n), p.k = int64_t(a->k);
+  p.epi = kEpiLinear;
+  p.act = int(a->act);
+  p.out = a->y, p.ldo = int64_t(a->ldy);
+  p.bias = a->bias;
+  p.residual = a->residual, p.ldr = int64_t(a->ldr);
+  p.pre = a->pre, p.ldp = int64_t(a->ldp);
+  ck(launch_tile(int(a->dtype), p, nullptr, nullptr, s), fn, "launch");
+}
+
+void check_linear_back(const tsb_linear_grad_args* a) {
+  const char* fn = "tsb_linear_backward";
+  need(a && a->struct_size >= sizeof *a, fn, "null or short argument struct");
+  need(a->dtype == TSB_BF16 || a->dtype == TSB_F16, fn, "dtype must be TSB_BF16 or TSB_F16");
+  need(a->act <= TSB_ACT_RELU, fn, "unknown activation");
+  need(a->n >= 1 && a->k >= 1 && a->n < kMaxDim && a->k < kMaxDim, fn, "n and k must be in [1, 2^22)");
+  need(a->rows < kMaxRows, fn, "rows must be below 2^28");
+  need(!a->dw || a->lddw >= a->k, fn, "a leading dimension is shorter than its row");
+  if (!a->rows) return;
+  need(a->dy && (!a->dx || a->w) && (!a->dw || a->x), fn, "null argument");
+  need(a->act == TSB_ACT_NONE || a->pre, fn, "an activation's slope needs pre");
+  need(a->lddy >= a->n && (!a->dx || (a->ldw >= a->k && a->lddx >= a->k)) && (!a->dw || a->ldx >= a->k) &&
+           (a->act == TSB_ACT_NONE || a->ldp >= a->n),
+       fn, "a leading dimension is shorter than its row");
+}
+
+struct LinearBackSpace {
+  void* dz;
+  uint64_t ldz;
+  float* part;
+  uint64_t bytes;
+};
+LinearBackSpace linear_back_space(const tsb_linear_grad_args* a) {
+  Arena w{static_cast<char*>(a->workspace)};
+  LinearBackSpace r{};
+  r.ldz = (a->n + 7) / 8 * 8;
+  if (a->rows && a->act != TSB_ACT_NONE) r.dz = w.take(a->rows * r.ldz * 2);
+  if (a->rows && a->db) r.part = static_cast<float*>(w.take(uint64_t(dz_chunks(a->rows, a->n)) * a->n * 4));
+  r.bytes = w.used;
+  return r;
+}
+
+void linear_back(const tsb_linear_grad_args* a) {
+  const char* fn = "tsb_linear_backward";
+  check_linear_back(a);
+  cudaStream_t s = static_cast<cudaStream_t>(a->stream);
+  if (!a->rows) {
+    if (a->dw) ck(int(cudaMemset2DAsync(a->dw, a->lddw * 2, 0, a->k * 2, a->n, s)), fn, "dw");
+    if (a->db) ck(int(cudaMemsetAsync(a->db, 0, a->n * 2, s)), fn, "db");
+    return;
+  }
+  const LinearBackSpace w = linear_back_space(a);
+  need_workspace(fn, a->workspace, a->workspace_bytes, w.bytes);
+  const void* dz = a->dy;
+  uint64_t ldz = a->lddy;
+  const bool slope = a->act != TSB_ACT_NONE;
+  if (slope) dz = w.dz, ldz = w.ldz;
+  if (slope || a->db)
+    ck(launch_dz(int(a->dtype), int(a->act), a->dy, a->lddy, a->pre, a->ldp, slope ? w.dz : nullptr, w.ldz, a->rows,
+                 a->n, a->db, w.part, s),
+       fn, "slope");
+  if (a->dx) {
+    Product p{};
+    p.segs = 1;
+    p.a[0] = dense(dz, int64_t(ldz), 1);
+    p.b[0] = dense(a->w, 1, int64_t(a->ldw));
+    p.m = int64_t(a->rows), p.n = int64_t(a->k), p.k = int64_t(a->n);
+    p.epi = kEpiStore;
+    p.out = a->dx, p.ldo = int64_t(a->lddx);
+    ck(launch_tile(int(a->dtype), p, nullptr, nullptr, s), fn, "dx");
+  }
+  if (a->dw) {
+    Product p{};
+    p.segs = 1;
+    p.a[0] = dense(dz, 1, int64_t(ldz), 1);
+    p.b[0] = dense(a->x, 1, int64_t(a->ldx), 1);
+    p.m = int64_t(a->n), p.n = int64_t(a->k), p.k = int64_t(a->rows);
+    p.epi = kEpiStore;
+    p.out = a->dw, p.ldo = int64_t(a->lddw);
+    ck(launch_tile(int(a->dtype), p, nullptr, nullptr, s), fn, "dw");
+  }
+}
+
+// ---- the gated feed-forward block ----
+Units units_of(const tsb_units* u) {
+  Units r{};
+  r.slot_of = u->slot_of;
+  r.unit_base = u->unit_base;
+  r.table = u->table;
+  r.abort = u->abort;
+  r.absent = u->absent_err;
+  r.n_units = u->n_units;
+  r.n_slots = u->n_slots;
+  for (int i = 0; i < 3; ++i) {
+    r.part[i] = static_cast<const char*>(u->part[i]);
+    r.stride[i] = u->stride[i];
+  }
+  return r;
+}
+
+template <class A>
+void check_ffn_shape(const A* a, const char* fn) {
+  need(a && a->struct_size >= sizeof *a, fn, "null or short argument struct");
+  need(a->dtype == TSB_BF16 || a->dtype == TSB_F16, fn, "dtype must be TSB_BF16 or TSB_F16");
+  need(a->act <= TSB_ACT_RELU, fn, "unknown activation");
+  need(a->hidden >= 1 && a->ffn >= 1 && a->hidden < kMaxDim && a->ffn < kMaxDim, fn,
+       "hidden and ffn must be in [1, 2^22)");
+  need(a->top >= 1 && a->top <= 64, fn, "top must be in [1, 64]");
+  need(a->rows <= kMaxRows / a->top, fn, "rows x top must be at most 2^28");
+  const tsb_units* u = a->units;
+  need(u && u->struct_size >= sizeof *u, fn, "null or short units struct");
+  need(u->n_units >= 1 && u->n_units <= 65535, fn, "n_units must be in [1, 65535]");
+  need(u->table || (u->part[0] && u->part[1] && u->part[2] && u->n_slots >= 1), fn, "no parts and no table");
+  need(u->stride[0] % 2 == 0 && u->stride[1] % 2 == 0 && u->stride[2] % 2 == 0, fn,
+       "the parts' strides must be whole elements");
+}
+
+struct FfnSpace {
+  Plan plan;
+  void* h;
+  float* rows32;
+  uint64_t bytes;
+};
+FfnSpace ffn_space(const tsb_ffn_args* a) {
+  Arena w{static_cast<char*>(a->workspace)};
+  FfnSpace r{};
+  const uint64_t pairs = a->rows * a->top;
+  r.plan = plan_at(w.take(plan_bytes(a->units->n_units, pairs, 1, 64)), a->units->n_units, pairs, 1, 64);
+  r.h = w.take(uint64_t(r.plan.max_rows) * a->ffn * 2);
+  r.rows32 = static_cast<float*>(w.take(uint64_t(r.plan.max_rows) * a->hidden * 4));
+  r.bytes = w.used;
+  return r;
+}
+
+void check_ffn(const tsb_ffn_args* a) {
+  const char* fn = "tsb_ffn";
+  check_ffn_shape(a, fn);
+  if (!a->rows) return;
+  need(a->x && a->ids && a->weights && a->y, fn, "null argument");
+  need(a->ldx >= a->hidden && a->ldy >= a->hidden && (!a->residual || a->ldr >= a->hidden), fn,
+       "a leading dimension is shorter than its row");
+}
+
+void ffn(const tsb_ffn_args* a) {
+  const char* fn = "tsb_ffn";
+  check_ffn(a);
+  if (!a->rows) return;
+  const FfnSpace w = ffn_space(a);
+  need_workspace(fn, a->workspace, a->workspace_bytes, w.bytes);
+  cudaStream_t s = static_cast<cudaStream_t>(a->stream);
+  const Units u = units_of(a->units);
+  const int64_t d = int64_t(a->hidden), f = int64_t(a->ffn);
+  ck(launch_plan(w.plan, u, a->ids, s), fn, "plan");
+  Product p{};
+  p.grouped = 1;
+  p.segs = 2;
+  p.a[0] = p.a[1] = gathered(a->x, int64_t(a->ldx), 1, w.plan, a->top);
+  p.b[0] = of_unit(0, d, 1);
+  p.b[1] = of_unit(1, d, 1);
+  p.acc[1] = 1;
+  p.n = f, p.k = d;
+  p.epi = kEpiUp;
+  p.act = int(a->act);
+  p.out = w.h, p.ldo = f;
+  ck(launch_tile(int(a->dtype), p, &w.plan, &u, s), fn, "gate and up");
+  Product q{};
+  q.grouped = 1;
+  q.segs = 1;
+  q.a[0] = dense(w.h, f, 1);
+  q.b[0] = of_unit(2, f, 1);
+  q.n = d, q.k = f;
+  q.epi = kEpiRows32;
+  q.rows32 = w.rows32;
+  ck(launch_tile(int(a->dtype), q, &w.plan, &u, s), fn, "down");
+  ck(launch_join(int(a->dtype), w.plan, w.rows32, 1, a->weights, a->top, a->rows, a->hidden, a->residual, a->ldr, a->y,
+                 a->ldy, s),
+     fn, "join");
+}
+
+struct FfnBackSpace {
+  Plan plan;
+  void *dg, *du, *hw;
+  float *dwp, *rows32;
+  uint32_t dw_tiles;
+  uint64_t bytes;
+};
+FfnBackSpace ffn_back_space(const tsb_ffn_grad_args* a) {
+  Arena w{static_cast<char*>(a->workspace)};
+  FfnBackSpace r{};
+  const uint64_t pairs = a->rows * a->top;
+  r.plan = plan_at(w.take(plan_bytes(a->units->n_units, pairs, 1, 64)), a->units->n_units, pairs, 1, 64);
+  r.dg = w.take(uint64_t(r.plan.max_rows) * a->ffn * 2);
+  r.du = w.take(uint64_t(r.plan.max_rows) * a->ffn * 2);
+  if (a->dgate) r.hw = w.take(uint64_t(r.plan.max_rows) * a->ffn * 2);
+  r.dw_tiles = uint32_t(ceil_div(a->ffn, kTileN));
+  if (a->dweights) r.dwp = static_cast<float*>(w.take(uint64_t(r.plan.max_rows) * r.dw_tiles * 4));
+  if (a->dx) r.rows32 = static_cast<float*>(w.take(uint64_t(r.plan.max_rows) * a->hidden * 4));
+  r.bytes = w.used;
+  return r;
+}
+
+void check_ffn_back(const tsb_ffn_grad_args* a) {
+  const char* fn = "tsb_ffn_backward";
+  check_ffn_shape(a, fn);
+  need((a->dgate && a->dup && a->ddown) || (!a->dgate && !a->dup && !a->ddown), fn,
+       "dgate, dup and ddown go together");
+  if (!a->rows) return;
+  need(a->dy && a->x && a->ids && a->weights, fn, "null argument");
+  need(a->ldx >= a->hidden && a->lddy >= a->hidden && (!a->dx || a->lddx >= a->hidden), fn,
+       "a leading dimension is shorter than its row");
+}
+
+void ffn_back(const tsb_ffn_grad_args* a) {
+  const char* fn = "tsb_ffn_backward";
+  check_ffn_back(a);
+  cudaStream_t s = static_cast<cudaStream_t>(a->stream);
+  const int64_t d = int64_t(a->hidden), f = int64_t(a->ffn);
+  if (!a->rows) {
+    for (void* g : {a->dgate, a->dup, a->ddown})
+      if (g) ck(int(cudaMemsetAsync(g, 0, uint64_t(a->units->n_units) * a->hidden * a->ffn * 2, s)), fn, "zeros");
+    return;
+  }
+  if (!a->dx && !a->dweights && !a->dgate) return;
+  const FfnBackSpace w = ffn_back_space(a);
+  need_workspace(fn, a->workspace, a->workspace_bytes, w.bytes);
+  const Units u = units_of(a->units);
+  const int dt = int(a->dtype);
+  ck(launch_plan(w.plan, u, a->ids, s), fn, "plan");
+  {
+    Product p{};
+    p.grouped = 1;
+    p.segs = 3;
+    p.a[0] = p.a[1] = gathered(a->x, int64_t(a->ldx), 1, w.plan, a->top);
+    p.a[2] = gathered(a->dy, int64_t(a->lddy), 1, w.plan, a->top);
+    p.b[0] = of_unit(0, d, 1);
+    p.b[1] = of_unit(1, d, 1);
+    p.b[2] = of_unit(2, 1, f);
+    p.acc[1] = 1, p.acc[2] = 2;
+    p.n = f, p.k = d;
+    p.epi = kEpiUpBack;
+    p.act = int(a->act);
+    p.dg = w.dg, p.du = w.du, p.hw = w.hw, p.ldo = f;
+    p.dwp = w.dwp, p.ld_dwp = w.dw_tiles;
+    p.weights = a->weights;
+    ck(launch_tile(dt, p, &w.plan, &u, s), fn, "gate, up and dh");
+  }
+  if (a->dweights) ck(launch_join_dw(dt, w.plan, w.dwp, w.dw_tiles, a->dweights, s), fn, "dweights");
+  if (a->dx) {
+    Product p{};
+    p.grouped = 1;
+    p.segs = 2;
+    p.a[0] = dense(w.dg, f, 1);
+    p.a[1] = dense(w.du, f, 1);
+    p.b[0] = of_unit(0, 1, d);
+    p.b[1] = of_unit(1, 1, d);
+    p.n = d, p.k = f;
+    p.epi = kEpiRows32;
+    p.rows32 = w.rows32;
+    ck(launch_tile(dt, p, &w.plan, &u, s), fn, "dx");
+    ck(launch_join(dt, w.plan, w.rows32, 1, nullptr, a->top, a->rows, a->hidden, nullptr, 0, a->dx, a->lddx, s), fn,
+       "join");
+  }
+  if (a->dgate) {
+    Product p{};
+    p.per_unit = 1;
+    p.k_rows = 1;
+    p.segs = 1;
+    p.epi = kEpiStore;
+    p.out_unit = d * f;
+    p.m = f, p.n = d, p.ldo = d;
+    p.b[0] = gathered(a->x, 1, int64_t(a->ldx), w.plan, a->top, 1);
+    p.a[0] = dense(w.dg, 1, f, 1);
+    p.out = a->dgate;
+    ck(launch_tile(dt, p, &w.plan, &u, s), fn, "dgate");
+    p.a[0] = dense(w.du, 1, f, 1);
+    p.out = a->dup;
+    ck(launch_tile(dt, p, &w.plan, &u, s), fn, "dup");
+    p.m = d, p.n = f, p.ldo = f;
+    p.a[0] = gathered(a->dy, 1, int64_t(a->lddy), w.plan, a->top, 1);
+    p.b[0] = dense(w.hw, 1, f, 1);
+    p.out = a->ddown;
+    ck(launch_tile(dt, p, &w.plan, &u, s), fn, "ddown");
+  }
+}
+
+template <class A, class F>
+uint64_t bytes_of(const A* a, void (*check)(const A*), F&& space) {
+  try {
+    check(a);
+    return a->rows ? space(a).bytes : 0;
+  } catch (const std::exception&) {
+    return 0;
+  }
+}
+
+}  // namespace
+
+extern "C" {
+
+uint64_t tsb_linear_workspace(const tsb_linear_args*) { return 0; }
+ss_status tsb_linear(const tsb_linear_args* a) {
+  return run([&] { linear(a); });
+}
+uint64_t tsb_linear_backward_workspace(const tsb_linear_grad_args* a) {
+  return bytes_of(a, check_linear_back, linear_back_space);
+}
+ss_status tsb_linear_backward(const tsb_linear_grad_args* a) {
+  return run([&] { linear_back(a); });
+}
+
+ss_status tsb_route(uint32_t dtype, const void* logits, uint64_t ld, uint64_t rows, uint32_t experts, uint32_t top,
+                    int norm, int32_t* ids, float* weights, void* stream) {
+  return run([&] {
+    const char* fn = "tsb_route";
+    need(dtype <= TSB_F32, fn, "dtype must be TSB_BF16, TSB_F16 or TSB_F32");
+    need(experts >= 1 && experts <= 1024, fn, "experts must be in [1, 1024]");
+    need(top >= 1 && top <= 32 && top <= experts, fn, "top must be in [1, 32] and at most experts");
+    need(rows < kMaxRows, fn, "rows must be below 2^28");
+    if (!rows) return;
+    need(logits && ids && weights, fn, "null argument");
+    need(ld >= experts, fn, "a leading dimension is shorter than its row");
+    ck(launch_route(int(dtype), logits, ld, rows, experts, top, norm, ids, weights, static_cast<cudaStream_t>(stream)),
+       fn, "launch");
+  });
+}
+ss_status tsb_route_backward(uint32_t dtype, uint32_t dw_dtype, const void* dweights, const void* logits, uint64_t ld,
+                             const int32_t* ids, const float* weights, uint64_t rows, uint32_t experts, uint32_t top,
+                             int norm, void* dlogits, uint64_t ldd, void* stream) {
+  return run([&] {
+    const char* fn = "tsb_route_backward";
+    need(dtype <= TSB_F32 && dw_dtype <= TSB_F32, fn, "dtypes must be TSB_BF16, TSB_F16 or TSB_F32");
+    need(experts >= 1 && experts <= 1024, fn, "experts must be in [1, 1024]");
+    need(top >= 1 && top <= 32 && top <= experts, fn, "top must be in [1, 32] and at most experts");
+    need(rows < kMaxRows, fn, "rows must be below 2^28");
+    if (!rows) return;
+    need(dweights && (norm || logits) && ids && weights && dlogits, fn, "null argument");
+    need((norm || ld >= experts) && ldd >= experts, fn, "a leading dimension is shorter than its row");
+    ck(launch_route_back(int(dtype), int(dw_dtype), dweights, logits, ld, ids, weights, rows, experts, top, norm,
+                         dlogits, ldd, static_cast<cudaStream_t>(stream)),
+       fn, "launch");
+  });
+}
+
+ss_status tsb_units_from_view(const ss_dg_device_view* v, uint32_t g, uint32_t n_units, uint64_t matrix_bytes,
+                              tsb_units* out) {
+  return run([&] {
+    const char* fn = "tsb_units_from_view";
+    need(v && out, fn, "null argument");
+    need(v->struct_size >= offsetof(ss_dg_device_view, absent_err), fn, "short view");
+    need(g < v->n_gated, fn, "no such gated layer");
+    need(v->n_parts >= 3, fn, "a unit needs the parts gate, up and down");
+    *out = tsb_units{};
+    out->struct_size = sizeof *out;
+    out->n_units = n_units;
+    out->n_slots = v->slots;
+    out->slot_of = v->slot_of;
+    out->unit_base = v->unit_base + g;
+    out->abort = v->abort;
+    out->absent_err = v->struct_size >= sizeof *v ? v->absent_err : nullptr;
+    for (int i = 0; i < 3; ++i) {
+      need(v->parts[i].bytes >= matrix_bytes, fn, "a part is smaller than its matrix");
+      out->part[i] = v->parts[i].base;
+      out->stride[i] = v->parts[i].stride;
+    }
+  });
+}
+
+uint64_t tsb_ffn_workspace(const tsb_ffn_args* a) { return bytes_of(a, check_ffn, ffn_space); }
+ss_status tsb_ffn(const tsb_ffn_args* a) {
+  return run([&] { ffn(a); });
+}
+uint64_t tsb_ffn_backward_workspace(const tsb_ffn_grad_args* a) {
+  return bytes_of(a, check_ffn_back, ffn_back_space);
+}
+ss_status tsb_ffn_backward(const tsb_ffn_grad_args* a) {
+  return run([&] { ffn_back(a); });
+}
+
+}  // extern "C"

@@ -1,0 +1,537 @@
+// What stands around the products: the grouping of (row, choice) pairs by unit, the joins of per-pair rows, the slope
+// times the incoming gradient with its column sums, and the router's selection with its backward pass. All of it moves
+// a few bytes per pair or element; every sum has a fixed order, so the same inputs give the same bits.
+#include <cfloat>
+
+#include "ops.hpp"
+
+namespace tsb {
+namespace ops {
+namespace {
+
+constexpr uint32_t kNone = 0xffffffffu;
+
+// ---------------------------------------------------------------------------------------------------------------
+// The plan. Counting first: CTA e counts unit e's pairs and resolves its slot. Then CTA e adds up the groups before its
+// own (padded rows, tiles) and writes its pairs in ascending order, found by scanning the ids with a ballot: no atomics,
+// so the order never changes. The scan reads the ids once per unit from L2 (256 units x 16,384 pairs: 16 MB).
+// ---------------------------------------------------------------------------------------------------------------
+constexpr int kPlanThreads = 256;
+
+__device__ __forceinline__ int32_t resolve(const Units& u, int32_t e) {
+  if (u.abort && *reinterpret_cast<const volatile uint32_t*>(u.abort)) return -1;
+  if (u.table) return u.table[e] ? e : -1;
+  if (!u.slot_of) return uint32_t(e) < u.n_slots ? e : -1;
+  const int32_t s = reinterpret_cast<const volatile int32_t*>(u.slot_of)[(u.unit_base ? *u.unit_base : 0u) + uint32_t(e)];
+  return uint32_t(s) < u.n_slots ? s : -1;
+}
+
+__device__ __forceinline__ int block_sum(int v, int* red) {
+  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+  __syncthreads();
+  int t = 0;
+  for (int w = 0; w < kPlanThreads / 32; ++w) t += red[w];
+  return t;
+}
+
+__global__ __launch_bounds__(kPlanThreads) void plan_count_kernel(const __grid_constant__ Plan p,
+                                                                  const __grid_constant__ Units u,
+                                                                  const int32_t* __restrict__ ids) {
+  __shared__ int red[kPlanThreads / 32];
+  const int32_t e = blockIdx.x;
+  int n = 0;
+  for (uint32_t i = threadIdx.x; i < p.pairs; i += kPlanThreads) n += ids[i] == e;
+  n = block_sum(n, red);
+  if (threadIdx.x) return;
+  const int32_t slot = n ? resolve(u, e) : -1;
+  if (n && slot < 0 && u.absent) atomicOr(u.absent, 1u);  // a routed unit that is not there: its rows are left out
+  p.cnt[e] = slot < 0 ? 0 : n;
+  p.slot[e] = slot < 0 ? 0 : slot;
+}
+
+__global__ __launch_bounds__(kPlanThreads) void plan_fill_kernel(const __grid_constant__ Plan p,
+                                                                 const int32_t* __restrict__ ids) {
+  __shared__ int red[kPlanThreads / 32];
+  __shared__ int warp_n[kPlanThreads / 32];
+  const uint32_t e = blockIdx.x;
+  int rows = 0, tiles = 0;
+  for (uint32_t j = threadIdx.x; j < e; j += kPlanThreads) {
+    const int c = p.cnt[j];
+    rows += (c + int(p.pad) - 1) / int(p.pad) * int(p.pad);
+    tiles += (c + int(p.bm) - 1) / int(p.bm);
+  }
+  rows = block_sum(rows, red);
+  tiles = block_sum(tiles, red);
+  const int cnt = p.cnt[e];
+  const int padded = (cnt + int(p.pad) - 1) / int(p.pad) * int(p.pad), mine = (cnt + int(p.bm) - 1) / int(p.bm);
+  if (threadIdx.x == 0) {
+    p.off[e] = rows;
+    if (e + 1 == p.units) {
+      p.head[0] = tiles + mine;
+      p.head[1] = rows + padded;
+    }
+  }
+  for (int i = threadIdx.x; i < mine; i += kPlanThreads) {
+    p.tile_unit[tiles + i] = int32_t(e);
+    p.tile_m0[tiles + i] = i * int(p.bm);
+  }
+  for (int i = cnt + threadIdx.x; i < padded; i += kPlanThreads) p.pair_of_row[rows + i] = -1;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int done = 0;  // pairs of this unit before the current span of ids
+  for (uint32_t i0 = 0; i0 < p.pairs && (cnt || e == 0); i0 += kPlanThreads) {
+    const uint32_t i = i0 + threadIdx.x;
+    const int32_t id = i < p.pairs ? ids[i] : -1;
+    if (e == 0 && i < p.pairs && (uint32_t(id) >= p.units || p.cnt[id] == 0)) p.row_of_pair[i] = -1;
+    const bool hit = cnt && i < p.pairs && id == int32_t(e);
+    const uint32_t m = __ballot_sync(0xffffffffu, hit);
+    __syncthreads();
+    if (lane == 0) warp_n[warp] = __popc(m);
+    __syncthreads();
+    int before = done;
+    for (int w = 0; w < kPlanThreads / 32; ++w) {
+      if (w < warp) before += warp_n[w];
+      done += warp_n[w];
+    }
+    if (hit) {
+      const int r = rows + before + __popc(m & ((1u << lane) - 1));
+      p.pair_of_row[r] = int32_t(i);
+      p.row_of_pair[i] = r;
+    }
+  }
+}
+
+// The same for few pairs in one launch: one CTA, the ids in shared memory, unit after unit by warps.
+constexpr int kSmallThreads = 1024;
+constexpr uint32_t kSmallPairs = 1024, kSmallUnits = 1024;
+
+__global__ __launch_bounds__(kSmallThreads) void plan_small_kernel(const __grid_constant__ Plan p,
+                                                                   const __grid_constant__ Units u,
+                                                                   const int32_t* __restrict__ ids) {
+  __shared__ int32_t id[kSmallPairs];
+  __shared__ int32_t cnt[kSmallUnits], rows[kSmallUnits], tiles[kSmallUnits];
+  __shared__ int32_t wr[32], wt[32];
+  const uint32_t t = threadIdx.x;
+  const int lane = t & 31, warp = t >> 5;
+  cnt[t] = 0;
+  if (t < p.pairs) id[t] = ids[t];
+  __syncthreads();
+  const int32_t mine = t < p.pairs ? id[t] : -1;
+  const bool valid = uint32_t(mine) < p.units;
+  if (valid) atomicAdd(&cnt[mine], 1);  // (counts only: their value does not depend on the order)
+  __syncthreads();
+  if (t < p.units && cnt[t]) {
+    const int32_t slot = resolve(u, int32_t(t));
+    if (slot < 0) {
+      if (u.absent) atomicOr(u.absent, 1u);
+      cnt[t] = 0;
+    } else {
+      p.slot[t] = slot;
+    }
+  }
+  __syncthreads();
+  const int c = t < p.units ? cnt[t] : 0;
+  const int padded = (c + int(p.pad) - 1) / int(p.pad) * int(p.pad), nt = (c + int(p.bm) - 1) / int(p.bm);
+  int r = padded, k = nt;  // inclusive scans over the units
+  for (int o = 1; o < 32; o <<= 1) {
+    const int a = __shfl_up_sync(0xffffffffu, r, o), b = __shfl_up_sync(0xffffffffu, k, o);
+    if (lane >= o) r += a, k += b;
+  }
+  if (lane == 31) wr[warp] = r, wt[warp] = k;
+  __syncthreads();
+  for (int w = 0; w < warp; ++w) r += wr[w], k += wt[w];
+  rows[t] = r - padded;
+  tiles[t] = k - nt;
+  __syncthreads();
+  if (t < p.units) {
+    p.cnt[t] = c;
+    p.off[t] = rows[t];
+    if (!c) p.slot[t] = 0;
+    if (t + 1 == p.units) p.head[0] = k, p.head[1] = r;
+    for (int i = 0; i < nt; ++i) {
+      p.tile_unit[tiles[t] + i] = int32_t(t);
+      p.tile_m0[tiles[t] + i] = i * int(p.bm);
+    }
+    for (int i = c; i < padded; ++i) p.pair_of_row[rows[t] + i] = -1;
+  }
+  if (t < p.pairs) {
+    int32_t row = -1;
+    if (valid && cnt[mine]) {
+      int before = 0;
+      for (uint32_t j = 0; j < t; ++j) before += id[j] == mine;
+      row = rows[mine] + before;
+      p.pair_of_row[row] = int32_t(t);
+    }
+    p.row_of_pair[t] = row;
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// Joins: a row's contributions from its choices (and from the splits of a long sum), added in order in 32 bits and
+// rounded once with the residual. V columns a thread; bound by the 32-bit rows' bytes.
+// ---------------------------------------------------------------------------------------------------------------
+template <class T, int V>
+__global__ __launch_bounds__(256) void join_kernel(const int32_t* __restrict__ row_of_pair, const float* __restrict__ src,
+                                                   uint32_t splits, uint64_t split_stride,
+                                                   const float* __restrict__ weights, uint32_t top, uint64_t n,
+                                                   const T* residual, uint64_t ldr, T* y, uint64_t ldy) {
+  const uint64_t t = blockIdx.x, c = (uint64_t(blockIdx.y) * 256 + threadIdx.x) * V;
+  if (c >= n) return;
+  float sum[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) sum[v] = residual ? to_f(residual[t * ldr + c + v]) : 0.f;
+  for (uint32_t k = 0; k < top; ++k) {
+    const int32_t row = row_of_pair[t * top + k];
+    if (row < 0) continue;
+    const float w = weights ? weights[t * top + k] : 1.f;
+    float part[V] = {};
+    for (uint32_t s = 0; s < splits; ++s) {
+      const float* p = src + s * split_stride + uint64_t(row) * n + c;
+      if constexpr (V == 4) {
+        const float4 f = *reinterpret_cast<const float4*>(p);
+        part[0] += f.x, part[1] += f.y, part[2] += f.z, part[3] += f.w;
+      } else {
+        part[0] += *p;
+      }
+    }
+#pragma unroll
+    for (int v = 0; v < V; ++v) sum[v] += w * part[v];
+  }
+#pragma unroll
+  for (int v = 0; v < V; ++v) y[t * ldy + c + v] = from_f<T>(sum[v]);
+}
+
+template <class T>
+__global__ void join_dw_kernel(const int32_t* __restrict__ row_of_pair, uint32_t pairs, const float* __restrict__ dwp,
+                               uint32_t tiles, T* __restrict__ dw) {
+  const uint32_t i = blockIdx.x * blockDim.x + threadIdx.x;
+  if (i >= pairs) return;
+  const int32_t row = row_of_pair[i];
+  float s = 0.f;
+  if (row >= 0)
+    for (uint32_t j = 0; j < tiles; ++j) s += dwp[uint64_t(row) * tiles + j];
+  dw[i] = from_f<T>(s);
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// dz = dy act'(pre), rounded once to the operands' type (the products take 16-bit operands), and db from the unrounded
+// values: each CTA sums kDzRows rows of 32 V columns, then one thread per column adds the CTAs' sums in order.
+// ---------------------------------------------------------------------------------------------------------------
+constexpr uint32_t kDzRows = 128;
+
+template <class T, int V>
+__global__ __launch_bounds__(256) void dz_kernel(int act, const T* __restrict__ dy, uint64_t ldy,
+                                                 const T* __restrict__ pre, uint64_t ldp, T* __restrict__ dz,
+                                                 uint64_t ldz, uint64_t rows, uint64_t n, float* __restrict__ part) {
+  __shared__ float red[8][32 * V];
+  const uint64_t c = (uint64_t(blockIdx.y) * 32 + threadIdx.x) * V;
+  const uint64_t r0 = uint64_t(blockIdx.x) * kDzRows, r1 = r0 + kDzRows < rows ? r0 + kDzRows : rows;
+  float sum[V] = {};
+  if (c < n)
+    for (uint64_t r = r0 + threadIdx.y; r < r1; r += 8) {
+      T a[V], z[V];
+      if constexpr (V == 8) {
+        *reinterpret_cast<uint4*>(a) = *reinterpret_cast<const uint4*>(dy + r * ldy + c);
+        if (dz) *reinterpret_cast<uint4*>(z) = *reinterpret_cast<const uint4*>(pre + r * ldp + c);
+      } else {
+        a[0] = dy[r * ldy + c];
+        if (dz) z[0] = pre[r * ldp + c];
+      }
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        const float d = to_f(a[v]) * (dz ? slope_rt(act, to_f(z[v])) : 1.f);
+        sum[v] += d;
+        a[v] = from_f<T>(d);
+      }
+      if (dz) {
+        if constexpr (V == 8) *reinterpret_cast<uint4*>(dz + r * ldz + c) = *reinterpret_cast<uint4*>(a);
+        else dz[r * ldz + c] = a[0];
+      }
+    }
+  if (!part) return;
+#pragma unroll
+  for (int v = 0; v < V; ++v) red[threadIdx.y][threadIdx.x * V + v] = sum[v];
+  __syncthreads();
+  for (uint32_t j = threadIdx.y * 32 + threadIdx.x; j < 32 * V; j += 256) {
+    const uint64_t col = uint64_t(blockIdx.y) * 32 * V + j;
+    if (col >= n) continue;
+    float s = 0.f;
+    for (int w = 0; w < 8; ++w) s += red[w][j];
+    part[uint64_t(blockIdx.x) * n + col] = s;
+  }
+}
+
+template <class T>
+__global__ void db_kernel(const float* __restrict__ part, uint32_t chunks, uint64_t n, T* __restrict__ db) {
+  const uint64_t c = uint64_t(blockIdx.x) * blockDim.x + threadIdx.x;
+  if (c >= n) return;
+  float s = 0.f;
+  for (uint32_t j = 0; j < chunks; ++j) s += part[j * n + c];
+  db[c] = from_f<T>(s);
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// The router. A warp holds a row's logits in registers (expert j in lane j % 32) and takes the largest `top` times: the
+// values as ordered unsigned words, so that one redux finds the maximum and one the lowest expert among the equal ones.
+// -inf and NaN order as 0 and are never taken; +inf counts as the largest finite value. Bound by the logits' bytes for
+// long prompts, by the launch for single tokens.
+// ---------------------------------------------------------------------------------------------------------------
+__device__ __forceinline__ float logit_of(float z) {
+  if (!(z > -INFINITY)) return -INFINITY;  // NaN too
+  return fminf(z, FLT_MAX) + 0.f;          // (+ 0: -0 equals +0)
+}
+__device__ __forceinline__ uint32_t ordered(float z) {
+  if (z == -INFINITY) return 0u;
+  const uint32_t b = __float_as_uint(z);
+  return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ float warp_add(float v) {
+  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+template <class T, int V>
+__global__ __launch_bounds__(256) void route_kernel(const T* __restrict__ logits, uint64_t ld, uint64_t rows,
+                                                    uint32_t experts, uint32_t top, int norm, int32_t* __restrict__ ids,
+                                                    float* __restrict__ weights) {
+  const uint64_t row = uint64_t(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  const uint32_t lane = threadIdx.x & 31;
+  if (row >= rows) return;
+  float z[V];
+  uint32_t key[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    const uint32_t j = lane + 32 * v;
+    z[v] = j < experts ? logit_of(to_f(logits[row * ld + j])) : -INFINITY;
+    key[v] = ordered(z[v]);
+  }
+  float best = 0.f, mine = 0.f;  // lane i keeps choice i
+  int32_t id = -1;
+  for (uint32_t i = 0; i < top; ++i) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int v = 0; v < V; ++v) m = key[v] > m ? key[v] : m;
+    m = __reduce_max_sync(0xffffffffu, m);
+    if (!m) break;
+    uint32_t at = kNone;
+#pragma unroll
+    for (int v = V - 1; v >= 0; --v)
+      if (key[v] == m) at = lane + 32 * v;
+    at = __reduce_min_sync(0xffffffffu, at);
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+      if (at == lane + 32 * v) key[v] = 0;
+    const float val = __uint_as_float(m & 0x80000000u ? m & 0x7fffffffu : ~m);
+    if (i == 0) best = val;
+    if (lane == i) id = int32_t(at), mine = val;
+  }
+  const float p = id >= 0 ? expf(mine - best) : 0.f;
+  float sum = 0.f;
+  if (norm) {
+    sum = p;
+  } else {
+#pragma unroll
+    for (int v = 0; v < V; ++v) sum += z[v] == -INFINITY ? 0.f : expf(z[v] - best);
+  }
+  sum = warp_add(sum);
+  if (lane < top) {
+    ids[row * top + lane] = id;
+    weights[row * top + lane] = id >= 0 ? p / sum : 0.f;
+  }
+}
+
+template <class T, class W, int V>
+__global__ __launch_bounds__(256) void route_back_kernel(const W* __restrict__ dw, const T* __restrict__ logits,
+                                                         uint64_t ld, const int32_t* __restrict__ ids,
+                                                         const float* __restrict__ weights, uint64_t rows,
+                                                         uint32_t experts, uint32_t top, int norm,
+                                                         T* __restrict__ dlogits, uint64_t ldd) {
+  const uint64_t row = uint64_t(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  const uint32_t lane = threadIdx.x & 31;
+  if (row >= rows) return;
+  const int32_t id = lane < top ? ids[row * top + lane] : -1;
+  const bool there = uint32_t(id) < experts;
+  const float d = there ? to_f(dw[row * top + lane]) : 0.f, w = there ? weights[row * top + lane] : 0.f;
+  const float s = warp_add(d * w);  // sum_i dw_i p_i
+  float p[V], g[V];
+  if (norm) {  // p is the chosen weights and zero elsewhere
+#pragma unroll
+    for (int v = 0; v < V; ++v) p[v] = 0.f;
+  } else {
+    float m = -INFINITY, sum = 0.f;
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      const uint32_t j = lane + 32 * v;
+      p[v] = j < experts ? logit_of(to_f(logits[row * ld + j])) : -INFINITY;
+      m = fmaxf(m, p[v]);
+    }
+    for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      p[v] = p[v] == -INFINITY ? 0.f : expf(p[v] - m);
+      sum += p[v];
+    }
+    sum = warp_add(sum);
+#pragma unroll
+    for (int v = 0; v < V; ++v) p[v] = sum > 0.f ? p[v] / sum : 0.f;
+  }
+#pragma unroll
+  for (int v = 0; v < V; ++v) g[v] = -s;
+  for (uint32_t i = 0; i < top; ++i) {
+    const int32_t e = __shfl_sync(0xffffffffu, id, i);
+    const float di = __shfl_sync(0xffffffffu, d, i), wi = __shfl_sync(0xffffffffu, w, i);
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+      if (e == int32_t(lane + 32 * v)) {
+        g[v] += di;
+        if (norm) p[v] = wi;
+      }
+  }
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    const uint32_t j = lane + 32 * v;
+    if (j < experts) dlogits[row * ldd + j] = from_f<T>(p[v] * g[v]);
+  }
+}
+
+template <class F>
+void by_experts(uint32_t experts, F&& f) {
+  if (experts <= 32) f(std::integral_constant<int, 1>());
+  else if (experts <= 64) f(std::integral_constant<int, 2>());
+  else if (experts <= 128) f(std::integral_constant<int, 4>());
+  else if (experts <= 256) f(std::integral_constant<int, 8>());
+  else if (experts <= 512) f(std::integral_constant<int, 16>());
+  else f(std::integral_constant<int, 32>());
+}
+template <class F>
+void by_type(int dtype, F&& f) {
+  if (dtype == TSB_BF16) f(__nv_bfloat16());
+  else if (dtype == TSB_F16) f(__half());
+  else f(float());
+}
+
+uint64_t aligned(uint64_t n) { return (n + 255) / 256 * 256; }
+bool on16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+}  // namespace
+
+// Plan arrays back to back, each on 256 bytes. A group of c rows has at most c / bm + 1 tiles and pad - 1 padding rows.
+Plan plan_at(void* ws, uint32_t units, uint64_t pairs, uint32_t pad, uint32_t bm) {
+  Plan p{};
+  const uint64_t met = pairs < units ? pairs : units;
+  p.units = units;
+  p.pairs = uint32_t(pairs);
+  p.pad = pad;
+  p.bm = bm;
+  p.max_rows = uint32_t(pairs + met * (pad - 1));
+  p.max_tiles = uint32_t(pairs / bm + met);
+  char* c = static_cast<char*>(ws);
+  auto take = [&](uint64_t n) {
+    int32_t* r = reinterpret_cast<int32_t*>(c);
+    c += aligned(n * 4);
+    return r;
+  };
+  p.head = take(2);
+  p.cnt = take(units);
+  p.off = take(units);
+  p.slot = take(units);
+  p.pair_of_row = take(p.max_rows);
+  p.row_of_pair = take(pairs);
+  p.tile_unit = take(p.max_tiles);
+  p.tile_m0 = take(p.max_tiles);
+  return p;
+}
+uint64_t plan_bytes(uint32_t units, uint64_t pairs, uint32_t pad, uint32_t bm) {
+  const uint64_t met = pairs < units ? pairs : units;
+  return aligned(8) + 3 * aligned(uint64_t(units) * 4) + aligned((pairs + met * (pad - 1)) * 4) + aligned(pairs * 4) +
+         2 * aligned((pairs / bm + met) * 4);
+}
+
+int launch_plan(const Plan& p, const Units& u, const int32_t* ids, cudaStream_t s) {
+  if (p.pairs <= kSmallPairs && p.units <= kSmallUnits) {
+    plan_small_kernel<<<1, kSmallThreads, 0, s>>>(p, u, ids);
+  } else {
+    plan_count_kernel<<<p.units, kPlanThreads, 0, s>>>(p, u, ids);
+    plan_fill_kernel<<<p.units, kPlanThreads, 0, s>>>(p, ids);
+  }
+  return int(cudaGetLastError());
+}
+
+int launch_join(int dtype, const Plan& p, const float* rows32, uint32_t splits, const float* weights, uint32_t top,
+                uint64_t rows, uint64_t n, const void* residual, uint64_t ldr, void* y, uint64_t ldy, cudaStream_t s) {
+  by_type(dtype, [&](auto v) {
+    using T = decltype(v);
+    const uint64_t stride = uint64_t(p.max_rows) * n;
+    const T* r = static_cast<const T*>(residual);
+    if (n % 4 == 0)
+      join_kernel<T, 4><<<dim3(unsigned(rows), unsigned(ceil_div(n, 1024))), 256, 0, s>>>(
+          p.row_of_pair, rows32, splits, stride, weights, top, n, r, ldr, static_cast<T*>(y), ldy);
+    else
+      join_kernel<T, 1><<<dim3(unsigned(rows), unsigned(ceil_div(n, 256))), 256, 0, s>>>(
+          p.row_of_pair, rows32, splits, stride, weights, top, n, r, ldr, static_cast<T*>(y), ldy);
+  });
+  return int(cudaGetLastError());
+}
+
+int launch_join_dw(int dtype, const Plan& p, const float* dwp, uint32_t tiles, void* dw, cudaStream_t s) {
+  by_type(dtype, [&](auto v) {
+    using T = decltype(v);
+    join_dw_kernel<T><<<unsigned(ceil_div(p.pairs, 128)), 128, 0, s>>>(p.row_of_pair, p.pairs, dwp, tiles,
+                                                                      static_cast<T*>(dw));
+  });
+  return int(cudaGetLastError());
+}
+
+uint32_t dz_chunks(uint64_t rows, uint64_t) { return uint32_t(ceil_div(rows, kDzRows)); }
+
+int launch_dz(int dtype, int act, const void* dy, uint64_t ldy, const void* pre, uint64_t ldp, void* dz, uint64_t ldz,
+              uint64_t rows, uint64_t n, void* db, float* part, cudaStream_t s) {
+  const bool wide = n % 8 == 0 && on16(dy) && ldy % 8 == 0 && (!dz || (on16(pre) && ldp % 8 == 0 && ldz % 8 == 0));
+  const uint32_t chunks = dz_chunks(rows, n);
+  by_type(dtype, [&](auto v) {
+    using T = decltype(v);
+    const T *a = static_cast<const T*>(dy), *b = static_cast<const T*>(pre);
+    T* z = static_cast<T*>(dz);
+    if (wide)
+      dz_kernel<T, 8><<<dim3(chunks, unsigned(ceil_div(n, 256))), dim3(32, 8), 0, s>>>(act, a, ldy, b, ldp, z, ldz, rows,
+                                                                                      n, db ? part : nullptr);
+    else
+      dz_kernel<T, 1><<<dim3(chunks, unsigned(ceil_div(n, 32))), dim3(32, 8), 0, s>>>(act, a, ldy, b, ldp, z, ldz, rows,
+                                                                                     n, db ? part : nullptr);
+    if (db) db_kernel<T><<<unsigned(ceil_div(n, 128)), 128, 0, s>>>(part, chunks, n, static_cast<T*>(db));
+  });
+  return int(cudaGetLastError());
+}
+
+int launch_route(int dtype, const void* logits, uint64_t ld, uint64_t rows, uint32_t experts, uint32_t top, int norm,
+                 int32_t* ids, float* weights, cudaStream_t s) {
+  by_type(dtype, [&](auto v) {
+    using T = decltype(v);
+    by_experts(experts, [&](auto c) {
+      route_kernel<T, c.value><<<unsigned(ceil_div(rows, 8)), 256, 0, s>>>(static_cast<const T*>(logits), ld, rows,
+                                                                          experts, top, norm, ids, weights);
+    });
+  });
+  return int(cudaGetLastError());
+}
+
+int launch_route_back(int dtype, int dw_dtype, const void* dw, const void* logits, uint64_t ld, const int32_t* ids,
+                      const float* weights, uint64_t rows, uint32_t experts, uint32_t top, int norm, void* dlogits,
+                      uint64_t ldd, cudaStream_t s) {
+  by_type(dtype, [&](auto v) {
+    by_type(dw_dtype, [&](auto x) {
+      using T = decltype(v);
+      using W = decltype(x);
+      by_experts(experts, [&](auto c) {
+        route_back_kernel<T, W, c.value><<<unsigned(ceil_div(rows, 8)), 256, 0, s>>>(
+            static_cast<const W*>(dw), static_cast<const T*>(logits), ld, ids, weights, rows, experts, top, norm,
+            static_cast<T*>(dlogits), ldd);
+      });
+    });
+  });
+  return int(cudaGetLastError());
+}
+
+}  // namespace ops
+}  // namespace tsb
