@@ -511,6 +511,10 @@ typedef struct tsb_ffn_grad_args {
 SS_API uint64_t tsb_ffn_backward_workspace(const tsb_ffn_grad_args* a);
 SS_API ss_status tsb_ffn_backward(const tsb_ffn_grad_args* a);
 
+/* The thread blocks of these operators whose staging or products did not complete within 2 s on the current device
+ * since the last call (their outputs are wrong), then reset; -1 on a device error. Synchronises. */
+SS_API int tsb_ops_timeouts(void);
+
 #ifdef __cplusplus
 }
 #endif

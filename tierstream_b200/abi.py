@@ -351,6 +351,7 @@ _PROTOS.update({
     "tsb_ffn": (C.c_int, [vp]),
     "tsb_ffn_backward_workspace": (u64, [vp]),
     "tsb_ffn_backward": (C.c_int, [vp]),
+    "tsb_ops_timeouts": (C.c_int, []),
 })
 
 _lib = None

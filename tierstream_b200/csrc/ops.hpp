@@ -180,5 +180,14 @@ int launch_dz(int dtype, int act, const void* dy, uint64_t ldy, const void* pre,
 constexpr uint32_t kTileM = 64, kTileN = 64;
 int launch_tile(int dtype, const Product& p, const Plan* plan, const Units* units, cudaStream_t s);
 
+
+// ops_tc.cu: products of many rows on tcgen05 (the plan made with bm = kTcRows). tc_fits: TMA can read the operand.
+// Gathered operands are gathered first: launch_gather copies n columns of every grouped row (n a multiple of 8).
+constexpr uint32_t kTcRows = 128;
+bool tc_fits(const Operand& o, const Units* units);
+int launch_gather(const Plan& plan, uint32_t top, const void* src, uint64_t ld, uint64_t n, void* dst, cudaStream_t s);
+int launch_tc(int dtype, const Product& p, const Plan* plan, const Units* units, cudaStream_t s);
+int ops_take_timeouts(uint32_t* out);
+
 }  // namespace ops
 }  // namespace tsb

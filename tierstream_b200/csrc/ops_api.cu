@@ -59,6 +59,13 @@ Operand gathered(const void* p, int64_t s_i, int64_t s_k, const Plan& plan, uint
 }
 Operand of_unit(int part, int64_t s_i, int64_t s_k) { return {nullptr, s_i, s_k, nullptr, 1, 0, part}; }
 
+// One matrix product: on the tensor cores' own path when TMA can read both operands (rows on 16 bytes), else by the
+// kernel for every alignment.
+int product(int dtype, const Product& p, cudaStream_t s) {
+  if (tc_fits(p.a[0], nullptr) && tc_fits(p.b[0], nullptr)) return launch_tc(dtype, p, nullptr, nullptr, s);
+  return launch_tile(dtype, p, nullptr, nullptr, s);
+}
+
 // ---- linear ----
 void check_linear(const tsb_linear_args* a) {
   const char* fn = "tsb_linear";
@@ -90,7 +97,7 @@ void linear(const tsb_linear_args* a) {
   p.bias = a->bias;
   p.residual = a->residual, p.ldr = int64_t(a->ldr);
   p.pre = a->pre, p.ldp = int64_t(a->ldp);
-  ck(launch_tile(int(a->dtype), p, nullptr, nullptr, s), fn, "launch");
+  ck(product(int(a->dtype), p, s), fn, "launch");
 }
 
 void check_linear_back(const tsb_linear_grad_args* a) {
@@ -152,7 +159,7 @@ void linear_back(const tsb_linear_grad_args* a) {
     p.m = int64_t(a->rows), p.n = int64_t(a->k), p.k = int64_t(a->n);
     p.epi = kEpiStore;
     p.out = a->dx, p.ldo = int64_t(a->lddx);
-    ck(launch_tile(int(a->dtype), p, nullptr, nullptr, s), fn, "dx");
+    ck(product(int(a->dtype), p, s), fn, "dx");
   }
   if (a->dw) {
     Product p{};
@@ -162,7 +169,7 @@ void linear_back(const tsb_linear_grad_args* a) {
     p.m = int64_t(a->n), p.n = int64_t(a->k), p.k = int64_t(a->rows);
     p.epi = kEpiStore;
     p.out = a->dw, p.ldo = int64_t(a->lddw);
-    ck(launch_tile(int(a->dtype), p, nullptr, nullptr, s), fn, "dw");
+    ck(product(int(a->dtype), p, s), fn, "dw");
   }
 }
 
@@ -200,8 +207,20 @@ void check_ffn_shape(const A* a, const char* fn) {
        "the parts' strides must be whole elements");
 }
 
+// Whether the block's products run on the tensor cores' own path: whole 16 bytes in every row, the units in slots.
+bool ffn_tc(const tsb_units* u, uint64_t hidden, uint64_t ffn, const void* x, uint64_t ldx, const void* dy,
+            uint64_t lddy) {
+  auto on16 = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; };
+  if (u->table || hidden % 8 || ffn % 8 || !on16(x) || ldx % 8 || !on16(dy) || lddy % 8) return false;
+  for (int i = 0; i < 3; ++i)
+    if (!on16(u->part[i]) || u->stride[i] % 16 || u->stride[i] >= (uint64_t(1) << 40)) return false;
+  return true;
+}
+
 struct FfnSpace {
   Plan plan;
+  bool tc;
+  void* xs;
   void* h;
   float* rows32;
   uint64_t bytes;
@@ -210,7 +229,10 @@ FfnSpace ffn_space(const tsb_ffn_args* a) {
   Arena w{static_cast<char*>(a->workspace)};
   FfnSpace r{};
   const uint64_t pairs = a->rows * a->top;
-  r.plan = plan_at(w.take(plan_bytes(a->units->n_units, pairs, 1, 64)), a->units->n_units, pairs, 1, 64);
+  r.tc = ffn_tc(a->units, a->hidden, a->ffn, a->x, a->ldx, nullptr, 0);
+  const uint32_t bm = r.tc ? kTcRows : kTileM;
+  r.plan = plan_at(w.take(plan_bytes(a->units->n_units, pairs, 1, bm)), a->units->n_units, pairs, 1, bm);
+  if (r.tc) r.xs = w.take(uint64_t(r.plan.max_rows) * a->hidden * 2);
   r.h = w.take(uint64_t(r.plan.max_rows) * a->ffn * 2);
   r.rows32 = static_cast<float*>(w.take(uint64_t(r.plan.max_rows) * a->hidden * 4));
   r.bytes = w.used;
@@ -247,7 +269,12 @@ void ffn(const tsb_ffn_args* a) {
   p.epi = kEpiUp;
   p.act = int(a->act);
   p.out = w.h, p.ldo = f;
-  ck(launch_tile(int(a->dtype), p, &w.plan, &u, s), fn, "gate and up");
+  const auto go = w.tc ? launch_tc : launch_tile;
+  if (w.tc) {
+    ck(launch_gather(w.plan, a->top, a->x, a->ldx, a->hidden, w.xs, s), fn, "gather");
+    p.a[0] = p.a[1] = dense(w.xs, d, 1);
+  }
+  ck(go(int(a->dtype), p, &w.plan, &u, s), fn, "gate and up");
   Product q{};
   q.grouped = 1;
   q.segs = 1;
@@ -256,7 +283,7 @@ void ffn(const tsb_ffn_args* a) {
   q.n = d, q.k = f;
   q.epi = kEpiRows32;
   q.rows32 = w.rows32;
-  ck(launch_tile(int(a->dtype), q, &w.plan, &u, s), fn, "down");
+  ck(go(int(a->dtype), q, &w.plan, &u, s), fn, "down");
   ck(launch_join(int(a->dtype), w.plan, w.rows32, 1, a->weights, a->top, a->rows, a->hidden, a->residual, a->ldr, a->y,
                  a->ldy, s),
      fn, "join");
@@ -264,7 +291,8 @@ void ffn(const tsb_ffn_args* a) {
 
 struct FfnBackSpace {
   Plan plan;
-  void *dg, *du, *hw;
+  bool tc;
+  void *xs, *dys, *dg, *du, *hw;
   float *dwp, *rows32;
   uint32_t dw_tiles;
   uint64_t bytes;
@@ -273,11 +301,18 @@ FfnBackSpace ffn_back_space(const tsb_ffn_grad_args* a) {
   Arena w{static_cast<char*>(a->workspace)};
   FfnBackSpace r{};
   const uint64_t pairs = a->rows * a->top;
-  r.plan = plan_at(w.take(plan_bytes(a->units->n_units, pairs, 1, 64)), a->units->n_units, pairs, 1, 64);
+  r.tc = ffn_tc(a->units, a->hidden, a->ffn, a->x, a->ldx, a->dy, a->lddy);
+  // (sums over a group's rows run in slices of 64 on the tensor cores: zero rows fill the last one)
+  const uint32_t bm = r.tc ? kTcRows : kTileM, pad = r.tc && a->dgate ? 64 : 1;
+  r.plan = plan_at(w.take(plan_bytes(a->units->n_units, pairs, pad, bm)), a->units->n_units, pairs, pad, bm);
+  if (r.tc) {
+    r.xs = w.take(uint64_t(r.plan.max_rows) * a->hidden * 2);
+    r.dys = w.take(uint64_t(r.plan.max_rows) * a->hidden * 2);
+  }
   r.dg = w.take(uint64_t(r.plan.max_rows) * a->ffn * 2);
   r.du = w.take(uint64_t(r.plan.max_rows) * a->ffn * 2);
   if (a->dgate) r.hw = w.take(uint64_t(r.plan.max_rows) * a->ffn * 2);
-  r.dw_tiles = uint32_t(ceil_div(a->ffn, kTileN));
+  r.dw_tiles = r.tc ? 2 * uint32_t(ceil_div(a->ffn, 128)) : uint32_t(ceil_div(a->ffn, kTileN));
   if (a->dweights) r.dwp = static_cast<float*>(w.take(uint64_t(r.plan.max_rows) * r.dw_tiles * 4));
   if (a->dx) r.rows32 = static_cast<float*>(w.take(uint64_t(r.plan.max_rows) * a->hidden * 4));
   r.bytes = w.used;
@@ -311,12 +346,25 @@ void ffn_back(const tsb_ffn_grad_args* a) {
   const Units u = units_of(a->units);
   const int dt = int(a->dtype);
   ck(launch_plan(w.plan, u, a->ids, s), fn, "plan");
+  const auto go = w.tc ? launch_tc : launch_tile;
+  Operand x_rows = gathered(a->x, int64_t(a->ldx), 1, w.plan, a->top),
+          dy_rows = gathered(a->dy, int64_t(a->lddy), 1, w.plan, a->top),
+          x_sum = gathered(a->x, 1, int64_t(a->ldx), w.plan, a->top, 1),
+          dy_sum = gathered(a->dy, 1, int64_t(a->lddy), w.plan, a->top, 1);
+  if (w.tc) {
+    ck(launch_gather(w.plan, a->top, a->x, a->ldx, a->hidden, w.xs, s), fn, "gather");
+    ck(launch_gather(w.plan, a->top, a->dy, a->lddy, a->hidden, w.dys, s), fn, "gather");
+    x_rows = dense(w.xs, d, 1);
+    dy_rows = dense(w.dys, d, 1);
+    x_sum = dense(w.xs, 1, d, 1);
+    dy_sum = dense(w.dys, 1, d, 1);
+  }
   {
     Product p{};
     p.grouped = 1;
     p.segs = 3;
-    p.a[0] = p.a[1] = gathered(a->x, int64_t(a->ldx), 1, w.plan, a->top);
-    p.a[2] = gathered(a->dy, int64_t(a->lddy), 1, w.plan, a->top);
+    p.a[0] = p.a[1] = x_rows;
+    p.a[2] = dy_rows;
     p.b[0] = of_unit(0, d, 1);
     p.b[1] = of_unit(1, d, 1);
     p.b[2] = of_unit(2, 1, f);
@@ -327,7 +375,7 @@ void ffn_back(const tsb_ffn_grad_args* a) {
     p.dg = w.dg, p.du = w.du, p.hw = w.hw, p.ldo = f;
     p.dwp = w.dwp, p.ld_dwp = w.dw_tiles;
     p.weights = a->weights;
-    ck(launch_tile(dt, p, &w.plan, &u, s), fn, "gate, up and dh");
+    ck(go(dt, p, &w.plan, &u, s), fn, "gate, up and dh");
   }
   if (a->dweights) ck(launch_join_dw(dt, w.plan, w.dwp, w.dw_tiles, a->dweights, s), fn, "dweights");
   if (a->dx) {
@@ -341,7 +389,7 @@ void ffn_back(const tsb_ffn_grad_args* a) {
     p.n = d, p.k = f;
     p.epi = kEpiRows32;
     p.rows32 = w.rows32;
-    ck(launch_tile(dt, p, &w.plan, &u, s), fn, "dx");
+    ck(go(dt, p, &w.plan, &u, s), fn, "dx");
     ck(launch_join(dt, w.plan, w.rows32, 1, nullptr, a->top, a->rows, a->hidden, nullptr, 0, a->dx, a->lddx, s), fn,
        "join");
   }
@@ -353,18 +401,18 @@ void ffn_back(const tsb_ffn_grad_args* a) {
     p.epi = kEpiStore;
     p.out_unit = d * f;
     p.m = f, p.n = d, p.ldo = d;
-    p.b[0] = gathered(a->x, 1, int64_t(a->ldx), w.plan, a->top, 1);
+    p.b[0] = x_sum;
     p.a[0] = dense(w.dg, 1, f, 1);
     p.out = a->dgate;
-    ck(launch_tile(dt, p, &w.plan, &u, s), fn, "dgate");
+    ck(go(dt, p, &w.plan, &u, s), fn, "dgate");
     p.a[0] = dense(w.du, 1, f, 1);
     p.out = a->dup;
-    ck(launch_tile(dt, p, &w.plan, &u, s), fn, "dup");
+    ck(go(dt, p, &w.plan, &u, s), fn, "dup");
     p.m = d, p.n = f, p.ldo = f;
-    p.a[0] = gathered(a->dy, 1, int64_t(a->lddy), w.plan, a->top, 1);
+    p.a[0] = dy_sum;
     p.b[0] = dense(w.hw, 1, f, 1);
     p.out = a->ddown;
-    ck(launch_tile(dt, p, &w.plan, &u, s), fn, "ddown");
+    ck(go(dt, p, &w.plan, &u, s), fn, "ddown");
   }
 }
 
@@ -459,6 +507,11 @@ uint64_t tsb_ffn_backward_workspace(const tsb_ffn_grad_args* a) {
 }
 ss_status tsb_ffn_backward(const tsb_ffn_grad_args* a) {
   return run([&] { ffn_back(a); });
+}
+
+int tsb_ops_timeouts(void) {
+  uint32_t v = 0;
+  return ops_take_timeouts(&v) == 0 ? int(v) : -1;
 }
 
 }  // extern "C"

@@ -1,0 +1,692 @@
+// The products for many rows, on the tensor cores (tcgen05) with both operands staged by TMA.
+//
+// A persistent CTA per SM computes 128-row tiles: one thread keeps TMA loads of 64-wide k slices in flight through a ring
+// of four stages (A 16 KiB, B up to 32 KiB, both 128-byte swizzled), one thread issues tcgen05.mma (128 x up to 256 x 16,
+// 32-bit sums in TMEM), and eight warps read finished sums back (tcgen05.ld), apply the epilogue of ops.hpp and store
+// through a small per-warp transpose in shared memory, so that global stores run along rows. With at most 256 columns a
+// tile the sums are double buffered in TMEM and the epilogue of one tile runs under the products of the next.
+//
+// Operands come either with k contiguous (K-major) or with m or n contiguous (MN-major), so that no backward product
+// needs a transposed copy. The gate and up products of a tile are one 256-column product (128 columns of each), whose two
+// halves of a row meet in the same thread's epilogue; the backward pass adds dy Wd as a third 128-column product, so that
+// g, u and dh are never stored. Rows of a group start anywhere; the rows of a tile behind its group's end are computed
+// and not stored.
+//
+// Every wait is bounded (2 s): one that runs out counts in a device word (tsb_ops_timeouts), and the CTA leaves after a
+// bounded wait for its copies and products in flight, its TMEM freed.
+#include <cuda.h>
+
+#include <cstring>
+
+#include "ops.hpp"
+
+namespace tsb {
+namespace ops {
+namespace {
+
+constexpr int kBM = 128, kBK = 64, kStages = 4;
+constexpr int kABytes = kBM * kBK * 2, kBBytes = 256 * kBK * 2, kStageBytes = kABytes + kBBytes;
+constexpr int kEpiWarps = 8, kThreads = 128 + 32 * kEpiWarps;
+constexpr int kRowBytes = 80, kStoreBytes = 32 * kRowBytes;  // a warp's 32 rows of 64 bytes, 16 apart: no bank twice
+constexpr int kSmemBytes = 1024 + kStages * kStageBytes + kEpiWarps * kStoreBytes + 256;
+constexpr unsigned long long kWaitNs = 2000000000ull;
+
+__device__ uint32_t g_ops_timeouts;
+
+enum Mode { kLin, kLinDx, kLinDw, kUp, kUpBack, kDown, kDx, kDw };
+
+struct Params {
+  Plan plan;
+  Product p;         // the epilogue's fields, n, and the groups
+  int32_t bn;        // columns of a tile (of each of gate and up)
+  int32_t n_tiles;   // tiles along n
+  int32_t m_tiles;   // tiles along m when not grouped
+  int32_t k_blocks;  // of a segment; with k_rows per unit: from the group
+  int32_t vec;       // 16-byte stores are possible
+};
+struct Maps {
+  CUtensorMap a[2], b[3];
+};
+
+__device__ __forceinline__ uint32_t smem_u32(const void* p) { return uint32_t(__cvta_generic_to_shared(p)); }
+__device__ __forceinline__ void bar_init(uint32_t b, uint32_t n) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(b), "r"(n) : "memory");
+}
+__device__ __forceinline__ void bar_expect(uint32_t b, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(b), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void bar_arrive(uint32_t b) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(b) : "memory");
+}
+__device__ __forceinline__ bool bar_try(uint32_t b, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(b), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+__device__ __forceinline__ unsigned long long now_ns() {
+  unsigned long long t;
+  asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
+  return t;
+}
+__device__ __noinline__ bool bar_wait_slow(uint32_t b, uint32_t parity, volatile uint32_t* dead) {
+  const unsigned long long t0 = now_ns();
+  for (;;) {
+    if (bar_try(b, parity)) return true;
+    if (*dead) return false;
+    if (now_ns() - t0 > kWaitNs) {
+      *dead = 1;
+      return false;
+    }
+  }
+}
+// false: the wait ran out, here or elsewhere in the CTA
+__device__ __forceinline__ bool bar_wait(uint32_t b, uint32_t parity, volatile uint32_t* dead) {
+  for (int i = 0; i < 8; ++i)
+    if (bar_try(b, parity)) return true;
+  return bar_wait_slow(b, parity, dead);
+}
+__device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
+          dst),
+      "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
+      : "memory");
+}
+// Shared memory descriptors, 128-byte swizzle. K-major: 8-row groups 1024 bytes apart. MN-major: a stage holds 64-wide
+// chunks of [64 k rows][128 bytes], 8 KiB apart, 8-row groups of k 1024 bytes apart.
+__device__ __forceinline__ uint64_t desc(uint32_t addr, bool mn) {
+  return uint64_t((addr & 0x3ffffu) >> 4) | (uint64_t(mn ? 8192 >> 4 : 1) << 16) | (uint64_t(1024 >> 4) << 32) |
+         (uint64_t(1) << 46) | (uint64_t(2) << 61);
+}
+__device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(uint32_t(add))
+      : "memory");
+}
+__device__ __forceinline__ void commit(uint32_t bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void tmem_ld16(uint32_t addr, float (&v)[16]) {
+  uint32_t r[16];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(addr));
+#pragma unroll
+  for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
+}
+__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+
+struct Tile {
+  int unit, slot, row0, rows, stored;  // row0: the group's first row; rows: m limit; stored: rows to store (padding too)
+  int m0, n, kb;
+};
+
+// Tile L of the launch: groups in unit order, inside a group chunks of up to 16 row tiles, inside a chunk the column
+// tiles, and the chunk's row tiles innermost, so that tiles running at the same time share a unit's columns from L2.
+template <int MODE>
+__device__ __forceinline__ bool tile_at(const Params& q, int L, Tile& t) {
+  constexpr int kChunk = 16;
+  int local, mt;
+  if constexpr (MODE == kUp || MODE == kUpBack || MODE == kDown || MODE == kDx) {
+    const int i = L / q.n_tiles;
+    if (i >= q.plan.head[0]) return false;
+    t.unit = q.plan.tile_unit[i];
+    t.rows = q.plan.cnt[t.unit];
+    t.stored = (t.rows + int(q.plan.pad) - 1) / int(q.plan.pad) * int(q.plan.pad);
+    t.row0 = q.plan.off[t.unit];
+    t.slot = q.plan.slot[t.unit];
+    mt = (t.rows + kBM - 1) / kBM;
+    local = L - (i - q.plan.tile_m0[i] / kBM) * q.n_tiles;
+    t.kb = q.k_blocks;
+  } else if constexpr (MODE == kDw) {
+    const int per = q.m_tiles * q.n_tiles;
+    t.unit = L / per;
+    if (t.unit >= int(q.plan.units)) return false;
+    t.row0 = q.plan.off[t.unit];
+    t.slot = 0;
+    t.rows = t.stored = int(q.p.m);
+    t.kb = (q.plan.cnt[t.unit] + kBK - 1) / kBK;
+    mt = q.m_tiles;
+    local = L - t.unit * per;
+  } else {
+    if (L >= q.m_tiles * q.n_tiles) return false;
+    t.unit = t.slot = t.row0 = 0;
+    t.rows = t.stored = int(q.p.m);
+    mt = q.m_tiles;
+    local = L;
+    t.kb = q.k_blocks;
+  }
+  const int chunk = local / (kChunk * q.n_tiles), in = local - chunk * kChunk * q.n_tiles;
+  const int width = min(kChunk, mt - chunk * kChunk);
+  t.n = in / width;
+  t.m0 = (chunk * kChunk + in - t.n * width) * kBM;
+  return true;
+}
+
+template <int MODE>
+struct Traits {
+  static constexpr bool grouped = MODE == kUp || MODE == kUpBack || MODE == kDown || MODE == kDx;
+  static constexpr int segs = MODE == kUpBack || MODE == kDx ? 2 : 1;
+  static constexpr bool a_mn = MODE == kLinDw || MODE == kDw;
+  static constexpr bool pair0 = MODE == kUp || MODE == kUpBack;  // segment 0's B: columns of gate, then of up
+  // B of segment s with n contiguous
+  __host__ __device__ static constexpr bool b_mn(int s) {
+    return MODE == kLinDx || MODE == kLinDw || MODE == kDx || MODE == kDw || (MODE == kUpBack && s == 1);
+  }
+  static constexpr int bufs = MODE == kUpBack ? 1 : 2;
+};
+
+template <class T>
+__device__ __forceinline__ uint32_t pack(float a, float b) {
+  T v[2] = {from_f<T>(a), from_f<T>(b)};
+  uint32_t r;
+  memcpy(&r, v, 4);
+  return r;
+}
+
+// A warp's 32 rows x 64 bytes (thread = row) written along rows: 8 rows of 64 bytes a store. `cols` elements of E bytes
+// are inside the matrix; vec: 16-byte stores fit.
+template <class E>
+__device__ __forceinline__ void store_rows(char* stage, const uint32_t (&v)[16], E* out, int64_t ld, int rows, int cols,
+                                           bool vec) {
+  const int lane = threadIdx.x & 31;
+  constexpr int kPer = 16 / int(sizeof(E));
+  uint4* mine = reinterpret_cast<uint4*>(stage + lane * kRowBytes);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) mine[i] = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+  __syncwarp();
+  const int c = (lane & 3) * kPer;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int r = i * 8 + (lane >> 2);
+    const uint4 w = *reinterpret_cast<const uint4*>(stage + r * kRowBytes + (lane & 3) * 16);
+    if (r >= rows) continue;
+    if (vec && c + kPer <= cols) {
+      *reinterpret_cast<uint4*>(out + r * ld + c) = w;
+    } else {
+      E e[kPer];
+      memcpy(e, &w, 16);
+#pragma unroll
+      for (int j = 0; j < kPer; ++j)
+        if (c + j < cols) out[r * ld + c + j] = e[j];
+    }
+  }
+  __syncwarp();
+}
+
+template <class T, int MODE, int ACT>
+__device__ __forceinline__ void epilogue(const Params& q, const Tile& t, uint32_t tmem, char* stage, int warp) {
+  const Product& p = q.p;
+  const int lane = threadIdx.x & 31, quad = warp & 3, half = warp >> 2;
+  const uint32_t base = tmem + (uint32_t(quad * 32) << 16);
+  const int m = t.m0 + quad * 32;                      // the warp's first row in the group
+  const int rows = min(32, t.stored - m);              // (may be <= 0: the loads below stay, they are collective)
+  const int64_t n0 = int64_t(t.n) * q.bn;
+  const int cols = int(min(int64_t(q.bn), p.n - n0));  // columns of this tile inside the matrix
+  const bool zero = MODE == kDw && t.kb == 0;          // a unit without rows: nothing was computed
+  if constexpr (MODE == kUp || MODE == kUpBack) {
+    float w = 0.f, dw = 0.f;
+    const int64_t row = int64_t(t.row0) + m + lane;
+    if (MODE == kUpBack && lane < rows && m + lane < t.rows) w = p.weights[q.plan.pair_of_row[row]];
+    for (int c = half * 32; c < q.bn; c += 64) {
+      uint32_t h[16], d1[16], d2[16];
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        float g[16], u[16], d[16];
+        const int cc = min(c + 16 * s, q.bn - 16);  // (bn is a multiple of 16: an odd half is loaded twice, not stored)
+        tmem_ld16(base + cc, g);
+        tmem_ld16(base + q.bn + cc, u);
+        if constexpr (MODE == kUpBack) tmem_ld16(base + 256 + cc, d);
+        tmem_wait_ld();
+        const bool in = c + 16 * s < q.bn;
+#pragma unroll
+        for (int i = 0; i < 16; i += 2) {
+          float k0 = act_of<ACT>(g[i]), k1 = act_of<ACT>(g[i + 1]);
+          if constexpr (MODE == kUp) {
+            h[s * 8 + i / 2] = pack<T>(k0 * u[i], k1 * u[i + 1]);
+          } else {
+            h[s * 8 + i / 2] = pack<T>(w * k0 * u[i], w * k1 * u[i + 1]);
+            d1[s * 8 + i / 2] = pack<T>(w * d[i] * u[i] * slope_of<ACT>(g[i]), w * d[i + 1] * u[i + 1] * slope_of<ACT>(g[i + 1]));
+            d2[s * 8 + i / 2] = pack<T>(w * d[i] * k0, w * d[i + 1] * k1);
+            if (in && c + 16 * s + i < cols) dw += d[i] * k0 * u[i];
+            if (in && c + 16 * s + i + 1 < cols) dw += d[i + 1] * k1 * u[i + 1];
+          }
+        }
+      }
+      const int64_t at = (int64_t(t.row0) + m) * p.ldo + n0 + c;
+      if constexpr (MODE == kUp) {
+        store_rows<T>(stage, h, static_cast<T*>(p.out) + at, p.ldo, rows, cols - c, q.vec);
+      } else {
+        store_rows<T>(stage, d1, static_cast<T*>(p.dg) + at, p.ldo, rows, cols - c, q.vec);
+        store_rows<T>(stage, d2, static_cast<T*>(p.du) + at, p.ldo, rows, cols - c, q.vec);
+        if (p.hw) store_rows<T>(stage, h, static_cast<T*>(p.hw) + at, p.ldo, rows, cols - c, q.vec);
+      }
+    }
+    if (MODE == kUpBack && p.dwp && lane < rows && m + lane < t.rows) p.dwp[row * p.ld_dwp + 2 * t.n + half] = dw;
+  } else if constexpr (MODE == kDown || MODE == kDx) {
+    for (int c = half * 16; c < q.bn; c += 32) {
+      float v[16];
+      tmem_ld16(base + c, v);
+      tmem_wait_ld();
+      uint32_t b[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) b[i] = __float_as_uint(v[i]);
+      store_rows<float>(stage, b, p.rows32 + (int64_t(t.row0) + m) * p.n + n0 + c, p.n, min(rows, t.rows - m), cols - c,
+                        true);
+    }
+  } else if constexpr (MODE == kLin) {
+    // the sums go through the transpose in 32 bits; bias, residual and both outputs are read and written along rows
+    for (int c = half * 16; c < q.bn; c += 32) {
+      float v[16];
+      tmem_ld16(base + c, v);
+      tmem_wait_ld();
+      float4* mine = reinterpret_cast<float4*>(stage + lane * kRowBytes);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) mine[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+      __syncwarp();
+      const int cc = c + (lane & 3) * 4;
+      const int64_t n = n0 + cc;
+      T bias[4] = {}, res[4] = {};
+      const bool whole = q.vec && cc + 4 <= cols;
+      if (p.bias)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (cc + j < cols) bias[j] = static_cast<const T*>(p.bias)[n + j];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int r = i * 8 + (lane >> 2);
+        const float4 f = *reinterpret_cast<const float4*>(stage + r * kRowBytes + (lane & 3) * 16);
+        if (r >= rows) continue;
+        const int64_t mm = m + r;
+        float z[4] = {f.x, f.y, f.z, f.w};
+        if (p.residual) {
+          const T* src = static_cast<const T*>(p.residual) + mm * p.ldr + n;
+          if (whole) {
+            *reinterpret_cast<uint2*>(res) = *reinterpret_cast<const uint2*>(src);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              if (cc + j < cols) res[j] = src[j];
+          }
+        }
+        T y[4], pre[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          z[j] += to_f(bias[j]);
+          pre[j] = from_f<T>(z[j]);
+          y[j] = from_f<T>(act_of<ACT>(z[j]) + to_f(res[j]));
+        }
+        T* out = static_cast<T*>(p.out) + mm * p.ldo + n;
+        T* keep = static_cast<T*>(p.pre) + mm * p.ldp + n;
+        if (whole) {
+          *reinterpret_cast<uint2*>(out) = *reinterpret_cast<uint2*>(y);
+          if (p.pre) *reinterpret_cast<uint2*>(keep) = *reinterpret_cast<uint2*>(pre);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (cc + j < cols) {
+              out[j] = y[j];
+              if (p.pre) keep[j] = pre[j];
+            }
+        }
+      }
+      __syncwarp();
+    }
+  } else {  // gradients: rounded once
+    T* out = static_cast<T*>(p.out) + int64_t(t.unit) * p.out_unit + m * p.ldo + n0;
+    for (int c = half * 32; c < q.bn; c += 64) {
+      uint32_t h[16] = {};
+      if (!zero) {
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          float v[16];
+          tmem_ld16(base + min(c + 16 * s, q.bn - 16), v);
+          tmem_wait_ld();
+#pragma unroll
+          for (int i = 0; i < 16; i += 2) h[s * 8 + i / 2] = pack<T>(v[i], v[i + 1]);
+        }
+      }
+      store_rows<T>(stage, h, out + c, p.ldo, rows, min(cols, q.bn) - c, q.vec);
+    }
+  }
+}
+
+template <class T, int MODE, int ACT>
+__global__ __launch_bounds__(kThreads, 1) void tc_kernel(const __grid_constant__ Maps maps,
+                                                         const __grid_constant__ Params q) {
+  using X = Traits<MODE>;
+  extern __shared__ char raw[];
+  char* smem = raw + ((1024 - (smem_u32(raw) & 1023)) & 1023);
+  char* store = smem + kStages * kStageBytes;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(store + kEpiWarps * kStoreBytes);
+  const uint32_t full = smem_u32(bars), empty = full + 8 * kStages, sums_full = empty + 8 * kStages,
+                 sums_empty = sums_full + 16;
+  uint32_t* words = reinterpret_cast<uint32_t*>(bars + 2 * kStages + 4);  // [0] TMEM address, [1] a wait ran out
+  volatile uint32_t* dead = words + 1;
+  const int warp = threadIdx.x >> 5;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kStages; ++s) {
+      bar_init(full + 8 * s, 1);
+      bar_init(empty + 8 * s, 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      bar_init(sums_full + 8 * b, 1);
+      bar_init(sums_empty + 8 * b, kEpiWarps);
+    }
+    words[1] = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(words)) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  fence_before();
+  __syncthreads();
+  fence_after();
+  const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(words);
+  const int chunks = (q.bn + 63) / 64;  // MN-major B
+
+  if (threadIdx.x == 0) {  // the loads
+    uint32_t it = 0;
+    bool ok = true;
+    Tile t;
+    for (int L = blockIdx.x; ok && tile_at<MODE>(q, L, t); L += gridDim.x) {
+#pragma unroll
+      for (int s = 0; s < X::segs; ++s) {
+        const bool pair = X::pair0 && s == 0;
+        const uint32_t b_bytes = X::b_mn(s) ? chunks * 8192 : (pair ? 2 : 1) * q.bn * 128;
+        for (int kb = 0; ok && kb < t.kb; ++kb, ++it) {
+          const int st = it % kStages;
+          ok = bar_wait(empty + 8 * st, ((it / kStages) & 1) ^ 1, dead);
+          if (!ok) break;
+          const uint32_t bar = full + 8 * st, sa = smem_u32(smem + st * kStageBytes), sb = sa + kABytes;
+          bar_expect(bar, kABytes + b_bytes);
+          const CUtensorMap* ma = &maps.a[s];
+          const int k0 = kb * kBK, krow = (MODE == kDw ? t.row0 : 0) + k0;
+          if constexpr (X::a_mn) {
+            tma_load(sa, ma, t.m0, krow, 0, bar);
+            tma_load(sa + 8192, ma, t.m0 + 64, krow, 0, bar);
+          } else {
+            tma_load(sa, ma, k0, t.row0 + t.m0, 0, bar);
+          }
+          const int n0 = t.n * q.bn, z = X::grouped ? t.slot : 0;
+          const CUtensorMap* mb = &maps.b[MODE == kUpBack && s == 1 ? 2 : s];
+          if (X::b_mn(s)) {
+            for (int c = 0; c < chunks; ++c) tma_load(sb + c * 8192, mb, n0 + 64 * c, krow, z, bar);
+          } else {
+            tma_load(sb, mb, k0, n0, z, bar);
+            if (pair) tma_load(sb + q.bn * 128, &maps.b[1], k0, n0, z, bar);
+          }
+        }
+      }
+    }
+    if (!ok)  // leave no copy in flight behind
+      for (uint32_t j = it > kStages ? it - kStages : 0; j < it; ++j) {
+        volatile uint32_t none = 0;
+        (void)bar_wait_slow(full + 8 * (j % kStages), (j / kStages) & 1, &none);
+      }
+  } else if (threadIdx.x == 32) {  // the products
+    uint32_t it = 0, nt = 0;
+    bool ok = true;
+    Tile t;
+    constexpr uint32_t type = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+    for (int L = blockIdx.x; ok && tile_at<MODE>(q, L, t); L += gridDim.x, ++nt) {
+      const int buf = nt % X::bufs;
+      ok = bar_wait(sums_empty + 8 * buf, ((nt / X::bufs) & 1) ^ 1, dead);
+      if (!ok) break;
+      fence_after();
+#pragma unroll
+      for (int s = 0; s < X::segs; ++s) {
+        const int n = X::pair0 && s == 0 ? 2 * q.bn : q.bn;
+        const uint32_t idesc = (1u << 4) | (type << 7) | (type << 10) | (uint32_t(X::a_mn) << 15) |
+                               (uint32_t(X::b_mn(s)) << 16) | (uint32_t(n >> 3) << 17) | (uint32_t(kBM >> 4) << 24);
+        const uint32_t d = tmem + buf * 256 + (MODE == kUpBack && s == 1 ? 256 : 0);
+        const bool fresh = !(MODE == kDx && s == 1);  // dx: both segments add into the same sums
+        for (int kb = 0; kb < t.kb; ++kb, ++it) {
+          const int st = it % kStages;
+          ok = bar_wait(full + 8 * st, (it / kStages) & 1, dead);
+          if (!ok) break;
+          fence_after();
+          const uint32_t sa = smem_u32(smem + st * kStageBytes), sb = sa + kABytes;
+          const uint64_t da = desc(sa, X::a_mn), db = desc(sb, X::b_mn(s));
+#pragma unroll
+          for (int k = 0; k < kBK / 16; ++k)
+            mma(d, da + uint64_t((X::a_mn ? 2048 : 32) * k >> 4), db + uint64_t((X::b_mn(s) ? 2048 : 32) * k >> 4), idesc,
+                !(fresh && kb == 0 && k == 0));
+          commit(empty + 8 * st);
+        }
+        if (!ok) break;
+      }
+      if (ok) commit(sums_full + 8 * buf);
+    }
+    if (!ok && it) {  // the products already issued read shared memory and TMEM: let them end
+      volatile uint32_t none = 0;
+      (void)bar_wait_slow(empty + 8 * ((it - 1) % kStages), ((it - 1) / kStages) & 1, &none);
+    }
+  } else if (warp >= 4) {  // the epilogue
+    uint32_t nt = 0;
+    Tile t;
+    for (int L = blockIdx.x; tile_at<MODE>(q, L, t); L += gridDim.x, ++nt) {
+      const int buf = nt % X::bufs;
+      if (!bar_wait(sums_full + 8 * buf, (nt / X::bufs) & 1, dead)) break;
+      __syncwarp();
+      fence_after();
+      epilogue<T, MODE, ACT>(q, t, tmem + buf * 256, store + (warp - 4) * kStoreBytes, warp - 4);
+      fence_before();
+      __syncwarp();
+      if ((threadIdx.x & 31) == 0) bar_arrive(sums_empty + 8 * buf);
+    }
+  }
+  fence_before();
+  __syncthreads();
+  fence_after();
+  if (warp == 1) {
+    __syncwarp();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+    if ((threadIdx.x & 31) == 0 && *dead) atomicAdd(&g_ops_timeouts, 1u);
+  }
+}
+
+// rows of grouped buffers: row r is source row pair_of_row[r] / top, padding rows are zeros
+__global__ __launch_bounds__(256) void gather_kernel(const __grid_constant__ Plan plan, uint32_t top, const uint4* src,
+                                                     uint64_t ld16, uint32_t n16, uint4* dst) {
+  const uint32_t r = blockIdx.x;
+  if (int32_t(r) >= plan.head[1]) return;
+  const int32_t pair = plan.pair_of_row[r];
+  const uint4* s = src + uint64_t(pair < 0 ? 0 : uint32_t(pair) / top) * ld16;
+  for (uint32_t c = threadIdx.x; c < n16; c += 256)
+    dst[uint64_t(r) * n16 + c] = pair < 0 ? make_uint4(0, 0, 0, 0) : s[c];
+}
+
+using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                            const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                            CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+Encode encoder() {
+  static const Encode e = [] {
+    void* fn = nullptr;
+    cudaDriverEntryPointQueryResult r{};
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &r) != cudaSuccess ||
+        r != cudaDriverEntryPointSuccess)
+      fn = nullptr;
+    return reinterpret_cast<Encode>(fn);
+  }();
+  return e;
+}
+
+// [slots][rows][cols] of 16-bit elements, boxes of 64 columns (128 swizzled bytes) x box_rows
+bool make_map(CUtensorMap* m, int dtype, const void* p, uint64_t cols, uint64_t rows, uint64_t ld, uint64_t slots,
+              uint64_t slot_bytes, uint32_t box_rows) {
+  const cuuint64_t dims[3] = {cols, rows, slots}, strides[2] = {ld * 2, slots > 1 ? slot_bytes : ld * 2};
+  const cuuint32_t box[3] = {64, box_rows, 1}, one[3] = {1, 1, 1};
+  return encoder()(m, dtype == TSB_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
+                   const_cast<void*>(p), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <class T, int MODE, int ACT>
+int go(const Maps& maps, const Params& q, int grid, cudaStream_t s) {
+  const auto kernel = tc_kernel<T, MODE, ACT>;
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
+  if (e != cudaSuccess) return int(e);
+  kernel<<<grid, kThreads, kSmemBytes, s>>>(maps, q);
+  return int(cudaGetLastError());
+}
+template <class T, int MODE>
+int go_act(int act, const Maps& maps, const Params& q, int grid, cudaStream_t s) {
+  switch (act) {
+    case TSB_ACT_SILU: return go<T, MODE, TSB_ACT_SILU>(maps, q, grid, s);
+    case TSB_ACT_GELU: return go<T, MODE, TSB_ACT_GELU>(maps, q, grid, s);
+    case TSB_ACT_GELU_TANH: return go<T, MODE, TSB_ACT_GELU_TANH>(maps, q, grid, s);
+    case TSB_ACT_RELU: return go<T, MODE, TSB_ACT_RELU>(maps, q, grid, s);
+  }
+  return go<T, MODE, TSB_ACT_NONE>(maps, q, grid, s);
+}
+template <int MODE>
+int go_type(int dtype, int act, const Maps& maps, const Params& q, int grid, cudaStream_t s) {
+  if constexpr (MODE == kLin || MODE == kUp || MODE == kUpBack)
+    return dtype == TSB_BF16 ? go_act<__nv_bfloat16, MODE>(act, maps, q, grid, s)
+                             : go_act<__half, MODE>(act, maps, q, grid, s);
+  else
+    return dtype == TSB_BF16 ? go<__nv_bfloat16, MODE, 0>(maps, q, grid, s) : go<__half, MODE, 0>(maps, q, grid, s);
+}
+
+bool on16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+int sm_count() {
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+    return 0;
+  return n;
+}
+
+// Columns a tile: of the multiples of 16 up to `most`, the one whose last wave of tiles wastes least. A tile costs its
+// columns plus about 32 (the narrower tile re-reads A for fewer products); 2047 x 7168 at 148 SMs takes 208 (4 waves of
+// 560 tiles) over 256 (4 waves of 448).
+int columns(int64_t m_tiles, int64_t n, int sms, int most) {
+  int best = 16;
+  int64_t cost = INT64_MAX;
+  for (int bn = most; bn >= 16; bn -= 16) {
+    const int64_t waves = ceil_div(uint64_t(m_tiles) * ceil_div(uint64_t(n), uint64_t(bn)), uint64_t(sms));
+    const int64_t c = waves * (bn + 32);
+    if (c < cost) cost = c, best = bn;
+  }
+  return best;
+}
+
+struct Shape {  // one operand as memory: [slots][rows][cols] with cols contiguous
+  const void* p;
+  uint64_t cols, rows, ld, slots, slot_bytes;
+};
+bool fits(const Shape& s) {
+  return on16(s.p) && s.ld % 8 == 0 && s.slot_bytes % 16 == 0 && s.slot_bytes < (uint64_t(1) << 40) && s.cols >= 1;
+}
+
+}  // namespace
+
+bool tc_fits(const Operand& o, const Units* u) {
+  // one of the two strides is 1, the other a multiple of 8 elements; a unit's matrices in slots (not by address)
+  if (o.part >= 0)
+    return !u->table && on16(u->part[o.part]) && u->stride[o.part] % 16 == 0 &&
+           u->stride[o.part] < (uint64_t(1) << 40) && (o.s_i == 1 ? o.s_k : o.s_i) % 8 == 0;
+  return on16(o.p) && (o.s_i == 1 || o.s_k == 1) && (o.s_k == 1 ? o.s_i : o.s_k) % 8 == 0 && (o.s_i != 1 || o.s_k != 1);
+}
+
+int launch_gather(const Plan& plan, uint32_t top, const void* src, uint64_t ld, uint64_t n, void* dst, cudaStream_t s) {
+  gather_kernel<<<plan.max_rows, 256, 0, s>>>(plan, top, static_cast<const uint4*>(src), ld / 8, uint32_t(n / 8),
+                                              static_cast<uint4*>(dst));
+  return int(cudaGetLastError());
+}
+
+int launch_tc(int dtype, const Product& p, const Plan* plan, const Units* u, cudaStream_t s) {
+  if (!encoder()) return int(cudaErrorNotSupported);
+  const int sms = sm_count();
+  if (!sms) return int(cudaErrorInvalidDevice);
+  Params q{};
+  q.p = p;
+  if (plan) q.plan = *plan;
+  const bool a_mn = p.a[0].s_k != 1;
+  Mode mode;
+  if (p.epi == kEpiLinear) mode = kLin;
+  else if (p.epi == kEpiUp) mode = kUp;
+  else if (p.epi == kEpiUpBack) mode = kUpBack;
+  else if (p.epi == kEpiRows32) mode = p.segs == 2 ? kDx : kDown;
+  else mode = p.per_unit ? kDw : (a_mn ? kLinDw : kLinDx);
+  q.k_blocks = int(ceil_div(uint64_t(p.k), kBK));
+  q.m_tiles = p.grouped ? 0 : int(ceil_div(uint64_t(p.m), kBM));
+  const int64_t m_tiles = p.grouped ? plan->max_tiles : p.per_unit ? int64_t(q.m_tiles) * plan->units : q.m_tiles;
+  const bool narrow = mode == kUp || mode == kUpBack;
+  q.bn = p.grouped || p.per_unit ? (narrow ? 128 : 256) : columns(m_tiles, p.n, sms, 256);
+  if (q.bn > (p.n + 15) / 16 * 16) q.bn = int((p.n + 15) / 16 * 16);
+  q.n_tiles = int(ceil_div(uint64_t(p.n), uint64_t(q.bn)));
+  q.vec = p.epi == kEpiRows32 ||
+          (p.epi == kEpiUpBack ? on16(p.dg) && on16(p.du) && on16(p.hw) && p.ldo % 8 == 0
+                               : on16(p.out) && p.ldo % 8 == 0 && p.out_unit % 8 == 0 &&
+                                     (!p.residual || (on16(p.residual) && p.ldr % 4 == 0)) &&
+                                     (!p.pre || (on16(p.pre) && p.ldp % 4 == 0)));
+  Maps maps;
+  std::memset(&maps, 0, sizeof maps);
+  auto shape = [&](const Operand& o, int64_t n_i, int64_t n_k) {
+    Shape r{};
+    const bool k_inner = o.s_k == 1;
+    r.cols = uint64_t(k_inner ? n_k : n_i);
+    r.rows = uint64_t(k_inner ? n_i : n_k);
+    r.ld = uint64_t(k_inner ? o.s_i : o.s_k);
+    r.slots = 1;
+    r.p = o.p;
+    if (o.part >= 0) {
+      r.p = u->part[o.part];
+      r.slots = u->n_slots;
+      r.slot_bytes = u->stride[o.part];
+    }
+    return r;
+  };
+  for (int i = 0; i < p.segs; ++i) {
+    // A's maps: one per k loop (gate and up share theirs)
+    const int64_t rows = p.grouped ? plan->max_rows : p.m, ks = p.per_unit ? plan->max_rows : p.k;
+    const Shape a = shape(p.a[i], rows, ks), b = shape(p.b[i], p.n, ks);
+    if (!fits(a) || !fits(b)) return int(cudaErrorInvalidValue);
+    const int ia = narrow ? (i == 2 ? 1 : 0) : i;
+    if (!make_map(&maps.a[ia], dtype, a.p, a.cols, a.rows, a.ld, a.slots, a.slot_bytes, a_mn ? 64 : kBM) ||
+        !make_map(&maps.b[i], dtype, b.p, b.cols, b.rows, b.ld, b.slots, b.slot_bytes,
+                  p.b[i].s_k == 1 ? uint32_t(q.bn) : 64))
+      return int(cudaErrorInvalidValue);
+  }
+  const int64_t tiles = m_tiles * q.n_tiles;
+  if (tiles >= (int64_t(1) << 30)) return int(cudaErrorInvalidValue);
+  const int grid = int(tiles < sms ? tiles : sms);
+  switch (mode) {
+    case kLin: return go_type<kLin>(dtype, p.act, maps, q, grid, s);
+    case kLinDx: return go_type<kLinDx>(dtype, 0, maps, q, grid, s);
+    case kLinDw: return go_type<kLinDw>(dtype, 0, maps, q, grid, s);
+    case kUp: return go_type<kUp>(dtype, p.act, maps, q, grid, s);
+    case kUpBack: return go_type<kUpBack>(dtype, p.act, maps, q, grid, s);
+    case kDown: return go_type<kDown>(dtype, 0, maps, q, grid, s);
+    case kDx: return go_type<kDx>(dtype, 0, maps, q, grid, s);
+    case kDw: return go_type<kDw>(dtype, 0, maps, q, grid, s);
+  }
+  return int(cudaErrorInvalidValue);
+}
+
+int ops_take_timeouts(uint32_t* out) {
+  uint32_t v = 0;
+  cudaError_t e = cudaMemcpyFromSymbol(&v, g_ops_timeouts, sizeof v);
+  if (e == cudaSuccess && v) {
+    const uint32_t zero = 0;
+    e = cudaMemcpyToSymbol(g_ops_timeouts, &zero, sizeof zero);
+  }
+  *out = v;
+  return int(e);
+}
+
+}  // namespace ops
+}  // namespace tsb
