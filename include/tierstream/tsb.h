@@ -442,8 +442,8 @@ SS_API ss_status tsb_route_backward(uint32_t dtype, uint32_t dw_dtype, const voi
 /* Where a layer's units live. Matrix p of unit u (0 gate [ffn][hidden], 1 up [ffn][hidden], 2 down [hidden][ffn]) is at
  * part[p] + slot x stride[p] bytes, slot = slot_of[*unit_base + u] (device memory, read when the kernels run; slot_of
  * NULL: slot = u; unit_base NULL: 0), or, with `table` (device array of n_units addresses, a host-mode
- * ss_layer_view.table_dev), at table[u] + stride[p] bytes. A slot outside [0, n_slots) or a zero address is a unit that
- * is not there: its rows contribute nothing and *absent_err (may be NULL) is set to 1; while *abort (may be NULL) is
+ * ss_layer_view.table_dev), at table[u] + stride[p] bytes. A slot outside [0, n_slots), a zero address or one that is
+ * not a multiple of 16 is a unit that is not there: its rows contribute nothing and *absent_err (may be NULL) is set to 1; while *abort (may be NULL) is
  * non-zero no unit is there. */
 typedef struct tsb_units {
   uint32_t struct_size, n_units, n_slots, reserved0;

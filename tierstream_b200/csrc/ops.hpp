@@ -39,6 +39,7 @@ struct Plan {
   int32_t* row_of_pair;
   int32_t* tile_unit;  // tiles of `bm` rows, group by group
   int32_t* tile_m0;    // the tile's first row inside its group
+  int4* tile_info;     // per tile up to max_tiles: slot, first grouped row, rows (0: no such tile), unit
   uint32_t units, pairs, max_rows, max_tiles, pad, bm;
 };
 
@@ -180,6 +181,11 @@ int launch_dz(int dtype, int act, const void* dy, uint64_t ldy, const void* pre,
 constexpr uint32_t kTileM = 64, kTileN = 64;
 int launch_tile(int dtype, const Product& p, const Plan* plan, const Units* units, cudaStream_t s);
 
+
+// ops_stream.cu: products of few rows, tiles of 8, 16 or 32 rows (the plan's bm). Rows of x and w start on 16 bytes and k
+// is a multiple of 8; gathered rows are read where they are (top: the pairs a row has).
+int launch_stream(int dtype, const Product& p, uint32_t rows_a_tile, uint32_t top, const Plan* plan, const Units* units,
+                  cudaStream_t s);
 
 // ops_tc.cu: products of many rows on tcgen05 (the plan made with bm = kTcRows). tc_fits: TMA can read the operand.
 // Gathered operands are gathered first: launch_gather copies n columns of every grouped row (n a multiple of 8).

@@ -59,9 +59,17 @@ Operand gathered(const void* p, int64_t s_i, int64_t s_k, const Plan& plan, uint
 }
 Operand of_unit(int part, int64_t s_i, int64_t s_k) { return {nullptr, s_i, s_k, nullptr, 1, 0, part}; }
 
+// Rows up to which the kernel that streams the weights beats the tensor cores' own path (whose 128-row tiles are then
+// mostly empty), and the tile's rows for it.
+constexpr uint64_t kStreamRows = 32;
+uint32_t stream_tile(uint64_t rows) { return rows <= 8 ? 8 : rows <= 16 ? 16 : 32; }
+
 // One matrix product: on the tensor cores' own path when TMA can read both operands (rows on 16 bytes), else by the
 // kernel for every alignment.
 int product(int dtype, const Product& p, cudaStream_t s) {
+  if (p.epi == kEpiLinear && uint64_t(p.m) <= kStreamRows && p.k % 8 == 0 && tc_fits(p.a[0], nullptr) &&
+      tc_fits(p.b[0], nullptr))
+    return launch_stream(dtype, p, stream_tile(uint64_t(p.m)), 1, nullptr, nullptr, s);
   if (tc_fits(p.a[0], nullptr) && tc_fits(p.b[0], nullptr)) return launch_tc(dtype, p, nullptr, nullptr, s);
   return launch_tile(dtype, p, nullptr, nullptr, s);
 }
@@ -207,19 +215,20 @@ void check_ffn_shape(const A* a, const char* fn) {
        "the parts' strides must be whole elements");
 }
 
-// Whether the block's products run on the tensor cores' own path: whole 16 bytes in every row, the units in slots.
-bool ffn_tc(const tsb_units* u, uint64_t hidden, uint64_t ffn, const void* x, uint64_t ldx, const void* dy,
+// Whether every row of the block's matrices starts on 16 bytes (a unit found by address: its slots are 256-byte aligned,
+// so its matrices' offsets decide).
+bool ffn_rows16(const tsb_units* u, uint64_t hidden, uint64_t ffn, const void* x, uint64_t ldx, const void* dy,
             uint64_t lddy) {
   auto on16 = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; };
-  if (u->table || hidden % 8 || ffn % 8 || !on16(x) || ldx % 8 || !on16(dy) || lddy % 8) return false;
+  if (hidden % 8 || ffn % 8 || !on16(x) || ldx % 8 || !on16(dy) || lddy % 8) return false;
   for (int i = 0; i < 3; ++i)
-    if (!on16(u->part[i]) || u->stride[i] % 16 || u->stride[i] >= (uint64_t(1) << 40)) return false;
+    if ((!u->table && !on16(u->part[i])) || u->stride[i] % 16 || u->stride[i] >= (uint64_t(1) << 40)) return false;
   return true;
 }
 
 struct FfnSpace {
   Plan plan;
-  bool tc;
+  bool tc, stream;
   void* xs;
   void* h;
   float* rows32;
@@ -229,8 +238,12 @@ FfnSpace ffn_space(const tsb_ffn_args* a) {
   Arena w{static_cast<char*>(a->workspace)};
   FfnSpace r{};
   const uint64_t pairs = a->rows * a->top;
-  r.tc = ffn_tc(a->units, a->hidden, a->ffn, a->x, a->ldx, nullptr, 0);
-  const uint32_t bm = r.tc ? kTcRows : kTileM;
+  // few rows for each unit that may be met: the weights are streamed (units by address too)
+  const uint64_t each = ceil_div(pairs, pairs < a->units->n_units ? pairs : a->units->n_units);
+  r.stream = each <= kStreamRows && pairs / 8 + a->units->n_units <= 65535 &&  // (a grid's y)
+             ffn_rows16(a->units, a->hidden, a->ffn, a->x, a->ldx, nullptr, 0);
+  r.tc = !r.stream && !a->units->table && ffn_rows16(a->units, a->hidden, a->ffn, a->x, a->ldx, nullptr, 0);
+  const uint32_t bm = r.stream ? stream_tile(each) : r.tc ? kTcRows : kTileM;
   r.plan = plan_at(w.take(plan_bytes(a->units->n_units, pairs, 1, bm)), a->units->n_units, pairs, 1, bm);
   if (r.tc) r.xs = w.take(uint64_t(r.plan.max_rows) * a->hidden * 2);
   r.h = w.take(uint64_t(r.plan.max_rows) * a->ffn * 2);
@@ -269,7 +282,11 @@ void ffn(const tsb_ffn_args* a) {
   p.epi = kEpiUp;
   p.act = int(a->act);
   p.out = w.h, p.ldo = f;
-  const auto go = w.tc ? launch_tc : launch_tile;
+  const auto go = [&](int dtype, const Product& pr, const Plan* pl, const Units* un, cudaStream_t st) {
+    return w.stream ? launch_stream(dtype, pr, pl->bm, a->top, pl, un, st)
+           : w.tc   ? launch_tc(dtype, pr, pl, un, st)
+                    : launch_tile(dtype, pr, pl, un, st);
+  };
   if (w.tc) {
     ck(launch_gather(w.plan, a->top, a->x, a->ldx, a->hidden, w.xs, s), fn, "gather");
     p.a[0] = p.a[1] = dense(w.xs, d, 1);
@@ -301,7 +318,7 @@ FfnBackSpace ffn_back_space(const tsb_ffn_grad_args* a) {
   Arena w{static_cast<char*>(a->workspace)};
   FfnBackSpace r{};
   const uint64_t pairs = a->rows * a->top;
-  r.tc = ffn_tc(a->units, a->hidden, a->ffn, a->x, a->ldx, a->dy, a->lddy);
+  r.tc = !a->units->table && ffn_rows16(a->units, a->hidden, a->ffn, a->x, a->ldx, a->dy, a->lddy);
   // (sums over a group's rows run in slices of 64 on the tensor cores: zero rows fill the last one)
   const uint32_t bm = r.tc ? kTcRows : kTileM, pad = r.tc && a->dgate ? 64 : 1;
   r.plan = plan_at(w.take(plan_bytes(a->units->n_units, pairs, pad, bm)), a->units->n_units, pairs, pad, bm);

@@ -20,7 +20,7 @@ constexpr int kPlanThreads = 256;
 
 __device__ __forceinline__ int32_t resolve(const Units& u, int32_t e) {
   if (u.abort && *reinterpret_cast<const volatile uint32_t*>(u.abort)) return -1;
-  if (u.table) return u.table[e] ? e : -1;
+  if (u.table) return u.table[e] && u.table[e] % 16 == 0 ? e : -1;
   if (!u.slot_of) return uint32_t(e) < u.n_slots ? e : -1;
   const int32_t s = reinterpret_cast<const volatile int32_t*>(u.slot_of)[(u.unit_base ? *u.unit_base : 0u) + uint32_t(e)];
   return uint32_t(s) < u.n_slots ? s : -1;
@@ -76,7 +76,11 @@ __global__ __launch_bounds__(kPlanThreads) void plan_fill_kernel(const __grid_co
   for (int i = threadIdx.x; i < mine; i += kPlanThreads) {
     p.tile_unit[tiles + i] = int32_t(e);
     p.tile_m0[tiles + i] = i * int(p.bm);
+    p.tile_info[tiles + i] = make_int4(p.slot[e], rows + i * int(p.bm), min(int(p.bm), cnt - i * int(p.bm)), int32_t(e));
   }
+  if (e + 1 == p.units)
+    for (uint32_t i = tiles + mine + threadIdx.x; i < p.max_tiles; i += kPlanThreads)
+      p.tile_info[i] = make_int4(0, 0, 0, 0);
   for (int i = cnt + threadIdx.x; i < padded; i += kPlanThreads) p.pair_of_row[rows + i] = -1;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int done = 0;  // pairs of this unit before the current span of ids
@@ -119,6 +123,7 @@ __global__ __launch_bounds__(kSmallThreads) void plan_small_kernel(const __grid_
   __syncthreads();
   const int32_t mine = t < p.pairs ? id[t] : -1;
   const bool valid = uint32_t(mine) < p.units;
+  int32_t my_slot = 0;
   if (valid) atomicAdd(&cnt[mine], 1);  // (counts only: their value does not depend on the order)
   __syncthreads();
   if (t < p.units && cnt[t]) {
@@ -127,7 +132,7 @@ __global__ __launch_bounds__(kSmallThreads) void plan_small_kernel(const __grid_
       if (u.absent) atomicOr(u.absent, 1u);
       cnt[t] = 0;
     } else {
-      p.slot[t] = slot;
+      my_slot = slot;
     }
   }
   __syncthreads();
@@ -147,14 +152,19 @@ __global__ __launch_bounds__(kSmallThreads) void plan_small_kernel(const __grid_
   if (t < p.units) {
     p.cnt[t] = c;
     p.off[t] = rows[t];
-    if (!c) p.slot[t] = 0;
+    p.slot[t] = my_slot;
     if (t + 1 == p.units) p.head[0] = k, p.head[1] = r;
     for (int i = 0; i < nt; ++i) {
       p.tile_unit[tiles[t] + i] = int32_t(t);
       p.tile_m0[tiles[t] + i] = i * int(p.bm);
+      p.tile_info[tiles[t] + i] =
+          make_int4(my_slot, rows[t] + i * int(p.bm), min(int(p.bm), c - i * int(p.bm)), int32_t(t));
     }
     for (int i = c; i < padded; ++i) p.pair_of_row[rows[t] + i] = -1;
   }
+  int all = 0;
+  for (int w = 0; w < 32; ++w) all += wt[w];
+  for (uint32_t i = uint32_t(all) + t; i < p.max_tiles; i += kSmallThreads) p.tile_info[i] = make_int4(0, 0, 0, 0);
   if (t < p.pairs) {
     int32_t row = -1;
     if (valid && cnt[mine]) {
@@ -440,12 +450,13 @@ Plan plan_at(void* ws, uint32_t units, uint64_t pairs, uint32_t pad, uint32_t bm
   p.row_of_pair = take(pairs);
   p.tile_unit = take(p.max_tiles);
   p.tile_m0 = take(p.max_tiles);
+  p.tile_info = reinterpret_cast<int4*>(take(uint64_t(p.max_tiles) * 4));
   return p;
 }
 uint64_t plan_bytes(uint32_t units, uint64_t pairs, uint32_t pad, uint32_t bm) {
   const uint64_t met = pairs < units ? pairs : units;
   return aligned(8) + 3 * aligned(uint64_t(units) * 4) + aligned((pairs + met * (pad - 1)) * 4) + aligned(pairs * 4) +
-         2 * aligned((pairs / bm + met) * 4);
+         2 * aligned((pairs / bm + met) * 4) + aligned((pairs / bm + met) * 16);
 }
 
 int launch_plan(const Plan& p, const Units& u, const int32_t* ids, cudaStream_t s) {
