@@ -187,7 +187,7 @@ int launch_tile(int dtype, const Product& p, const Plan* plan, const Units* unit
 int launch_stream(int dtype, const Product& p, uint32_t rows_a_tile, uint32_t top, const Plan* plan, const Units* units,
                   cudaStream_t s);
 
-// ops_tc.cu: products of many rows on tcgen05 (the plan made with bm = kTcRows). tc_fits: TMA can read the operand.
+// ops_tc.cu: products of many rows on tcgen05 (the plan made with bm = kTcRows, or twice that: pairs of CTAs). tc_fits: TMA can read the operand.
 // Gathered operands are gathered first: launch_gather copies n columns of every grouped row (n a multiple of 8).
 constexpr uint32_t kTcRows = 128;
 bool tc_fits(const Operand& o, const Units* units);

@@ -226,6 +226,9 @@ bool ffn_rows16(const tsb_units* u, uint64_t hidden, uint64_t ffn, const void* x
   return true;
 }
 
+// Rows of a tile on the tensor cores' own path: pairs of CTAs (256 rows) when the units' groups fill them.
+uint32_t tc_tile(uint64_t each) { return each > kTcRows + kTcRows / 4 ? 2 * kTcRows : kTcRows; }
+
 struct FfnSpace {
   Plan plan;
   bool tc, stream;
@@ -243,7 +246,7 @@ FfnSpace ffn_space(const tsb_ffn_args* a) {
   r.stream = each <= kStreamRows && pairs / 8 + a->units->n_units <= 65535 &&  // (a grid's y)
              ffn_rows16(a->units, a->hidden, a->ffn, a->x, a->ldx, nullptr, 0);
   r.tc = !r.stream && !a->units->table && ffn_rows16(a->units, a->hidden, a->ffn, a->x, a->ldx, nullptr, 0);
-  const uint32_t bm = r.stream ? stream_tile(each) : r.tc ? kTcRows : kTileM;
+  const uint32_t bm = r.stream ? stream_tile(each) : r.tc ? tc_tile(each) : kTileM;
   r.plan = plan_at(w.take(plan_bytes(a->units->n_units, pairs, 1, bm)), a->units->n_units, pairs, 1, bm);
   if (r.tc) r.xs = w.take(uint64_t(r.plan.max_rows) * a->hidden * 2);
   r.h = w.take(uint64_t(r.plan.max_rows) * a->ffn * 2);
@@ -320,7 +323,8 @@ FfnBackSpace ffn_back_space(const tsb_ffn_grad_args* a) {
   const uint64_t pairs = a->rows * a->top;
   r.tc = !a->units->table && ffn_rows16(a->units, a->hidden, a->ffn, a->x, a->ldx, a->dy, a->lddy);
   // (sums over a group's rows run in slices of 64 on the tensor cores: zero rows fill the last one)
-  const uint32_t bm = r.tc ? kTcRows : kTileM, pad = r.tc && a->dgate ? 64 : 1;
+  const uint64_t each = ceil_div(pairs, pairs < a->units->n_units ? pairs : a->units->n_units);
+  const uint32_t bm = r.tc ? tc_tile(each) : kTileM, pad = r.tc && a->dgate ? 64 : 1;
   r.plan = plan_at(w.take(plan_bytes(a->units->n_units, pairs, pad, bm)), a->units->n_units, pairs, pad, bm);
   if (r.tc) {
     r.xs = w.take(uint64_t(r.plan.max_rows) * a->hidden * 2);

@@ -24,11 +24,11 @@ namespace tsb {
 namespace ops {
 namespace {
 
-constexpr int kBM = 128, kBK = 64, kStages = 4;
-constexpr int kABytes = kBM * kBK * 2, kBBytes = 256 * kBK * 2, kStageBytes = kABytes + kBBytes;
+constexpr int kBM = 128, kBK = 64;  // (a CTA's rows)
+constexpr int kABytes = kBM * kBK * 2, kRingBytes = 4 * (kABytes + 256 * kBK * 2);  // 192 KiB of stages
 constexpr int kEpiWarps = 8, kThreads = 128 + 32 * kEpiWarps;
 constexpr int kRowBytes = 80, kStoreBytes = 32 * kRowBytes;  // a warp's 32 rows of 64 bytes, 16 apart: no bank twice
-constexpr int kSmemBytes = 1024 + kStages * kStageBytes + kEpiWarps * kStoreBytes + 256;
+constexpr int kSmemBytes = 1024 + kRingBytes + kEpiWarps * kStoreBytes + 256;
 constexpr unsigned long long kWaitNs = 2000000000ull;
 
 __device__ uint32_t g_ops_timeouts;
@@ -43,6 +43,7 @@ struct Params {
   int32_t m_tiles;   // tiles along m when not grouped
   int32_t k_blocks;  // of a segment; with k_rows per unit: from the group
   int32_t vec;       // 16-byte stores are possible
+  int32_t pair;      // two CTAs to a tile of 256 rows
 };
 struct Maps {
   CUtensorMap a[2], b[3];
@@ -61,7 +62,7 @@ __device__ __forceinline__ void bar_arrive(uint32_t b) {
 __device__ __forceinline__ bool bar_try(uint32_t b, uint32_t parity) {
   uint32_t ok;
   asm volatile(
-      "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+      "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, 20000;\n\tselp.u32 %0, 1, 0, p;\n\t}"
       : "=r"(ok)
       : "r"(b), "r"(parity)
       : "memory");
@@ -72,29 +73,60 @@ __device__ __forceinline__ unsigned long long now_ns() {
   asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
   return t;
 }
-__device__ __noinline__ bool bar_wait_slow(uint32_t b, uint32_t parity, volatile uint32_t* dead) {
-  const unsigned long long t0 = now_ns();
+// false: the wait ran out, here or elsewhere in the CTA. A try sleeps in hardware for up to 20 us; the clock is read
+// between runs of tries.
+__device__ __forceinline__ bool bar_wait(uint32_t b, uint32_t parity, volatile uint32_t* dead) {
+  unsigned long long t0 = 0;
   for (;;) {
-    if (bar_try(b, parity)) return true;
+    for (int i = 0; i < 256; ++i)
+      if (bar_try(b, parity)) return true;
     if (*dead) return false;
-    if (now_ns() - t0 > kWaitNs) {
+    const unsigned long long t = now_ns();
+    if (!t0) t0 = t;
+    if (t - t0 > kWaitNs) {
       *dead = 1;
       return false;
     }
   }
 }
-// false: the wait ran out, here or elsewhere in the CTA
-__device__ __forceinline__ bool bar_wait(uint32_t b, uint32_t parity, volatile uint32_t* dead) {
-  for (int i = 0; i < 8; ++i)
-    if (bar_try(b, parity)) return true;
-  return bar_wait_slow(b, parity, dead);
-}
+// CG = 2: `bar` may be the peer's
+template <int CG>
 __device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
-          dst),
-      "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
-      : "memory");
+  if constexpr (CG == 1)
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
+            dst),
+        "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
+        : "memory");
+  else
+    asm volatile(
+        "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, "
+        "%4}], [%5];" ::"r"(dst),
+        "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
+        : "memory");
+}
+__device__ __forceinline__ uint32_t cta_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ uint32_t in_cta(uint32_t addr, uint32_t rank) {
+  uint32_t a;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(addr), "r"(rank));
+  return a;
+}
+__device__ __forceinline__ void bar_arrive_cluster(uint32_t b) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(b) : "memory");
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+}
+// One lane of a whole warp, always the same. The loading and the issuing warp run their loops as whole warps, so that
+// addresses and descriptors stay in uniform registers (a loop of one thread spent about 500 clocks a k slice).
+__device__ __forceinline__ bool elect() {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+  return r != 0;
 }
 // Shared memory descriptors, 128-byte swizzle. K-major: 8-row groups 1024 bytes apart. MN-major: a stage holds 64-wide
 // chunks of [64 k rows][128 bytes], 8 KiB apart, 8-row groups of k 1024 bytes apart.
@@ -102,15 +134,31 @@ __device__ __forceinline__ uint64_t desc(uint32_t addr, bool mn) {
   return uint64_t((addr & 0x3ffffu) >> 4) | (uint64_t(mn ? 8192 >> 4 : 1) << 16) | (uint64_t(1024 >> 4) << 32) |
          (uint64_t(1) << 46) | (uint64_t(2) << 61);
 }
+template <int CG>
 __device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(uint32_t(add))
-      : "memory");
+  if constexpr (CG == 1)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(uint32_t(add))
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(uint32_t(add))
+        : "memory");
 }
+// the barrier at this offset, in both CTAs of a pair
+template <int CG>
 __device__ __forceinline__ void commit(uint32_t bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+  if constexpr (CG == 1)
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+  else
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
+        "h"(uint16_t(3))
+        : "memory");
 }
 __device__ __forceinline__ void tmem_ld16(uint32_t addr, float (&v)[16]) {
   uint32_t r[16];
@@ -133,9 +181,9 @@ struct Tile {
 
 // Tile L of the launch: groups in unit order, inside a group chunks of up to 16 row tiles, inside a chunk the column
 // tiles, and the chunk's row tiles innermost, so that tiles running at the same time share a unit's columns from L2.
-template <int MODE>
+template <int MODE, int CG>
 __device__ __forceinline__ bool tile_at(const Params& q, int L, Tile& t) {
-  constexpr int kChunk = 16;
+  constexpr int kRows = kBM * CG, kChunk = 16 / CG;
   int local, mt;
   if constexpr (MODE == kUp || MODE == kUpBack || MODE == kDown || MODE == kDx) {
     const int i = L / q.n_tiles;
@@ -145,8 +193,8 @@ __device__ __forceinline__ bool tile_at(const Params& q, int L, Tile& t) {
     t.stored = (t.rows + int(q.plan.pad) - 1) / int(q.plan.pad) * int(q.plan.pad);
     t.row0 = q.plan.off[t.unit];
     t.slot = q.plan.slot[t.unit];
-    mt = (t.rows + kBM - 1) / kBM;
-    local = L - (i - q.plan.tile_m0[i] / kBM) * q.n_tiles;
+    mt = (t.rows + kRows - 1) / kRows;
+    local = L - (i - q.plan.tile_m0[i] / kRows) * q.n_tiles;
     t.kb = q.k_blocks;
   } else if constexpr (MODE == kDw) {
     const int per = q.m_tiles * q.n_tiles;
@@ -169,7 +217,7 @@ __device__ __forceinline__ bool tile_at(const Params& q, int L, Tile& t) {
   const int chunk = local / (kChunk * q.n_tiles), in = local - chunk * kChunk * q.n_tiles;
   const int width = min(kChunk, mt - chunk * kChunk);
   t.n = in / width;
-  t.m0 = (chunk * kChunk + in - t.n * width) * kBM;
+  t.m0 = (chunk * kChunk + in - t.n * width) * kRows;
   return true;
 }
 
@@ -361,19 +409,22 @@ __device__ __forceinline__ void epilogue(const Params& q, const Tile& t, uint32_
   }
 }
 
-template <class T, int MODE, int ACT>
+template <class T, int MODE, int ACT, int CG>
 __global__ __launch_bounds__(kThreads, 1) void tc_kernel(const __grid_constant__ Maps maps,
                                                          const __grid_constant__ Params q) {
   using X = Traits<MODE>;
+  constexpr int kStageBytes = kABytes + 256 / CG * kBK * 2, kStages = kRingBytes / kStageBytes;
   extern __shared__ char raw[];
   char* smem = raw + ((1024 - (smem_u32(raw) & 1023)) & 1023);
-  char* store = smem + kStages * kStageBytes;
+  char* store = smem + kRingBytes;
   uint64_t* bars = reinterpret_cast<uint64_t*>(store + kEpiWarps * kStoreBytes);
   const uint32_t full = smem_u32(bars), empty = full + 8 * kStages, sums_full = empty + 8 * kStages,
                  sums_empty = sums_full + 16;
   uint32_t* words = reinterpret_cast<uint32_t*>(bars + 2 * kStages + 4);  // [0] TMEM address, [1] a wait ran out
   volatile uint32_t* dead = words + 1;
-  const int warp = threadIdx.x >> 5;
+  const int warp = __shfl_sync(0xffffffffu, int(threadIdx.x >> 5), 0);
+  const uint32_t rank = CG == 2 ? cta_rank() : 0;
+  const int first = blockIdx.x / CG, stride = gridDim.x / CG;
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) {
       bar_init(full + 8 * s, 1);
@@ -381,66 +432,83 @@ __global__ __launch_bounds__(kThreads, 1) void tc_kernel(const __grid_constant__
     }
     for (int b = 0; b < 2; ++b) {
       bar_init(sums_full + 8 * b, 1);
-      bar_init(sums_empty + 8 * b, kEpiWarps);
+      bar_init(sums_empty + 8 * b, CG * kEpiWarps);
     }
     words[1] = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 1) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(words)) : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    if constexpr (CG == 1) {
+      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(words))
+                   : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    } else {
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(words))
+                   : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+    }
   }
   fence_before();
   __syncthreads();
+  if constexpr (CG == 2) cluster_sync();
   fence_after();
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(words);
-  const int chunks = (q.bn + 63) / 64;  // MN-major B
+  const int half_n = q.bn / CG;              // columns of B that this CTA stages (of a single B)
+  const int chunks = (half_n + 63) / 64;     // MN-major B
 
-  if (threadIdx.x == 0) {  // the loads
-    uint32_t it = 0;
+  if (warp == 0) {  // the loads: each CTA its rows of A and its columns of B, all arriving at the first CTA's barrier
+    uint32_t it = 0, st = 0, parity = 1;
     bool ok = true;
     Tile t;
-    for (int L = blockIdx.x; ok && tile_at<MODE>(q, L, t); L += gridDim.x) {
+    const uint32_t ring = smem_u32(smem), arrive = CG == 2 ? in_cta(full, 0) : full;
+    for (int L = first; ok && tile_at<MODE, CG>(q, L, t); L += stride) {
+      t.m0 += int(rank) * kBM;
 #pragma unroll
       for (int s = 0; s < X::segs; ++s) {
         const bool pair = X::pair0 && s == 0;
-        const uint32_t b_bytes = X::b_mn(s) ? chunks * 8192 : (pair ? 2 : 1) * q.bn * 128;
-        for (int kb = 0; ok && kb < t.kb; ++kb, ++it) {
-          const int st = it % kStages;
-          ok = bar_wait(empty + 8 * st, ((it / kStages) & 1) ^ 1, dead);
+        const uint32_t bytes = kABytes + (X::b_mn(s) ? chunks * 8192 : pair ? 2 / CG * q.bn * 128 : half_n * 128);
+        const CUtensorMap* ma = &maps.a[s];
+        const CUtensorMap* mb = &maps.b[MODE == kUpBack && s == 1 ? 2 : pair && CG == 2 ? rank : s];
+        const int z = X::grouped ? t.slot : 0, n0 = t.n * q.bn + (pair ? 0 : int(rank) * half_n);
+        const int m0 = X::a_mn ? t.m0 : t.row0 + t.m0;
+        int k0 = 0, krow = MODE == kDw ? t.row0 : 0;
+        for (int kb = 0; kb < t.kb; ++kb, k0 += kBK, krow += kBK) {
+          ok = bar_wait(empty + 8 * st, parity, dead);
           if (!ok) break;
-          const uint32_t bar = full + 8 * st, sa = smem_u32(smem + st * kStageBytes), sb = sa + kABytes;
-          bar_expect(bar, kABytes + b_bytes);
-          const CUtensorMap* ma = &maps.a[s];
-          const int k0 = kb * kBK, krow = (MODE == kDw ? t.row0 : 0) + k0;
-          if constexpr (X::a_mn) {
-            tma_load(sa, ma, t.m0, krow, 0, bar);
-            tma_load(sa + 8192, ma, t.m0 + 64, krow, 0, bar);
-          } else {
-            tma_load(sa, ma, k0, t.row0 + t.m0, 0, bar);
+          const uint32_t sa = ring + st * kStageBytes, sb = sa + kABytes, bar = arrive + 8 * st;
+          if (elect()) {
+            if (rank == 0) bar_expect(bar, CG * bytes);
+            if constexpr (X::a_mn) {
+              tma_load<CG>(sa, ma, m0, krow, 0, bar);
+              tma_load<CG>(sa + 8192, ma, m0 + 64, krow, 0, bar);
+            } else {
+              tma_load<CG>(sa, ma, k0, m0, 0, bar);
+            }
+            if (X::b_mn(s)) {
+              for (int c = 0; c < chunks; ++c) tma_load<CG>(sb + c * 8192, mb, n0 + 64 * c, krow, z, bar);
+            } else {
+              tma_load<CG>(sb, mb, k0, n0, z, bar);
+              if (pair && CG == 1) tma_load<CG>(sb + q.bn * 128, &maps.b[1], k0, n0, z, bar);
+            }
           }
-          const int n0 = t.n * q.bn, z = X::grouped ? t.slot : 0;
-          const CUtensorMap* mb = &maps.b[MODE == kUpBack && s == 1 ? 2 : s];
-          if (X::b_mn(s)) {
-            for (int c = 0; c < chunks; ++c) tma_load(sb + c * 8192, mb, n0 + 64 * c, krow, z, bar);
-          } else {
-            tma_load(sb, mb, k0, n0, z, bar);
-            if (pair) tma_load(sb + q.bn * 128, &maps.b[1], k0, n0, z, bar);
-          }
+          ++it;
+          if (++st == kStages) st = 0, parity ^= 1;
         }
+        if (!ok) break;
       }
     }
     if (!ok)  // leave no copy in flight behind
       for (uint32_t j = it > kStages ? it - kStages : 0; j < it; ++j) {
         volatile uint32_t none = 0;
-        (void)bar_wait_slow(full + 8 * (j % kStages), (j / kStages) & 1, &none);
+        (void)bar_wait((rank == 0 ? full : empty) + 8 * (j % kStages), (j / kStages) & 1, &none);
       }
-  } else if (threadIdx.x == 32) {  // the products
-    uint32_t it = 0, nt = 0;
+  } else if (warp == 1 && rank == 0) {  // the products, for both CTAs
+    uint32_t it = 0, nt = 0, st = 0, parity = 0;
     bool ok = true;
     Tile t;
+    const uint64_t ring_a = desc(smem_u32(smem), X::a_mn);
     constexpr uint32_t type = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
-    for (int L = blockIdx.x; ok && tile_at<MODE>(q, L, t); L += gridDim.x, ++nt) {
+    for (int L = first; ok && tile_at<MODE, CG>(q, L, t); L += stride, ++nt) {
       const int buf = nt % X::bufs;
       ok = bar_wait(sums_empty + 8 * buf, ((nt / X::bufs) & 1) ^ 1, dead);
       if (!ok) break;
@@ -449,34 +517,39 @@ __global__ __launch_bounds__(kThreads, 1) void tc_kernel(const __grid_constant__
       for (int s = 0; s < X::segs; ++s) {
         const int n = X::pair0 && s == 0 ? 2 * q.bn : q.bn;
         const uint32_t idesc = (1u << 4) | (type << 7) | (type << 10) | (uint32_t(X::a_mn) << 15) |
-                               (uint32_t(X::b_mn(s)) << 16) | (uint32_t(n >> 3) << 17) | (uint32_t(kBM >> 4) << 24);
+                               (uint32_t(X::b_mn(s)) << 16) | (uint32_t(n >> 3) << 17) |
+                               (uint32_t(CG * kBM >> 4) << 24);
         const uint32_t d = tmem + buf * 256 + (MODE == kUpBack && s == 1 ? 256 : 0);
         const bool fresh = !(MODE == kDx && s == 1);  // dx: both segments add into the same sums
-        for (int kb = 0; kb < t.kb; ++kb, ++it) {
-          const int st = it % kStages;
-          ok = bar_wait(full + 8 * st, (it / kStages) & 1, dead);
+        const uint64_t ring_b = desc(smem_u32(smem) + kABytes, X::b_mn(s));
+        for (int kb = 0; kb < t.kb; ++kb) {
+          ok = bar_wait(full + 8 * st, parity, dead);
           if (!ok) break;
           fence_after();
-          const uint32_t sa = smem_u32(smem + st * kStageBytes), sb = sa + kABytes;
-          const uint64_t da = desc(sa, X::a_mn), db = desc(sb, X::b_mn(s));
+          const uint64_t da = ring_a + st * (kStageBytes >> 4), db = ring_b + st * (kStageBytes >> 4);
+          if (elect()) {
 #pragma unroll
-          for (int k = 0; k < kBK / 16; ++k)
-            mma(d, da + uint64_t((X::a_mn ? 2048 : 32) * k >> 4), db + uint64_t((X::b_mn(s) ? 2048 : 32) * k >> 4), idesc,
-                !(fresh && kb == 0 && k == 0));
-          commit(empty + 8 * st);
+            for (int k = 0; k < kBK / 16; ++k)
+              mma<CG>(d, da + uint64_t((X::a_mn ? 2048 : 32) * k >> 4), db + uint64_t((X::b_mn(s) ? 2048 : 32) * k >> 4),
+                      idesc, !(fresh && kb == 0 && k == 0));
+            commit<CG>(empty + 8 * st);
+          }
+          ++it;
+          if (++st == kStages) st = 0, parity ^= 1;
         }
         if (!ok) break;
       }
-      if (ok) commit(sums_full + 8 * buf);
+      if (ok && elect()) commit<CG>(sums_full + 8 * buf);
     }
     if (!ok && it) {  // the products already issued read shared memory and TMEM: let them end
       volatile uint32_t none = 0;
-      (void)bar_wait_slow(empty + 8 * ((it - 1) % kStages), ((it - 1) / kStages) & 1, &none);
+      (void)bar_wait(empty + 8 * ((it - 1) % kStages), ((it - 1) / kStages) & 1, &none);
     }
   } else if (warp >= 4) {  // the epilogue
     uint32_t nt = 0;
     Tile t;
-    for (int L = blockIdx.x; tile_at<MODE>(q, L, t); L += gridDim.x, ++nt) {
+    for (int L = first; tile_at<MODE, CG>(q, L, t); L += stride, ++nt) {
+      t.m0 += int(rank) * kBM;
       const int buf = nt % X::bufs;
       if (!bar_wait(sums_full + 8 * buf, (nt / X::bufs) & 1, dead)) break;
       __syncwarp();
@@ -484,15 +557,20 @@ __global__ __launch_bounds__(kThreads, 1) void tc_kernel(const __grid_constant__
       epilogue<T, MODE, ACT>(q, t, tmem + buf * 256, store + (warp - 4) * kStoreBytes, warp - 4);
       fence_before();
       __syncwarp();
-      if ((threadIdx.x & 31) == 0) bar_arrive(sums_empty + 8 * buf);
+      if ((threadIdx.x & 31) == 0) {
+        if constexpr (CG == 2) bar_arrive_cluster(in_cta(sums_empty + 8 * buf, 0));
+        else bar_arrive(sums_empty + 8 * buf);
+      }
     }
   }
   fence_before();
   __syncthreads();
+  if constexpr (CG == 2) cluster_sync();  // neither CTA's memory goes while the other's copies, products or arrivals use it
   fence_after();
   if (warp == 1) {
     __syncwarp();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+    if constexpr (CG == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+    else asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem));
     if ((threadIdx.x & 31) == 0 && *dead) atomicAdd(&g_ops_timeouts, 1u);
   }
 }
@@ -534,13 +612,27 @@ bool make_map(CUtensorMap* m, int dtype, const void* p, uint64_t cols, uint64_t 
                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <class T, int MODE, int ACT>
-int go(const Maps& maps, const Params& q, int grid, cudaStream_t s) {
-  const auto kernel = tc_kernel<T, MODE, ACT>;
+template <class T, int MODE, int ACT, int CG>
+int go_pair(const Maps& maps, const Params& q, int grid, cudaStream_t s) {
+  const auto kernel = tc_kernel<T, MODE, ACT, CG>;
   const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
   if (e != cudaSuccess) return int(e);
-  kernel<<<grid, kThreads, kSmemBytes, s>>>(maps, q);
-  return int(cudaGetLastError());
+  cudaLaunchConfig_t c{};
+  c.gridDim = dim3(unsigned(grid * CG));
+  c.blockDim = dim3(kThreads);
+  c.dynamicSmemBytes = kSmemBytes;
+  c.stream = s;
+  cudaLaunchAttribute a[1];
+  a[0].id = cudaLaunchAttributeClusterDimension;
+  a[0].val.clusterDim.x = CG;
+  a[0].val.clusterDim.y = a[0].val.clusterDim.z = 1;
+  c.attrs = a;
+  c.numAttrs = 1;
+  return int(cudaLaunchKernelEx(&c, kernel, maps, q));
+}
+template <class T, int MODE, int ACT>
+int go(const Maps& maps, const Params& q, int grid, cudaStream_t s) {
+  return q.pair ? go_pair<T, MODE, ACT, 2>(maps, q, grid, s) : go_pair<T, MODE, ACT, 1>(maps, q, grid, s);
 }
 template <class T, int MODE>
 int go_act(int act, const Maps& maps, const Params& q, int grid, cudaStream_t s) {
@@ -569,13 +661,13 @@ int sm_count() {
   return n;
 }
 
-// Columns a tile: of the multiples of 16 up to `most`, the one whose last wave of tiles wastes least. A tile costs its
+// Columns a tile: of the multiples of `step` up to `most`, the one whose last wave of tiles wastes least. A tile costs its
 // columns plus about 32 (the narrower tile re-reads A for fewer products); 2047 x 7168 at 148 SMs takes 208 (4 waves of
 // 560 tiles) over 256 (4 waves of 448).
-int columns(int64_t m_tiles, int64_t n, int sms, int most) {
-  int best = 16;
+int columns(int64_t m_tiles, int64_t n, int sms, int most, int step) {
+  int best = step;
   int64_t cost = INT64_MAX;
-  for (int bn = most; bn >= 16; bn -= 16) {
+  for (int bn = most; bn >= step; bn -= step) {
     const int64_t waves = ceil_div(uint64_t(m_tiles) * ceil_div(uint64_t(n), uint64_t(bn)), uint64_t(sms));
     const int64_t c = waves * (bn + 32);
     if (c < cost) cost = c, best = bn;
@@ -621,12 +713,17 @@ int launch_tc(int dtype, const Product& p, const Plan* plan, const Units* u, cud
   else if (p.epi == kEpiUpBack) mode = kUpBack;
   else if (p.epi == kEpiRows32) mode = p.segs == 2 ? kDx : kDown;
   else mode = p.per_unit ? kDw : (a_mn ? kLinDw : kLinDx);
+  // Pairs of CTAs share a 256-row tile when there are rows for it: each stages half of B, so a tile's operands cross from
+  // L2 once for 256 x 256 sums instead of 128 x 256 (the SM's 64 bytes a clock from L2 bound the single CTA).
+  q.pair = p.grouped ? plan->bm == 2 * kBM : p.m > kBM;
+  const int cg = q.pair ? 2 : 1;
   q.k_blocks = int(ceil_div(uint64_t(p.k), kBK));
-  q.m_tiles = p.grouped ? 0 : int(ceil_div(uint64_t(p.m), kBM));
+  q.m_tiles = p.grouped ? 0 : int(ceil_div(uint64_t(p.m), uint64_t(cg * kBM)));
   const int64_t m_tiles = p.grouped ? plan->max_tiles : p.per_unit ? int64_t(q.m_tiles) * plan->units : q.m_tiles;
   const bool narrow = mode == kUp || mode == kUpBack;
-  q.bn = p.grouped || p.per_unit ? (narrow ? 128 : 256) : columns(m_tiles, p.n, sms, 256);
-  if (q.bn > (p.n + 15) / 16 * 16) q.bn = int((p.n + 15) / 16 * 16);
+  q.bn = p.grouped || p.per_unit ? (narrow ? 128 : 256) : columns(m_tiles, p.n, sms / cg, 256, 16 * cg);
+  const int64_t step = 16 * cg;  // a product's columns: whole 16 for one CTA, 32 for a pair
+  if (q.bn > (p.n + step - 1) / step * step) q.bn = int((p.n + step - 1) / step * step);
   q.n_tiles = int(ceil_div(uint64_t(p.n), uint64_t(q.bn)));
   q.vec = p.epi == kEpiRows32 ||
           (p.epi == kEpiUpBack ? on16(p.dg) && on16(p.du) && on16(p.hw) && p.ldo % 8 == 0
@@ -658,12 +755,12 @@ int launch_tc(int dtype, const Product& p, const Plan* plan, const Units* u, cud
     const int ia = narrow ? (i == 2 ? 1 : 0) : i;
     if (!make_map(&maps.a[ia], dtype, a.p, a.cols, a.rows, a.ld, a.slots, a.slot_bytes, a_mn ? 64 : kBM) ||
         !make_map(&maps.b[i], dtype, b.p, b.cols, b.rows, b.ld, b.slots, b.slot_bytes,
-                  p.b[i].s_k == 1 ? uint32_t(q.bn) : 64))
+                  p.b[i].s_k == 1 ? uint32_t(narrow ? q.bn : q.bn / cg) : 64))
       return int(cudaErrorInvalidValue);
   }
   const int64_t tiles = m_tiles * q.n_tiles;
   if (tiles >= (int64_t(1) << 30)) return int(cudaErrorInvalidValue);
-  const int grid = int(tiles < sms ? tiles : sms);
+  const int grid = int(tiles < sms / cg ? tiles : sms / cg);
   switch (mode) {
     case kLin: return go_type<kLin>(dtype, p.act, maps, q, grid, s);
     case kLinDx: return go_type<kLinDx>(dtype, 0, maps, q, grid, s);
