@@ -50,27 +50,29 @@ __device__ __forceinline__ const char* unit_part(const Units& u, int p, int32_t 
   return u.table ? reinterpret_cast<const char*>(u.table[e]) + u.stride[p] : u.part[p] + uint64_t(slot) * u.stride[p];
 }
 
-// Activations and their slopes in 32 bits, by the accurate library functions: their cost hides behind the products.
+// Activations and their slopes in 32 bits. The exponentials and quotients are the fast intrinsics, off by a few 2^-22 of
+// the value where the results are rounded to 2^-9 or 2^-12; (1 + tanh q) / 2 is the logistic of 2 q.
+__device__ __forceinline__ float logistic(float z) { return __fdividef(1.f, 1.f + __expf(-z)); }
+constexpr float kGelu1 = 1.5957691216057308f, kGelu3 = 0.071354816272600250f;  // 2 sqrt(2 / pi), and times 0.044715
 template <int ACT>
 __device__ __forceinline__ float act_of(float z) {
-  if constexpr (ACT == TSB_ACT_SILU) return z / (1.f + expf(-z));
+  if constexpr (ACT == TSB_ACT_SILU) return z * logistic(z);
   if constexpr (ACT == TSB_ACT_GELU) return 0.5f * z * (1.f + erff(z * 0.70710678118654752f));
-  if constexpr (ACT == TSB_ACT_GELU_TANH)
-    return 0.5f * z * (1.f + tanhf(0.79788456080286536f * (z + 0.044715f * z * z * z)));
+  if constexpr (ACT == TSB_ACT_GELU_TANH) return z * logistic(z * (kGelu1 + kGelu3 * z * z));
   if constexpr (ACT == TSB_ACT_RELU) return z < 0.f ? 0.f : z;  // (a NaN stays one)
   return z;
 }
 template <int ACT>
 __device__ __forceinline__ float slope_of(float z) {
   if constexpr (ACT == TSB_ACT_SILU) {
-    const float p = 1.f / (1.f + expf(-z));
+    const float p = logistic(z);
     return p * (1.f + z * (1.f - p));
   }
   if constexpr (ACT == TSB_ACT_GELU)
-    return 0.5f * (1.f + erff(z * 0.70710678118654752f)) + z * expf(-0.5f * z * z) * 0.39894228040143268f;
+    return 0.5f * (1.f + erff(z * 0.70710678118654752f)) + z * __expf(-0.5f * z * z) * 0.39894228040143268f;
   if constexpr (ACT == TSB_ACT_GELU_TANH) {
-    const float p = tanhf(0.79788456080286536f * (z + 0.044715f * z * z * z));
-    return 0.5f * (1.f + p) + 0.5f * z * (1.f - p * p) * 0.79788456080286536f * (1.f + 0.134145f * z * z);
+    const float p = logistic(z * (kGelu1 + kGelu3 * z * z));
+    return p + z * p * (1.f - p) * (kGelu1 + 3.f * kGelu3 * z * z);
   }
   if constexpr (ACT == TSB_ACT_RELU) return z > 0.f ? 1.f : 0.f;
   return 1.f;

@@ -25,7 +25,8 @@ namespace ops {
 namespace {
 
 constexpr int kBM = 128, kBK = 64;  // (a CTA's rows)
-constexpr int kABytes = kBM * kBK * 2, kRingBytes = 4 * (kABytes + 256 * kBK * 2);  // 192 KiB of stages
+constexpr int kABytes = kBM * kBK * 2, kRingBytes = 192 << 10;  // the stages'
+constexpr int kMaxStages = 12;
 constexpr int kEpiWarps = 8, kThreads = 128 + 32 * kEpiWarps;
 constexpr int kRowBytes = 80, kStoreBytes = 32 * kRowBytes;  // a warp's 32 rows of 64 bytes, 16 apart: no bank twice
 constexpr int kSmemBytes = 1024 + kRingBytes + kEpiWarps * kStoreBytes + 256;
@@ -43,6 +44,7 @@ struct Params {
   int32_t m_tiles;   // tiles along m when not grouped
   int32_t k_blocks;  // of a segment; with k_rows per unit: from the group
   int32_t vec;       // 16-byte stores are possible
+  int32_t stages, stage_bytes;
   int32_t pair;      // two CTAs to a tile of 256 rows
 };
 struct Maps {
@@ -272,6 +274,19 @@ __device__ __forceinline__ void store_rows(char* stage, const uint32_t (&v)[16],
   __syncwarp();
 }
 
+// 32 elements of a row into registers, `cols` of them inside the matrix
+template <class T>
+__device__ __forceinline__ void read32(T (&v)[32], const T* p, int cols, bool whole) {
+  if (whole) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) reinterpret_cast<uint4*>(v)[i] = reinterpret_cast<const uint4*>(p)[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < 32; ++i)
+      if (i < cols) v[i] = p[i];
+  }
+}
+
 template <class T, int MODE, int ACT>
 __device__ __forceinline__ void epilogue(const Params& q, const Tile& t, uint32_t tmem, char* stage, int warp) {
   const Product& p = q.p;
@@ -333,62 +348,29 @@ __device__ __forceinline__ void epilogue(const Params& q, const Tile& t, uint32_
                         true);
     }
   } else if constexpr (MODE == kLin) {
-    // the sums go through the transpose in 32 bits; bias, residual and both outputs are read and written along rows
-    for (int c = half * 16; c < q.bn; c += 32) {
-      float v[16];
-      tmem_ld16(base + c, v);
-      tmem_wait_ld();
-      float4* mine = reinterpret_cast<float4*>(stage + lane * kRowBytes);
+    const int64_t row = m + lane;
+    const T *bias = static_cast<const T*>(p.bias), *res = static_cast<const T*>(p.residual) + row * p.ldr;
+    for (int c = half * 32; c < q.bn; c += 64) {
+      const int64_t n = n0 + c;
+      const bool whole = q.vec && c + 32 <= cols;
+      T b[32] = {}, r[32] = {};
+      if (bias) read32(b, bias + n, cols - c, whole);
+      if (p.residual && lane < rows) read32(r, res + n, cols - c, whole);
+      uint32_t y[16], pre[16];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) mine[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
-      __syncwarp();
-      const int cc = c + (lane & 3) * 4;
-      const int64_t n = n0 + cc;
-      T bias[4] = {}, res[4] = {};
-      const bool whole = q.vec && cc + 4 <= cols;
-      if (p.bias)
+      for (int s = 0; s < 2; ++s) {
+        float v[16];
+        tmem_ld16(base + min(c + 16 * s, q.bn - 16), v);
+        tmem_wait_ld();
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (cc + j < cols) bias[j] = static_cast<const T*>(p.bias)[n + j];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int r = i * 8 + (lane >> 2);
-        const float4 f = *reinterpret_cast<const float4*>(stage + r * kRowBytes + (lane & 3) * 16);
-        if (r >= rows) continue;
-        const int64_t mm = m + r;
-        float z[4] = {f.x, f.y, f.z, f.w};
-        if (p.residual) {
-          const T* src = static_cast<const T*>(p.residual) + mm * p.ldr + n;
-          if (whole) {
-            *reinterpret_cast<uint2*>(res) = *reinterpret_cast<const uint2*>(src);
-          } else {
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-              if (cc + j < cols) res[j] = src[j];
-          }
-        }
-        T y[4], pre[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          z[j] += to_f(bias[j]);
-          pre[j] = from_f<T>(z[j]);
-          y[j] = from_f<T>(act_of<ACT>(z[j]) + to_f(res[j]));
-        }
-        T* out = static_cast<T*>(p.out) + mm * p.ldo + n;
-        T* keep = static_cast<T*>(p.pre) + mm * p.ldp + n;
-        if (whole) {
-          *reinterpret_cast<uint2*>(out) = *reinterpret_cast<uint2*>(y);
-          if (p.pre) *reinterpret_cast<uint2*>(keep) = *reinterpret_cast<uint2*>(pre);
-        } else {
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            if (cc + j < cols) {
-              out[j] = y[j];
-              if (p.pre) keep[j] = pre[j];
-            }
+        for (int i = 0; i < 16; i += 2) {
+          const float z0 = v[i] + to_f(b[16 * s + i]), z1 = v[i + 1] + to_f(b[16 * s + i + 1]);
+          pre[8 * s + i / 2] = pack<T>(z0, z1);
+          y[8 * s + i / 2] = pack<T>(act_of<ACT>(z0) + to_f(r[16 * s + i]), act_of<ACT>(z1) + to_f(r[16 * s + i + 1]));
         }
       }
-      __syncwarp();
+      store_rows<T>(stage, y, static_cast<T*>(p.out) + m * p.ldo + n, p.ldo, rows, cols - c, q.vec);
+      if (p.pre) store_rows<T>(stage, pre, static_cast<T*>(p.pre) + m * p.ldp + n, p.ldp, rows, cols - c, q.vec);
     }
   } else {  // gradients: rounded once
     T* out = static_cast<T*>(p.out) + int64_t(t.unit) * p.out_unit + m * p.ldo + n0;
@@ -413,20 +395,20 @@ template <class T, int MODE, int ACT, int CG>
 __global__ __launch_bounds__(kThreads, 1) void tc_kernel(const __grid_constant__ Maps maps,
                                                          const __grid_constant__ Params q) {
   using X = Traits<MODE>;
-  constexpr int kStageBytes = kABytes + 256 / CG * kBK * 2, kStages = kRingBytes / kStageBytes;
+  const uint32_t stages = uint32_t(q.stages), stage_bytes = uint32_t(q.stage_bytes);
   extern __shared__ char raw[];
   char* smem = raw + ((1024 - (smem_u32(raw) & 1023)) & 1023);
   char* store = smem + kRingBytes;
   uint64_t* bars = reinterpret_cast<uint64_t*>(store + kEpiWarps * kStoreBytes);
-  const uint32_t full = smem_u32(bars), empty = full + 8 * kStages, sums_full = empty + 8 * kStages,
+  const uint32_t full = smem_u32(bars), empty = full + 8 * kMaxStages, sums_full = empty + 8 * kMaxStages,
                  sums_empty = sums_full + 16;
-  uint32_t* words = reinterpret_cast<uint32_t*>(bars + 2 * kStages + 4);  // [0] TMEM address, [1] a wait ran out
+  uint32_t* words = reinterpret_cast<uint32_t*>(bars + 2 * kMaxStages + 4);  // [0] TMEM address, [1] a wait ran out
   volatile uint32_t* dead = words + 1;
   const int warp = __shfl_sync(0xffffffffu, int(threadIdx.x >> 5), 0);
   const uint32_t rank = CG == 2 ? cta_rank() : 0;
   const int first = blockIdx.x / CG, stride = gridDim.x / CG;
   if (threadIdx.x == 0) {
-    for (int s = 0; s < kStages; ++s) {
+    for (uint32_t s = 0; s < stages; ++s) {
       bar_init(full + 8 * s, 1);
       bar_init(empty + 8 * s, 1);
     }
@@ -475,7 +457,7 @@ __global__ __launch_bounds__(kThreads, 1) void tc_kernel(const __grid_constant__
         for (int kb = 0; kb < t.kb; ++kb, k0 += kBK, krow += kBK) {
           ok = bar_wait(empty + 8 * st, parity, dead);
           if (!ok) break;
-          const uint32_t sa = ring + st * kStageBytes, sb = sa + kABytes, bar = arrive + 8 * st;
+          const uint32_t sa = ring + st * stage_bytes, sb = sa + kABytes, bar = arrive + 8 * st;
           if (elect()) {
             if (rank == 0) bar_expect(bar, CG * bytes);
             if constexpr (X::a_mn) {
@@ -492,15 +474,15 @@ __global__ __launch_bounds__(kThreads, 1) void tc_kernel(const __grid_constant__
             }
           }
           ++it;
-          if (++st == kStages) st = 0, parity ^= 1;
+          if (++st == stages) st = 0, parity ^= 1;
         }
         if (!ok) break;
       }
     }
     if (!ok)  // leave no copy in flight behind
-      for (uint32_t j = it > kStages ? it - kStages : 0; j < it; ++j) {
+      for (uint32_t j = it > stages ? it - stages : 0; j < it; ++j) {
         volatile uint32_t none = 0;
-        (void)bar_wait((rank == 0 ? full : empty) + 8 * (j % kStages), (j / kStages) & 1, &none);
+        (void)bar_wait((rank == 0 ? full : empty) + 8 * (j % stages), (j / stages) & 1, &none);
       }
   } else if (warp == 1 && rank == 0) {  // the products, for both CTAs
     uint32_t it = 0, nt = 0, st = 0, parity = 0;
@@ -526,7 +508,7 @@ __global__ __launch_bounds__(kThreads, 1) void tc_kernel(const __grid_constant__
           ok = bar_wait(full + 8 * st, parity, dead);
           if (!ok) break;
           fence_after();
-          const uint64_t da = ring_a + st * (kStageBytes >> 4), db = ring_b + st * (kStageBytes >> 4);
+          const uint64_t da = ring_a + st * (stage_bytes >> 4), db = ring_b + st * (stage_bytes >> 4);
           if (elect()) {
 #pragma unroll
             for (int k = 0; k < kBK / 16; ++k)
@@ -535,7 +517,7 @@ __global__ __launch_bounds__(kThreads, 1) void tc_kernel(const __grid_constant__
             commit<CG>(empty + 8 * st);
           }
           ++it;
-          if (++st == kStages) st = 0, parity ^= 1;
+          if (++st == stages) st = 0, parity ^= 1;
         }
         if (!ok) break;
       }
@@ -543,7 +525,7 @@ __global__ __launch_bounds__(kThreads, 1) void tc_kernel(const __grid_constant__
     }
     if (!ok && it) {  // the products already issued read shared memory and TMEM: let them end
       volatile uint32_t none = 0;
-      (void)bar_wait(empty + 8 * ((it - 1) % kStages), ((it - 1) / kStages) & 1, &none);
+      (void)bar_wait(empty + 8 * ((it - 1) % stages), ((it - 1) / stages) & 1, &none);
     }
   } else if (warp >= 4) {  // the epilogue
     uint32_t nt = 0;
@@ -728,8 +710,8 @@ int launch_tc(int dtype, const Product& p, const Plan* plan, const Units* u, cud
   q.vec = p.epi == kEpiRows32 ||
           (p.epi == kEpiUpBack ? on16(p.dg) && on16(p.du) && on16(p.hw) && p.ldo % 8 == 0
                                : on16(p.out) && p.ldo % 8 == 0 && p.out_unit % 8 == 0 &&
-                                     (!p.residual || (on16(p.residual) && p.ldr % 4 == 0)) &&
-                                     (!p.pre || (on16(p.pre) && p.ldp % 4 == 0)));
+                                     on16(p.bias) && on16(p.residual) && p.ldr % 8 == 0 && on16(p.pre) &&
+                                     p.ldp % 8 == 0);
   Maps maps;
   std::memset(&maps, 0, sizeof maps);
   auto shape = [&](const Operand& o, int64_t n_i, int64_t n_k) {
@@ -758,6 +740,10 @@ int launch_tc(int dtype, const Product& p, const Plan* plan, const Units* u, cud
                   p.b[i].s_k == 1 ? uint32_t(narrow ? q.bn : q.bn / cg) : 64))
       return int(cudaErrorInvalidValue);
   }
+  // as many stages as the ring holds: narrow tiles are bound by the loads' latency
+  const int b_cols = (narrow && cg == 1 ? 2 : 1) * (narrow ? q.bn : q.bn / cg);
+  q.stage_bytes = kABytes + int(ceil_div(uint64_t(b_cols), 64)) * 8192;
+  q.stages = kRingBytes / q.stage_bytes < kMaxStages ? kRingBytes / q.stage_bytes : kMaxStages;
   const int64_t tiles = m_tiles * q.n_tiles;
   if (tiles >= (int64_t(1) << 30)) return int(cudaErrorInvalidValue);
   const int grid = int(tiles < sms / cg ? tiles : sms / cg);
