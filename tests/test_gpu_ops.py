@@ -608,9 +608,11 @@ def test_refusals_on_tensors():
                 lambda: ops.ffn(x[:, :8], ids, p, un), lambda: ops.ffn(x.half(), ids, p, un),
                 lambda: ops.ffn(x, ids.T, p, un),
                 lambda: ops.Units(un.keep[0], un.keep[1], un.keep[1]),
-                lambda: ops.Units(un.keep[0], un.keep[1], un.keep[2], ids.float())):
+                lambda: ops.Units(un.keep[0], un.keep[1], un.keep[2], ids.float()), lambda: ops.route(x, 17),
+                lambda: ops.route(x, 0), lambda: ops.linear(x, torch.zeros((16, 16), dtype=t, device="cuda"), out=x),
+                lambda: ops.ffn(x, ids, p, un, out=x), lambda: ops.ffn(x, ids, p, un, residual=x, out=x[:2]),
+                lambda: ops.route_backward(p, x[:2], ids, p)):
         with pytest.raises(ValueError):
             bad()
-    for bad in (lambda: ops.route(x, 17), lambda: ops.route(x, 0)):
-        with pytest.raises(abi.TsError):
-            bad()
+    with pytest.raises(abi.TsError):  # the library's own refusals
+        ops.ffn(x, torch.zeros((4, 65), dtype=torch.int32, device="cuda"), torch.zeros((4, 65), device="cuda"), un)

@@ -184,10 +184,10 @@ constexpr uint32_t kTileM = 64, kTileN = 64;
 int launch_tile(int dtype, const Product& p, const Plan* plan, const Units* units, cudaStream_t s);
 
 
-// ops_stream.cu: products of few rows, tiles of 8, 16 or 32 rows (the plan's bm). Rows of x and w start on 16 bytes and k
+// ops_stream.cu: products of few rows, in tiles of 8 (the plan's bm). Rows of x and w start on 16 bytes and k
 // is a multiple of 8; gathered rows are read where they are (top: the pairs a row has).
-int launch_stream(int dtype, const Product& p, uint32_t rows_a_tile, uint32_t top, const Plan* plan, const Units* units,
-                  cudaStream_t s);
+constexpr uint32_t kStreamTile = 8;
+int launch_stream(int dtype, const Product& p, uint32_t top, const Plan* plan, const Units* units, cudaStream_t s);
 
 // ops_tc.cu: products of many rows on tcgen05 (the plan made with bm = kTcRows, or twice that: pairs of CTAs). tc_fits: TMA can read the operand.
 // Gathered operands are gathered first: launch_gather copies n columns of every grouped row (n a multiple of 8).

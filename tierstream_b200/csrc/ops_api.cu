@@ -59,17 +59,19 @@ Operand gathered(const void* p, int64_t s_i, int64_t s_k, const Plan& plan, uint
 }
 Operand of_unit(int part, int64_t s_i, int64_t s_k) { return {nullptr, s_i, s_k, nullptr, 1, 0, part}; }
 
-// Rows up to which the kernel that streams the weights beats the tensor cores' own path (whose 128-row tiles are then
-// mostly empty), and the tile's rows for it.
-constexpr uint64_t kStreamRows = 32;
-uint32_t stream_tile(uint64_t rows) { return rows <= 8 ? 8 : rows <= 16 ? 16 : 32; }
+// Where the kernel that streams the weights (8 rows a tile) beats the tensor cores' own path, whose 128-row tiles are
+// mostly empty then: a plain product of at most 8 rows (32 us against 58 at 6 x 8192 x 8192, 34 against 48 at 8 x 4096 x
+// 14336, where the other's 128 column tiles cannot keep enough bytes in flight), and the feed-forward block with at most
+// two rows for each unit that may be met (730 us against 767 at two of 64 units of 88 MB, 327 against 362 at one of 8 of
+// 352 MB, 663 against 644 at two of 128 of 38 MB; at four 800 against 750 there).
+constexpr uint64_t kStreamRows = kStreamTile, kStreamEach = 2;
 
 // One matrix product: on the tensor cores' own path when TMA can read both operands (rows on 16 bytes), else by the
 // kernel for every alignment.
 int product(int dtype, const Product& p, cudaStream_t s) {
   if (p.epi == kEpiLinear && uint64_t(p.m) <= kStreamRows && p.k % 8 == 0 && tc_fits(p.a[0], nullptr) &&
       tc_fits(p.b[0], nullptr))
-    return launch_stream(dtype, p, stream_tile(uint64_t(p.m)), 1, nullptr, nullptr, s);
+    return launch_stream(dtype, p, 1, nullptr, nullptr, s);
   if (tc_fits(p.a[0], nullptr) && tc_fits(p.b[0], nullptr)) return launch_tc(dtype, p, nullptr, nullptr, s);
   return launch_tile(dtype, p, nullptr, nullptr, s);
 }
@@ -241,12 +243,12 @@ FfnSpace ffn_space(const tsb_ffn_args* a) {
   Arena w{static_cast<char*>(a->workspace)};
   FfnSpace r{};
   const uint64_t pairs = a->rows * a->top;
-  // few rows for each unit that may be met: the weights are streamed (units by address too)
+  // few rows for each unit that may be met, or units by address, which TMA cannot find: the weights are streamed
   const uint64_t each = ceil_div(pairs, pairs < a->units->n_units ? pairs : a->units->n_units);
-  r.stream = each <= kStreamRows && pairs / 8 + a->units->n_units <= 65535 &&  // (a grid's y)
+  r.stream = (each <= kStreamEach || a->units->table) && pairs / kStreamTile + a->units->n_units <= 65535 &&  // (a grid's y)
              ffn_rows16(a->units, a->hidden, a->ffn, a->x, a->ldx, nullptr, 0);
   r.tc = !r.stream && !a->units->table && ffn_rows16(a->units, a->hidden, a->ffn, a->x, a->ldx, nullptr, 0);
-  const uint32_t bm = r.stream ? stream_tile(each) : r.tc ? tc_tile(each) : kTileM;
+  const uint32_t bm = r.stream ? kStreamTile : r.tc ? tc_tile(each) : kTileM;
   r.plan = plan_at(w.take(plan_bytes(a->units->n_units, pairs, 1, bm)), a->units->n_units, pairs, 1, bm);
   if (r.tc) r.xs = w.take(uint64_t(r.plan.max_rows) * a->hidden * 2);
   r.h = w.take(uint64_t(r.plan.max_rows) * a->ffn * 2);
@@ -286,7 +288,7 @@ void ffn(const tsb_ffn_args* a) {
   p.act = int(a->act);
   p.out = w.h, p.ldo = f;
   const auto go = [&](int dtype, const Product& pr, const Plan* pl, const Units* un, cudaStream_t st) {
-    return w.stream ? launch_stream(dtype, pr, pl->bm, a->top, pl, un, st)
+    return w.stream ? launch_stream(dtype, pr, a->top, pl, un, st)
            : w.tc   ? launch_tc(dtype, pr, pl, un, st)
                     : launch_tile(dtype, pr, pl, un, st);
   };

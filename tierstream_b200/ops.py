@@ -17,6 +17,10 @@ ACTIVATIONS = {"none": abi.TSB_ACT_NONE, "silu": abi.TSB_ACT_SILU, "gelu": abi.T
                "gelu_tanh": abi.TSB_ACT_GELU_TANH, "relu": abi.TSB_ACT_RELU}
 _HALF = {torch.bfloat16: abi.TSB_BF16, torch.float16: abi.TSB_F16}
 _ANY = {**_HALF, torch.float32: abi.TSB_F32}
+_LINEAR, _LINEAR_GRAD = C.sizeof(abi.tsb_linear_args), C.sizeof(abi.tsb_linear_grad_args)
+_FFN, _FFN_GRAD, _UNITS = C.sizeof(abi.tsb_ffn_args), C.sizeof(abi.tsb_ffn_grad_args), C.sizeof(abi.tsb_units)
+# the current stream's handle; torch.cuda.current_stream() builds an object around it, which costs 4 us a call
+_raw_stream = torch._C._cuda_getCurrentRawStream
 
 
 def _act(name):
@@ -26,73 +30,95 @@ def _act(name):
         raise ValueError("unknown activation %r: one of %s" % (name, ", ".join(ACTIVATIONS))) from None
 
 
-def _mat(name, t, rows, cols, like):
-    """A [rows][cols] matrix of like's type on like's device: (address, elements between rows)."""
-    if t.dtype != like.dtype or t.device != like.device:
-        raise ValueError("%s: %s on %s is wanted, got %s on %s" % (name, like.dtype, like.device, t.dtype, t.device))
-    if t.dim() != 2 or t.shape[0] != rows or t.shape[1] != cols:
-        raise ValueError("%s: shape %s is wanted, got %s" % (name, (rows, cols), tuple(t.shape)))
-    s0, s1 = t.stride()
-    if cols > 1 and s1 != 1:
-        raise ValueError("%s: the elements of a row must be adjacent" % name)
-    if rows > 1 and s0 < cols:
-        raise ValueError("%s: rows overlap" % name)
-    return t.data_ptr(), s0 if rows > 1 else max(s0, cols)
-
-
-def _flat(name, t, shape, dtype, device):
-    """A contiguous tensor of the given shape: its address."""
-    if t.dtype != dtype or t.device != device or t.shape != shape or not t.is_contiguous():
-        raise ValueError("%s: a contiguous %s of shape %s on %s is wanted, got %s %s on %s" %
-                         (name, dtype, tuple(shape), device, t.dtype, tuple(t.shape), t.device))
-    return t.data_ptr()
-
-
 def _first(name, t, types):
-    if t.dtype not in types:
+    """The type code and the device of an operator's first matrix."""
+    dt = types.get(t.dtype)
+    if dt is None:
         raise ValueError("%s: %s is not served (%s)" % (name, t.dtype, ", ".join(str(d) for d in types)))
     if t.dim() != 2:
         raise ValueError("%s: two dimensions are wanted, got %s" % (name, tuple(t.shape)))
     if not t.is_cuda:
         raise ValueError("%s: a CUDA tensor is wanted" % name)
-    return types[t.dtype]
+    return dt, t.get_device()
 
 
-def _call(fn, args, device, size=None):
-    """Runs one entry point on the current stream of `device` with scratch of the size it asks for."""
-    if torch.cuda.current_device() != device.index:
-        with torch.cuda.device(device):
-            return _call(fn, args, device, size)
-    args.stream = torch.cuda.current_stream().cuda_stream
-    scratch = None
-    n = size(C.byref(args)) if size else 0
+def _mat(name, t, rows, cols, dtype, dev):
+    """A [rows][cols] matrix of that type on that device: (address, elements between rows)."""
+    if t.dtype is not dtype or t.get_device() != dev:
+        raise ValueError("%s: %s on cuda:%d is wanted, got %s on %s" % (name, dtype, dev, t.dtype, t.device))
+    if t.shape != (rows, cols):
+        raise ValueError("%s: shape %s is wanted, got %s" % (name, (rows, cols), tuple(t.shape)))
+    if t.is_contiguous():
+        return t.data_ptr(), cols
+    s0, s1 = t.stride()
+    if cols > 1 and s1 != 1:
+        raise ValueError("%s: the elements of a row must be adjacent" % name)
+    if rows > 1 and s0 < cols:
+        raise ValueError("%s: rows overlap" % name)
+    return t.data_ptr(), s0 if rows > 1 else cols
+
+
+def _flat(name, t, shape, dtype, dev):
+    """A contiguous tensor of the given shape: its address."""
+    if t.dtype is not dtype or t.get_device() != dev or t.shape != shape or not t.is_contiguous():
+        raise ValueError("%s: a contiguous %s of shape %s on cuda:%d is wanted, got %s %s on %s" %
+                         (name, dtype, tuple(shape), dev, t.dtype, tuple(t.shape), t.device))
+    return t.data_ptr()
+
+
+def _apart(name, out, *inputs):
+    """Refuses an output that shares memory with an input (its residual apart, element by element)."""
+    def span(t):
+        n = sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1 if t.numel() else 0
+        return t.data_ptr(), t.data_ptr() + n * t.element_size()
+    lo, hi = span(out)
+    for t in inputs:
+        a, b = span(t)
+        if a < hi and lo < b:
+            raise ValueError("%s: overlaps an input" % name)
+
+
+def _call(fn, args, dev, size=None):
+    """Runs one entry point on the current stream of device `dev` with scratch of the size it asks for."""
+    if torch.cuda.current_device() != dev:
+        with torch.cuda.device(dev):
+            return _call(fn, args, dev, size)
+    args.stream = _raw_stream(dev)
+    ref = C.byref(args)
+    n = size(ref) if size else 0
     if n:
-        scratch = torch.empty(n + 256, dtype=torch.uint8, device=device)
+        scratch = torch.empty(n + 256, dtype=torch.uint8, device="cuda")
         args.workspace = (scratch.data_ptr() + 255) & ~255
         args.workspace_bytes = n
-    abi.check(fn(C.byref(args)))
+    st = fn(ref)
+    if st:
+        abi.check(st)
 
 
 def linear(x, w, bias=None, residual=None, act="none", pre=None, out=None):
     """act(x w^T + bias) + residual: x [rows][k], w [n][k], bias [n], residual [rows][n]. pre: a [rows][n] tensor that
     receives x w^T + bias for linear_backward. out: where to write (may be the residual)."""
     lib = abi.load()
-    dt = _first("x", x, _HALF)
-    rows, k = x.shape
-    n = w.shape[0]
-    a = abi.tsb_linear_args(C.sizeof(abi.tsb_linear_args), dt, _act(act), 0, rows, n, k)
-    a.x, a.ldx = _mat("x", x, rows, k, x)
-    a.w, a.ldw = _mat("w", w, n, k, x)
+    dt, dev = _first("x", x, _HALF)
+    (rows, k), n, t = x.shape, w.shape[0], x.dtype
+    px, ldx = _mat("x", x, rows, k, t, dev)
+    pw, ldw = _mat("w", w, n, k, t, dev)
+    pb = pr = pp = None
+    ldr = ldp = 0
     if bias is not None:
-        a.bias = _flat("bias", bias, (n,), x.dtype, x.device)
+        pb = _flat("bias", bias, (n,), t, dev)
     if residual is not None:
-        a.residual, a.ldr = _mat("residual", residual, rows, n, x)
+        pr, ldr = _mat("residual", residual, rows, n, t, dev)
     if pre is not None:
-        a.pre, a.ldp = _mat("pre", pre, rows, n, x)
+        pp, ldp = _mat("pre", pre, rows, n, t, dev)
+        _apart("pre", pre, x, w)
     if out is None:
-        out = torch.empty((rows, n), dtype=x.dtype, device=x.device)
-    a.y, a.ldy = _mat("out", out, rows, n, x)
-    _call(lib.tsb_linear, a, x.device, lib.tsb_linear_workspace)
+        out = x.new_empty((rows, n))
+    else:
+        _apart("out", out, x, w)
+    py, ldy = _mat("out", out, rows, n, t, dev)
+    a = abi.tsb_linear_args(_LINEAR, dt, _act(act), 0, rows, n, k, px, ldx, pw, ldw, pb, pr, ldr, py, ldy, pp, ldp)
+    _call(lib.tsb_linear, a, dev, lib.tsb_linear_workspace)
     return out
 
 
@@ -100,29 +126,40 @@ def linear_backward(dy, x, w, act="none", pre=None, need=("x", "w", "bias")):
     """(dx, dw, dbias) of linear() from dy [rows][n]; None for what `need` does not name. pre: what the forward pass
     wrote there (needed unless act is "none"). The residual's gradient is dy."""
     lib = abi.load()
-    dt = _first("dy", dy, _HALF)
-    rows, n = dy.shape
+    dt, dev = _first("dy", dy, _HALF)
+    (rows, n), t = dy.shape, dy.dtype
+    if x.dim() != 2:
+        raise ValueError("x: two dimensions are wanted, got %s" % (tuple(x.shape),))
     k = x.shape[1]
-    a = abi.tsb_linear_grad_args(C.sizeof(abi.tsb_linear_grad_args), dt, _act(act), 0, rows, n, k)
-    a.dy, a.lddy = _mat("dy", dy, rows, n, dy)
-    a.x, a.ldx = _mat("x", x, rows, k, dy)
-    a.w, a.ldw = _mat("w", w, n, k, dy)
+    a = abi.tsb_linear_grad_args(_LINEAR_GRAD, dt, _act(act), 0, rows, n, k)
+    a.dy, a.lddy = _mat("dy", dy, rows, n, t, dev)
+    a.x, a.ldx = _mat("x", x, rows, k, t, dev)
+    a.w, a.ldw = _mat("w", w, n, k, t, dev)
     if act != "none":
         if pre is None:
             raise ValueError("pre: an activation's slope needs it")
-        a.pre, a.ldp = _mat("pre", pre, rows, n, dy)
+        a.pre, a.ldp = _mat("pre", pre, rows, n, t, dev)
     dx = dw = db = None
     if "x" in need:
-        dx = torch.empty((rows, k), dtype=dy.dtype, device=dy.device)
+        dx = dy.new_empty((rows, k))
         a.dx, a.lddx = dx.data_ptr(), k
     if "w" in need:
-        dw = torch.empty((n, k), dtype=dy.dtype, device=dy.device)
+        dw = dy.new_empty((n, k))
         a.dw, a.lddw = dw.data_ptr(), k
     if "bias" in need:
-        db = torch.empty(n, dtype=dy.dtype, device=dy.device)
+        db = dy.new_empty((n,))
         a.db = db.data_ptr()
-    _call(lib.tsb_linear_backward, a, dy.device, lib.tsb_linear_backward_workspace)
+    _call(lib.tsb_linear_backward, a, dev, lib.tsb_linear_backward_workspace)
     return dx, dw, db
+
+
+def _route_call(dev, fn, *args):
+    if torch.cuda.current_device() != dev:
+        with torch.cuda.device(dev):
+            return _route_call(dev, fn, *args)
+    st = fn(*args, _raw_stream(dev))
+    if st:
+        abi.check(st)
 
 
 def route(logits, top, norm=True):
@@ -130,44 +167,34 @@ def route(logits, top, norm=True):
     first among equal ones; weights by softmax over the chosen (norm) or over the whole row. -inf and NaN are never
     chosen: a row with fewer than `top` others ends in ids -1 with weight 0."""
     lib = abi.load()
-    dt = _first("logits", logits, _ANY)
+    dt, dev = _first("logits", logits, _ANY)
     rows, experts = logits.shape
-    p, ld = _mat("logits", logits, rows, experts, logits)
-    ids = torch.empty((rows, top), dtype=torch.int32, device=logits.device)
-    weights = torch.empty((rows, top), dtype=torch.float32, device=logits.device)
-
-    def go():
-        abi.check(lib.tsb_route(dt, p, ld, rows, experts, top, 1 if norm else 0, ids.data_ptr(), weights.data_ptr(),
-                                torch.cuda.current_stream().cuda_stream))
-    _on(logits.device, go)
+    p, ld = _mat("logits", logits, rows, experts, logits.dtype, dev)
+    if not 1 <= top <= min(32, experts):
+        raise ValueError("top: must be in [1, 32] and at most the experts, got %d" % top)
+    ids = logits.new_empty((rows, top), dtype=torch.int32)
+    weights = logits.new_empty((rows, top), dtype=torch.float32)
+    _route_call(dev, lib.tsb_route, dt, p, ld, rows, experts, top, 1 if norm else 0, ids.data_ptr(),
+                weights.data_ptr())
     return ids, weights
-
-
-def _on(device, go):
-    if torch.cuda.current_device() == device.index:
-        go()
-    else:
-        with torch.cuda.device(device):
-            go()
 
 
 def route_backward(dweights, logits, ids, weights, norm=True):
     """dlogits [rows][experts] (logits' type) of route() from dweights [rows][top] and the ids and weights it gave."""
     lib = abi.load()
-    dt = _first("logits", logits, _ANY)
-    wt = _first("dweights", dweights, _ANY)
+    dt, dev = _first("logits", logits, _ANY)
+    wt, _ = _first("dweights", dweights, _ANY)
     rows, experts = logits.shape
-    top = ids.shape[1]
-    p, ld = _mat("logits", logits, rows, experts, logits)
-    d = _flat("dweights", dweights, (rows, top), dweights.dtype, logits.device)
-    i = _flat("ids", ids, (rows, top), torch.int32, logits.device)
-    w = _flat("weights", weights, (rows, top), torch.float32, logits.device)
-    out = torch.empty((rows, experts), dtype=logits.dtype, device=logits.device)
-
-    def go():
-        abi.check(lib.tsb_route_backward(dt, wt, d, p, ld, i, w, rows, experts, top, 1 if norm else 0, out.data_ptr(),
-                                         experts, torch.cuda.current_stream().cuda_stream))
-    _on(logits.device, go)
+    shape = dweights.shape
+    p, ld = _mat("logits", logits, rows, experts, logits.dtype, dev)
+    if shape[0] != rows:
+        raise ValueError("dweights: %d rows are wanted, got %d" % (rows, shape[0]))
+    d = _flat("dweights", dweights, shape, dweights.dtype, dev)
+    i = _flat("ids", ids, shape, torch.int32, dev)
+    w = _flat("weights", weights, shape, torch.float32, dev)
+    out = logits.new_empty((rows, experts))
+    _route_call(dev, lib.tsb_route_backward, dt, wt, d, p, ld, i, w, rows, experts, shape[1], 1 if norm else 0,
+                out.data_ptr(), experts)
     return out
 
 
@@ -177,23 +204,27 @@ class Units:
     slot is outside the arrays is not there: its rows contribute nothing."""
 
     def __init__(self, gate, up, down, slot_of=None):
-        _first("gate", gate[:, 0] if gate.dim() == 3 else gate, _HALF)
+        if gate.dim() != 3 or gate.dtype not in _HALF or not gate.is_cuda:
+            raise ValueError("gate: [slots][ffn][hidden] of bfloat16 or float16 on a CUDA device is wanted, got %s %s on "
+                             "%s" % (gate.dtype, tuple(gate.shape), gate.device))
         slots, ffn, hidden = gate.shape
-        self.dtype, self.device, self.hidden, self.ffn = gate.dtype, gate.device, hidden, ffn
-        self.n_units = slots if slot_of is None else slot_of.numel()
+        t, dev = gate.dtype, gate.get_device()
+        self.dtype, self.dev, self.hidden, self.ffn = t, dev, hidden, ffn
+        self.n_units = n = slots if slot_of is None else slot_of.numel()
         self.keep = (gate, up, down, slot_of)  # the tensors behind the addresses
-        s = abi.tsb_units(C.sizeof(abi.tsb_units), self.n_units, slots)
-        for i, (name, t, shape) in enumerate((("gate", gate, (slots, ffn, hidden)), ("up", up, (slots, ffn, hidden)),
-                                              ("down", down, (slots, hidden, ffn)))):
-            if t.dtype != gate.dtype or t.device != gate.device or t.shape != shape:
-                raise ValueError("%s: %s of shape %s on %s is wanted" % (name, gate.dtype, shape, gate.device))
-            if t.stride()[1:] != (shape[2], 1) or (slots > 1 and t.stride(0) < ffn * hidden):
-                raise ValueError("%s: a slot's matrix must be contiguous, and slots apart" % name)
-            s.part[i] = t.data_ptr()
-            s.stride[i] = t.stride(0) * 2
+        self.struct = s = abi.tsb_units(_UNITS, n, slots)
+        for i, (m, shape) in enumerate(((gate, (slots, ffn, hidden)), (up, (slots, ffn, hidden)),
+                                        (down, (slots, hidden, ffn)))):
+            if m.dtype is not t or m.get_device() != dev or m.shape != shape:
+                raise ValueError("%s: %s of shape %s on cuda:%d is wanted, got %s %s on %s" %
+                                 (("gate", "up", "down")[i], t, shape, dev, m.dtype, tuple(m.shape), m.device))
+            s0, s1, s2 = m.stride()
+            if not m.is_contiguous() and (s1 != shape[2] or s2 != 1 or (slots > 1 and s0 < ffn * hidden)):
+                raise ValueError("%s: a slot's matrix must be contiguous, and slots apart" % ("gate", "up", "down")[i])
+            s.part[i] = m.data_ptr()
+            s.stride[i] = s0 * 2
         if slot_of is not None:
-            s.slot_of = _flat("slot_of", slot_of, (self.n_units,), torch.int32, gate.device)
-        self.struct = s
+            s.slot_of = _flat("slot_of", slot_of, (n,), torch.int32, dev)
 
     @classmethod
     def of_context(cls, ctx, g, n_units, hidden, ffn, dtype=torch.bfloat16, device=None):
@@ -203,7 +234,7 @@ class Units:
         if dtype not in _HALF:
             raise ValueError("%s is not served" % dtype)
         self.dtype, self.hidden, self.ffn, self.n_units = dtype, hidden, ffn, n_units
-        self.device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
+        self.dev = torch.cuda.current_device() if device is None else torch.device(device).index
         self.keep, self.struct = (ctx,), abi.tsb_units()
         v = ctx.view()
         abi.check(abi.load().tsb_units_from_view(C.byref(v), g, n_units, hidden * ffn * 2, C.byref(self.struct)))
@@ -217,7 +248,7 @@ class Units:
         if dtype not in _HALF:
             raise ValueError("%s is not served" % dtype)
         self.dtype, self.hidden, self.ffn, self.n_units = dtype, hidden, ffn, n_units
-        self.device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
+        self.dev = torch.cuda.current_device() if device is None else torch.device(device).index
         self.keep = ()
         s = self.struct = abi.tsb_units(C.sizeof(abi.tsb_units), n_units, 0)
         s.table = table
@@ -226,20 +257,23 @@ class Units:
         return self
 
 
-def _ffn_args(struct, x, ids, weights, units, act):
-    dt = _first("x", x, _HALF)
+def _ffn_args(struct, size, x, ids, weights, units, act):
+    dt, dev = _first("x", x, _HALF)
     rows, hidden = x.shape
     if ids.dim() != 2:
         raise ValueError("ids: two dimensions are wanted, got %s" % (tuple(ids.shape),))
-    top = ids.shape[1]
-    if units.dtype != x.dtype or units.hidden != hidden or units.device != x.device:
-        raise ValueError("units: %s with hidden %d on %s is wanted" % (x.dtype, hidden, x.device))
-    a = struct(C.sizeof(struct), dt, _act(act), top, rows, hidden, units.ffn)
-    a.x, a.ldx = _mat("x", x, rows, hidden, x)
-    a.ids = _flat("ids", ids, (rows, top), torch.int32, x.device)
-    a.weights = _flat("weights", weights, (rows, top), torch.float32, x.device)
-    a.units = C.addressof(units.struct)
-    return a
+    shape = (rows, ids.shape[1])
+    if units.dtype is not x.dtype or units.hidden != hidden or units.dev != dev:
+        raise ValueError("units: %s with hidden %d on cuda:%d is wanted" % (x.dtype, hidden, dev))
+    px, ldx = _mat("x", x, rows, hidden, x.dtype, dev)
+    pi = _flat("ids", ids, shape, torch.int32, dev)
+    pw = _flat("weights", weights, shape, torch.float32, dev)
+    pu = C.addressof(units.struct)
+    if struct is abi.tsb_ffn_args:
+        a = struct(size, dt, _act(act), shape[1], rows, hidden, units.ffn, px, ldx, pi, pw, pu)
+    else:
+        a = struct(size, dt, _act(act), shape[1], rows, hidden, units.ffn, None, 0, px, ldx, pi, pw, pu)
+    return a, dev
 
 
 def ffn(x, ids, weights, units, act="silu", residual=None, out=None):
@@ -247,14 +281,16 @@ def ffn(x, ids, weights, units, act="silu", residual=None, out=None):
     weights float32 [rows][top]. An id outside the units (-1: a padded row) contributes nothing. out: where to write
     (may be the residual)."""
     lib = abi.load()
-    a = _ffn_args(abi.tsb_ffn_args, x, ids, weights, units, act)
+    a, dev = _ffn_args(abi.tsb_ffn_args, _FFN, x, ids, weights, units, act)
     rows, hidden = x.shape
     if residual is not None:
-        a.residual, a.ldr = _mat("residual", residual, rows, hidden, x)
+        a.residual, a.ldr = _mat("residual", residual, rows, hidden, x.dtype, dev)
     if out is None:
-        out = torch.empty((rows, hidden), dtype=x.dtype, device=x.device)
-    a.y, a.ldy = _mat("out", out, rows, hidden, x)
-    _call(lib.tsb_ffn, a, x.device, lib.tsb_ffn_workspace)
+        out = x.new_empty((rows, hidden))
+    elif out.data_ptr() != x.data_ptr() or residual is not x:  # (in place on x as its own residual: x is read first)
+        _apart("out", out, x)
+    a.y, a.ldy = _mat("out", out, rows, hidden, x.dtype, dev)
+    _call(lib.tsb_ffn, a, dev, lib.tsb_ffn_workspace)
     return out
 
 
@@ -262,21 +298,20 @@ def ffn_backward(dy, x, ids, weights, units, act="silu", need=("x", "weights", "
     """The gradients of ffn() from dy [rows][hidden] as a dict: dx, dweights [rows][top], and dgate, dup, ddown by unit
     (zeros for a unit without rows); None for what `need` ("x", "weights", "units") does not name. All of x's type."""
     lib = abi.load()
-    a = _ffn_args(abi.tsb_ffn_grad_args, x, ids, weights, units, act)
+    a, dev = _ffn_args(abi.tsb_ffn_grad_args, _FFN_GRAD, x, ids, weights, units, act)
     rows, hidden = x.shape
-    a.dy, a.lddy = _mat("dy", dy, rows, hidden, x)
-    like = dict(dtype=x.dtype, device=x.device)
+    a.dy, a.lddy = _mat("dy", dy, rows, hidden, x.dtype, dev)
     g = dict.fromkeys(("dx", "dweights", "dgate", "dup", "ddown"))
     if "x" in need:
-        g["dx"] = torch.empty((rows, hidden), **like)
+        g["dx"] = x.new_empty((rows, hidden))
         a.dx, a.lddx = g["dx"].data_ptr(), hidden
     if "weights" in need:
-        g["dweights"] = torch.empty(tuple(ids.shape), **like)
+        g["dweights"] = x.new_empty(tuple(ids.shape))
         a.dweights = g["dweights"].data_ptr()
     if "units" in need:
-        g["dgate"] = torch.empty((units.n_units, units.ffn, hidden), **like)
-        g["dup"] = torch.empty((units.n_units, units.ffn, hidden), **like)
-        g["ddown"] = torch.empty((units.n_units, hidden, units.ffn), **like)
+        g["dgate"] = x.new_empty((units.n_units, units.ffn, hidden))
+        g["dup"] = x.new_empty((units.n_units, units.ffn, hidden))
+        g["ddown"] = x.new_empty((units.n_units, hidden, units.ffn))
         a.dgate, a.dup, a.ddown = (g[k].data_ptr() for k in ("dgate", "dup", "ddown"))
-    _call(lib.tsb_ffn_backward, a, x.device, lib.tsb_ffn_backward_workspace)
+    _call(lib.tsb_ffn_backward, a, dev, lib.tsb_ffn_backward_workspace)
     return g
