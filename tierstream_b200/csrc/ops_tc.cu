@@ -28,7 +28,7 @@ constexpr int kBM = 128, kBK = 64;  // (a CTA's rows)
 constexpr int kABytes = kBM * kBK * 2, kRingBytes = 192 << 10;  // the stages'
 constexpr int kMaxStages = 12;
 constexpr int kEpiWarps = 8, kThreads = 128 + 32 * kEpiWarps;
-constexpr int kRowBytes = 80, kStoreBytes = 32 * kRowBytes;  // a warp's 32 rows of 64 bytes, 16 apart: no bank twice
+constexpr int kRowBytes = 64, kStoreBytes = 2 * 32 * kRowBytes;  // a warp's two buffers of 32 rows x 64 bytes
 constexpr int kSmemBytes = 1024 + kRingBytes + kEpiWarps * kStoreBytes + 256;
 constexpr unsigned long long kWaitNs = 2000000000ull;
 
@@ -43,12 +43,12 @@ struct Params {
   int32_t n_tiles;   // tiles along n
   int32_t m_tiles;   // tiles along m when not grouped
   int32_t k_blocks;  // of a segment; with k_rows per unit: from the group
-  int32_t vec;       // 16-byte stores are possible
+  int32_t vec;       // 16-byte stores are possible: `out` maps are made
   int32_t stages, stage_bytes;
   int32_t pair;      // two CTAs to a tile of 256 rows
 };
 struct Maps {
-  CUtensorMap a[2], b[3];
+  CUtensorMap a[2], b[3], out[3];
 };
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return uint32_t(__cvta_generic_to_shared(p)); }
@@ -228,10 +228,11 @@ struct Traits {
   static constexpr bool grouped = MODE == kUp || MODE == kUpBack || MODE == kDown || MODE == kDx;
   static constexpr int segs = MODE == kUpBack || MODE == kDx ? 2 : 1;
   static constexpr bool a_mn = MODE == kLinDw || MODE == kDw;
-  static constexpr bool pair0 = MODE == kUp || MODE == kUpBack;  // segment 0's B: columns of gate, then of up
+  // the segment whose B is columns of gate, then of up (the last: in the backward pass dh comes first)
+  __host__ __device__ static constexpr bool both(int s) { return (MODE == kUp && s == 0) || (MODE == kUpBack && s == 1); }
   // B of segment s with n contiguous
   __host__ __device__ static constexpr bool b_mn(int s) {
-    return MODE == kLinDx || MODE == kLinDw || MODE == kDx || MODE == kDw || (MODE == kUpBack && s == 1);
+    return MODE == kLinDx || MODE == kLinDw || MODE == kDx || MODE == kDw || (MODE == kUpBack && s == 0);
   }
   static constexpr int bufs = MODE == kUpBack ? 1 : 2;
 };
@@ -244,33 +245,63 @@ __device__ __forceinline__ uint32_t pack(float a, float b) {
   return r;
 }
 
-// A warp's 32 rows x 64 bytes (thread = row) written along rows: 8 rows of 64 bytes a store. `cols` elements of E bytes
-// are inside the matrix; vec: 16-byte stores fit.
+// A warp's 32 rows x 64 bytes (thread = row) on their way out: into one of its two buffers in shared memory, 64-byte
+// swizzled so that no bank is met twice, and from there by a TMA store that runs while the next block is computed. Blocks
+// at an edge that TMA must not cross (the rows behind a group's end, columns of the next tile) and outputs whose rows do
+// not start on 16 bytes are written along rows by the lanes instead.
+struct Out {
+  const CUtensorMap* map;
+  int z;  // the unit
+  char* buf;
+  uint32_t flip;
+  bool tma;
+};
+// E out[rows][cols] from row `y`, column `x` of the map; `p` is its address
 template <class E>
-__device__ __forceinline__ void store_rows(char* stage, const uint32_t (&v)[16], E* out, int64_t ld, int rows, int cols,
-                                           bool vec) {
+__device__ __forceinline__ void store_rows(Out& o, int which, const uint32_t (&v)[16], int64_t x, int64_t y, E* p,
+                                           int64_t ld, int rows, int cols, bool whole) {
   const int lane = threadIdx.x & 31;
   constexpr int kPer = 16 / int(sizeof(E));
-  uint4* mine = reinterpret_cast<uint4*>(stage + lane * kRowBytes);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) mine[i] = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+  char* stage = o.buf + (o.flip & 1u) * (32 * kRowBytes);
+  o.flip ^= 1u;
+  if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");  // the store before the last has read
   __syncwarp();
-  const int c = (lane & 3) * kPer;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int r = i * 8 + (lane >> 2);
-    const uint4 w = *reinterpret_cast<const uint4*>(stage + r * kRowBytes + (lane & 3) * 16);
-    if (r >= rows) continue;
-    if (vec && c + kPer <= cols) {
-      *reinterpret_cast<uint4*>(out + r * ld + c) = w;
-    } else {
-      E e[kPer];
-      memcpy(e, &w, 16);
-#pragma unroll
-      for (int j = 0; j < kPer; ++j)
-        if (c + j < cols) out[r * ld + c + j] = e[j];
+  for (int i = 0; i < 4; ++i)
+    *reinterpret_cast<uint4*>(stage + lane * kRowBytes + ((i ^ ((lane >> 1) & 3)) * 16)) =
+        make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+  if (o.tma && whole) {
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    __syncwarp();
+    if (lane == 0) {
+      asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%1, %2, %3}], [%4];" ::"l"(o.map + which),
+                   "r"(int(x)), "r"(int(y)), "r"(o.z), "r"(smem_u32(stage))
+                   : "memory");
     }
+  } else {
+    __syncwarp();
+    const int c = (lane & 3) * kPer;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = i * 8 + (lane >> 2);
+      const uint4 w = *reinterpret_cast<const uint4*>(stage + r * kRowBytes + (((lane & 3) ^ ((r >> 1) & 3)) * 16));
+      if (r >= rows) continue;
+      if (o.tma && c + kPer <= cols) {
+        *reinterpret_cast<uint4*>(p + r * ld + c) = w;
+      } else {
+        E e[kPer];
+        memcpy(e, &w, 16);
+#pragma unroll
+        for (int j = 0; j < kPer; ++j)
+          if (c + j < cols) p[r * ld + c + j] = e[j];
+      }
+    }
+    __syncwarp();
   }
+  if (lane == 0) asm volatile("cp.async.bulk.commit_group;" ::: "memory");  // (an empty group keeps the count)
+}
+__device__ __forceinline__ void stores_done() {
+  if ((threadIdx.x & 31) == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
   __syncwarp();
 }
 
@@ -287,8 +318,15 @@ __device__ __forceinline__ void read32(T (&v)[32], const T* p, int cols, bool wh
   }
 }
 
+// 32 columns of sums, 16 at a time (bn is a multiple of 16: the second half of a last odd block is loaded twice and not
+// stored)
+__device__ __forceinline__ void sums32(uint32_t base, int c, int bn, float (&v)[2][16]) {
+  tmem_ld16(base + c, v[0]);
+  tmem_ld16(base + min(c + 16, bn - 16), v[1]);
+}
+
 template <class T, int MODE, int ACT>
-__device__ __forceinline__ void epilogue(const Params& q, const Tile& t, uint32_t tmem, char* stage, int warp) {
+__device__ __forceinline__ void epilogue(const Params& q, const Tile& t, uint32_t tmem, uint32_t tmem_dh, Out& o, int warp) {
   const Product& p = q.p;
   const int lane = threadIdx.x & 31, quad = warp & 3, half = warp >> 2;
   const uint32_t base = tmem + (uint32_t(quad * 32) << 16);
@@ -297,96 +335,95 @@ __device__ __forceinline__ void epilogue(const Params& q, const Tile& t, uint32_
   const int64_t n0 = int64_t(t.n) * q.bn;
   const int cols = int(min(int64_t(q.bn), p.n - n0));  // columns of this tile inside the matrix
   const bool zero = MODE == kDw && t.kb == 0;          // a unit without rows: nothing was computed
+  // TMA clips at the matrix' edges: a block is whole unless it crosses its group's rows or its tile's columns
+  const bool whole_rows = rows == 32 || (!Traits<MODE>::grouped && rows > 0);
+  const int64_t y = int64_t(t.row0) + m;
+  o.z = MODE == kDw ? t.unit : 0;
   if constexpr (MODE == kUp || MODE == kUpBack) {
     float w = 0.f, dw = 0.f;
-    const int64_t row = int64_t(t.row0) + m + lane;
-    if (MODE == kUpBack && lane < rows && m + lane < t.rows) w = p.weights[q.plan.pair_of_row[row]];
-    for (int c = half * 32; c < q.bn; c += 64) {
+    if (MODE == kUpBack && lane < rows && m + lane < t.rows) w = p.weights[q.plan.pair_of_row[y + lane]];
+    for (int c = half * 32; c < cols; c += 64) {
       uint32_t h[16], d1[16], d2[16];
+      float g[2][16], u[2][16], d[2][16];
+      sums32(base, c, q.bn, g);
+      sums32(base + q.bn, c, q.bn, u);
+      if constexpr (MODE == kUpBack) sums32(tmem_dh + (uint32_t(quad * 32) << 16), c, q.bn, d);
+      tmem_wait_ld();
 #pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        float g[16], u[16], d[16];
-        const int cc = min(c + 16 * s, q.bn - 16);  // (bn is a multiple of 16: an odd half is loaded twice, not stored)
-        tmem_ld16(base + cc, g);
-        tmem_ld16(base + q.bn + cc, u);
-        if constexpr (MODE == kUpBack) tmem_ld16(base + 256 + cc, d);
-        tmem_wait_ld();
-        const bool in = c + 16 * s < q.bn;
+      for (int s = 0; s < 2; ++s)
 #pragma unroll
         for (int i = 0; i < 16; i += 2) {
-          float k0 = act_of<ACT>(g[i]), k1 = act_of<ACT>(g[i + 1]);
+          const float k0 = act_of<ACT>(g[s][i]), k1 = act_of<ACT>(g[s][i + 1]), u0 = u[s][i], u1 = u[s][i + 1];
           if constexpr (MODE == kUp) {
-            h[s * 8 + i / 2] = pack<T>(k0 * u[i], k1 * u[i + 1]);
+            h[s * 8 + i / 2] = pack<T>(k0 * u0, k1 * u1);
           } else {
-            h[s * 8 + i / 2] = pack<T>(w * k0 * u[i], w * k1 * u[i + 1]);
-            d1[s * 8 + i / 2] = pack<T>(w * d[i] * u[i] * slope_of<ACT>(g[i]), w * d[i + 1] * u[i + 1] * slope_of<ACT>(g[i + 1]));
-            d2[s * 8 + i / 2] = pack<T>(w * d[i] * k0, w * d[i + 1] * k1);
-            if (in && c + 16 * s + i < cols) dw += d[i] * k0 * u[i];
-            if (in && c + 16 * s + i + 1 < cols) dw += d[i + 1] * k1 * u[i + 1];
+            const float e0 = d[s][i], e1 = d[s][i + 1];
+            h[s * 8 + i / 2] = pack<T>(w * k0 * u0, w * k1 * u1);
+            d1[s * 8 + i / 2] = pack<T>(w * e0 * u0 * slope_of<ACT>(g[s][i]), w * e1 * u1 * slope_of<ACT>(g[s][i + 1]));
+            d2[s * 8 + i / 2] = pack<T>(w * e0 * k0, w * e1 * k1);
+            if (c + 16 * s + i < cols) dw += e0 * k0 * u0;
+            if (c + 16 * s + i + 1 < cols) dw += e1 * k1 * u1;
           }
         }
-      }
-      const int64_t at = (int64_t(t.row0) + m) * p.ldo + n0 + c;
+      const int64_t at = y * p.ldo + n0 + c;
+      const bool whole = whole_rows && c + 32 <= q.bn;
       if constexpr (MODE == kUp) {
-        store_rows<T>(stage, h, static_cast<T*>(p.out) + at, p.ldo, rows, cols - c, q.vec);
+        store_rows<T>(o, 0, h, n0 + c, y, static_cast<T*>(p.out) + at, p.ldo, rows, cols - c, whole);
       } else {
-        store_rows<T>(stage, d1, static_cast<T*>(p.dg) + at, p.ldo, rows, cols - c, q.vec);
-        store_rows<T>(stage, d2, static_cast<T*>(p.du) + at, p.ldo, rows, cols - c, q.vec);
-        if (p.hw) store_rows<T>(stage, h, static_cast<T*>(p.hw) + at, p.ldo, rows, cols - c, q.vec);
+        store_rows<T>(o, 0, d1, n0 + c, y, static_cast<T*>(p.dg) + at, p.ldo, rows, cols - c, whole);
+        store_rows<T>(o, 1, d2, n0 + c, y, static_cast<T*>(p.du) + at, p.ldo, rows, cols - c, whole);
+        if (p.hw) store_rows<T>(o, 2, h, n0 + c, y, static_cast<T*>(p.hw) + at, p.ldo, rows, cols - c, whole);
       }
     }
-    if (MODE == kUpBack && p.dwp && lane < rows && m + lane < t.rows) p.dwp[row * p.ld_dwp + 2 * t.n + half] = dw;
+    if (MODE == kUpBack && p.dwp && lane < rows && m + lane < t.rows) p.dwp[(y + lane) * p.ld_dwp + 2 * t.n + half] = dw;
   } else if constexpr (MODE == kDown || MODE == kDx) {
-    for (int c = half * 16; c < q.bn; c += 32) {
+    for (int c = half * 16; c < cols; c += 32) {
       float v[16];
       tmem_ld16(base + c, v);
       tmem_wait_ld();
       uint32_t b[16];
 #pragma unroll
       for (int i = 0; i < 16; ++i) b[i] = __float_as_uint(v[i]);
-      store_rows<float>(stage, b, p.rows32 + (int64_t(t.row0) + m) * p.n + n0 + c, p.n, min(rows, t.rows - m), cols - c,
-                        true);
+      store_rows<float>(o, 0, b, n0 + c, y, p.rows32 + y * p.n + n0 + c, p.n, rows, cols - c, whole_rows);
     }
   } else if constexpr (MODE == kLin) {
-    const int64_t row = m + lane;
-    const T *bias = static_cast<const T*>(p.bias), *res = static_cast<const T*>(p.residual) + row * p.ldr;
-    for (int c = half * 32; c < q.bn; c += 64) {
+    const T *bias = static_cast<const T*>(p.bias), *res = static_cast<const T*>(p.residual) + (m + lane) * p.ldr;
+    for (int c = half * 32; c < cols; c += 64) {
       const int64_t n = n0 + c;
-      const bool whole = q.vec && c + 32 <= cols;
+      const bool inside = q.vec && c + 32 <= cols;
       T b[32] = {}, r[32] = {};
-      if (bias) read32(b, bias + n, cols - c, whole);
-      if (p.residual && lane < rows) read32(r, res + n, cols - c, whole);
-      uint32_t y[16], pre[16];
+      if (bias) read32(b, bias + n, cols - c, inside);
+      if (p.residual && lane < rows) read32(r, res + n, cols - c, inside);
+      uint32_t out[16], pre[16];
+      float v[2][16];
+      sums32(base, c, q.bn, v);
+      tmem_wait_ld();
 #pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        float v[16];
-        tmem_ld16(base + min(c + 16 * s, q.bn - 16), v);
-        tmem_wait_ld();
+      for (int s = 0; s < 2; ++s)
 #pragma unroll
         for (int i = 0; i < 16; i += 2) {
-          const float z0 = v[i] + to_f(b[16 * s + i]), z1 = v[i + 1] + to_f(b[16 * s + i + 1]);
+          const float z0 = v[s][i] + to_f(b[16 * s + i]), z1 = v[s][i + 1] + to_f(b[16 * s + i + 1]);
           pre[8 * s + i / 2] = pack<T>(z0, z1);
-          y[8 * s + i / 2] = pack<T>(act_of<ACT>(z0) + to_f(r[16 * s + i]), act_of<ACT>(z1) + to_f(r[16 * s + i + 1]));
+          out[8 * s + i / 2] = pack<T>(act_of<ACT>(z0) + to_f(r[16 * s + i]), act_of<ACT>(z1) + to_f(r[16 * s + i + 1]));
         }
-      }
-      store_rows<T>(stage, y, static_cast<T*>(p.out) + m * p.ldo + n, p.ldo, rows, cols - c, q.vec);
-      if (p.pre) store_rows<T>(stage, pre, static_cast<T*>(p.pre) + m * p.ldp + n, p.ldp, rows, cols - c, q.vec);
+      const bool whole = whole_rows && c + 32 <= q.bn;
+      store_rows<T>(o, 0, out, n, y, static_cast<T*>(p.out) + m * p.ldo + n, p.ldo, rows, cols - c, whole);
+      if (p.pre) store_rows<T>(o, 1, pre, n, y, static_cast<T*>(p.pre) + m * p.ldp + n, p.ldp, rows, cols - c, whole);
     }
   } else {  // gradients: rounded once
     T* out = static_cast<T*>(p.out) + int64_t(t.unit) * p.out_unit + m * p.ldo + n0;
-    for (int c = half * 32; c < q.bn; c += 64) {
+    for (int c = half * 32; c < cols; c += 64) {
       uint32_t h[16] = {};
       if (!zero) {
+        float v[2][16];
+        sums32(base, c, q.bn, v);
+        tmem_wait_ld();
 #pragma unroll
-        for (int s = 0; s < 2; ++s) {
-          float v[16];
-          tmem_ld16(base + min(c + 16 * s, q.bn - 16), v);
-          tmem_wait_ld();
+        for (int s = 0; s < 2; ++s)
 #pragma unroll
-          for (int i = 0; i < 16; i += 2) h[s * 8 + i / 2] = pack<T>(v[i], v[i + 1]);
-        }
+          for (int i = 0; i < 16; i += 2) h[s * 8 + i / 2] = pack<T>(v[s][i], v[s][i + 1]);
       }
-      store_rows<T>(stage, h, out + c, p.ldo, rows, min(cols, q.bn) - c, q.vec);
+      store_rows<T>(o, 0, h, n0 + c, MODE == kDw ? m : y, out + c, p.ldo, rows, cols - c, whole_rows && c + 32 <= q.bn);
     }
   }
 }
@@ -447,10 +484,10 @@ __global__ __launch_bounds__(kThreads, 1) void tc_kernel(const __grid_constant__
       t.m0 += int(rank) * kBM;
 #pragma unroll
       for (int s = 0; s < X::segs; ++s) {
-        const bool pair = X::pair0 && s == 0;
+        const bool pair = X::both(s);
         const uint32_t bytes = kABytes + (X::b_mn(s) ? chunks * 8192 : pair ? 2 / CG * q.bn * 128 : half_n * 128);
-        const CUtensorMap* ma = &maps.a[s];
-        const CUtensorMap* mb = &maps.b[MODE == kUpBack && s == 1 ? 2 : pair && CG == 2 ? rank : s];
+        const CUtensorMap* ma = &maps.a[MODE == kUpBack ? 1 - s : s];
+        const CUtensorMap* mb = &maps.b[MODE == kUpBack && s == 0 ? 2 : pair ? (CG == 2 ? rank : 0) : s];
         const int z = X::grouped ? t.slot : 0, n0 = t.n * q.bn + (pair ? 0 : int(rank) * half_n);
         const int m0 = X::a_mn ? t.m0 : t.row0 + t.m0;
         int k0 = 0, krow = MODE == kDw ? t.row0 : 0;
@@ -492,16 +529,19 @@ __global__ __launch_bounds__(kThreads, 1) void tc_kernel(const __grid_constant__
     constexpr uint32_t type = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
     for (int L = first; ok && tile_at<MODE, CG>(q, L, t); L += stride, ++nt) {
       const int buf = nt % X::bufs;
-      ok = bar_wait(sums_empty + 8 * buf, ((nt / X::bufs) & 1) ^ 1, dead);
-      if (!ok) break;
-      fence_after();
 #pragma unroll
       for (int s = 0; s < X::segs; ++s) {
-        const int n = X::pair0 && s == 0 ? 2 * q.bn : q.bn;
+        // (dh of tile nt goes where tile nt - 2 had its own: read before tile nt - 1's gate and up could start)
+        if (s == X::segs - 1 || !(MODE == kUpBack)) {
+          ok = ok && bar_wait(sums_empty + 8 * buf, ((nt / X::bufs) & 1) ^ 1, dead);
+          if (!ok) break;
+        }
+        fence_after();
+        const int n = X::both(s) ? 2 * q.bn : q.bn;
         const uint32_t idesc = (1u << 4) | (type << 7) | (type << 10) | (uint32_t(X::a_mn) << 15) |
                                (uint32_t(X::b_mn(s)) << 16) | (uint32_t(n >> 3) << 17) |
                                (uint32_t(CG * kBM >> 4) << 24);
-        const uint32_t d = tmem + buf * 256 + (MODE == kUpBack && s == 1 ? 256 : 0);
+        const uint32_t d = tmem + (MODE == kUpBack && s == 0 ? 256 + 128 * (nt & 1) : buf * 256);
         const bool fresh = !(MODE == kDx && s == 1);  // dx: both segments add into the same sums
         const uint64_t ring_b = desc(smem_u32(smem) + kABytes, X::b_mn(s));
         for (int kb = 0; kb < t.kb; ++kb) {
@@ -530,13 +570,14 @@ __global__ __launch_bounds__(kThreads, 1) void tc_kernel(const __grid_constant__
   } else if (warp >= 4) {  // the epilogue
     uint32_t nt = 0;
     Tile t;
+    Out out{maps.out, 0, store + (warp - 4) * kStoreBytes, 0, q.vec != 0};
     for (int L = first; tile_at<MODE, CG>(q, L, t); L += stride, ++nt) {
       t.m0 += int(rank) * kBM;
       const int buf = nt % X::bufs;
       if (!bar_wait(sums_full + 8 * buf, (nt / X::bufs) & 1, dead)) break;
       __syncwarp();
       fence_after();
-      epilogue<T, MODE, ACT>(q, t, tmem + buf * 256, store + (warp - 4) * kStoreBytes, warp - 4);
+      epilogue<T, MODE, ACT>(q, t, tmem + buf * 256, tmem + 256 + 128 * (nt & 1), out, warp - 4);
       fence_before();
       __syncwarp();
       if ((threadIdx.x & 31) == 0) {
@@ -544,6 +585,7 @@ __global__ __launch_bounds__(kThreads, 1) void tc_kernel(const __grid_constant__
         else bar_arrive(sums_empty + 8 * buf);
       }
     }
+    stores_done();
   }
   fence_before();
   __syncthreads();
@@ -583,14 +625,18 @@ Encode encoder() {
   return e;
 }
 
-// [slots][rows][cols] of 16-bit elements, boxes of 64 columns (128 swizzled bytes) x box_rows
+// [slots][rows][cols], boxes of box_rows rows of 128 (an output: 64) swizzled bytes
 bool make_map(CUtensorMap* m, int dtype, const void* p, uint64_t cols, uint64_t rows, uint64_t ld, uint64_t slots,
-              uint64_t slot_bytes, uint32_t box_rows) {
-  const cuuint64_t dims[3] = {cols, rows, slots}, strides[2] = {ld * 2, slots > 1 ? slot_bytes : ld * 2};
-  const cuuint32_t box[3] = {64, box_rows, 1}, one[3] = {1, 1, 1};
-  return encoder()(m, dtype == TSB_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
-                   const_cast<void*>(p), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              uint64_t slot_bytes, uint32_t box_rows, bool out = false) {
+  const uint32_t size = dtype == TSB_F32 ? 4 : 2;
+  const cuuint64_t dims[3] = {cols, rows, slots}, strides[2] = {ld * size, slots > 1 ? slot_bytes : ld * size};
+  const cuuint32_t box[3] = {(out ? 64 : 128) / size, box_rows, 1}, one[3] = {1, 1, 1};
+  return encoder()(m,
+                   dtype == TSB_BF16  ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                   : dtype == TSB_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                      : CU_TENSOR_MAP_DATA_TYPE_FLOAT32,
+                   3, const_cast<void*>(p), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                   out ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
@@ -707,7 +753,7 @@ int launch_tc(int dtype, const Product& p, const Plan* plan, const Units* u, cud
   const int64_t step = 16 * cg;  // a product's columns: whole 16 for one CTA, 32 for a pair
   if (q.bn > (p.n + step - 1) / step * step) q.bn = int((p.n + step - 1) / step * step);
   q.n_tiles = int(ceil_div(uint64_t(p.n), uint64_t(q.bn)));
-  q.vec = p.epi == kEpiRows32 ||
+  q.vec = (p.epi == kEpiRows32 && p.n % 4 == 0) ||
           (p.epi == kEpiUpBack ? on16(p.dg) && on16(p.du) && on16(p.hw) && p.ldo % 8 == 0
                                : on16(p.out) && p.ldo % 8 == 0 && p.out_unit % 8 == 0 &&
                                      on16(p.bias) && on16(p.residual) && p.ldr % 8 == 0 && on16(p.pre) &&
@@ -739,6 +785,17 @@ int launch_tc(int dtype, const Product& p, const Plan* plan, const Units* u, cud
         !make_map(&maps.b[i], dtype, b.p, b.cols, b.rows, b.ld, b.slots, b.slot_bytes,
                   p.b[i].s_k == 1 ? uint32_t(narrow ? q.bn : q.bn / cg) : 64))
       return int(cudaErrorInvalidValue);
+  }
+  if (q.vec) {  // where the results go, by TMA
+    const uint64_t rows = uint64_t(p.grouped ? plan->max_rows : p.m), n = uint64_t(p.n);
+    void* const outs[3] = {p.epi == kEpiRows32 ? p.rows32 : p.epi == kEpiUpBack ? p.dg : p.out,
+                           p.epi == kEpiUpBack ? p.du : p.pre, p.hw};
+    const uint64_t lds[3] = {uint64_t(p.epi == kEpiRows32 ? p.n : p.ldo), uint64_t(p.epi == kEpiUpBack ? p.ldo : p.ldp),
+                             uint64_t(p.ldo)};
+    for (int i = 0; i < 3; ++i)
+      if (outs[i] && !make_map(&maps.out[i], p.epi == kEpiRows32 ? TSB_F32 : dtype, outs[i], n, rows, lds[i],
+                               p.per_unit ? plan->units : 1, uint64_t(p.out_unit) * 2, 32, true))
+        return int(cudaErrorInvalidValue);
   }
   // as many stages as the ring holds: narrow tiles are bound by the loads' latency
   const int b_cols = (narrow && cg == 1 ? 2 : 1) * (narrow ? q.bn : q.bn / cg);
