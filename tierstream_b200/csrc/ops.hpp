@@ -31,15 +31,15 @@ struct Units {
 // The (row, choice) pairs grouped by unit, built on the device by launch_plan: unit e's pairs, in ascending order, are
 // rows [off[e], off[e] + cnt[e]) of every grouped buffer; rows up to the next multiple of `pad` have no pair (-1).
 struct Plan {
-  int32_t* head;  // [0] tiles, [1] grouped rows (padding included)
+  int32_t* head;  // [0] tiles of `bm` rows, [1] grouped rows (padding included), [2] tiles of 2 `bm` rows
   int32_t* cnt;
   int32_t* off;
   int32_t* slot;
   int32_t* pair_of_row;
   int32_t* row_of_pair;
-  int32_t* tile_unit;  // tiles of `bm` rows, group by group
-  int32_t* tile_m0;    // the tile's first row inside its group
-  int4* tile_info;     // per tile up to max_tiles: slot, first grouped row, rows (0: no such tile), unit
+  int32_t* tile_unit[2];  // tiles of `bm` and of 2 `bm` rows, group by group
+  int32_t* tile_m0[2];    // the tile's first row inside its group
+  int4* tile_info;        // per tile of `bm` rows up to max_tiles: slot, first grouped row, rows (0: no such tile), unit
   uint32_t units, pairs, max_rows, max_tiles, pad, bm;
 };
 
@@ -189,13 +189,18 @@ int launch_tile(int dtype, const Product& p, const Plan* plan, const Units* unit
 constexpr uint32_t kStreamTile = 8;
 int launch_stream(int dtype, const Product& p, uint32_t top, const Plan* plan, const Units* units, cudaStream_t s);
 
-// ops_tc.cu: products of many rows on tcgen05 (the plan made with bm = kTcRows, or twice that: pairs of CTAs). tc_fits: TMA can read the operand.
+// ops_tc.cu: products of many rows on tcgen05; grouped ones take tiles of kTcRows rows (the plan's bm). tc_fits: TMA can read the operand.
 // Gathered operands are gathered first: launch_gather copies n columns of every grouped row (n a multiple of 8).
-constexpr uint32_t kTcRows = 128;
+constexpr uint32_t kTcRows = 256;
 bool tc_fits(const Operand& o, const Units* units);
 int launch_gather(const Plan& plan, uint32_t top, const void* src, uint64_t ld, uint64_t n, void* dst, cudaStream_t s);
 int launch_tc(int dtype, const Product& p, const Plan* plan, const Units* units, cudaStream_t s);
 int ops_take_timeouts(uint32_t* out);
+
+// ops_group.cu: the grouped products with the unit's matrix as rows, for groups of any length (the plan's bm kGroupRows)
+constexpr uint32_t kGroupRows = 128;
+int launch_group(int dtype, const Product& p, const Plan* plan, const Units* units, cudaStream_t s);
+int group_take_timeouts(uint32_t* out);
 
 }  // namespace ops
 }  // namespace tsb

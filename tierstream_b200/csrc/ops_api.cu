@@ -228,9 +228,12 @@ bool ffn_rows16(const tsb_units* u, uint64_t hidden, uint64_t ffn, const void* x
   return true;
 }
 
-// Rows of a tile on the tensor cores' own path: a group wastes half a tile on average, so pairs of CTAs (256 rows) pay
-// only for long groups (their products run at 1540 TFLOP/s against 1456 with single CTAs).
-uint32_t tc_tile(uint64_t each) { return each >= 8 * kTcRows ? 2 * kTcRows : kTcRows; }
+// On the tensor cores' own path a unit's matrix supplies the rows and the group's rows the columns, except for groups so
+// long that whole 256-row tiles waste little of them.
+uint32_t tc_tile(uint64_t each) { return each >= 4 * kTcRows ? kTcRows : kGroupRows; }
+int launch_grouped(int dtype, const Product& p, const Plan* plan, const Units* u, cudaStream_t s) {
+  return p.grouped && plan->bm == kGroupRows ? launch_group(dtype, p, plan, u, s) : launch_tc(dtype, p, plan, u, s);
+}
 
 struct FfnSpace {
   Plan plan;
@@ -290,7 +293,7 @@ void ffn(const tsb_ffn_args* a) {
   p.out = w.h, p.ldo = f;
   const auto go = [&](int dtype, const Product& pr, const Plan* pl, const Units* un, cudaStream_t st) {
     return w.stream ? launch_stream(dtype, pr, a->top, pl, un, st)
-           : w.tc   ? launch_tc(dtype, pr, pl, un, st)
+           : w.tc   ? launch_grouped(dtype, pr, pl, un, st)
                     : launch_tile(dtype, pr, pl, un, st);
   };
   if (w.tc) {
@@ -336,7 +339,7 @@ FfnBackSpace ffn_back_space(const tsb_ffn_grad_args* a) {
   r.dg = w.take(uint64_t(r.plan.max_rows) * a->ffn * 2);
   r.du = w.take(uint64_t(r.plan.max_rows) * a->ffn * 2);
   if (a->dgate) r.hw = w.take(uint64_t(r.plan.max_rows) * a->ffn * 2);
-  r.dw_tiles = r.tc ? 2 * uint32_t(ceil_div(a->ffn, 128)) : uint32_t(ceil_div(a->ffn, kTileN));
+  r.dw_tiles = r.tc ? (bm == kGroupRows ? 8 * uint32_t(ceil_div(a->ffn, 256)) : 2 * uint32_t(ceil_div(a->ffn, 128))) : uint32_t(ceil_div(a->ffn, kTileN));
   if (a->dweights) r.dwp = static_cast<float*>(w.take(uint64_t(r.plan.max_rows) * r.dw_tiles * 4));
   if (a->dx) r.rows32 = static_cast<float*>(w.take(uint64_t(r.plan.max_rows) * a->hidden * 4));
   r.bytes = w.used;
@@ -370,7 +373,7 @@ void ffn_back(const tsb_ffn_grad_args* a) {
   const Units u = units_of(a->units);
   const int dt = int(a->dtype);
   ck(launch_plan(w.plan, u, a->ids, s), fn, "plan");
-  const auto go = w.tc ? launch_tc : launch_tile;
+  const auto go = w.tc ? launch_grouped : launch_tile;
   Operand x_rows = gathered(a->x, int64_t(a->ldx), 1, w.plan, a->top),
           dy_rows = gathered(a->dy, int64_t(a->lddy), 1, w.plan, a->top),
           x_sum = gathered(a->x, 1, int64_t(a->ldx), w.plan, a->top, 1),
@@ -534,8 +537,9 @@ ss_status tsb_ffn_backward(const tsb_ffn_grad_args* a) {
 }
 
 int tsb_ops_timeouts(void) {
-  uint32_t v = 0;
-  return ops_take_timeouts(&v) == 0 ? int(v) : -1;
+  uint32_t v = 0, w = 0;
+  const int a = ops_take_timeouts(&v), b = group_take_timeouts(&w);
+  return a == 0 && b == 0 ? int(v + w) : -1;
 }
 
 }  // extern "C"

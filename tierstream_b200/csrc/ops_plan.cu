@@ -56,27 +56,35 @@ __global__ __launch_bounds__(kPlanThreads) void plan_fill_kernel(const __grid_co
   __shared__ int red[kPlanThreads / 32];
   __shared__ int warp_n[kPlanThreads / 32];
   const uint32_t e = blockIdx.x;
-  int rows = 0, tiles = 0;
+  int rows = 0, tiles = 0, twice = 0;
   for (uint32_t j = threadIdx.x; j < e; j += kPlanThreads) {
     const int c = p.cnt[j];
     rows += (c + int(p.pad) - 1) / int(p.pad) * int(p.pad);
     tiles += (c + int(p.bm) - 1) / int(p.bm);
+    twice += (c + 2 * int(p.bm) - 1) / (2 * int(p.bm));
   }
   rows = block_sum(rows, red);
   tiles = block_sum(tiles, red);
+  twice = block_sum(twice, red);
   const int cnt = p.cnt[e];
-  const int padded = (cnt + int(p.pad) - 1) / int(p.pad) * int(p.pad), mine = (cnt + int(p.bm) - 1) / int(p.bm);
+  const int padded = (cnt + int(p.pad) - 1) / int(p.pad) * int(p.pad), mine = (cnt + int(p.bm) - 1) / int(p.bm),
+            mine2 = (mine + 1) / 2;
   if (threadIdx.x == 0) {
     p.off[e] = rows;
     if (e + 1 == p.units) {
       p.head[0] = tiles + mine;
       p.head[1] = rows + padded;
+      p.head[2] = twice + mine2;
     }
   }
   for (int i = threadIdx.x; i < mine; i += kPlanThreads) {
-    p.tile_unit[tiles + i] = int32_t(e);
-    p.tile_m0[tiles + i] = i * int(p.bm);
+    p.tile_unit[0][tiles + i] = int32_t(e);
+    p.tile_m0[0][tiles + i] = i * int(p.bm);
     p.tile_info[tiles + i] = make_int4(p.slot[e], rows + i * int(p.bm), min(int(p.bm), cnt - i * int(p.bm)), int32_t(e));
+  }
+  for (int i = threadIdx.x; i < mine2; i += kPlanThreads) {
+    p.tile_unit[1][twice + i] = int32_t(e);
+    p.tile_m0[1][twice + i] = i * 2 * int(p.bm);
   }
   if (e + 1 == p.units)
     for (uint32_t i = tiles + mine + threadIdx.x; i < p.max_tiles; i += kPlanThreads)
@@ -115,7 +123,7 @@ __global__ __launch_bounds__(kSmallThreads) void plan_small_kernel(const __grid_
                                                                    const int32_t* __restrict__ ids) {
   __shared__ int32_t id[kSmallPairs];
   __shared__ int32_t cnt[kSmallUnits], rows[kSmallUnits], tiles[kSmallUnits];
-  __shared__ int32_t wr[32], wt[32];
+  __shared__ int32_t wr[32], wt[32], wd[32];
   const uint32_t t = threadIdx.x;
   const int lane = t & 31, warp = t >> 5;
   cnt[t] = 0;
@@ -138,14 +146,16 @@ __global__ __launch_bounds__(kSmallThreads) void plan_small_kernel(const __grid_
   __syncthreads();
   const int c = t < p.units ? cnt[t] : 0;
   const int padded = (c + int(p.pad) - 1) / int(p.pad) * int(p.pad), nt = (c + int(p.bm) - 1) / int(p.bm);
-  int r = padded, k = nt;  // inclusive scans over the units
+  const int nd = (nt + 1) / 2;
+  int r = padded, k = nt, d = nd;  // inclusive scans over the units
   for (int o = 1; o < 32; o <<= 1) {
-    const int a = __shfl_up_sync(0xffffffffu, r, o), b = __shfl_up_sync(0xffffffffu, k, o);
-    if (lane >= o) r += a, k += b;
+    const int a = __shfl_up_sync(0xffffffffu, r, o), b = __shfl_up_sync(0xffffffffu, k, o),
+              e = __shfl_up_sync(0xffffffffu, d, o);
+    if (lane >= o) r += a, k += b, d += e;
   }
-  if (lane == 31) wr[warp] = r, wt[warp] = k;
+  if (lane == 31) wr[warp] = r, wt[warp] = k, wd[warp] = d;
   __syncthreads();
-  for (int w = 0; w < warp; ++w) r += wr[w], k += wt[w];
+  for (int w = 0; w < warp; ++w) r += wr[w], k += wt[w], d += wd[w];
   rows[t] = r - padded;
   tiles[t] = k - nt;
   __syncthreads();
@@ -153,12 +163,16 @@ __global__ __launch_bounds__(kSmallThreads) void plan_small_kernel(const __grid_
     p.cnt[t] = c;
     p.off[t] = rows[t];
     p.slot[t] = my_slot;
-    if (t + 1 == p.units) p.head[0] = k, p.head[1] = r;
+    if (t + 1 == p.units) p.head[0] = k, p.head[1] = r, p.head[2] = d;
     for (int i = 0; i < nt; ++i) {
-      p.tile_unit[tiles[t] + i] = int32_t(t);
-      p.tile_m0[tiles[t] + i] = i * int(p.bm);
+      p.tile_unit[0][tiles[t] + i] = int32_t(t);
+      p.tile_m0[0][tiles[t] + i] = i * int(p.bm);
       p.tile_info[tiles[t] + i] =
           make_int4(my_slot, rows[t] + i * int(p.bm), min(int(p.bm), c - i * int(p.bm)), int32_t(t));
+    }
+    for (int i = 0; i < nd; ++i) {
+      p.tile_unit[1][d - nd + i] = int32_t(t);
+      p.tile_m0[1][d - nd + i] = i * 2 * int(p.bm);
     }
     for (int i = c; i < padded; ++i) p.pair_of_row[rows[t] + i] = -1;
   }
@@ -212,16 +226,18 @@ __global__ __launch_bounds__(256) void join_kernel(const int32_t* __restrict__ r
   for (int v = 0; v < V; ++v) y[t * ldy + c + v] = from_f<T>(sum[v]);
 }
 
+// a warp adds a pair's sums, lane by lane and then over the lanes
 template <class T>
-__global__ void join_dw_kernel(const int32_t* __restrict__ row_of_pair, uint32_t pairs, const float* __restrict__ dwp,
-                               uint32_t tiles, T* __restrict__ dw) {
-  const uint32_t i = blockIdx.x * blockDim.x + threadIdx.x;
+__global__ __launch_bounds__(256) void join_dw_kernel(const int32_t* __restrict__ row_of_pair, uint32_t pairs,
+                                                      const float* __restrict__ dwp, uint32_t tiles, T* __restrict__ dw) {
+  const uint32_t i = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
   if (i >= pairs) return;
   const int32_t row = row_of_pair[i];
   float s = 0.f;
   if (row >= 0)
-    for (uint32_t j = 0; j < tiles; ++j) s += dwp[uint64_t(row) * tiles + j];
-  dw[i] = from_f<T>(s);
+    for (uint32_t j = lane; j < tiles; j += 32) s += dwp[uint64_t(row) * tiles + j];
+  for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  if (lane == 0) dw[i] = from_f<T>(s);
 }
 
 // ---------------------------------------------------------------------------------------------------------------
@@ -442,21 +458,23 @@ Plan plan_at(void* ws, uint32_t units, uint64_t pairs, uint32_t pad, uint32_t bm
     c += aligned(n * 4);
     return r;
   };
-  p.head = take(2);
+  p.head = take(3);
   p.cnt = take(units);
   p.off = take(units);
   p.slot = take(units);
   p.pair_of_row = take(p.max_rows);
   p.row_of_pair = take(pairs);
-  p.tile_unit = take(p.max_tiles);
-  p.tile_m0 = take(p.max_tiles);
+  for (int i = 0; i < 2; ++i) {
+    p.tile_unit[i] = take(p.max_tiles);
+    p.tile_m0[i] = take(p.max_tiles);
+  }
   p.tile_info = reinterpret_cast<int4*>(take(uint64_t(p.max_tiles) * 4));
   return p;
 }
 uint64_t plan_bytes(uint32_t units, uint64_t pairs, uint32_t pad, uint32_t bm) {
   const uint64_t met = pairs < units ? pairs : units;
-  return aligned(8) + 3 * aligned(uint64_t(units) * 4) + aligned((pairs + met * (pad - 1)) * 4) + aligned(pairs * 4) +
-         2 * aligned((pairs / bm + met) * 4) + aligned((pairs / bm + met) * 16);
+  return aligned(12) + 3 * aligned(uint64_t(units) * 4) + aligned((pairs + met * (pad - 1)) * 4) + aligned(pairs * 4) +
+         4 * aligned((pairs / bm + met) * 4) + aligned((pairs / bm + met) * 16);
 }
 
 int launch_plan(const Plan& p, const Units& u, const int32_t* ids, cudaStream_t s) {
@@ -488,7 +506,7 @@ int launch_join(int dtype, const Plan& p, const float* rows32, uint32_t splits, 
 int launch_join_dw(int dtype, const Plan& p, const float* dwp, uint32_t tiles, void* dw, cudaStream_t s) {
   by_type(dtype, [&](auto v) {
     using T = decltype(v);
-    join_dw_kernel<T><<<unsigned(ceil_div(p.pairs, 128)), 128, 0, s>>>(p.row_of_pair, p.pairs, dwp, tiles,
+    join_dw_kernel<T><<<unsigned(ceil_div(p.pairs, 8)), 256, 0, s>>>(p.row_of_pair, p.pairs, dwp, tiles,
                                                                       static_cast<T*>(dw));
   });
   return int(cudaGetLastError());

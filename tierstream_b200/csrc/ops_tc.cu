@@ -14,23 +14,13 @@
 //
 // Every wait is bounded (2 s): one that runs out counts in a device word (tsb_ops_timeouts), and the CTA leaves after a
 // bounded wait for its copies and products in flight, its TMEM freed.
-#include <cuda.h>
-
-#include <cstring>
-
-#include "ops.hpp"
+#include "tc.cuh"
 
 namespace tsb {
 namespace ops {
 namespace {
 
-constexpr int kBM = 128, kBK = 64;  // (a CTA's rows)
-constexpr int kABytes = kBM * kBK * 2, kRingBytes = 192 << 10;  // the stages'
-constexpr int kMaxStages = 12;
-constexpr int kEpiWarps = 8, kThreads = 128 + 32 * kEpiWarps;
-constexpr int kRowBytes = 64, kStoreBytes = 2 * 32 * kRowBytes;  // a warp's two buffers of 32 rows x 64 bytes
-constexpr int kSmemBytes = 1024 + kRingBytes + kEpiWarps * kStoreBytes + 256;
-constexpr unsigned long long kWaitNs = 2000000000ull;
+constexpr int kRowBytes = 64;  // a store buffer: 32 rows x 64 bytes
 
 __device__ uint32_t g_ops_timeouts;
 
@@ -51,131 +41,6 @@ struct Maps {
   CUtensorMap a[2], b[3], out[3];
 };
 
-__device__ __forceinline__ uint32_t smem_u32(const void* p) { return uint32_t(__cvta_generic_to_shared(p)); }
-__device__ __forceinline__ void bar_init(uint32_t b, uint32_t n) {
-  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(b), "r"(n) : "memory");
-}
-__device__ __forceinline__ void bar_expect(uint32_t b, uint32_t bytes) {
-  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(b), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void bar_arrive(uint32_t b) {
-  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(b) : "memory");
-}
-__device__ __forceinline__ bool bar_try(uint32_t b, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, 20000;\n\tselp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(ok)
-      : "r"(b), "r"(parity)
-      : "memory");
-  return ok != 0;
-}
-__device__ __forceinline__ unsigned long long now_ns() {
-  unsigned long long t;
-  asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
-  return t;
-}
-// false: the wait ran out, here or elsewhere in the CTA. A try sleeps in hardware for up to 20 us; the clock is read
-// between runs of tries.
-__device__ __forceinline__ bool bar_wait(uint32_t b, uint32_t parity, volatile uint32_t* dead) {
-  unsigned long long t0 = 0;
-  for (;;) {
-    for (int i = 0; i < 256; ++i)
-      if (bar_try(b, parity)) return true;
-    if (*dead) return false;
-    const unsigned long long t = now_ns();
-    if (!t0) t0 = t;
-    if (t - t0 > kWaitNs) {
-      *dead = 1;
-      return false;
-    }
-  }
-}
-// CG = 2: `bar` may be the peer's
-template <int CG>
-__device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
-  if constexpr (CG == 1)
-    asm volatile(
-        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
-            dst),
-        "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
-        : "memory");
-  else
-    asm volatile(
-        "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, "
-        "%4}], [%5];" ::"r"(dst),
-        "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
-        : "memory");
-}
-__device__ __forceinline__ uint32_t cta_rank() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %cluster_ctarank;" : "=r"(r));
-  return r;
-}
-__device__ __forceinline__ uint32_t in_cta(uint32_t addr, uint32_t rank) {
-  uint32_t a;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(addr), "r"(rank));
-  return a;
-}
-__device__ __forceinline__ void bar_arrive_cluster(uint32_t b) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(b) : "memory");
-}
-__device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
-}
-// One lane of a whole warp, always the same. The loading and the issuing warp run their loops as whole warps, so that
-// addresses and descriptors stay in uniform registers (a loop of one thread spent about 500 clocks a k slice).
-__device__ __forceinline__ bool elect() {
-  uint32_t r;
-  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
-  return r != 0;
-}
-// Shared memory descriptors, 128-byte swizzle. K-major: 8-row groups 1024 bytes apart. MN-major: a stage holds 64-wide
-// chunks of [64 k rows][128 bytes], 8 KiB apart, 8-row groups of k 1024 bytes apart.
-__device__ __forceinline__ uint64_t desc(uint32_t addr, bool mn) {
-  return uint64_t((addr & 0x3ffffu) >> 4) | (uint64_t(mn ? 8192 >> 4 : 1) << 16) | (uint64_t(1024 >> 4) << 32) |
-         (uint64_t(1) << 46) | (uint64_t(2) << 61);
-}
-template <int CG>
-__device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
-  if constexpr (CG == 1)
-    asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"(uint32_t(add))
-        : "memory");
-  else
-    asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"(uint32_t(add))
-        : "memory");
-}
-// the barrier at this offset, in both CTAs of a pair
-template <int CG>
-__device__ __forceinline__ void commit(uint32_t bar) {
-  if constexpr (CG == 1)
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
-  else
-    asm volatile(
-        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
-        "h"(uint16_t(3))
-        : "memory");
-}
-__device__ __forceinline__ void tmem_ld16(uint32_t addr, float (&v)[16]) {
-  uint32_t r[16];
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-      : "r"(addr));
-#pragma unroll
-  for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
-}
-__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
-__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-
 struct Tile {
   int unit, slot, row0, rows, stored;  // row0: the group's first row; rows: m limit; stored: rows to store (padding too)
   int m0, n, kb;
@@ -190,13 +55,13 @@ __device__ __forceinline__ bool tile_at(const Params& q, int L, Tile& t) {
   if constexpr (MODE == kUp || MODE == kUpBack || MODE == kDown || MODE == kDx) {
     const int i = L / q.n_tiles;
     if (i >= q.plan.head[0]) return false;
-    t.unit = q.plan.tile_unit[i];
+    t.unit = q.plan.tile_unit[0][i];
     t.rows = q.plan.cnt[t.unit];
     t.stored = (t.rows + int(q.plan.pad) - 1) / int(q.plan.pad) * int(q.plan.pad);
     t.row0 = q.plan.off[t.unit];
     t.slot = q.plan.slot[t.unit];
     mt = (t.rows + kRows - 1) / kRows;
-    local = L - (i - q.plan.tile_m0[i] / kRows) * q.n_tiles;
+    local = L - (i - q.plan.tile_m0[0][i] / kRows) * q.n_tiles;
     t.kb = q.k_blocks;
   } else if constexpr (MODE == kDw) {
     const int per = q.m_tiles * q.n_tiles;
@@ -236,14 +101,6 @@ struct Traits {
   }
   static constexpr int bufs = MODE == kUpBack ? 1 : 2;
 };
-
-template <class T>
-__device__ __forceinline__ uint32_t pack(float a, float b) {
-  T v[2] = {from_f<T>(a), from_f<T>(b)};
-  uint32_t r;
-  memcpy(&r, v, 4);
-  return r;
-}
 
 // A warp's 32 rows x 64 bytes (thread = row) on their way out: into one of its two buffers in shared memory, 64-byte
 // swizzled so that no bank is met twice, and from there by a TMA store that runs while the next block is computed. Blocks
@@ -485,9 +342,9 @@ __global__ __launch_bounds__(kThreads, 1) void tc_kernel(const __grid_constant__
 #pragma unroll
       for (int s = 0; s < X::segs; ++s) {
         const bool pair = X::both(s);
-        const uint32_t bytes = kABytes + (X::b_mn(s) ? chunks * 8192 : pair ? 2 / CG * q.bn * 128 : half_n * 128);
+        const uint32_t bytes = kABytes + (X::b_mn(s) ? chunks * 8192 : pair ? q.bn * 128 : half_n * 128);
         const CUtensorMap* ma = &maps.a[MODE == kUpBack ? 1 - s : s];
-        const CUtensorMap* mb = &maps.b[MODE == kUpBack && s == 0 ? 2 : pair ? (CG == 2 ? rank : 0) : s];
+        const CUtensorMap* mb = &maps.b[MODE == kUpBack && s == 0 ? 2 : pair ? rank : s];
         const int z = X::grouped ? t.slot : 0, n0 = t.n * q.bn + (pair ? 0 : int(rank) * half_n);
         const int m0 = X::a_mn ? t.m0 : t.row0 + t.m0;
         int k0 = 0, krow = MODE == kDw ? t.row0 : 0;
@@ -507,7 +364,6 @@ __global__ __launch_bounds__(kThreads, 1) void tc_kernel(const __grid_constant__
               for (int c = 0; c < chunks; ++c) tma_load<CG>(sb + c * 8192, mb, n0 + 64 * c, krow, z, bar);
             } else {
               tma_load<CG>(sb, mb, k0, n0, z, bar);
-              if (pair && CG == 1) tma_load<CG>(sb + q.bn * 128, &maps.b[1], k0, n0, z, bar);
             }
           }
           ++it;
@@ -610,36 +466,6 @@ __global__ __launch_bounds__(256) void gather_kernel(const __grid_constant__ Pla
     dst[uint64_t(r) * n16 + c] = pair < 0 ? make_uint4(0, 0, 0, 0) : s[c];
 }
 
-using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
-                            const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
-                            CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-Encode encoder() {
-  static const Encode e = [] {
-    void* fn = nullptr;
-    cudaDriverEntryPointQueryResult r{};
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &r) != cudaSuccess ||
-        r != cudaDriverEntryPointSuccess)
-      fn = nullptr;
-    return reinterpret_cast<Encode>(fn);
-  }();
-  return e;
-}
-
-// [slots][rows][cols], boxes of box_rows rows of 128 (an output: 64) swizzled bytes
-bool make_map(CUtensorMap* m, int dtype, const void* p, uint64_t cols, uint64_t rows, uint64_t ld, uint64_t slots,
-              uint64_t slot_bytes, uint32_t box_rows, bool out = false) {
-  const uint32_t size = dtype == TSB_F32 ? 4 : 2;
-  const cuuint64_t dims[3] = {cols, rows, slots}, strides[2] = {ld * size, slots > 1 ? slot_bytes : ld * size};
-  const cuuint32_t box[3] = {(out ? 64 : 128) / size, box_rows, 1}, one[3] = {1, 1, 1};
-  return encoder()(m,
-                   dtype == TSB_BF16  ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
-                   : dtype == TSB_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
-                                      : CU_TENSOR_MAP_DATA_TYPE_FLOAT32,
-                   3, const_cast<void*>(p), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                   out ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
 template <class T, int MODE, int ACT, int CG>
 int go_pair(const Maps& maps, const Params& q, int grid, cudaStream_t s) {
   const auto kernel = tc_kernel<T, MODE, ACT, CG>;
@@ -660,7 +486,8 @@ int go_pair(const Maps& maps, const Params& q, int grid, cudaStream_t s) {
 }
 template <class T, int MODE, int ACT>
 int go(const Maps& maps, const Params& q, int grid, cudaStream_t s) {
-  return q.pair ? go_pair<T, MODE, ACT, 2>(maps, q, grid, s) : go_pair<T, MODE, ACT, 1>(maps, q, grid, s);
+  if constexpr (Traits<MODE>::grouped) return go_pair<T, MODE, ACT, 2>(maps, q, grid, s);
+  else return q.pair ? go_pair<T, MODE, ACT, 2>(maps, q, grid, s) : go_pair<T, MODE, ACT, 1>(maps, q, grid, s);
 }
 template <class T, int MODE>
 int go_act(int act, const Maps& maps, const Params& q, int grid, cudaStream_t s) {
@@ -679,14 +506,6 @@ int go_type(int dtype, int act, const Maps& maps, const Params& q, int grid, cud
                              : go_act<__half, MODE>(act, maps, q, grid, s);
   else
     return dtype == TSB_BF16 ? go<__nv_bfloat16, MODE, 0>(maps, q, grid, s) : go<__half, MODE, 0>(maps, q, grid, s);
-}
-
-bool on16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
-int sm_count() {
-  int dev = 0, n = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
-    return 0;
-  return n;
 }
 
 // Columns a tile: of the multiples of `step` up to `most`, the one whose last wave of tiles wastes least. A tile costs its
@@ -743,7 +562,7 @@ int launch_tc(int dtype, const Product& p, const Plan* plan, const Units* u, cud
   else mode = p.per_unit ? kDw : (a_mn ? kLinDw : kLinDx);
   // Pairs of CTAs share a 256-row tile when there are rows for it: each stages half of B, so a tile's operands cross from
   // L2 once for 256 x 256 sums instead of 128 x 256 (the SM's 64 bytes a clock from L2 bound the single CTA).
-  q.pair = p.grouped ? plan->bm == 2 * kBM : p.m > kBM;
+  q.pair = p.grouped || p.m > kBM;
   const int cg = q.pair ? 2 : 1;
   q.k_blocks = int(ceil_div(uint64_t(p.k), kBK));
   q.m_tiles = p.grouped ? 0 : int(ceil_div(uint64_t(p.m), uint64_t(cg * kBM)));
@@ -798,7 +617,7 @@ int launch_tc(int dtype, const Product& p, const Plan* plan, const Units* u, cud
         return int(cudaErrorInvalidValue);
   }
   // as many stages as the ring holds: narrow tiles are bound by the loads' latency
-  const int b_cols = (narrow && cg == 1 ? 2 : 1) * (narrow ? q.bn : q.bn / cg);
+  const int b_cols = narrow ? q.bn : q.bn / cg;
   q.stage_bytes = kABytes + int(ceil_div(uint64_t(b_cols), 64)) * 8192;
   q.stages = kRingBytes / q.stage_bytes < kMaxStages ? kRingBytes / q.stage_bytes : kMaxStages;
   const int64_t tiles = m_tiles * q.n_tiles;

@@ -79,8 +79,8 @@ __global__ __launch_bounds__(kThreads) void tile_kernel(const __grid_constant__ 
   int64_t m0 = int64_t(blockIdx.x) * 64;
   if (p.grouped) {
     if (int32_t(blockIdx.x) >= plan.head[0]) return;
-    g.unit = plan.tile_unit[blockIdx.x];
-    m0 = plan.tile_m0[blockIdx.x];
+    g.unit = plan.tile_unit[0][blockIdx.x];
+    m0 = plan.tile_m0[0][blockIdx.x];
     g.rows = plan.cnt[g.unit];
     g.row0 = plan.off[g.unit];
     g.slot = plan.slot[g.unit];
