@@ -13,10 +13,10 @@ constexpr uint32_t kNone = 0xffffffffu;
 
 // ---------------------------------------------------------------------------------------------------------------
 // The plan. Counting first: CTA e counts unit e's pairs and resolves its slot. Then CTA e adds up the groups before its
-// own (padded rows, tiles) and writes its pairs in ascending order, found by scanning the ids with a ballot: no atomics,
+// own (padded rows, tiles) and writes its pairs in ascending order, found by scanning the ids: no atomics,
 // so the order never changes. The scan reads the ids once per unit from L2 (256 units x 16,384 pairs: 16 MB).
 // ---------------------------------------------------------------------------------------------------------------
-constexpr int kPlanThreads = 256;
+constexpr int kPlanThreads = 1024, kPlanEach = 4;  // ids a thread and step
 
 __device__ __forceinline__ int32_t resolve(const Units& u, int32_t e) {
   if (u.abort && *reinterpret_cast<const volatile uint32_t*>(u.abort)) return -1;
@@ -42,6 +42,7 @@ __global__ __launch_bounds__(kPlanThreads) void plan_count_kernel(const __grid_c
   __shared__ int red[kPlanThreads / 32];
   const int32_t e = blockIdx.x;
   int n = 0;
+#pragma unroll 4
   for (uint32_t i = threadIdx.x; i < p.pairs; i += kPlanThreads) n += ids[i] == e;
   n = block_sum(n, red);
   if (threadIdx.x) return;
@@ -92,25 +93,35 @@ __global__ __launch_bounds__(kPlanThreads) void plan_fill_kernel(const __grid_co
   for (int i = cnt + threadIdx.x; i < padded; i += kPlanThreads) p.pair_of_row[rows + i] = -1;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int done = 0;  // pairs of this unit before the current span of ids
-  for (uint32_t i0 = 0; i0 < p.pairs && (cnt || e == 0); i0 += kPlanThreads) {
-    const uint32_t i = i0 + threadIdx.x;
-    const int32_t id = i < p.pairs ? ids[i] : -1;
-    if (e == 0 && i < p.pairs && (uint32_t(id) >= p.units || p.cnt[id] == 0)) p.row_of_pair[i] = -1;
-    const bool hit = cnt && i < p.pairs && id == int32_t(e);
-    const uint32_t m = __ballot_sync(0xffffffffu, hit);
+  for (uint32_t i0 = 0; i0 < p.pairs && (cnt || e == 0); i0 += kPlanThreads * kPlanEach) {
+    const uint32_t i = i0 + threadIdx.x * kPlanEach;
+    int hits = 0;
+    uint32_t hit = 0;
+#pragma unroll
+    for (int j = 0; j < kPlanEach; ++j) {
+      const int32_t id = i + j < p.pairs ? ids[i + j] : -1;
+      if (e == 0 && i + j < p.pairs && (uint32_t(id) >= p.units || p.cnt[id] == 0)) p.row_of_pair[i + j] = -1;
+      if (cnt && i + j < p.pairs && id == int32_t(e)) hit |= 1u << j, ++hits;
+    }
+    int upto = hits;  // inclusive over the warp
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += v;
+    }
     __syncthreads();
-    if (lane == 0) warp_n[warp] = __popc(m);
+    if (lane == 31) warp_n[warp] = upto;
     __syncthreads();
-    int before = done;
+    int r = rows + done + upto - hits;
     for (int w = 0; w < kPlanThreads / 32; ++w) {
-      if (w < warp) before += warp_n[w];
+      if (w < warp) r += warp_n[w];
       done += warp_n[w];
     }
-    if (hit) {
-      const int r = rows + before + __popc(m & ((1u << lane) - 1));
-      p.pair_of_row[r] = int32_t(i);
-      p.row_of_pair[i] = r;
-    }
+#pragma unroll
+    for (int j = 0; j < kPlanEach; ++j)
+      if (hit >> j & 1) {
+        p.pair_of_row[r] = int32_t(i + j);
+        p.row_of_pair[i + j] = r++;
+      }
   }
 }
 
