@@ -362,7 +362,9 @@ SS_API ss_status tsb_dg_peer_retier(ss_ctx* c, const tsb_peer_tier* peer);
  * needed; on a refused argument 0 too, and the call itself names the refusal), a 256-byte aligned device area that
  * belongs to the call until the stream has passed it (two calls that may run at the same time, or two graphs, need one
  * each). No result depends on the order in which anything ran: the same inputs give the same bits. Outputs must not
- * overlap inputs, except that y may be the residual. Sums are held in 32 bits; what is 16 bits wide between two
+ * overlap inputs, except that y may be the residual (of the feed-forward block even when that is x). On a device-gated
+ * context, capture the calls, or make a first call of each before a token runs: a kernel's first call loads it, which a
+ * token's waiting kernel holds up. Sums are held in 32 bits; what is 16 bits wide between two
  * products of a call is said at each. */
 #define TSB_BF16 0
 #define TSB_F16 1
@@ -462,8 +464,8 @@ SS_API ss_status tsb_units_from_view(const ss_dg_device_view* v, uint32_t g, uin
 
 /* The gated feed-forward block of the routed units: y[t] = residual[t] + sum over k of weights[t][k] x
  * Wd_e (act(Wg_e x[t]) * (Wu_e x[t])), e = ids[t][k]; x and y [rows][hidden], ids and weights [rows][top] (device
- * memory). An id outside [0, n_units) contributes nothing (a padded row's -1); a row with none gives its residual, or
- * zeros. The same unit twice in a row counts twice. act(..) * (..) is rounded to dtype between the products; the
+ * memory). An id outside [0, n_units) contributes nothing (a padded row's -1, which is not to be exported); a row with
+ * none gives its residual, or zeros. The same unit twice in a row counts twice. act(..) * (..) is rounded to dtype between the products; the
  * choices' sums are added in 32 bits. residual may be NULL. top is at most 64, rows x top at most 2^28. */
 typedef struct tsb_ffn_args {
   uint32_t struct_size, dtype, act, top;

@@ -165,6 +165,13 @@ class tsb_ffn_grad_args(C.Structure):
                 ("workspace", vp), ("workspace_bytes", u64), ("stream", vp)]
 
 
+class tse_layers(C.Structure):
+    """The engine stand-in's stack of layers (engine_sim.cu)."""
+    _fields_ = [("rows", u32), ("top", u32), ("units", u32), ("dtype", u32), ("act", u32), ("reserved", u32),
+                ("hidden", u64), ("ffn", u64), ("router", C.POINTER(vp)), ("x", vp), ("logits", vp), ("ids", vp),
+                ("weights", vp), ("workspace", vp), ("workspace_bytes", u64)]
+
+
 class ss_dg_stats(C.Structure):
     """The leading fields of ss_dg_stats (a versioned struct: the library writes min(size, its own) bytes)."""
     _fields_ = [("struct_size", u32), ("reserved0", u32)] + [(n, u64) for n in _DG_STATS_U64_1]
@@ -337,6 +344,8 @@ _ENGINE_PROTOS = {
     "tse_read_table16": (C.c_int, [vp, vp, u32, u64, vp, u32, C.c_int, vp]),
     "tse_host_forward": (C.c_int, [vp, vp, vp, u32, vp, vp, vp, u32, C.c_int, vp]),
     "tse_expect_sums": (C.c_int, [u64, vp, u32, u64, C.c_int, vp, u32, vp]),
+    "tse_layers_workspace": (u64, [vp, vp]),
+    "tse_capture_layers": (C.c_int, [vp, u32, vp, vp, P(vp)]),
 }
 
 _PROTOS.update({

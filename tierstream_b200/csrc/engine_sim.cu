@@ -6,6 +6,9 @@
 // then ss_dg_enqueue_end. The reader's result per (layer, id) is a checksum of the unit's bytes:
 //   mode 0: sum(byte * (pos % 251 + 1)) over the unit (the reference GPU tests' check, tests/test_dg_cuda.cu:103-114);
 //   mode 1: the sum of the unit's 32-bit little-endian words (a read at HBM speed, the bench's engine work).
+// tse_capture_layers captures the step of an engine that computes instead: per gated layer the router's logits, its
+// selection, the export and wait of the ids it chose, and the gated feed-forward block of the units in their slots, by
+// the library's own operators (tsb_linear, tsb_route, tsb_ffn).
 // This library is not part of the runtime (libtierstream.so never links it).
 #include <cuda_runtime.h>
 
@@ -15,6 +18,7 @@
 #include <vector>
 
 #include "strix_stream/ss.h"
+#include "tierstream/tsb.h"
 
 namespace {
 
@@ -239,6 +243,93 @@ __attribute__((visibility("default"))) int tse_capture_token(ss_ctx* c, uint32_t
   if (side) cudaStreamDestroy(side);
   if (fork) cudaEventDestroy(fork);
   if (join) cudaEventDestroy(join);
+  if (err) {
+    if (graph) cudaGraphDestroy(graph);
+    return err;
+  }
+  CK(ec);
+  cudaGraphExec_t exec = nullptr;
+  const cudaError_t ei = cudaGraphInstantiate(&exec, graph, 0);
+  cudaGraphDestroy(graph);
+  CK(ei);
+  *exec_out = exec;
+  return 0;
+}
+
+// A stack of mixture-of-experts layers over the context's gated layers, `rows` rows of [hidden] 16-bit values at a time:
+// x = x + block(x) for each. router[g]: gated layer g's router matrix [units][hidden] (device); x, logits [rows][units],
+// ids and weights [n_gated][rows x top] (device) are read and written by the graph; the workspace is
+// tse_layers_workspace(m) bytes on 256.
+struct tse_layers {
+  uint32_t rows, top, units, dtype, act, reserved;
+  uint64_t hidden, ffn;
+  const void* const* router;
+  void* x;
+  void* logits;
+  int32_t* ids;
+  float* weights;
+  void* workspace;
+  uint64_t workspace_bytes;
+};
+static void layer_args(const tse_layers* m, const tsb_units* u, tsb_ffn_args* f) {
+  *f = tsb_ffn_args{};
+  f->struct_size = sizeof *f;
+  f->dtype = m->dtype, f->act = m->act, f->top = m->top;
+  f->rows = m->rows, f->hidden = m->hidden, f->ffn = m->ffn;
+  f->x = m->x, f->ldx = m->hidden;
+  f->residual = m->x, f->ldr = m->hidden;
+  f->y = m->x, f->ldy = m->hidden;
+  f->ids = m->ids, f->weights = m->weights;
+  f->units = u;
+  f->workspace = m->workspace, f->workspace_bytes = m->workspace_bytes;
+}
+__attribute__((visibility("default"))) uint64_t tse_layers_workspace(ss_ctx* c, const tse_layers* m) {
+  ss_dg_device_view v;
+  tsb_units u;
+  if (ss_dg_get_device_view(c, &v) != SS_OK || tsb_units_from_view(&v, 0, m->units, m->hidden * m->ffn * 2, &u) != SS_OK)
+    return 0;
+  tsb_ffn_args f;
+  layer_args(m, &u, &f);
+  return tsb_ffn_workspace(&f);
+}
+__attribute__((visibility("default"))) int tse_capture_layers(ss_ctx* c, uint32_t n_gated, const tse_layers* m,
+                                                              void* stream, void** exec_out) {
+  ss_dg_device_view v;
+  SS(ss_dg_get_device_view(c, &v));
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const uint32_t n = m->rows * m->top;
+  cudaGraph_t graph = nullptr;
+  CK(cudaStreamBeginCapture(s, cudaStreamCaptureModeThreadLocal));
+  auto layers = [&]() -> int {
+    SS(ss_dg_enqueue_begin(c, s));
+    for (uint32_t g = 0; g < n_gated; ++g) {
+      tsb_linear_args a{};
+      a.struct_size = sizeof a;
+      a.dtype = m->dtype;
+      a.rows = m->rows, a.n = m->units, a.k = m->hidden;
+      a.x = m->x, a.ldx = m->hidden;
+      a.w = m->router[g], a.ldw = m->hidden;
+      a.y = m->logits, a.ldy = m->units;
+      a.stream = s;
+      SS(tsb_linear(&a));
+      int32_t* ids = m->ids + uint64_t(g) * n;
+      float* weights = m->weights + uint64_t(g) * n;
+      SS(tsb_route(m->dtype, m->logits, m->units, m->rows, m->units, m->top, 1, ids, weights, s));
+      SS(ss_dg_enqueue_export(c, int(g), ids, int(n), 0, s));
+      SS(ss_dg_enqueue_wait(c, int(g), s));
+      tsb_units u;
+      SS(tsb_units_from_view(&v, g, m->units, m->hidden * m->ffn * 2, &u));
+      tsb_ffn_args f;
+      layer_args(m, &u, &f);
+      f.ids = ids, f.weights = weights;
+      f.stream = s;
+      SS(tsb_ffn(&f));
+    }
+    SS(ss_dg_enqueue_end(c, s));
+    return 0;
+  };
+  const int err = layers();
+  const cudaError_t ec = cudaStreamEndCapture(s, &graph);
   if (err) {
     if (graph) cudaGraphDestroy(graph);
     return err;

@@ -9,7 +9,7 @@ import os
 import numpy as np
 import torch
 
-from . import abi, runtime, synth
+from . import abi, ops, runtime, synth
 
 
 class DgSetup:
@@ -148,6 +148,53 @@ class DgRun:
         for g in getattr(self, "graphs", {}).values():
             g.close()
         self.graphs = {}
+        if getattr(self, "graph", None):
+            self.graph.close()
+        if getattr(self, "ctx", None):
+            self.ctx.close()
+
+
+class DgLayers:
+    """A device-gated context whose engine computes: a stack of mixture-of-experts layers (router logits, selection,
+    export and wait of the chosen ids, gated feed-forward block of the units in their slots, residual) captured as one
+    graph. model: units of three parts, gate and up [ffn][hidden] and down [hidden][ffn] of `dtype`; routers
+    [layers][units][hidden] on the device."""
+
+    def __init__(self, model, hidden, ffn, routers, rows=1, top=2, dtype=torch.bfloat16, act="silu", **setup):
+        G, U = model.layers, model.units
+        n = rows * top
+        s = DgSetup(model, max_ids=n, **setup)
+        self.setup, self.rows, self.top, self.G = s, rows, top, G
+        s.options.device = torch.cuda.current_device()
+        self.ctx = runtime.DgContext(s.desc, s.plan, s.options)
+        self.stream = torch.cuda.Stream()
+        self.routers = routers
+        self.x = torch.zeros((rows, hidden), dtype=dtype, device="cuda")
+        self.logits = torch.zeros((rows, U), dtype=dtype, device="cuda")
+        self.ids = torch.zeros((G, rows, top), dtype=torch.int32, device="cuda")
+        self.weights = torch.zeros((G, rows, top), dtype=torch.float32, device="cuda")
+        self.ptrs = (C.c_void_p * G)(*[routers[g].data_ptr() for g in range(G)])
+        m = abi.tse_layers(rows, top, U, ops.HALF[dtype], ops.ACTIVATIONS[act], 0, hidden, ffn, self.ptrs,
+                           self.x.data_ptr(), self.logits.data_ptr(), self.ids.data_ptr(), self.weights.data_ptr())
+        m.workspace_bytes = abi.load_engine().tse_layers_workspace(self.ctx.h, C.byref(m))
+        self.scratch = torch.empty(m.workspace_bytes + 256, dtype=torch.uint8, device="cuda")
+        m.workspace = (self.scratch.data_ptr() + 255) & ~255
+        self.stream.wait_stream(torch.cuda.current_stream())
+        self.graph = runtime.LayerGraph(self.ctx, G, m, self.stream.cuda_stream)
+
+    def step(self, x):
+        """One step: the stack's output for x [rows][hidden]; ids and weights [layers][rows][top] of the step are in
+        self.ids and self.weights."""
+        self.ctx.begin()
+        self.stream.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(self.stream):
+            self.x.copy_(x)
+            self.graph.launch()
+        self.stream.synchronize()
+        self.ctx.end()
+        return self.x.clone()
+
+    def close(self):
         if getattr(self, "graph", None):
             self.graph.close()
         if getattr(self, "ctx", None):

@@ -12,7 +12,7 @@ import json
 
 import torch
 
-from . import abi
+from . import abi, ops
 
 
 def _events(stream, fn, reps, warmup):
@@ -91,6 +91,43 @@ def xxh64(units, part_bytes, n_parts, reps, warmup):
             "gbs": round(total / ms / 1e6, 2), "per_unit_gbs": round(unit_bytes / ms / 1e6, 3)}
 
 
+def operator(name, rows, hidden, ffn, units, top, reps, warmup, back):
+    """One of the operators (ops.linear [rows][hidden] x [ffn][hidden], ops.route, ops.ffn) or its backward pass, bf16,
+    rotating over three inputs; bytes and flops as the operator cannot do without, units met counted."""
+    t = torch.bfloat16
+    s = torch.cuda.current_stream()
+    sets = []
+    for _ in range(3):
+        x, dy = torch.randn((rows, hidden), device="cuda", dtype=t), torch.randn((rows, hidden), device="cuda", dtype=t)
+        logits = torch.randn((rows, units), device="cuda")
+        ids, w = ops.route(logits, top)
+        sets.append((x, dy, logits, ids, w, torch.randn((rows, ffn), device="cuda", dtype=t)))
+    met = sum(int(torch.unique(v[3]).numel()) for v in sets) / 3
+    if name == "linear":
+        ws = [torch.randn((ffn, hidden), device="cuda", dtype=t) for _ in range(3)]
+        calls = [(lambda v=v, m=m: ops.linear_backward(v[5], v[0], m)) if back else (lambda v=v, m=m: ops.linear(v[0], m))
+                 for v, m in zip(sets, ws)]
+        nbytes = 2 * (rows * hidden + ffn * hidden + rows * ffn) + back * 2 * (rows * hidden + ffn * hidden)
+        flops = 2 * rows * hidden * ffn * (2 if back else 1)
+    elif name == "route":
+        calls = [(lambda v=v: ops.route_backward(v[4], v[2], v[3], v[4])) if back else (lambda v=v: ops.route(v[2], top))
+                 for v in sets]
+        nbytes, flops = rows * (4 * units * (1 + back) + 8 * top), 4 * rows * units
+    else:
+        gate, up = (torch.randn((units, ffn, hidden), device="cuda", dtype=t) * hidden ** -0.5 for _ in range(2))
+        un = ops.Units(gate, up, torch.randn((units, hidden, ffn), device="cuda", dtype=t) * ffn ** -0.5)
+        calls = [(lambda v=v: ops.ffn_backward(v[1], v[0], v[3], v[4], un)) if back
+                 else (lambda v=v: ops.ffn(v[0], v[3], v[4], un)) for v in sets]
+        nbytes = 2 * (3 * met * hidden * ffn + 2 * rows * hidden) + back * 2 * (3 * units * hidden * ffn + rows * hidden)
+        flops = rows * top * hidden * ffn * (16 if back else 6)
+    turn = iter(range(1 << 30))
+    times = sorted(_events(s, lambda: calls[next(turn) % 3](), reps, warmup))
+    ms = times[len(times) // 2]
+    return {"kernel": name + ("_backward" if back else ""), "rows": rows, "hidden": hidden, "ffn": ffn, "units": units,
+            "top": top, "ms_median": round(ms, 4), "gbs": round(nbytes / ms / 1e6, 2),
+            "tflops": round(flops / ms / 1e9, 2)}
+
+
 def main():
     ap = argparse.ArgumentParser()
     sub = ap.add_subparsers(dest="what", required=True)
@@ -104,13 +141,23 @@ def main():
     a2.add_argument("--units", type=int, default=296)
     a2.add_argument("--part-bytes", type=int, default=12582912)
     a2.add_argument("--n-parts", type=int, default=3)
-    for p in (a1, a2):
+    a3 = [sub.add_parser(n, help="the operator ops.%s (--back: its backward pass)" % n) for n in ("linear", "route", "ffn")]
+    for p in a3:
+        p.add_argument("--rows", type=int, default=1)
+        p.add_argument("--hidden", type=int, default=4096)
+        p.add_argument("--ffn", type=int, default=14336)
+        p.add_argument("--units", type=int, default=8)
+        p.add_argument("--top", type=int, default=2)
+        p.add_argument("--back", action="store_true")
+    for p in (a1, a2, *a3):
         p.add_argument("--reps", type=int, default=10)
         p.add_argument("--warmup", type=int, default=3)
     a = ap.parse_args()
     if a.what == "land":
         assert a.kernel == "land" or a.dir == "d2d", "the move kernel copies HBM -> HBM only"
         r = land(a.dir, a.part_bytes, a.parts, a.reps, a.warmup, a.kernel)
+    elif a.what in ("linear", "route", "ffn"):
+        r = operator(a.what, a.rows, a.hidden, a.ffn, a.units, a.top, a.reps, a.warmup, a.back)
     else:
         r = xxh64(a.units, a.part_bytes, a.n_parts, a.reps, a.warmup)
     print(json.dumps(r), flush=True)

@@ -15,8 +15,8 @@ from . import abi
 
 ACTIVATIONS = {"none": abi.TSB_ACT_NONE, "silu": abi.TSB_ACT_SILU, "gelu": abi.TSB_ACT_GELU,
                "gelu_tanh": abi.TSB_ACT_GELU_TANH, "relu": abi.TSB_ACT_RELU}
-_HALF = {torch.bfloat16: abi.TSB_BF16, torch.float16: abi.TSB_F16}
-_ANY = {**_HALF, torch.float32: abi.TSB_F32}
+HALF = {torch.bfloat16: abi.TSB_BF16, torch.float16: abi.TSB_F16}
+_ANY = {**HALF, torch.float32: abi.TSB_F32}
 _LINEAR, _LINEAR_GRAD = C.sizeof(abi.tsb_linear_args), C.sizeof(abi.tsb_linear_grad_args)
 _FFN, _FFN_GRAD, _UNITS = C.sizeof(abi.tsb_ffn_args), C.sizeof(abi.tsb_ffn_grad_args), C.sizeof(abi.tsb_units)
 # the current stream's handle; torch.cuda.current_stream() builds an object around it, which costs 4 us a call
@@ -99,7 +99,7 @@ def linear(x, w, bias=None, residual=None, act="none", pre=None, out=None):
     """act(x w^T + bias) + residual: x [rows][k], w [n][k], bias [n], residual [rows][n]. pre: a [rows][n] tensor that
     receives x w^T + bias for linear_backward. out: where to write (may be the residual)."""
     lib = abi.load()
-    dt, dev = _first("x", x, _HALF)
+    dt, dev = _first("x", x, HALF)
     (rows, k), n, t = x.shape, w.shape[0], x.dtype
     px, ldx = _mat("x", x, rows, k, t, dev)
     pw, ldw = _mat("w", w, n, k, t, dev)
@@ -126,7 +126,7 @@ def linear_backward(dy, x, w, act="none", pre=None, need=("x", "w", "bias")):
     """(dx, dw, dbias) of linear() from dy [rows][n]; None for what `need` does not name. pre: what the forward pass
     wrote there (needed unless act is "none"). The residual's gradient is dy."""
     lib = abi.load()
-    dt, dev = _first("dy", dy, _HALF)
+    dt, dev = _first("dy", dy, HALF)
     (rows, n), t = dy.shape, dy.dtype
     if x.dim() != 2:
         raise ValueError("x: two dimensions are wanted, got %s" % (tuple(x.shape),))
@@ -204,7 +204,7 @@ class Units:
     slot is outside the arrays is not there: its rows contribute nothing."""
 
     def __init__(self, gate, up, down, slot_of=None):
-        if gate.dim() != 3 or gate.dtype not in _HALF or not gate.is_cuda:
+        if gate.dim() != 3 or gate.dtype not in HALF or not gate.is_cuda:
             raise ValueError("gate: [slots][ffn][hidden] of bfloat16 or float16 on a CUDA device is wanted, got %s %s on "
                              "%s" % (gate.dtype, tuple(gate.shape), gate.device))
         slots, ffn, hidden = gate.shape
@@ -231,7 +231,7 @@ class Units:
         """Gated layer g of a runtime.DgContext whose units are gate, up and down parts of this type: valid between
         ss_dg_enqueue_wait(g) and the token's end, for the context's life."""
         self = cls.__new__(cls)
-        if dtype not in _HALF:
+        if dtype not in HALF:
             raise ValueError("%s is not served" % dtype)
         self.dtype, self.hidden, self.ffn, self.n_units = dtype, hidden, ffn, n_units
         self.dev = torch.cuda.current_device() if device is None else torch.device(device).index
@@ -245,7 +245,7 @@ class Units:
         """A layer acquired in host forward mode: `table` the device address of its n_units unit addresses
         (ss_layer_view.table_dev), each unit gate, up and down back to back. Valid until the layer's release."""
         self = cls.__new__(cls)
-        if dtype not in _HALF:
+        if dtype not in HALF:
             raise ValueError("%s is not served" % dtype)
         self.dtype, self.hidden, self.ffn, self.n_units = dtype, hidden, ffn, n_units
         self.dev = torch.cuda.current_device() if device is None else torch.device(device).index
@@ -258,7 +258,7 @@ class Units:
 
 
 def _ffn_args(struct, size, x, ids, weights, units, act):
-    dt, dev = _first("x", x, _HALF)
+    dt, dev = _first("x", x, HALF)
     rows, hidden = x.shape
     if ids.dim() != 2:
         raise ValueError("ids: two dimensions are wanted, got %s" % (tuple(ids.shape),))

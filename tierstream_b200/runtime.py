@@ -276,6 +276,20 @@ class TokenGraph:
         self.close()
 
 
+class LayerGraph(TokenGraph):
+    """One decode step of a stack of layers captured once (libtsb_engine.so tse_capture_layers): per layer the router's
+    logits, its selection, export / wait of the ids it chose, and the units' gated feed-forward block. layers: a filled
+    abi.tse_layers; what its addresses point to has to outlive the graph."""
+
+    def __init__(self, ctx, n_gated, layers, stream):
+        self.exec = C.c_void_p()
+        self.stream = stream
+        rc = abi.load_engine().tse_capture_layers(ctx.h, n_gated, C.byref(layers), stream, C.byref(self.exec))
+        if rc != 0:
+            msg = abi.load().ss_last_error().decode(errors="replace") if rc >= 1000 else ""
+            raise RuntimeError("tse_capture_layers failed: %d %s" % (rc, msg))
+
+
 def replay_config(n_units, part_bytes, persistent_slots, bank_slots, blocks, spare_target, order, tokens, n_ids,
                   n_pred=0, prefetch_reserve=0xFFFFFFFF, prefetch_per_layer=4, prefetch_per_token=48, wb_defer=1,
                   wb_on_d2h=1, wb_layer_bytes=0, wb_max_outstanding=0, move_bytes=0, inclusive=0, disk=None,
