@@ -167,6 +167,7 @@ void linear_back(const tsb_linear_grad_args* a) {
     p.a[0] = dense(dz, int64_t(ldz), 1);
     p.b[0] = dense(a->w, 1, int64_t(a->ldw));
     p.m = int64_t(a->rows), p.n = int64_t(a->k), p.k = int64_t(a->n);
+    p.after = slope || a->db;
     p.epi = kEpiStore;
     p.out = a->dx, p.ldo = int64_t(a->lddx);
     ck(product(int(a->dtype), p, s), fn, "dx");
@@ -177,6 +178,7 @@ void linear_back(const tsb_linear_grad_args* a) {
     p.a[0] = dense(dz, 1, int64_t(ldz), 1);
     p.b[0] = dense(a->x, 1, int64_t(a->ldx), 1);
     p.m = int64_t(a->n), p.n = int64_t(a->k), p.k = int64_t(a->rows);
+    p.after = slope || a->db || a->dx;
     p.epi = kEpiStore;
     p.out = a->dw, p.ldo = int64_t(a->lddw);
     ck(product(int(a->dtype), p, s), fn, "dw");
@@ -282,6 +284,7 @@ void ffn(const tsb_ffn_args* a) {
   ck(launch_plan(w.plan, u, a->ids, s), fn, "plan");
   Product p{};
   p.grouped = 1;
+  p.after = true;
   p.segs = 2;
   p.a[0] = p.a[1] = gathered(a->x, int64_t(a->ldx), 1, w.plan, a->top);
   p.b[0] = of_unit(0, d, 1);
@@ -303,6 +306,7 @@ void ffn(const tsb_ffn_args* a) {
   ck(go(int(a->dtype), p, &w.plan, &u, s), fn, "gate and up");
   Product q{};
   q.grouped = 1;
+  q.after = true;
   q.segs = 1;
   q.a[0] = dense(w.h, f, 1);
   q.b[0] = of_unit(2, f, 1);
@@ -389,6 +393,7 @@ void ffn_back(const tsb_ffn_grad_args* a) {
   {
     Product p{};
     p.grouped = 1;
+    p.after = true;
     p.segs = 3;
     p.a[0] = p.a[1] = x_rows;
     p.a[2] = dy_rows;
@@ -408,6 +413,7 @@ void ffn_back(const tsb_ffn_grad_args* a) {
   if (a->dx) {
     Product p{};
     p.grouped = 1;
+    p.after = true;
     p.segs = 2;
     p.a[0] = dense(w.dg, f, 1);
     p.a[1] = dense(w.du, f, 1);
@@ -423,6 +429,7 @@ void ffn_back(const tsb_ffn_grad_args* a) {
   if (a->dgate) {
     Product p{};
     p.per_unit = 1;
+    p.after = true;
     p.k_rows = 1;
     p.segs = 1;
     p.epi = kEpiStore;

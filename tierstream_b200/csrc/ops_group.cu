@@ -250,6 +250,7 @@ __global__ __launch_bounds__(kThreads, 1) void group_kernel(const __grid_constan
   cluster_sync();
   fence_after();
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(words);
+  begin_after();
 
   if (warp == 0) {  // the loads: 128 rows of the matrix and half of the group's rows, arriving at the first CTA's barrier
     uint32_t it = 0, st = 0, parity = 1;
@@ -371,21 +372,10 @@ __global__ __launch_bounds__(kThreads, 1) void group_kernel(const __grid_constan
 
 template <class T, int MODE, int ACT>
 int go(const Maps& maps, const Params& q, int pairs, cudaStream_t s) {
+  static std::atomic<uint64_t> devices{0};
   const auto kernel = group_kernel<T, MODE, ACT>;
-  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
-  if (e != cudaSuccess) return int(e);
-  cudaLaunchConfig_t c{};
-  c.gridDim = dim3(unsigned(pairs * 2));
-  c.blockDim = dim3(kThreads);
-  c.dynamicSmemBytes = kSmemBytes;
-  c.stream = s;
-  cudaLaunchAttribute a[1];
-  a[0].id = cudaLaunchAttributeClusterDimension;
-  a[0].val.clusterDim.x = 2;
-  a[0].val.clusterDim.y = a[0].val.clusterDim.z = 1;
-  c.attrs = a;
-  c.numAttrs = 1;
-  return int(cudaLaunchKernelEx(&c, kernel, maps, q));
+  if (const int e = allow_smem(reinterpret_cast<const void*>(kernel), devices)) return e;
+  return launch(kernel, unsigned(pairs * 2), kThreads, kSmemBytes, 2, q.p.after, s, maps, q);
 }
 template <class T, int MODE>
 int go_act(int act, const Maps& maps, const Params& q, int pairs, cudaStream_t s) {

@@ -39,6 +39,7 @@ __device__ __forceinline__ int block_sum(int v, int* red) {
 __global__ __launch_bounds__(kPlanThreads) void plan_count_kernel(const __grid_constant__ Plan p,
                                                                   const __grid_constant__ Units u,
                                                                   const int32_t* __restrict__ ids) {
+  begin_after();
   __shared__ int red[kPlanThreads / 32];
   const int32_t e = blockIdx.x;
   int n = 0;
@@ -56,6 +57,7 @@ __global__ __launch_bounds__(kPlanThreads) void plan_fill_kernel(const __grid_co
                                                                  const int32_t* __restrict__ ids) {
   __shared__ int red[kPlanThreads / 32];
   __shared__ int warp_n[kPlanThreads / 32];
+  begin_after();
   const uint32_t e = blockIdx.x;
   int rows = 0, tiles = 0, twice = 0;
   for (uint32_t j = threadIdx.x; j < e; j += kPlanThreads) {
@@ -137,6 +139,7 @@ __global__ __launch_bounds__(kSmallThreads) void plan_small_kernel(const __grid_
   __shared__ int32_t wr[32], wt[32], wd[32];
   const uint32_t t = threadIdx.x;
   const int lane = t & 31, warp = t >> 5;
+  begin_after();
   cnt[t] = 0;
   if (t < p.pairs) id[t] = ids[t];
   __syncthreads();
@@ -211,6 +214,7 @@ __global__ __launch_bounds__(256) void join_kernel(const int32_t* __restrict__ r
                                                    uint32_t splits, uint64_t split_stride,
                                                    const float* __restrict__ weights, uint32_t top, uint64_t n,
                                                    const T* residual, uint64_t ldr, T* y, uint64_t ldy) {
+  begin_after();
   const uint64_t t = blockIdx.x, c = (uint64_t(blockIdx.y) * 256 + threadIdx.x) * V;
   if (c >= n) return;
   float sum[V];
@@ -241,6 +245,7 @@ __global__ __launch_bounds__(256) void join_kernel(const int32_t* __restrict__ r
 template <class T>
 __global__ __launch_bounds__(256) void join_dw_kernel(const int32_t* __restrict__ row_of_pair, uint32_t pairs,
                                                       const float* __restrict__ dwp, uint32_t tiles, T* __restrict__ dw) {
+  begin_after();
   const uint32_t i = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
   if (i >= pairs) return;
   const int32_t row = row_of_pair[i];
@@ -261,6 +266,7 @@ template <class T, int V>
 __global__ __launch_bounds__(256) void dz_kernel(int act, const T* __restrict__ dy, uint64_t ldy,
                                                  const T* __restrict__ pre, uint64_t ldp, T* __restrict__ dz,
                                                  uint64_t ldz, uint64_t rows, uint64_t n, float* __restrict__ part) {
+  begin_after();
   __shared__ float red[8][32 * V];
   const uint64_t c = (uint64_t(blockIdx.y) * 32 + threadIdx.x) * V;
   const uint64_t r0 = uint64_t(blockIdx.x) * kDzRows, r1 = r0 + kDzRows < rows ? r0 + kDzRows : rows;
@@ -301,6 +307,7 @@ __global__ __launch_bounds__(256) void dz_kernel(int act, const T* __restrict__ 
 
 template <class T>
 __global__ void db_kernel(const float* __restrict__ part, uint32_t chunks, uint64_t n, T* __restrict__ db) {
+  begin_after();
   const uint64_t c = uint64_t(blockIdx.x) * blockDim.x + threadIdx.x;
   if (c >= n) return;
   float s = 0.f;
@@ -490,37 +497,34 @@ uint64_t plan_bytes(uint32_t units, uint64_t pairs, uint32_t pad, uint32_t bm) {
 
 int launch_plan(const Plan& p, const Units& u, const int32_t* ids, cudaStream_t s) {
   if (p.pairs <= kSmallPairs && p.units <= kSmallUnits) {
-    plan_small_kernel<<<1, kSmallThreads, 0, s>>>(p, u, ids);
-  } else {
-    plan_count_kernel<<<p.units, kPlanThreads, 0, s>>>(p, u, ids);
-    plan_fill_kernel<<<p.units, kPlanThreads, 0, s>>>(p, ids);
+    return launch(plan_small_kernel, 1, kSmallThreads, 0, 1, false, s, p, u, ids);
   }
-  return int(cudaGetLastError());
+  if (const int e = launch(plan_count_kernel, p.units, kPlanThreads, 0, 1, false, s, p, u, ids)) return e;
+  return launch(plan_fill_kernel, p.units, kPlanThreads, 0, 1, true, s, p, ids);
 }
 
 int launch_join(int dtype, const Plan& p, const float* rows32, uint32_t splits, const float* weights, uint32_t top,
                 uint64_t rows, uint64_t n, const void* residual, uint64_t ldr, void* y, uint64_t ldy, cudaStream_t s) {
+  int e = 0;
   by_type(dtype, [&](auto v) {
     using T = decltype(v);
     const uint64_t stride = uint64_t(p.max_rows) * n;
     const T* r = static_cast<const T*>(residual);
-    if (n % 4 == 0)
-      join_kernel<T, 4><<<dim3(unsigned(rows), unsigned(ceil_div(n, 1024))), 256, 0, s>>>(
-          p.row_of_pair, rows32, splits, stride, weights, top, n, r, ldr, static_cast<T*>(y), ldy);
-    else
-      join_kernel<T, 1><<<dim3(unsigned(rows), unsigned(ceil_div(n, 256))), 256, 0, s>>>(
-          p.row_of_pair, rows32, splits, stride, weights, top, n, r, ldr, static_cast<T*>(y), ldy);
+    const unsigned v4 = n % 4 == 0 ? 4 : 1;
+    e = launch(v4 == 4 ? join_kernel<T, 4> : join_kernel<T, 1>, dim3(unsigned(rows), unsigned(ceil_div(n, 256 * v4))), 256, 0,
+               1, true, s, p.row_of_pair, rows32, splits, stride, weights, top, n, r, ldr, static_cast<T*>(y), ldy);
   });
-  return int(cudaGetLastError());
+  return e;
 }
 
 int launch_join_dw(int dtype, const Plan& p, const float* dwp, uint32_t tiles, void* dw, cudaStream_t s) {
+  int e = 0;
   by_type(dtype, [&](auto v) {
     using T = decltype(v);
-    join_dw_kernel<T><<<unsigned(ceil_div(p.pairs, 8)), 256, 0, s>>>(p.row_of_pair, p.pairs, dwp, tiles,
-                                                                      static_cast<T*>(dw));
+    e = launch(join_dw_kernel<T>, unsigned(ceil_div(p.pairs, 8)), 256, 0, 1, true, s, p.row_of_pair, p.pairs, dwp, tiles,
+               static_cast<T*>(dw));
   });
-  return int(cudaGetLastError());
+  return e;
 }
 
 uint32_t dz_chunks(uint64_t rows, uint64_t) { return uint32_t(ceil_div(rows, kDzRows)); }
@@ -529,19 +533,19 @@ int launch_dz(int dtype, int act, const void* dy, uint64_t ldy, const void* pre,
               uint64_t rows, uint64_t n, void* db, float* part, cudaStream_t s) {
   const bool wide = n % 8 == 0 && on16(dy) && ldy % 8 == 0 && (!dz || (on16(pre) && ldp % 8 == 0 && ldz % 8 == 0));
   const uint32_t chunks = dz_chunks(rows, n);
+  int e = 0;
   by_type(dtype, [&](auto v) {
     using T = decltype(v);
     const T *a = static_cast<const T*>(dy), *b = static_cast<const T*>(pre);
     T* z = static_cast<T*>(dz);
-    if (wide)
-      dz_kernel<T, 8><<<dim3(chunks, unsigned(ceil_div(n, 256))), dim3(32, 8), 0, s>>>(act, a, ldy, b, ldp, z, ldz, rows,
-                                                                                      n, db ? part : nullptr);
-    else
-      dz_kernel<T, 1><<<dim3(chunks, unsigned(ceil_div(n, 32))), dim3(32, 8), 0, s>>>(act, a, ldy, b, ldp, z, ldz, rows,
-                                                                                     n, db ? part : nullptr);
-    if (db) db_kernel<T><<<unsigned(ceil_div(n, 128)), 128, 0, s>>>(part, chunks, n, static_cast<T*>(db));
+    float* sums = db ? part : nullptr;
+    const unsigned each = wide ? 8 : 1;
+    e = launch(wide ? dz_kernel<T, 8> : dz_kernel<T, 1>, dim3(chunks, unsigned(ceil_div(n, 32 * each))), dim3(32, 8), 0, 1,
+               false, s, act, a, ldy, b, ldp, z, ldz, rows, n, sums);
+    if (!e && db)
+      e = launch(db_kernel<T>, unsigned(ceil_div(n, 128)), 128, 0, 1, true, s, part, chunks, n, static_cast<T*>(db));
   });
-  return int(cudaGetLastError());
+  return e;
 }
 
 int launch_route(int dtype, const void* logits, uint64_t ld, uint64_t rows, uint32_t experts, uint32_t top, int norm,

@@ -94,6 +94,7 @@ __global__ __launch_bounds__(kThreads) void stream_kernel(const __grid_constant_
   constexpr int kHalf = 8, kRows = MODE == kUp ? kHalf : 2 * kHalf, kTok = kStreamTile;
   __shared__ float red[kWarps][2 * kHalf][kTok + 1];
   __shared__ float sum[2 * kHalf][kTok + 1];
+  begin_after();
   const Product& p = q.p;
   const uint32_t rank = blockIdx.x % uint32_t(q.splits);
   const int64_t n0 = int64_t(blockIdx.x / uint32_t(q.splits)) * kRows;
@@ -183,23 +184,10 @@ __global__ __launch_bounds__(kThreads) void stream_kernel(const __grid_constant_
   }
 }
 
-template <class T, int MODE, bool WIDE>
-int go(const Params& q, dim3 grid, cudaStream_t s) {
-  cudaLaunchConfig_t c{};
-  c.gridDim = grid;
-  c.blockDim = dim3(kThreads);
-  c.stream = s;
-  cudaLaunchAttribute a[1];
-  a[0].id = cudaLaunchAttributeClusterDimension;
-  a[0].val.clusterDim.x = unsigned(q.splits);
-  a[0].val.clusterDim.y = a[0].val.clusterDim.z = 1;
-  c.attrs = a;
-  c.numAttrs = 1;
-  return int(cudaLaunchKernelEx(&c, stream_kernel<T, MODE, WIDE>, q));
-}
 template <class T, int MODE>
-int go_wide(bool wide, const Params& q, dim3 grid, cudaStream_t s) {
-  return wide ? go<T, MODE, true>(q, grid, s) : go<T, MODE, false>(q, grid, s);
+int go(bool wide, const Params& q, dim3 grid, cudaStream_t s) {
+  return launch(wide ? stream_kernel<T, MODE, true> : stream_kernel<T, MODE, false>, grid, kThreads, 0, q.splits, q.p.after, s,
+                q);
 }
 
 // CTAs of a cluster that split k: enough that the GPU's 148 SMs hold about six CTAs each, as long as a warp keeps a span
@@ -241,12 +229,12 @@ int launch_stream(int dtype, const Product& p, uint32_t top, const Plan* plan, c
   q.splits = splits_for(m_tiles * n_tiles, p.k);
   const dim3 grid(unsigned(n_tiles * q.splits), unsigned(m_tiles));
   if (dtype == TSB_BF16)
-    return mode == kLin ? go_wide<__nv_bfloat16, kLin>(wide, q, grid, s)
-           : mode == kUp ? go_wide<__nv_bfloat16, kUp>(wide, q, grid, s)
-                         : go_wide<__nv_bfloat16, kDown>(wide, q, grid, s);
-  return mode == kLin ? go_wide<__half, kLin>(wide, q, grid, s)
-         : mode == kUp ? go_wide<__half, kUp>(wide, q, grid, s)
-                       : go_wide<__half, kDown>(wide, q, grid, s);
+    return mode == kLin ? go<__nv_bfloat16, kLin>(wide, q, grid, s)
+           : mode == kUp ? go<__nv_bfloat16, kUp>(wide, q, grid, s)
+                         : go<__nv_bfloat16, kDown>(wide, q, grid, s);
+  return mode == kLin ? go<__half, kLin>(wide, q, grid, s)
+         : mode == kUp ? go<__half, kUp>(wide, q, grid, s)
+                       : go<__half, kDown>(wide, q, grid, s);
 }
 
 }  // namespace ops

@@ -329,6 +329,7 @@ __global__ __launch_bounds__(kThreads, 1) void tc_kernel(const __grid_constant__
   if constexpr (CG == 2) cluster_sync();
   fence_after();
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(words);
+  begin_after();
   const int half_n = q.bn / CG;              // columns of B that this CTA stages (of a single B)
   const int chunks = (half_n + 63) / 64;     // MN-major B
 
@@ -458,6 +459,7 @@ __global__ __launch_bounds__(kThreads, 1) void tc_kernel(const __grid_constant__
 // rows of grouped buffers: row r is source row pair_of_row[r] / top, padding rows are zeros
 __global__ __launch_bounds__(256) void gather_kernel(const __grid_constant__ Plan plan, uint32_t top, const uint4* src,
                                                      uint64_t ld16, uint32_t n16, uint4* dst) {
+  begin_after();
   const uint32_t r = blockIdx.x;
   if (int32_t(r) >= plan.head[1]) return;
   const int32_t pair = plan.pair_of_row[r];
@@ -468,21 +470,10 @@ __global__ __launch_bounds__(256) void gather_kernel(const __grid_constant__ Pla
 
 template <class T, int MODE, int ACT, int CG>
 int go_pair(const Maps& maps, const Params& q, int grid, cudaStream_t s) {
+  static std::atomic<uint64_t> devices{0};
   const auto kernel = tc_kernel<T, MODE, ACT, CG>;
-  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
-  if (e != cudaSuccess) return int(e);
-  cudaLaunchConfig_t c{};
-  c.gridDim = dim3(unsigned(grid * CG));
-  c.blockDim = dim3(kThreads);
-  c.dynamicSmemBytes = kSmemBytes;
-  c.stream = s;
-  cudaLaunchAttribute a[1];
-  a[0].id = cudaLaunchAttributeClusterDimension;
-  a[0].val.clusterDim.x = CG;
-  a[0].val.clusterDim.y = a[0].val.clusterDim.z = 1;
-  c.attrs = a;
-  c.numAttrs = 1;
-  return int(cudaLaunchKernelEx(&c, kernel, maps, q));
+  if (const int e = allow_smem(reinterpret_cast<const void*>(kernel), devices)) return e;
+  return launch(kernel, unsigned(grid * CG), kThreads, kSmemBytes, CG, q.p.after, s, maps, q);
 }
 template <class T, int MODE, int ACT>
 int go(const Maps& maps, const Params& q, int grid, cudaStream_t s) {
@@ -541,9 +532,8 @@ bool tc_fits(const Operand& o, const Units* u) {
 }
 
 int launch_gather(const Plan& plan, uint32_t top, const void* src, uint64_t ld, uint64_t n, void* dst, cudaStream_t s) {
-  gather_kernel<<<plan.max_rows, 256, 0, s>>>(plan, top, static_cast<const uint4*>(src), ld / 8, uint32_t(n / 8),
-                                              static_cast<uint4*>(dst));
-  return int(cudaGetLastError());
+  return launch(gather_kernel, plan.max_rows, 256, 0, 1, true, s, plan, top, static_cast<const uint4*>(src), ld / 8,
+                uint32_t(n / 8), static_cast<uint4*>(dst));
 }
 
 int launch_tc(int dtype, const Product& p, const Plan* plan, const Units* u, cudaStream_t s) {

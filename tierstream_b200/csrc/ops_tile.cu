@@ -75,6 +75,7 @@ __global__ __launch_bounds__(kThreads) void tile_kernel(const __grid_constant__ 
   __shared__ __align__(16) T sa[64 * kLd];
   __shared__ __align__(16) T sb[64 * kLd];
   __shared__ float red[2][64];
+  begin_after();
   Group g{0, 0, 0, p.m};
   int64_t m0 = int64_t(blockIdx.x) * 64;
   if (p.grouped) {
@@ -189,16 +190,14 @@ __global__ __launch_bounds__(kThreads) void tile_kernel(const __grid_constant__ 
 }
 
 template <class T>
-int launch(const Product& p, const Plan& plan, const Units& u, cudaStream_t s) {
+int go(const Product& p, const Plan& plan, const Units& u, cudaStream_t s) {
   // unit tiles of `plan.bm` rows are walked as 64-row tiles: the plan handed here was made with bm = 64
   const dim3 grid(p.grouped ? plan.max_tiles : unsigned(ceil_div(p.m, 64)), unsigned(ceil_div(p.n, 64)),
                   p.per_unit ? plan.units : 1);
   int accs = 1;
   for (int i = 0; i < p.segs; ++i) accs = p.acc[i] + 1 > accs ? p.acc[i] + 1 : accs;
-  if (accs == 1) tile_kernel<T, 1><<<grid, kThreads, 0, s>>>(p, plan, u);
-  else if (accs == 2) tile_kernel<T, 2><<<grid, kThreads, 0, s>>>(p, plan, u);
-  else tile_kernel<T, 3><<<grid, kThreads, 0, s>>>(p, plan, u);
-  return int(cudaGetLastError());
+  return launch(accs == 1 ? tile_kernel<T, 1> : accs == 2 ? tile_kernel<T, 2> : tile_kernel<T, 3>, grid, kThreads, 0, 1,
+                p.after, s, p, plan, u);
 }
 
 }  // namespace
@@ -206,7 +205,7 @@ int launch(const Product& p, const Plan& plan, const Units& u, cudaStream_t s) {
 int launch_tile(int dtype, const Product& p, const Plan* plan, const Units* units, cudaStream_t s) {
   const Plan pl = plan ? *plan : Plan{};
   const Units u = units ? *units : Units{};
-  return dtype == TSB_BF16 ? launch<__nv_bfloat16>(p, pl, u, s) : launch<__half>(p, pl, u, s);
+  return dtype == TSB_BF16 ? go<__nv_bfloat16>(p, pl, u, s) : go<__half>(p, pl, u, s);
 }
 
 }  // namespace ops
