@@ -85,10 +85,18 @@ __device__ __forceinline__ const char* unit_part(const Units& u, int p, int32_t 
 // the value where the results are rounded to 2^-9 or 2^-12; (1 + tanh q) / 2 is the logistic of 2 q.
 __device__ __forceinline__ float logistic(float z) { return __fdividef(1.f, 1.f + __expf(-z)); }
 constexpr float kGelu1 = 1.5957691216057308f, kGelu3 = 0.071354816272600250f;  // 2 sqrt(2 / pi), and times 0.044715
+// The normal distribution's integral up to z by Abramowitz and Stegun's 7.1.26, off by at most 7.5e-8 (32-bit
+// (1 + erf) / 2 is off by 6e-8); `e` is exp(-z^2 / 2), which its slope needs too.
+__device__ __forceinline__ float normal_upto(float z, float e) {
+  const float t = __fdividef(1.f, 1.f + 0.23164189f * fabsf(z));  // 0.3275911 / sqrt 2
+  const float tail = 0.5f * e * t *
+                     (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f))));
+  return z < 0.f ? tail : 1.f - tail;
+}
 template <int ACT>
 __device__ __forceinline__ float act_of(float z) {
   if constexpr (ACT == TSB_ACT_SILU) return z * logistic(z);
-  if constexpr (ACT == TSB_ACT_GELU) return 0.5f * z * (1.f + erff(z * 0.70710678118654752f));
+  if constexpr (ACT == TSB_ACT_GELU) return z * normal_upto(z, __expf(-0.5f * z * z));
   if constexpr (ACT == TSB_ACT_GELU_TANH) return z * logistic(z * (kGelu1 + kGelu3 * z * z));
   if constexpr (ACT == TSB_ACT_RELU) return z < 0.f ? 0.f : z;  // (a NaN stays one)
   return z;
@@ -99,8 +107,10 @@ __device__ __forceinline__ float slope_of(float z) {
     const float p = logistic(z);
     return p * (1.f + z * (1.f - p));
   }
-  if constexpr (ACT == TSB_ACT_GELU)
-    return 0.5f * (1.f + erff(z * 0.70710678118654752f)) + z * __expf(-0.5f * z * z) * 0.39894228040143268f;
+  if constexpr (ACT == TSB_ACT_GELU) {
+    const float e = __expf(-0.5f * z * z);
+    return normal_upto(z, e) + z * e * 0.39894228040143268f;
+  }
   if constexpr (ACT == TSB_ACT_GELU_TANH) {
     const float p = logistic(z * (kGelu1 + kGelu3 * z * z));
     return p + z * p * (1.f - p) * (kGelu1 + 3.f * kGelu3 * z * z);
@@ -199,6 +209,10 @@ int launch_plan(const Plan& p, const Units& u, const int32_t* ids, cudaStream_t 
 // y[t] = residual[t] + sum over k, then over the splits, of w[t][k] x rows32[split][row_of_pair[t top + k]]
 int launch_join(int dtype, const Plan& p, const float* rows32, uint32_t splits, const float* weights, uint32_t top,
                 uint64_t rows, uint64_t n, const void* residual, uint64_t ldr, void* y, uint64_t ldy, cudaStream_t s);
+// y = act(sum over the splits of rows32 + bias) + residual, pre the sum itself
+int launch_join_linear(int dtype, int act, const float* rows32, uint32_t splits, uint64_t rows, uint64_t n,
+                       const void* bias, const void* residual, uint64_t ldr, void* y, uint64_t ldy, void* pre,
+                       uint64_t ldp, cudaStream_t s);
 // dweights[pair] = sum over tiles of dwp[row][tile]
 int launch_join_dw(int dtype, const Plan& p, const float* dwp, uint32_t tiles, void* dw, cudaStream_t s);
 int launch_route(int dtype, const void* logits, uint64_t ld, uint64_t rows, uint32_t experts, uint32_t top, int norm,
@@ -225,13 +239,16 @@ int launch_stream(int dtype, const Product& p, uint32_t top, const Plan* plan, c
 // Gathered operands are gathered first: launch_gather copies n columns of every grouped row (n a multiple of 8).
 constexpr uint32_t kTcRows = 256;
 bool tc_fits(const Operand& o, const Units* units);
+int tc_columns(int64_t m, int64_t n, int sms);
 int launch_gather(const Plan& plan, uint32_t top, const void* src, uint64_t ld, uint64_t n, void* dst, cudaStream_t s);
 int launch_tc(int dtype, const Product& p, const Plan* plan, const Units* units, cudaStream_t s);
 int ops_take_timeouts(uint32_t* out);
 
 // ops_group.cu: the grouped products with the unit's matrix as rows, for groups of any length (the plan's bm kGroupRows)
 constexpr uint32_t kGroupRows = 128;
-int launch_group(int dtype, const Product& p, const Plan* plan, const Units* units, cudaStream_t s);
+// plan NULL: one matrix p.b[0] and p.m rows of p.a[0]. kEpiRows32 may split the sum over k: split j's rows at rows32 +
+// j x rows x n (rows: the plan's max_rows, or p.m).
+int launch_group(int dtype, const Product& p, int splits, const Plan* plan, const Units* units, cudaStream_t s);
 int group_take_timeouts(uint32_t* out);
 
 }  // namespace ops

@@ -1,5 +1,7 @@
 // The entry points of the operators (include/tierstream/tsb.h): argument checks, the workspace's layout and the choice
 // of kernels.
+#include <algorithm>
+#include <cmath>
 #include <cstring>
 #include <string>
 
@@ -66,14 +68,58 @@ Operand of_unit(int part, int64_t s_i, int64_t s_k) { return {nullptr, s_i, s_k,
 // 352 MB, 663 against 644 at two of 128 of 38 MB; at four 800 against 750 there).
 constexpr uint64_t kStreamRows = kStreamTile, kStreamEach = 2;
 
-// One matrix product: on the tensor cores' own path when TMA can read both operands (rows on 16 bytes), else by the
-// kernel for every alignment.
-int product(int dtype, const Product& p, cudaStream_t s) {
-  if (p.epi == kEpiLinear && uint64_t(p.m) <= kStreamRows && p.k % 8 == 0 && tc_fits(p.a[0], nullptr) &&
-      tc_fits(p.b[0], nullptr))
-    return launch_stream(dtype, p, 1, nullptr, nullptr, s);
-  if (tc_fits(p.a[0], nullptr) && tc_fits(p.b[0], nullptr)) return launch_tc(dtype, p, nullptr, nullptr, s);
-  return launch_tile(dtype, p, nullptr, nullptr, s);
+// How a plain product runs. The times are fits, in us, to what the kernels took a 64-wide slice of k on this GPU (148 SMs):
+// 0.10 + 0.0012 columns for a pair of CTAs (0.254 measured at 128 columns, 0.405 at 256; 0.2 at least), 0.17 + 0.00098
+// columns for a single one, about 6 for a launch's start and end, 3 for the join's, which reads 32-bit rows at 6 TB/s.
+struct How {
+  enum Kind { kAny, kStream, kTc, kGroup } kind;
+  int splits;
+};
+constexpr int kSms = 148;
+double slice_us(double columns) { return columns < 84 ? 0.2 : 0.10 + 0.0012 * columns; }
+
+How how(const Product& p) {
+  if (!tc_fits(p.a[0], nullptr) || !tc_fits(p.b[0], nullptr)) return {How::kAny, 1};
+  const bool forward = p.epi == kEpiLinear;
+  if (forward && uint64_t(p.m) <= kStreamRows && p.k % 8 == 0) return {How::kStream, 1};
+  if (p.a[0].s_k != 1) return {How::kTc, 1};  // (dw: a sum over rows)
+  const double kb = double(ceil_div(uint64_t(p.k), 64)), bytes = 2.0 * double(p.n) * double(p.k) / 6.5e6;
+  // the matrix as columns, in the columns a tile that launch_tc would take
+  const int cg = p.m > 128 ? 2 : 1;
+  const int bn = tc_columns(p.m, p.n, kSms);
+  const double waves = double(ceil_div(ceil_div(uint64_t(p.m), 128 * cg) * ceil_div(uint64_t(p.n), uint64_t(bn)), uint64_t(kSms / cg)));
+  const double tc = 6 + std::max(bytes, waves * kb * (cg == 2 ? slice_us(bn) : 0.17 + 0.00098 * bn));
+  // the matrix as rows, k split
+  const uint64_t tiles = ceil_div(uint64_t(p.m), 2 * kGroupRows);
+  const double cols = double((ceil_div(uint64_t(p.m), tiles) + 31) / 32 * 32);
+  How best{How::kTc, 1};
+  double least = tc;
+  for (int s = 1; s <= 8 && s * 4 <= kb; ++s) {
+    const double w = double(ceil_div(tiles * ceil_div(uint64_t(p.n), 256) * s, kSms / 2));
+    const double us = 9 + std::max(bytes, w * std::ceil(kb / s) * slice_us(cols)) + s * double(p.m) * double(p.n) * 8 / 6e6;
+    if (us < least) least = us, best = {How::kGroup, s};
+  }
+  return best;
+}
+
+uint64_t product_bytes(const Product& p) {
+  const How h = how(p);
+  return h.kind == How::kGroup ? uint64_t(h.splits) * uint64_t(p.m) * uint64_t(p.n) * 4 : 0;
+}
+int product(int dtype, const Product& p, float* rows32, cudaStream_t s) {
+  const How h = how(p);
+  switch (h.kind) {
+    case How::kStream: return launch_stream(dtype, p, 1, nullptr, nullptr, s);
+    case How::kTc: return launch_tc(dtype, p, nullptr, nullptr, s);
+    case How::kAny: return launch_tile(dtype, p, nullptr, nullptr, s);
+    case How::kGroup: break;
+  }
+  Product r = p;
+  r.epi = kEpiRows32;
+  r.rows32 = rows32;
+  if (const int e = launch_group(dtype, r, h.splits, nullptr, nullptr, s)) return e;
+  return launch_join_linear(dtype, p.act, rows32, uint32_t(h.splits), uint64_t(p.m), uint64_t(p.n), p.bias, p.residual,
+                            uint64_t(p.ldr), p.out, uint64_t(p.ldo), p.pre, uint64_t(p.ldp), s);
 }
 
 // ---- linear ----
@@ -91,11 +137,17 @@ void check_linear(const tsb_linear_args* a) {
        fn, "a leading dimension is shorter than its row");
 }
 
+Product linear_product(const tsb_linear_args* a);
 void linear(const tsb_linear_args* a) {
   const char* fn = "tsb_linear";
   check_linear(a);
   if (!a->rows) return;
-  cudaStream_t s = static_cast<cudaStream_t>(a->stream);
+  const Product p = linear_product(a);
+  need_workspace(fn, a->workspace, a->workspace_bytes, product_bytes(p));
+  ck(product(int(a->dtype), p, static_cast<float*>(a->workspace), static_cast<cudaStream_t>(a->stream)), fn, "launch");
+}
+
+Product linear_product(const tsb_linear_args* a) {
   Product p{};
   p.segs = 1;
   p.a[0] = dense(a->x, int64_t(a->ldx), 1);
@@ -107,7 +159,7 @@ void linear(const tsb_linear_args* a) {
   p.bias = a->bias;
   p.residual = a->residual, p.ldr = int64_t(a->ldr);
   p.pre = a->pre, p.ldp = int64_t(a->ldp);
-  ck(product(int(a->dtype), p, s), fn, "launch");
+  return p;
 }
 
 void check_linear_back(const tsb_linear_grad_args* a) {
@@ -126,18 +178,33 @@ void check_linear_back(const tsb_linear_grad_args* a) {
        fn, "a leading dimension is shorter than its row");
 }
 
+Product dx_product(const tsb_linear_grad_args* a, const void* dz, uint64_t ldz) {
+  Product p{};
+  p.segs = 1;
+  p.a[0] = dense(dz, int64_t(ldz), 1);
+  p.b[0] = dense(a->w, 1, int64_t(a->ldw));
+  p.m = int64_t(a->rows), p.n = int64_t(a->k), p.k = int64_t(a->n);
+  p.epi = kEpiStore;
+  p.out = a->dx, p.ldo = int64_t(a->lddx);
+  return p;
+}
+
 struct LinearBackSpace {
-  void* dz;
+  const void* dz;  // dy itself without an activation
   uint64_t ldz;
-  float* part;
+  float *part, *rows32;
   uint64_t bytes;
 };
 LinearBackSpace linear_back_space(const tsb_linear_grad_args* a) {
   Arena w{static_cast<char*>(a->workspace)};
-  LinearBackSpace r{};
-  r.ldz = (a->n + 7) / 8 * 8;
-  if (a->rows && a->act != TSB_ACT_NONE) r.dz = w.take(a->rows * r.ldz * 2);
-  if (a->rows && a->db) r.part = static_cast<float*>(w.take(uint64_t(dz_chunks(a->rows, a->n)) * a->n * 4));
+  LinearBackSpace r{a->dy, a->lddy, nullptr, nullptr, 0};
+  if (!a->rows) return r;
+  if (a->act != TSB_ACT_NONE) {
+    r.ldz = (a->n + 7) / 8 * 8;
+    r.dz = w.take(a->rows * r.ldz * 2);
+  }
+  if (a->db) r.part = static_cast<float*>(w.take(uint64_t(dz_chunks(a->rows, a->n)) * a->n * 4));
+  if (a->dx) r.rows32 = static_cast<float*>(w.take(product_bytes(dx_product(a, r.dz, r.ldz))));
   r.bytes = w.used;
   return r;
 }
@@ -153,35 +220,26 @@ void linear_back(const tsb_linear_grad_args* a) {
   }
   const LinearBackSpace w = linear_back_space(a);
   need_workspace(fn, a->workspace, a->workspace_bytes, w.bytes);
-  const void* dz = a->dy;
-  uint64_t ldz = a->lddy;
   const bool slope = a->act != TSB_ACT_NONE;
-  if (slope) dz = w.dz, ldz = w.ldz;
   if (slope || a->db)
-    ck(launch_dz(int(a->dtype), int(a->act), a->dy, a->lddy, a->pre, a->ldp, slope ? w.dz : nullptr, w.ldz, a->rows,
-                 a->n, a->db, w.part, s),
+    ck(launch_dz(int(a->dtype), int(a->act), a->dy, a->lddy, a->pre, a->ldp, slope ? const_cast<void*>(w.dz) : nullptr,
+                 w.ldz, a->rows, a->n, a->db, w.part, s),
        fn, "slope");
   if (a->dx) {
-    Product p{};
-    p.segs = 1;
-    p.a[0] = dense(dz, int64_t(ldz), 1);
-    p.b[0] = dense(a->w, 1, int64_t(a->ldw));
-    p.m = int64_t(a->rows), p.n = int64_t(a->k), p.k = int64_t(a->n);
+    Product p = dx_product(a, w.dz, w.ldz);
     p.after = slope || a->db;
-    p.epi = kEpiStore;
-    p.out = a->dx, p.ldo = int64_t(a->lddx);
-    ck(product(int(a->dtype), p, s), fn, "dx");
+    ck(product(int(a->dtype), p, w.rows32, s), fn, "dx");
   }
   if (a->dw) {
     Product p{};
     p.segs = 1;
-    p.a[0] = dense(dz, 1, int64_t(ldz), 1);
+    p.a[0] = dense(w.dz, 1, int64_t(w.ldz), 1);
     p.b[0] = dense(a->x, 1, int64_t(a->ldx), 1);
     p.m = int64_t(a->n), p.n = int64_t(a->k), p.k = int64_t(a->rows);
     p.after = slope || a->db || a->dx;
     p.epi = kEpiStore;
     p.out = a->dw, p.ldo = int64_t(a->lddw);
-    ck(product(int(a->dtype), p, s), fn, "dw");
+    ck(product(int(a->dtype), p, nullptr, s), fn, "dw");
   }
 }
 
@@ -233,12 +291,29 @@ bool ffn_rows16(const tsb_units* u, uint64_t hidden, uint64_t ffn, const void* x
 // On the tensor cores' own path a unit's matrix supplies the rows and the group's rows the columns, except for groups so
 // long that whole 256-row tiles waste little of them.
 uint32_t tc_tile(uint64_t each) { return each >= 4 * kTcRows ? kTcRows : kGroupRows; }
-int launch_grouped(int dtype, const Product& p, const Plan* plan, const Units* u, cudaStream_t s) {
-  return p.grouped && plan->bm == kGroupRows ? launch_group(dtype, p, plan, u, s) : launch_tc(dtype, p, plan, u, s);
+int launch_grouped(int dtype, const Product& p, int splits, const Plan* plan, const Units* u, cudaStream_t s) {
+  return p.grouped && plan->bm == kGroupRows ? launch_group(dtype, p, splits, plan, u, s) : launch_tc(dtype, p, plan, u, s);
+}
+
+// Into how many parts a grouped product's sum over `kb` slices is cut: the tiles of about half-full groups, dealt to 74
+// pairs, end in waves, which shorter tiles fill better; each part costs its 32-bit rows' way to the join and back.
+int grouped_splits(const Plan& plan, uint64_t n, double kb) {
+  if (plan.bm != kGroupRows) return 1;
+  const double met = double(std::min<uint64_t>(plan.pairs, plan.units)), each = plan.pairs / met;
+  const double tiles = double(ceil_div(n, 256)) * (plan.pairs / 256.0 + met / 2);
+  const double us = slice_us(std::min(256.0, std::ceil(each / 32) * 32));
+  int best = 1;
+  double least = 0;
+  for (int s = 1; s <= 4 && s * 8 <= kb; ++s) {
+    const double c = std::ceil(tiles * s / (kSms / 2)) * (kb / s * us + 2) + s * double(plan.max_rows) * double(n) * 8 / 6e6;
+    if (s == 1 || c < least) least = c, best = s;
+  }
+  return best;
 }
 
 struct FfnSpace {
   Plan plan;
+  int splits;
   bool tc, stream;
   void* xs;
   void* h;
@@ -258,7 +333,8 @@ FfnSpace ffn_space(const tsb_ffn_args* a) {
   r.plan = plan_at(w.take(plan_bytes(a->units->n_units, pairs, 1, bm)), a->units->n_units, pairs, 1, bm);
   if (r.tc) r.xs = w.take(uint64_t(r.plan.max_rows) * a->hidden * 2);
   r.h = w.take(uint64_t(r.plan.max_rows) * a->ffn * 2);
-  r.rows32 = static_cast<float*>(w.take(uint64_t(r.plan.max_rows) * a->hidden * 4));
+  r.splits = r.tc ? grouped_splits(r.plan, a->hidden, double(ceil_div(a->ffn, 64))) : 1;
+  r.rows32 = static_cast<float*>(w.take(uint64_t(r.splits) * r.plan.max_rows * a->hidden * 4));
   r.bytes = w.used;
   return r;
 }
@@ -294,16 +370,16 @@ void ffn(const tsb_ffn_args* a) {
   p.epi = kEpiUp;
   p.act = int(a->act);
   p.out = w.h, p.ldo = f;
-  const auto go = [&](int dtype, const Product& pr, const Plan* pl, const Units* un, cudaStream_t st) {
-    return w.stream ? launch_stream(dtype, pr, a->top, pl, un, st)
-           : w.tc   ? launch_grouped(dtype, pr, pl, un, st)
-                    : launch_tile(dtype, pr, pl, un, st);
+  const auto go = [&](const Product& pr, int splits) {
+    return w.stream ? launch_stream(int(a->dtype), pr, a->top, &w.plan, &u, s)
+           : w.tc   ? launch_grouped(int(a->dtype), pr, splits, &w.plan, &u, s)
+                    : launch_tile(int(a->dtype), pr, &w.plan, &u, s);
   };
   if (w.tc) {
     ck(launch_gather(w.plan, a->top, a->x, a->ldx, a->hidden, w.xs, s), fn, "gather");
     p.a[0] = p.a[1] = dense(w.xs, d, 1);
   }
-  ck(go(int(a->dtype), p, &w.plan, &u, s), fn, "gate and up");
+  ck(go(p, 1), fn, "gate and up");
   Product q{};
   q.grouped = 1;
   q.after = true;
@@ -313,14 +389,15 @@ void ffn(const tsb_ffn_args* a) {
   q.n = d, q.k = f;
   q.epi = kEpiRows32;
   q.rows32 = w.rows32;
-  ck(go(int(a->dtype), q, &w.plan, &u, s), fn, "down");
-  ck(launch_join(int(a->dtype), w.plan, w.rows32, 1, a->weights, a->top, a->rows, a->hidden, a->residual, a->ldr, a->y,
+  ck(go(q, w.splits), fn, "down");
+  ck(launch_join(int(a->dtype), w.plan, w.rows32, uint32_t(w.splits), a->weights, a->top, a->rows, a->hidden, a->residual, a->ldr, a->y,
                  a->ldy, s),
      fn, "join");
 }
 
 struct FfnBackSpace {
   Plan plan;
+  int splits;
   bool tc;
   void *xs, *dys, *dg, *du, *hw;
   float *dwp, *rows32;
@@ -345,7 +422,8 @@ FfnBackSpace ffn_back_space(const tsb_ffn_grad_args* a) {
   if (a->dgate) r.hw = w.take(uint64_t(r.plan.max_rows) * a->ffn * 2);
   r.dw_tiles = r.tc ? (bm == kGroupRows ? 8 * uint32_t(ceil_div(a->ffn, 256)) : 2 * uint32_t(ceil_div(a->ffn, 128))) : uint32_t(ceil_div(a->ffn, kTileN));
   if (a->dweights) r.dwp = static_cast<float*>(w.take(uint64_t(r.plan.max_rows) * r.dw_tiles * 4));
-  if (a->dx) r.rows32 = static_cast<float*>(w.take(uint64_t(r.plan.max_rows) * a->hidden * 4));
+  r.splits = r.tc ? grouped_splits(r.plan, a->hidden, 2 * double(ceil_div(a->ffn, 64))) : 1;
+  if (a->dx) r.rows32 = static_cast<float*>(w.take(uint64_t(r.splits) * r.plan.max_rows * a->hidden * 4));
   r.bytes = w.used;
   return r;
 }
@@ -377,7 +455,9 @@ void ffn_back(const tsb_ffn_grad_args* a) {
   const Units u = units_of(a->units);
   const int dt = int(a->dtype);
   ck(launch_plan(w.plan, u, a->ids, s), fn, "plan");
-  const auto go = w.tc ? launch_grouped : launch_tile;
+  const auto go = [&](const Product& pr, int splits) {
+    return w.tc ? launch_grouped(dt, pr, splits, &w.plan, &u, s) : launch_tile(dt, pr, &w.plan, &u, s);
+  };
   Operand x_rows = gathered(a->x, int64_t(a->ldx), 1, w.plan, a->top),
           dy_rows = gathered(a->dy, int64_t(a->lddy), 1, w.plan, a->top),
           x_sum = gathered(a->x, 1, int64_t(a->ldx), w.plan, a->top, 1),
@@ -407,7 +487,7 @@ void ffn_back(const tsb_ffn_grad_args* a) {
     p.dg = w.dg, p.du = w.du, p.hw = w.hw, p.ldo = f;
     p.dwp = w.dwp, p.ld_dwp = w.dw_tiles;
     p.weights = a->weights;
-    ck(go(dt, p, &w.plan, &u, s), fn, "gate, up and dh");
+    ck(go(p, 1), fn, "gate, up and dh");
   }
   if (a->dweights) ck(launch_join_dw(dt, w.plan, w.dwp, w.dw_tiles, a->dweights, s), fn, "dweights");
   if (a->dx) {
@@ -422,8 +502,8 @@ void ffn_back(const tsb_ffn_grad_args* a) {
     p.n = d, p.k = f;
     p.epi = kEpiRows32;
     p.rows32 = w.rows32;
-    ck(go(dt, p, &w.plan, &u, s), fn, "dx");
-    ck(launch_join(dt, w.plan, w.rows32, 1, nullptr, a->top, a->rows, a->hidden, nullptr, 0, a->dx, a->lddx, s), fn,
+    ck(go(p, w.splits), fn, "dx");
+    ck(launch_join(dt, w.plan, w.rows32, uint32_t(w.splits), nullptr, a->top, a->rows, a->hidden, nullptr, 0, a->dx, a->lddx, s), fn,
        "join");
   }
   if (a->dgate) {
@@ -438,15 +518,15 @@ void ffn_back(const tsb_ffn_grad_args* a) {
     p.b[0] = x_sum;
     p.a[0] = dense(w.dg, 1, f, 1);
     p.out = a->dgate;
-    ck(go(dt, p, &w.plan, &u, s), fn, "dgate");
+    ck(go(p, 1), fn, "dgate");
     p.a[0] = dense(w.du, 1, f, 1);
     p.out = a->dup;
-    ck(go(dt, p, &w.plan, &u, s), fn, "dup");
+    ck(go(p, 1), fn, "dup");
     p.m = d, p.n = f, p.ldo = f;
     p.a[0] = dy_sum;
     p.b[0] = dense(w.hw, 1, f, 1);
     p.out = a->ddown;
-    ck(go(dt, p, &w.plan, &u, s), fn, "ddown");
+    ck(go(p, 1), fn, "ddown");
   }
 }
 
@@ -464,7 +544,14 @@ uint64_t bytes_of(const A* a, void (*check)(const A*), F&& space) {
 
 extern "C" {
 
-uint64_t tsb_linear_workspace(const tsb_linear_args*) { return 0; }
+uint64_t tsb_linear_workspace(const tsb_linear_args* a) {
+  return bytes_of(a, check_linear, [](const tsb_linear_args* b) {
+    struct {
+      uint64_t bytes;
+    } r{product_bytes(linear_product(b))};
+    return r;
+  });
+}
 ss_status tsb_linear(const tsb_linear_args* a) {
   return run([&] { linear(a); });
 }

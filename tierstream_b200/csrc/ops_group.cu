@@ -19,7 +19,8 @@ namespace {
 
 __device__ uint32_t g_group_timeouts;
 
-enum Mode { kUp, kUpBack, kDown, kDx };
+// kLin, kLinDx: one matrix (k contiguous, or its rows contiguous) and host-known rows, as a single group
+enum Mode { kUp, kUpBack, kDown, kDx, kLin, kLinDx };
 
 struct Params {
   Plan plan;
@@ -28,6 +29,9 @@ struct Params {
   int32_t list;      // which of the plan's tile lists has them
   int32_t f_tiles;   // tiles of 256 rows of the matrix
   int32_t k_blocks;  // of a segment
+  int32_t rows;      // kLin, kLinDx: rows of x
+  int32_t splits;    // parts of the sum over k, each with its own 32-bit rows
+  int32_t split_rows;  // rows of a split's 32-bit rows
   int32_t vec;       // `out` maps are made
   int32_t stages, stage_bytes;
 };
@@ -36,28 +40,47 @@ struct Maps {
 };
 
 struct Tile {
-  int unit, slot, row0;  // row0: the tile's first grouped row
+  int slot, row0;        // row0: the tile's first grouped row
   int rows, cols;        // rows of the group to store, and the products' columns (a multiple of 32)
   int f0;
+  int split, kb0, kb1;   // its slices of k, over all segments
 };
 
 // Tile L: groups in unit order, inside a group chunks of up to 8 tiles of its rows, inside a chunk the matrix' tiles, the
 // chunk's row tiles innermost: tiles running at the same time share a unit's matrix rows from L2.
+template <int MODE>
 __device__ __forceinline__ bool tile_at(const Params& q, int L, Tile& t) {
   constexpr int kChunk = 8;
-  const int i = L / q.f_tiles;
-  if (i >= q.plan.head[2 * q.list]) return false;
-  t.unit = q.plan.tile_unit[q.list][i];
-  t.slot = q.plan.slot[t.unit];
-  const int cnt = (q.plan.cnt[t.unit] + int(q.plan.pad) - 1) / int(q.plan.pad) * int(q.plan.pad);  // padding rows too
+  const int all = (MODE == kDx ? 2 : 1) * q.k_blocks;
+  t.split = 0, t.kb0 = 0, t.kb1 = all;
+  if (MODE != kUp && MODE != kUpBack && q.splits > 1) {
+    t.split = L % q.splits;
+    L /= q.splits;
+    t.kb0 = all * t.split / q.splits;
+    t.kb1 = all * (t.split + 1) / q.splits;
+  }
+  int cnt, local, first;
+  if constexpr (MODE == kLin || MODE == kLinDx) {
+    cnt = q.rows;
+    local = L;
+    first = t.slot = 0;
+  } else {
+    const int i = L / q.f_tiles;
+    if (i >= q.plan.head[2 * q.list]) return false;
+    const int unit = q.plan.tile_unit[q.list][i];
+    t.slot = q.plan.slot[unit];
+    cnt = (q.plan.cnt[unit] + int(q.plan.pad) - 1) / int(q.plan.pad) * int(q.plan.pad);  // padding rows too
+    local = L - (i - q.plan.tile_m0[q.list][i] / q.bm) * q.f_tiles;
+    first = q.plan.off[unit];
+  }
   const int tiles = (cnt + q.bm - 1) / q.bm;
+  if ((MODE == kLin || MODE == kLinDx) && local >= tiles * q.f_tiles) return false;
   const int size = ((cnt + tiles - 1) / tiles + 31) & ~31;
-  const int local = L - (i - q.plan.tile_m0[q.list][i] / q.bm) * q.f_tiles;
   const int chunk = local / (kChunk * q.f_tiles), in = local - chunk * kChunk * q.f_tiles;
   const int width = min(kChunk, tiles - chunk * kChunk);
   const int f = in / width, m0 = (chunk * kChunk + in - f * width) * size;
   t.f0 = f * 2 * kBM;
-  t.row0 = q.plan.off[t.unit] + m0;
+  t.row0 = first + m0;
   t.rows = min(size, cnt - m0);
   t.cols = (t.rows + 31) & ~31;
   return true;
@@ -65,15 +88,15 @@ __device__ __forceinline__ bool tile_at(const Params& q, int L, Tile& t) {
 
 template <int MODE>
 struct Traits {
-  static constexpr int segs = MODE == kUpBack || MODE == kDx ? 2 : 1;
+  static constexpr int segs = MODE == kUpBack ? 2 : 1;  // sums of their own (dx's two matrices add into one)
   static constexpr int bufs = MODE == kUpBack ? 1 : 2;
   __host__ __device__ static constexpr bool both(int s) { return (MODE == kUp && s == 0) || (MODE == kUpBack && s == 1); }
   // the matrix with its rows (of the tile) contiguous
-  __host__ __device__ static constexpr bool a_mn(int s) { return MODE == kDx || (MODE == kUpBack && s == 0); }
+  __host__ __device__ static constexpr bool a_mn(int s) { return MODE == kDx || MODE == kLinDx || (MODE == kUpBack && s == 0); }
   __host__ __device__ static constexpr int a_map(int s) {
-    return MODE == kDown ? 2 : MODE == kUpBack && s == 0 ? 2 : MODE == kDx ? s : 0;
+    return MODE == kDown || (MODE == kUpBack && s == 0) ? 2 : 0;
   }
-  __host__ __device__ static constexpr int b_map(int s) { return MODE == kUpBack ? 1 - s : MODE == kDx ? s : 0; }
+  __host__ __device__ static constexpr int b_map(int s) { return MODE == kUpBack ? 1 - s : 0; }
 };
 
 // A warp's buffer of rows of the group by its 32 features, on its way out (see ops_tc.cu): 32 rows of 16-bit values, or 16
@@ -98,7 +121,8 @@ __device__ __forceinline__ uint32_t out_at(int r, int lane) {
   else return uint32_t(r * 128 + (((lane >> 2) ^ (r & 7)) * 16) + (lane & 3) * 4);
 }
 template <class E>
-__device__ __forceinline__ void out_end(Out& o, char* b, int which, int x, int y, E* p, int64_t ld, int rows, int cols) {
+__device__ __forceinline__ void out_end(Out& o, char* b, int which, int x, int y, int z, E* p, int64_t ld, int rows,
+                                        int cols) {
   constexpr int kRows = 64 / int(sizeof(E));
   const int lane = threadIdx.x & 31;
   if (o.tma && rows >= kRows && cols > 0) {
@@ -106,7 +130,7 @@ __device__ __forceinline__ void out_end(Out& o, char* b, int which, int x, int y
     __syncwarp();
     if (lane == 0)
       asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%1, %2, %3}], [%4];" ::"l"(o.map + which),
-                   "r"(x), "r"(y), "r"(0), "r"(smem_u32(b))
+                   "r"(x), "r"(y), "r"(z), "r"(smem_u32(b))
                    : "memory");
   } else {
     __syncwarp();
@@ -164,7 +188,7 @@ __device__ __forceinline__ void epilogue(const Params& q, const Tile& t, uint32_
 #pragma unroll
           for (int i = 0; i < 16; ++i)
             *reinterpret_cast<T*>(b + out_at<T>(16 * s + i, lane)) = from_f<T>(act_of<ACT>(g[s][i]) * u[s][i]);
-        out_end<T>(o, b, 0, f, y, static_cast<T*>(p.out) + at, p.ldo, rows, cols);
+        out_end<T>(o, b, 0, f, y, 0, static_cast<T*>(p.out) + at, p.ldo, rows, cols);
       } else {
         float dw[32];
         char* b = out_begin(o);
@@ -179,20 +203,20 @@ __device__ __forceinline__ void epilogue(const Params& q, const Tile& t, uint32_
             d[s][i] = wr * dh * k;
             g[s][i] = wr * k * u[s][i];
           }
-        out_end<T>(o, b, 0, f, y, static_cast<T*>(p.dg) + at, p.ldo, rows, cols);
+        out_end<T>(o, b, 0, f, y, 0, static_cast<T*>(p.dg) + at, p.ldo, rows, cols);
         b = out_begin(o);
 #pragma unroll
         for (int s = 0; s < 2; ++s)
 #pragma unroll
           for (int i = 0; i < 16; ++i) *reinterpret_cast<T*>(b + out_at<T>(16 * s + i, lane)) = from_f<T>(d[s][i]);
-        out_end<T>(o, b, 1, f, y, static_cast<T*>(p.du) + at, p.ldo, rows, cols);
+        out_end<T>(o, b, 1, f, y, 0, static_cast<T*>(p.du) + at, p.ldo, rows, cols);
         if (p.hw) {
           b = out_begin(o);
 #pragma unroll
           for (int s = 0; s < 2; ++s)
 #pragma unroll
             for (int i = 0; i < 16; ++i) *reinterpret_cast<T*>(b + out_at<T>(16 * s + i, lane)) = from_f<T>(g[s][i]);
-          out_end<T>(o, b, 2, f, y, static_cast<T*>(p.hw) + at, p.ldo, rows, cols);
+          out_end<T>(o, b, 2, f, y, 0, static_cast<T*>(p.hw) + at, p.ldo, rows, cols);
         }
         if (p.dwp) {  // features outside the matrix have u = 0
           const float sum = lane_sums(dw);
@@ -209,7 +233,8 @@ __device__ __forceinline__ void epilogue(const Params& q, const Tile& t, uint32_
 #pragma unroll
       for (int i = 0; i < 16; ++i) *reinterpret_cast<float*>(b + out_at<float>(i, lane)) = v[i];
       const int y = t.row0 + c;
-      out_end<float>(o, b, 0, f, y, p.rows32 + int64_t(y) * p.n + f, p.n, t.rows - c, cols);
+      out_end<float>(o, b, 0, f, y, t.split, p.rows32 + (int64_t(t.split) * q.split_rows + y) * p.n + f, p.n, t.rows - c,
+                     cols);
     }
   }
 }
@@ -257,7 +282,7 @@ __global__ __launch_bounds__(kThreads, 1) void group_kernel(const __grid_constan
     bool ok = true;
     Tile t;
     const uint32_t ring = smem_u32(smem), arrive = in_cta(full, 0);
-    for (int L = first; ok && tile_at(q, L, t); L += stride) {
+    for (int L = first; ok && tile_at<MODE>(q, L, t); L += stride) {
       const int boxes = t.cols / 32;  // of 16 rows
       const int r0 = t.row0 + int(rank) * (t.cols / 2), f0 = t.f0 + int(rank) * kBM;
 #pragma unroll
@@ -266,8 +291,10 @@ __global__ __launch_bounds__(kThreads, 1) void group_kernel(const __grid_constan
         const int a_bytes = X::both(s) ? 2 * kA : kA;
         const uint32_t bytes = uint32_t(a_bytes + boxes * 2048);
         const CUtensorMap *ma = &maps.a[X::a_map(s)], *mb = &maps.b[X::b_map(s)];
-        int k0 = 0;
-        for (int kb = 0; kb < q.k_blocks; ++kb, k0 += kBK) {
+        int k0 = t.kb0 * kBK;
+        for (int kb = t.kb0; kb < t.kb1; ++kb, k0 += kBK) {
+          if (MODE == kDx && kb >= q.k_blocks && mb == maps.b)  // on to up's matrix and du
+            ma = maps.a + 1, mb = maps.b + 1, k0 -= q.k_blocks * kBK;
           ok = bar_wait(empty + 8 * st, parity, dead);
           if (!ok) break;
           const uint32_t sa = ring + st * stage_bytes, sb = sa + a_bytes, bar = arrive + 8 * st;
@@ -299,7 +326,7 @@ __global__ __launch_bounds__(kThreads, 1) void group_kernel(const __grid_constan
     Tile t;
     constexpr uint32_t type = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
     const uint32_t ring = smem_u32(smem);
-    for (int L = first; ok && tile_at(q, L, t); L += stride, ++nt) {
+    for (int L = first; ok && tile_at<MODE>(q, L, t); L += stride, ++nt) {
       const int buf = nt % X::bufs;
 #pragma unroll
       for (int s = 0; s < X::segs; ++s) {
@@ -312,10 +339,9 @@ __global__ __launch_bounds__(kThreads, 1) void group_kernel(const __grid_constan
         const uint32_t idesc = (1u << 4) | (type << 7) | (type << 10) | (uint32_t(X::a_mn(s)) << 15) |
                                (uint32_t(t.cols >> 3) << 17) | (uint32_t(2 * kBM >> 4) << 24);
         const uint32_t d = tmem + (MODE == kUpBack && s == 0 ? 256 + 128 * (nt & 1) : buf * 256);
-        const bool fresh = !(MODE == kDx && s == 1);  // dx: both segments add into the same sums
         const uint64_t ring_a = desc(ring, X::a_mn(s)), ring_a2 = desc(ring + kABytes, false),
                        ring_b = desc(ring + (X::both(s) ? 2 : 1) * kABytes, false);
-        for (int kb = 0; kb < q.k_blocks; ++kb) {
+        for (int kb = t.kb0; kb < t.kb1; ++kb) {
           ok = bar_wait(full + 8 * st, parity, dead);
           if (!ok) break;
           fence_after();
@@ -323,7 +349,7 @@ __global__ __launch_bounds__(kThreads, 1) void group_kernel(const __grid_constan
           if (elect()) {
 #pragma unroll
             for (int k = 0; k < kBK / 16; ++k) {
-              const bool add = !(fresh && kb == 0 && k == 0);
+              const bool add = kb > t.kb0 || k > 0;
               mma<2>(d, ring_a + at + uint64_t((X::a_mn(s) ? 2048 : 32) * k >> 4), ring_b + at + uint64_t(32 * k >> 4),
                      idesc, add);
               if (X::both(s)) mma<2>(d + 128, ring_a2 + at + uint64_t(32 * k >> 4), ring_b + at + uint64_t(32 * k >> 4),
@@ -346,7 +372,7 @@ __global__ __launch_bounds__(kThreads, 1) void group_kernel(const __grid_constan
     uint32_t nt = 0;
     Tile t;
     Out out{maps.out, store + (warp - 4) * kStoreBytes, 0, q.vec != 0};
-    for (int L = first; tile_at(q, L, t); L += stride, ++nt) {
+    for (int L = first; tile_at<MODE>(q, L, t); L += stride, ++nt) {
       const int buf = nt % X::bufs;
       if (!bar_wait(sums_full + 8 * buf, (nt / X::bufs) & 1, dead)) break;
       __syncwarp();
@@ -394,26 +420,33 @@ int go_mode(Mode mode, int act, const Maps& maps, const Params& q, int pairs, cu
     case kUpBack: return go_act<T, kUpBack>(act, maps, q, pairs, s);
     case kDown: return go<T, kDown, 0>(maps, q, pairs, s);
     case kDx: return go<T, kDx, 0>(maps, q, pairs, s);
+    case kLin: return go<T, kLin, 0>(maps, q, pairs, s);
+    case kLinDx: return go<T, kLinDx, 0>(maps, q, pairs, s);
   }
   return int(cudaErrorInvalidValue);
 }
 
 }  // namespace
 
-int launch_group(int dtype, const Product& p, const Plan* plan, const Units* u, cudaStream_t s) {
+int launch_group(int dtype, const Product& p, int splits, const Plan* plan, const Units* u, cudaStream_t s) {
   if (!encoder()) return int(cudaErrorNotSupported);
   const int sms = sm_count();
   if (!sms) return int(cudaErrorInvalidDevice);
   Params q{};
   q.p = p;
-  q.plan = *plan;
-  const Mode mode = p.epi == kEpiUp ? kUp : p.epi == kEpiUpBack ? kUpBack : p.segs == 2 ? kDx : kDown;
+  const bool rows32 = p.epi == kEpiRows32;
+  Mode mode;
+  if (!plan) mode = p.b[0].s_k == 1 ? kLin : kLinDx;
+  else mode = p.epi == kEpiUp ? kUp : p.epi == kEpiUpBack ? kUpBack : p.segs == 2 ? kDx : kDown;
   // gate and up (and dh) share TMEM: 128 columns each; one product's sums take 256
-  q.list = mode == kUp || mode == kUpBack ? 0 : 1;
-  q.bm = int(plan->bm << q.list);
+  q.list = rows32 ? 1 : 0;
+  q.bm = int(kGroupRows << q.list);
+  if (plan) q.plan = *plan;
+  q.rows = int(p.m);
+  q.splits = splits;
+  q.split_rows = plan ? int(plan->max_rows) : int(p.m);
   q.f_tiles = int(ceil_div(uint64_t(p.n), 2 * kBM));
   q.k_blocks = int(ceil_div(uint64_t(p.k), kBK));
-  const bool rows32 = p.epi == kEpiRows32;
   q.vec = rows32 ? p.n % 4 == 0 : mode == kUp ? on16(p.out) && p.ldo % 8 == 0
                                               : on16(p.dg) && on16(p.du) && on16(p.hw) && p.ldo % 8 == 0;
   Maps maps;
@@ -421,22 +454,25 @@ int launch_group(int dtype, const Product& p, const Plan* plan, const Units* u, 
   for (int i = 0; i < p.segs; ++i) {
     const Operand &b = p.a[i], &a = p.b[i];  // (the group's rows are the products' second operand here)
     const bool k_inner = a.s_k == 1;
-    if (!make_map(&maps.a[a.part], dtype, u->part[a.part], uint64_t(k_inner ? p.k : p.n), uint64_t(k_inner ? p.n : p.k),
-                  uint64_t(k_inner ? a.s_i : a.s_k), u->n_slots, u->stride[a.part], k_inner ? kBM : 64) ||
-        !make_map(&maps.b[mode == kUpBack ? i / 2 : mode == kDx ? i : 0], dtype, b.p, uint64_t(p.k), plan->max_rows,
-                  uint64_t(b.s_i), 1, 0, 16))
+    const int part = a.part < 0 ? 0 : a.part;
+    if (!make_map(&maps.a[part], dtype, plan ? u->part[part] : a.p, uint64_t(k_inner ? p.k : p.n),
+                  uint64_t(k_inner ? p.n : p.k), uint64_t(k_inner ? a.s_i : a.s_k), plan ? u->n_slots : 1,
+                  plan ? u->stride[part] : 0, k_inner ? kBM : 64) ||
+        !make_map(&maps.b[mode == kUpBack ? i / 2 : mode == kDx ? i : 0], dtype, b.p, uint64_t(p.k),
+                  uint64_t(q.split_rows), uint64_t(b.s_i), 1, 0, 16))
       return int(cudaErrorInvalidValue);
   }
   if (q.vec) {
     void* const outs[3] = {rows32 ? p.rows32 : mode == kUp ? p.out : p.dg, p.du, p.hw};
     for (int i = 0; i < 3; ++i)
-      if (outs[i] && !make_map(&maps.out[i], rows32 ? TSB_F32 : dtype, outs[i], uint64_t(p.n), plan->max_rows,
-                               uint64_t(rows32 ? p.n : p.ldo), 1, 0, rows32 ? 16 : 32, !rows32))
+      if (outs[i] && !make_map(&maps.out[i], rows32 ? TSB_F32 : dtype, outs[i], uint64_t(p.n), uint64_t(q.split_rows),
+                               uint64_t(rows32 ? p.n : p.ldo), uint64_t(splits), uint64_t(q.split_rows) * uint64_t(p.n) * 4,
+                               rows32 ? 16 : 32, !rows32))
         return int(cudaErrorInvalidValue);
   }
   q.stage_bytes = q.list == 0 ? 2 * kABytes + 8192 : 2 * kABytes;
   q.stages = kRingBytes / q.stage_bytes;
-  const int64_t tiles = int64_t(plan->max_tiles) * q.f_tiles;
+  const int64_t tiles = (plan ? int64_t(plan->max_tiles) : int64_t(ceil_div(uint64_t(p.m), uint64_t(q.bm)))) * q.f_tiles * splits;
   if (tiles >= (int64_t(1) << 30)) return int(cudaErrorInvalidValue);
   const int pairs = int(tiles < sms / 2 ? tiles : sms / 2);
   return dtype == TSB_BF16 ? go_mode<__nv_bfloat16>(mode, p.act, maps, q, pairs, s)

@@ -241,6 +241,32 @@ __global__ __launch_bounds__(256) void join_kernel(const int32_t* __restrict__ r
   for (int v = 0; v < V; ++v) y[t * ldy + c + v] = from_f<T>(sum[v]);
 }
 
+template <class T, int V>
+__global__ __launch_bounds__(256) void join_linear_kernel(int act, const float* __restrict__ src, uint32_t splits,
+                                                          uint64_t split_stride, uint64_t n, const T* __restrict__ bias,
+                                                          const T* residual, uint64_t ldr, T* y, uint64_t ldy, T* pre,
+                                                          uint64_t ldp) {
+  begin_after();
+  const uint64_t r = blockIdx.x, c = (uint64_t(blockIdx.y) * 256 + threadIdx.x) * V;
+  if (c >= n) return;
+  float z[V] = {};
+  for (uint32_t s = 0; s < splits; ++s) {
+    const float* p = src + s * split_stride + r * n + c;
+    if constexpr (V == 4) {
+      const float4 f = *reinterpret_cast<const float4*>(p);
+      z[0] += f.x, z[1] += f.y, z[2] += f.z, z[3] += f.w;
+    } else {
+      z[0] += *p;
+    }
+  }
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    if (bias) z[v] += to_f(bias[c + v]);
+    if (pre) pre[r * ldp + c + v] = from_f<T>(z[v]);
+    y[r * ldy + c + v] = from_f<T>(act_rt(act, z[v]) + (residual ? to_f(residual[r * ldr + c + v]) : 0.f));
+  }
+}
+
 // a warp adds a pair's sums, lane by lane and then over the lanes
 template <class T>
 __global__ __launch_bounds__(256) void join_dw_kernel(const int32_t* __restrict__ row_of_pair, uint32_t pairs,
@@ -513,6 +539,21 @@ int launch_join(int dtype, const Plan& p, const float* rows32, uint32_t splits, 
     const unsigned v4 = n % 4 == 0 ? 4 : 1;
     e = launch(v4 == 4 ? join_kernel<T, 4> : join_kernel<T, 1>, dim3(unsigned(rows), unsigned(ceil_div(n, 256 * v4))), 256, 0,
                1, true, s, p.row_of_pair, rows32, splits, stride, weights, top, n, r, ldr, static_cast<T*>(y), ldy);
+  });
+  return e;
+}
+
+int launch_join_linear(int dtype, int act, const float* rows32, uint32_t splits, uint64_t rows, uint64_t n,
+                       const void* bias, const void* residual, uint64_t ldr, void* y, uint64_t ldy, void* pre,
+                       uint64_t ldp, cudaStream_t s) {
+  int e = 0;
+  by_type(dtype, [&](auto v) {
+    using T = decltype(v);
+    const unsigned v4 = n % 4 == 0 ? 4 : 1;
+    e = launch(v4 == 4 ? join_linear_kernel<T, 4> : join_linear_kernel<T, 1>,
+               dim3(unsigned(rows), unsigned(ceil_div(n, 256 * v4))), 256, 0, 1, true, s, act, rows32, splits, rows * n, n,
+               static_cast<const T*>(bias), static_cast<const T*>(residual), ldr, static_cast<T*>(y), ldy,
+               static_cast<T*>(pre), ldp);
   });
   return e;
 }

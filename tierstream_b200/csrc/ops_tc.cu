@@ -499,20 +499,6 @@ int go_type(int dtype, int act, const Maps& maps, const Params& q, int grid, cud
     return dtype == TSB_BF16 ? go<__nv_bfloat16, MODE, 0>(maps, q, grid, s) : go<__half, MODE, 0>(maps, q, grid, s);
 }
 
-// Columns a tile: of the multiples of `step` up to `most`, the one whose last wave of tiles wastes least. A tile costs its
-// columns plus about 32 (the narrower tile re-reads A for fewer products); 2047 x 7168 at 148 SMs takes 208 (4 waves of
-// 560 tiles) over 256 (4 waves of 448).
-int columns(int64_t m_tiles, int64_t n, int sms, int most, int step) {
-  int best = step;
-  int64_t cost = INT64_MAX;
-  for (int bn = most; bn >= step; bn -= step) {
-    const int64_t waves = ceil_div(uint64_t(m_tiles) * ceil_div(uint64_t(n), uint64_t(bn)), uint64_t(sms));
-    const int64_t c = waves * (bn + 32);
-    if (c < cost) cost = c, best = bn;
-  }
-  return best;
-}
-
 struct Shape {  // one operand as memory: [slots][rows][cols] with cols contiguous
   const void* p;
   uint64_t cols, rows, ld, slots, slot_bytes;
@@ -522,6 +508,22 @@ bool fits(const Shape& s) {
 }
 
 }  // namespace
+
+// Columns a tile: of the multiples of 16 (32 for a pair) up to 256, the one whose last wave of tiles wastes least. A tile
+// costs its columns plus about 32 (the narrower tile re-reads A for fewer products); 2047 x 7168 on 74 pairs takes 224
+// (four waves) over 256 (four waves).
+int tc_columns(int64_t m, int64_t n, int sms) {
+  const int cg = m > kBM ? 2 : 1, step = 16 * cg;
+  const uint64_t m_tiles = ceil_div(uint64_t(m), uint64_t(kBM * cg));
+  int best = step;
+  int64_t cost = INT64_MAX;
+  for (int bn = 256; bn >= step; bn -= step) {
+    const int64_t waves = int64_t(ceil_div(m_tiles * ceil_div(uint64_t(n), uint64_t(bn)), uint64_t(sms / cg)));
+    const int64_t c = waves * (bn + 32);
+    if (c < cost) cost = c, best = bn;
+  }
+  return best;
+}
 
 bool tc_fits(const Operand& o, const Units* u) {
   // one of the two strides is 1, the other a multiple of 8 elements; a unit's matrices in slots (not by address)
@@ -558,7 +560,7 @@ int launch_tc(int dtype, const Product& p, const Plan* plan, const Units* u, cud
   q.m_tiles = p.grouped ? 0 : int(ceil_div(uint64_t(p.m), uint64_t(cg * kBM)));
   const int64_t m_tiles = p.grouped ? plan->max_tiles : p.per_unit ? int64_t(q.m_tiles) * plan->units : q.m_tiles;
   const bool narrow = mode == kUp || mode == kUpBack;
-  q.bn = p.grouped || p.per_unit ? (narrow ? 128 : 256) : columns(m_tiles, p.n, sms / cg, 256, 16 * cg);
+  q.bn = p.grouped || p.per_unit ? (narrow ? 128 : 256) : tc_columns(p.m, p.n, sms);
   const int64_t step = 16 * cg;  // a product's columns: whole 16 for one CTA, 32 for a pair
   if (q.bn > (p.n + step - 1) / step * step) q.bn = int((p.n + step - 1) / step * step);
   q.n_tiles = int(ceil_div(uint64_t(p.n), uint64_t(q.bn)));
