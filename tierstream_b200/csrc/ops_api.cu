@@ -291,29 +291,12 @@ bool ffn_rows16(const tsb_units* u, uint64_t hidden, uint64_t ffn, const void* x
 // On the tensor cores' own path a unit's matrix supplies the rows and the group's rows the columns, except for groups so
 // long that whole 256-row tiles waste little of them.
 uint32_t tc_tile(uint64_t each) { return each >= 4 * kTcRows ? kTcRows : kGroupRows; }
-int launch_grouped(int dtype, const Product& p, int splits, const Plan* plan, const Units* u, cudaStream_t s) {
-  return p.grouped && plan->bm == kGroupRows ? launch_group(dtype, p, splits, plan, u, s) : launch_tc(dtype, p, plan, u, s);
-}
-
-// Into how many parts a grouped product's sum over `kb` slices is cut: the tiles of about half-full groups, dealt to 74
-// pairs, end in waves, which shorter tiles fill better; each part costs its 32-bit rows' way to the join and back.
-int grouped_splits(const Plan& plan, uint64_t n, double kb) {
-  if (plan.bm != kGroupRows) return 1;
-  const double met = double(std::min<uint64_t>(plan.pairs, plan.units)), each = plan.pairs / met;
-  const double tiles = double(ceil_div(n, 256)) * (plan.pairs / 256.0 + met / 2);
-  const double us = slice_us(std::min(256.0, std::ceil(each / 32) * 32));
-  int best = 1;
-  double least = 0;
-  for (int s = 1; s <= 4 && s * 8 <= kb; ++s) {
-    const double c = std::ceil(tiles * s / (kSms / 2)) * (kb / s * us + 2) + s * double(plan.max_rows) * double(n) * 8 / 6e6;
-    if (s == 1 || c < least) least = c, best = s;
-  }
-  return best;
+int launch_grouped(int dtype, const Product& p, const Plan* plan, const Units* u, cudaStream_t s) {
+  return p.grouped && plan->bm == kGroupRows ? launch_group(dtype, p, 1, plan, u, s) : launch_tc(dtype, p, plan, u, s);
 }
 
 struct FfnSpace {
   Plan plan;
-  int splits;
   bool tc, stream;
   void* xs;
   void* h;
@@ -333,8 +316,7 @@ FfnSpace ffn_space(const tsb_ffn_args* a) {
   r.plan = plan_at(w.take(plan_bytes(a->units->n_units, pairs, 1, bm)), a->units->n_units, pairs, 1, bm);
   if (r.tc) r.xs = w.take(uint64_t(r.plan.max_rows) * a->hidden * 2);
   r.h = w.take(uint64_t(r.plan.max_rows) * a->ffn * 2);
-  r.splits = r.tc ? grouped_splits(r.plan, a->hidden, double(ceil_div(a->ffn, 64))) : 1;
-  r.rows32 = static_cast<float*>(w.take(uint64_t(r.splits) * r.plan.max_rows * a->hidden * 4));
+  r.rows32 = static_cast<float*>(w.take(uint64_t(r.plan.max_rows) * a->hidden * 4));
   r.bytes = w.used;
   return r;
 }
@@ -370,16 +352,16 @@ void ffn(const tsb_ffn_args* a) {
   p.epi = kEpiUp;
   p.act = int(a->act);
   p.out = w.h, p.ldo = f;
-  const auto go = [&](const Product& pr, int splits) {
+  const auto go = [&](const Product& pr) {
     return w.stream ? launch_stream(int(a->dtype), pr, a->top, &w.plan, &u, s)
-           : w.tc   ? launch_grouped(int(a->dtype), pr, splits, &w.plan, &u, s)
+           : w.tc   ? launch_grouped(int(a->dtype), pr, &w.plan, &u, s)
                     : launch_tile(int(a->dtype), pr, &w.plan, &u, s);
   };
   if (w.tc) {
     ck(launch_gather(w.plan, a->top, a->x, a->ldx, a->hidden, w.xs, s), fn, "gather");
     p.a[0] = p.a[1] = dense(w.xs, d, 1);
   }
-  ck(go(p, 1), fn, "gate and up");
+  ck(go(p), fn, "gate and up");
   Product q{};
   q.grouped = 1;
   q.after = true;
@@ -389,15 +371,14 @@ void ffn(const tsb_ffn_args* a) {
   q.n = d, q.k = f;
   q.epi = kEpiRows32;
   q.rows32 = w.rows32;
-  ck(go(q, w.splits), fn, "down");
-  ck(launch_join(int(a->dtype), w.plan, w.rows32, uint32_t(w.splits), a->weights, a->top, a->rows, a->hidden, a->residual, a->ldr, a->y,
+  ck(go(q), fn, "down");
+  ck(launch_join(int(a->dtype), w.plan, w.rows32, 1, a->weights, a->top, a->rows, a->hidden, a->residual, a->ldr, a->y,
                  a->ldy, s),
      fn, "join");
 }
 
 struct FfnBackSpace {
   Plan plan;
-  int splits;
   bool tc;
   void *xs, *dys, *dg, *du, *hw;
   float *dwp, *rows32;
@@ -422,8 +403,7 @@ FfnBackSpace ffn_back_space(const tsb_ffn_grad_args* a) {
   if (a->dgate) r.hw = w.take(uint64_t(r.plan.max_rows) * a->ffn * 2);
   r.dw_tiles = r.tc ? (bm == kGroupRows ? 8 * uint32_t(ceil_div(a->ffn, 256)) : 2 * uint32_t(ceil_div(a->ffn, 128))) : uint32_t(ceil_div(a->ffn, kTileN));
   if (a->dweights) r.dwp = static_cast<float*>(w.take(uint64_t(r.plan.max_rows) * r.dw_tiles * 4));
-  r.splits = r.tc ? grouped_splits(r.plan, a->hidden, 2 * double(ceil_div(a->ffn, 64))) : 1;
-  if (a->dx) r.rows32 = static_cast<float*>(w.take(uint64_t(r.splits) * r.plan.max_rows * a->hidden * 4));
+  if (a->dx) r.rows32 = static_cast<float*>(w.take(uint64_t(r.plan.max_rows) * a->hidden * 4));
   r.bytes = w.used;
   return r;
 }
@@ -455,8 +435,8 @@ void ffn_back(const tsb_ffn_grad_args* a) {
   const Units u = units_of(a->units);
   const int dt = int(a->dtype);
   ck(launch_plan(w.plan, u, a->ids, s), fn, "plan");
-  const auto go = [&](const Product& pr, int splits) {
-    return w.tc ? launch_grouped(dt, pr, splits, &w.plan, &u, s) : launch_tile(dt, pr, &w.plan, &u, s);
+  const auto go = [&](const Product& pr) {
+    return w.tc ? launch_grouped(dt, pr, &w.plan, &u, s) : launch_tile(dt, pr, &w.plan, &u, s);
   };
   Operand x_rows = gathered(a->x, int64_t(a->ldx), 1, w.plan, a->top),
           dy_rows = gathered(a->dy, int64_t(a->lddy), 1, w.plan, a->top),
@@ -487,7 +467,7 @@ void ffn_back(const tsb_ffn_grad_args* a) {
     p.dg = w.dg, p.du = w.du, p.hw = w.hw, p.ldo = f;
     p.dwp = w.dwp, p.ld_dwp = w.dw_tiles;
     p.weights = a->weights;
-    ck(go(p, 1), fn, "gate, up and dh");
+    ck(go(p), fn, "gate, up and dh");
   }
   if (a->dweights) ck(launch_join_dw(dt, w.plan, w.dwp, w.dw_tiles, a->dweights, s), fn, "dweights");
   if (a->dx) {
@@ -502,8 +482,8 @@ void ffn_back(const tsb_ffn_grad_args* a) {
     p.n = d, p.k = f;
     p.epi = kEpiRows32;
     p.rows32 = w.rows32;
-    ck(go(p, w.splits), fn, "dx");
-    ck(launch_join(dt, w.plan, w.rows32, uint32_t(w.splits), nullptr, a->top, a->rows, a->hidden, nullptr, 0, a->dx, a->lddx, s), fn,
+    ck(go(p), fn, "dx");
+    ck(launch_join(dt, w.plan, w.rows32, 1, nullptr, a->top, a->rows, a->hidden, nullptr, 0, a->dx, a->lddx, s), fn,
        "join");
   }
   if (a->dgate) {
@@ -518,15 +498,15 @@ void ffn_back(const tsb_ffn_grad_args* a) {
     p.b[0] = x_sum;
     p.a[0] = dense(w.dg, 1, f, 1);
     p.out = a->dgate;
-    ck(go(p, 1), fn, "dgate");
+    ck(go(p), fn, "dgate");
     p.a[0] = dense(w.du, 1, f, 1);
     p.out = a->dup;
-    ck(go(p, 1), fn, "dup");
+    ck(go(p), fn, "dup");
     p.m = d, p.n = f, p.ldo = f;
     p.a[0] = dy_sum;
     p.b[0] = dense(w.hw, 1, f, 1);
     p.out = a->ddown;
-    ck(go(p, 1), fn, "ddown");
+    ck(go(p), fn, "ddown");
   }
 }
 
