@@ -193,3 +193,40 @@ def test_struct_layouts_match_the_header():
         want.append(C.sizeof(s))
         want += [getattr(s, f[0]).offset for f in s._fields_]
     assert got == want
+
+
+def test_tensors_that_do_not_fit_are_refused_on_the_host():
+    """ops.py's checks of types, shapes, strides and devices raise ValueError naming the tensor, before any device work."""
+    torch = pytest.importorskip("torch")
+    from tierstream_b200 import ops
+    x = torch.zeros((4, 16), dtype=torch.bfloat16)
+    w = torch.zeros((8, 16), dtype=torch.bfloat16)
+    g, d = torch.zeros((3, 8, 16), dtype=torch.bfloat16), torch.zeros((3, 16, 8), dtype=torch.bfloat16)
+    i, p = torch.zeros((4, 2), dtype=torch.int32), torch.zeros((4, 2))
+    y = torch.zeros((4, 8), dtype=torch.bfloat16)
+    for call, text in (
+            (lambda: ops.linear(x.float(), w), "x: Float is not served"), (lambda: ops.linear(x, w), "CUDA tensors"),
+            (lambda: ops.linear(g, w), "x: two dimensions"), (lambda: ops.linear(x, 3), "w: a tensor is wanted"),
+            (lambda: ops.linear(x, w.half()), "w: BFloat16 on the CPU is wanted, got Half"),
+            (lambda: ops.linear(x, w[:, :8]), r"w: shape \[8, 16\] is wanted, got \[8, 8\]"),
+            (lambda: ops.linear(x.T.contiguous().T, w), "x: the elements of a row must be adjacent"),
+            (lambda: ops.linear(x[:1].expand(4, 16), w), "x: rows overlap"), (lambda: ops.linear(x, x[0]), "w: two dim"),
+            (lambda: ops.linear(x, w, bias=x), r"bias: a contiguous BFloat16 of shape \[8\]"),
+            (lambda: ops.linear(x, w, residual=x), "residual: shape"), (lambda: ops.linear(x, w, pre=x), "pre: shape"),
+            (lambda: ops.linear(x, w, act="tanh"), "unknown activation"),
+            (lambda: ops.linear_backward(x.double(), x, x), "dy: Double is not served"),
+            (lambda: ops.linear_backward(y, x, w), "CUDA tensors"), (lambda: ops.linear_backward(y, x, x), "w: shape"),
+            (lambda: ops.linear_backward(y, x[0], w), "x: two dimensions"),
+            (lambda: ops.linear_backward(y, x, w, act="silu"), "pre: an activation"),
+            (lambda: ops.route(x.double(), 2), "logits: Double"), (lambda: ops.route(g, 2), "logits: two dimensions"),
+            (lambda: ops.route(x, 2), "CUDA tensors"), (lambda: ops.route(x, 17), "top: must be"),
+            (lambda: ops.route(x, 0), "top: must be"), (lambda: ops.route_backward(p, x, i, p), "CUDA tensors"),
+            (lambda: ops.route_backward(p, x, p, p), "ids: a contiguous Int"),
+            (lambda: ops.route_backward(p[:2], x, i, p), "dweights: 4 rows"),
+            (lambda: ops.Units(g, g, d), "CUDA tensors"), (lambda: ops.Units(g, g, g), "down: BFloat16 of shape"),
+            (lambda: ops.Units(x, x, x), "gate: .slots"), (lambda: ops.Units(g.double(), g, d), "gate: Double"),
+            (lambda: ops.Units(None, g, d), "gate: a tensor"), (lambda: ops.Units(g, g[:, :, ::2], d), "up: BFloat16"),
+            (lambda: ops.Units(g, g.mT.contiguous().mT, d), "up: a slot's matrix must be contiguous"),
+            (lambda: ops.Units(g, g, d, p), "slot_of: a contiguous Int")):
+        with pytest.raises(ValueError, match=text):
+            call()

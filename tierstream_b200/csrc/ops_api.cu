@@ -227,7 +227,6 @@ void linear_back(const tsb_linear_grad_args* a) {
        fn, "slope");
   if (a->dx) {
     Product p = dx_product(a, w.dz, w.ldz);
-    p.after = slope || a->db;
     ck(product(int(a->dtype), p, w.rows32, s), fn, "dx");
   }
   if (a->dw) {
@@ -236,7 +235,6 @@ void linear_back(const tsb_linear_grad_args* a) {
     p.a[0] = dense(w.dz, 1, int64_t(w.ldz), 1);
     p.b[0] = dense(a->x, 1, int64_t(a->ldx), 1);
     p.m = int64_t(a->n), p.n = int64_t(a->k), p.k = int64_t(a->rows);
-    p.after = slope || a->db || a->dx;
     p.epi = kEpiStore;
     p.out = a->dw, p.ldo = int64_t(a->lddw);
     ck(product(int(a->dtype), p, nullptr, s), fn, "dw");
@@ -342,7 +340,6 @@ void ffn(const tsb_ffn_args* a) {
   ck(launch_plan(w.plan, u, a->ids, s), fn, "plan");
   Product p{};
   p.grouped = 1;
-  p.after = true;
   p.segs = 2;
   p.a[0] = p.a[1] = gathered(a->x, int64_t(a->ldx), 1, w.plan, a->top);
   p.b[0] = of_unit(0, d, 1);
@@ -364,7 +361,6 @@ void ffn(const tsb_ffn_args* a) {
   ck(go(p), fn, "gate and up");
   Product q{};
   q.grouped = 1;
-  q.after = true;
   q.segs = 1;
   q.a[0] = dense(w.h, f, 1);
   q.b[0] = of_unit(2, f, 1);
@@ -453,8 +449,7 @@ void ffn_back(const tsb_ffn_grad_args* a) {
   {
     Product p{};
     p.grouped = 1;
-    p.after = true;
-    p.segs = 3;
+      p.segs = 3;
     p.a[0] = p.a[1] = x_rows;
     p.a[2] = dy_rows;
     p.b[0] = of_unit(0, d, 1);
@@ -473,8 +468,7 @@ void ffn_back(const tsb_ffn_grad_args* a) {
   if (a->dx) {
     Product p{};
     p.grouped = 1;
-    p.after = true;
-    p.segs = 2;
+      p.segs = 2;
     p.a[0] = dense(w.dg, f, 1);
     p.a[1] = dense(w.du, f, 1);
     p.b[0] = of_unit(0, 1, d);
@@ -489,8 +483,7 @@ void ffn_back(const tsb_ffn_grad_args* a) {
   if (a->dgate) {
     Product p{};
     p.per_unit = 1;
-    p.after = true;
-    p.k_rows = 1;
+      p.k_rows = 1;
     p.segs = 1;
     p.epi = kEpiStore;
     p.out_unit = d * f;

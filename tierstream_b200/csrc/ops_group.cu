@@ -401,7 +401,7 @@ int go(const Maps& maps, const Params& q, int pairs, cudaStream_t s) {
   static std::atomic<uint64_t> devices{0};
   const auto kernel = group_kernel<T, MODE, ACT>;
   if (const int e = allow_smem(reinterpret_cast<const void*>(kernel), devices)) return e;
-  return launch(kernel, unsigned(pairs * 2), kThreads, kSmemBytes, 2, q.p.after, s, maps, q);
+  return launch(kernel, unsigned(pairs * 2), kThreads, kSmemBytes, 2, s, maps, q);
 }
 template <class T, int MODE>
 int go_act(int act, const Maps& maps, const Params& q, int pairs, cudaStream_t s) {

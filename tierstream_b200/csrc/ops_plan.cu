@@ -365,6 +365,7 @@ template <class T, int V>
 __global__ __launch_bounds__(256) void route_kernel(const T* __restrict__ logits, uint64_t ld, uint64_t rows,
                                                     uint32_t experts, uint32_t top, int norm, int32_t* __restrict__ ids,
                                                     float* __restrict__ weights) {
+  begin_after();
   const uint64_t row = uint64_t(blockIdx.x) * 8 + (threadIdx.x >> 5);
   const uint32_t lane = threadIdx.x & 31;
   if (row >= rows) return;
@@ -417,6 +418,7 @@ __global__ __launch_bounds__(256) void route_back_kernel(const W* __restrict__ d
                                                          const float* __restrict__ weights, uint64_t rows,
                                                          uint32_t experts, uint32_t top, int norm,
                                                          T* __restrict__ dlogits, uint64_t ldd) {
+  begin_after();
   const uint64_t row = uint64_t(blockIdx.x) * 8 + (threadIdx.x >> 5);
   const uint32_t lane = threadIdx.x & 31;
   if (row >= rows) return;
@@ -523,10 +525,10 @@ uint64_t plan_bytes(uint32_t units, uint64_t pairs, uint32_t pad, uint32_t bm) {
 
 int launch_plan(const Plan& p, const Units& u, const int32_t* ids, cudaStream_t s) {
   if (p.pairs <= kSmallPairs && p.units <= kSmallUnits) {
-    return launch(plan_small_kernel, 1, kSmallThreads, 0, 1, false, s, p, u, ids);
+    return launch(plan_small_kernel, 1, kSmallThreads, 0, 1, s, p, u, ids);
   }
-  if (const int e = launch(plan_count_kernel, p.units, kPlanThreads, 0, 1, false, s, p, u, ids)) return e;
-  return launch(plan_fill_kernel, p.units, kPlanThreads, 0, 1, true, s, p, ids);
+  if (const int e = launch(plan_count_kernel, p.units, kPlanThreads, 0, 1, s, p, u, ids)) return e;
+  return launch(plan_fill_kernel, p.units, kPlanThreads, 0, 1, s, p, ids);
 }
 
 int launch_join(int dtype, const Plan& p, const float* rows32, uint32_t splits, const float* weights, uint32_t top,
@@ -538,7 +540,7 @@ int launch_join(int dtype, const Plan& p, const float* rows32, uint32_t splits, 
     const T* r = static_cast<const T*>(residual);
     const unsigned v4 = n % 4 == 0 ? 4 : 1;
     e = launch(v4 == 4 ? join_kernel<T, 4> : join_kernel<T, 1>, dim3(unsigned(rows), unsigned(ceil_div(n, 256 * v4))), 256, 0,
-               1, true, s, p.row_of_pair, rows32, splits, stride, weights, top, n, r, ldr, static_cast<T*>(y), ldy);
+               1, s, p.row_of_pair, rows32, splits, stride, weights, top, n, r, ldr, static_cast<T*>(y), ldy);
   });
   return e;
 }
@@ -551,7 +553,7 @@ int launch_join_linear(int dtype, int act, const float* rows32, uint32_t splits,
     using T = decltype(v);
     const unsigned v4 = n % 4 == 0 ? 4 : 1;
     e = launch(v4 == 4 ? join_linear_kernel<T, 4> : join_linear_kernel<T, 1>,
-               dim3(unsigned(rows), unsigned(ceil_div(n, 256 * v4))), 256, 0, 1, true, s, act, rows32, splits, rows * n, n,
+               dim3(unsigned(rows), unsigned(ceil_div(n, 256 * v4))), 256, 0, 1, s, act, rows32, splits, rows * n, n,
                static_cast<const T*>(bias), static_cast<const T*>(residual), ldr, static_cast<T*>(y), ldy,
                static_cast<T*>(pre), ldp);
   });
@@ -562,7 +564,7 @@ int launch_join_dw(int dtype, const Plan& p, const float* dwp, uint32_t tiles, v
   int e = 0;
   by_type(dtype, [&](auto v) {
     using T = decltype(v);
-    e = launch(join_dw_kernel<T>, unsigned(ceil_div(p.pairs, 8)), 256, 0, 1, true, s, p.row_of_pair, p.pairs, dwp, tiles,
+    e = launch(join_dw_kernel<T>, unsigned(ceil_div(p.pairs, 8)), 256, 0, 1, s, p.row_of_pair, p.pairs, dwp, tiles,
                static_cast<T*>(dw));
   });
   return e;
@@ -582,40 +584,41 @@ int launch_dz(int dtype, int act, const void* dy, uint64_t ldy, const void* pre,
     float* sums = db ? part : nullptr;
     const unsigned each = wide ? 8 : 1;
     e = launch(wide ? dz_kernel<T, 8> : dz_kernel<T, 1>, dim3(chunks, unsigned(ceil_div(n, 32 * each))), dim3(32, 8), 0, 1,
-               false, s, act, a, ldy, b, ldp, z, ldz, rows, n, sums);
+               s, act, a, ldy, b, ldp, z, ldz, rows, n, sums);
     if (!e && db)
-      e = launch(db_kernel<T>, unsigned(ceil_div(n, 128)), 128, 0, 1, true, s, part, chunks, n, static_cast<T*>(db));
+      e = launch(db_kernel<T>, unsigned(ceil_div(n, 128)), 128, 0, 1, s, part, chunks, n, static_cast<T*>(db));
   });
   return e;
 }
 
 int launch_route(int dtype, const void* logits, uint64_t ld, uint64_t rows, uint32_t experts, uint32_t top, int norm,
                  int32_t* ids, float* weights, cudaStream_t s) {
+  int e = 0;
   by_type(dtype, [&](auto v) {
     using T = decltype(v);
     by_experts(experts, [&](auto c) {
-      route_kernel<T, c.value><<<unsigned(ceil_div(rows, 8)), 256, 0, s>>>(static_cast<const T*>(logits), ld, rows,
-                                                                          experts, top, norm, ids, weights);
+      e = launch(route_kernel<T, c.value>, unsigned(ceil_div(rows, 8)), 256, 0, 1, s, static_cast<const T*>(logits), ld, rows,
+                 experts, top, norm, ids, weights);
     });
   });
-  return int(cudaGetLastError());
+  return e;
 }
 
 int launch_route_back(int dtype, int dw_dtype, const void* dw, const void* logits, uint64_t ld, const int32_t* ids,
                       const float* weights, uint64_t rows, uint32_t experts, uint32_t top, int norm, void* dlogits,
                       uint64_t ldd, cudaStream_t s) {
+  int e = 0;
   by_type(dtype, [&](auto v) {
     by_type(dw_dtype, [&](auto x) {
       using T = decltype(v);
       using W = decltype(x);
       by_experts(experts, [&](auto c) {
-        route_back_kernel<T, W, c.value><<<unsigned(ceil_div(rows, 8)), 256, 0, s>>>(
-            static_cast<const W*>(dw), static_cast<const T*>(logits), ld, ids, weights, rows, experts, top, norm,
-            static_cast<T*>(dlogits), ldd);
+        e = launch(route_back_kernel<T, W, c.value>, unsigned(ceil_div(rows, 8)), 256, 0, 1, s, static_cast<const W*>(dw),
+                   static_cast<const T*>(logits), ld, ids, weights, rows, experts, top, norm, static_cast<T*>(dlogits), ldd);
       });
     });
   });
-  return int(cudaGetLastError());
+  return e;
 }
 
 }  // namespace ops

@@ -186,7 +186,7 @@ __global__ __launch_bounds__(kThreads) void stream_kernel(const __grid_constant_
 
 template <class T, int MODE>
 int go(bool wide, const Params& q, dim3 grid, cudaStream_t s) {
-  return launch(wide ? stream_kernel<T, MODE, true> : stream_kernel<T, MODE, false>, grid, kThreads, 0, q.splits, q.p.after, s,
+  return launch(wide ? stream_kernel<T, MODE, true> : stream_kernel<T, MODE, false>, grid, kThreads, 0, q.splits, s,
                 q);
 }
 

@@ -473,7 +473,7 @@ int go_pair(const Maps& maps, const Params& q, int grid, cudaStream_t s) {
   static std::atomic<uint64_t> devices{0};
   const auto kernel = tc_kernel<T, MODE, ACT, CG>;
   if (const int e = allow_smem(reinterpret_cast<const void*>(kernel), devices)) return e;
-  return launch(kernel, unsigned(grid * CG), kThreads, kSmemBytes, CG, q.p.after, s, maps, q);
+  return launch(kernel, unsigned(grid * CG), kThreads, kSmemBytes, CG, s, maps, q);
 }
 template <class T, int MODE, int ACT>
 int go(const Maps& maps, const Params& q, int grid, cudaStream_t s) {
@@ -534,7 +534,7 @@ bool tc_fits(const Operand& o, const Units* u) {
 }
 
 int launch_gather(const Plan& plan, uint32_t top, const void* src, uint64_t ld, uint64_t n, void* dst, cudaStream_t s) {
-  return launch(gather_kernel, plan.max_rows, 256, 0, 1, true, s, plan, top, static_cast<const uint4*>(src), ld / 8,
+  return launch(gather_kernel, plan.max_rows, 256, 0, 1, s, plan, top, static_cast<const uint4*>(src), ld / 8,
                 uint32_t(n / 8), static_cast<uint4*>(dst));
 }
 

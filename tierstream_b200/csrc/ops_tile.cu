@@ -197,7 +197,7 @@ int go(const Product& p, const Plan& plan, const Units& u, cudaStream_t s) {
   int accs = 1;
   for (int i = 0; i < p.segs; ++i) accs = p.acc[i] + 1 > accs ? p.acc[i] + 1 : accs;
   return launch(accs == 1 ? tile_kernel<T, 1> : accs == 2 ? tile_kernel<T, 2> : tile_kernel<T, 3>, grid, kThreads, 0, 1,
-                p.after, s, p, plan, u);
+                s, p, plan, u);
 }
 
 }  // namespace
