@@ -37,9 +37,9 @@ struct Plan {
   int32_t* slot;
   int32_t* pair_of_row;
   int32_t* row_of_pair;
-  int32_t* tile_unit[2];  // tiles of `bm` and of 2 `bm` rows, group by group
-  int32_t* tile_m0[2];    // the tile's first row inside its group
-  int4* tile_info;        // per tile of `bm` rows up to max_tiles: slot, first grouped row, rows (0: no such tile), unit
+  // per tile of `bm` and of 2 `bm` rows, group by group: the unit's slot, the group's first row, its rows, and its first
+  // tile; behind the last tile of `bm` rows, up to max_tiles, zeros
+  int4* tiles[2];
   uint32_t units, pairs, max_rows, max_tiles, pad, bm;
 };
 
@@ -75,8 +75,9 @@ int launch(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, int cluster
   return int(cudaLaunchKernelEx(&c, kernel, P(args)...));
 }
 
-__device__ __forceinline__ const char* unit_part(const Units& u, int p, int32_t e, int32_t slot) {
-  return u.table ? reinterpret_cast<const char*>(u.table[e]) + u.stride[p] : u.part[p] + uint64_t(slot) * u.stride[p];
+// (units found by address have their index for a slot)
+__device__ __forceinline__ const char* unit_part(const Units& u, int p, int32_t slot) {
+  return u.table ? reinterpret_cast<const char*>(u.table[slot]) + u.stride[p] : u.part[p] + uint64_t(slot) * u.stride[p];
 }
 
 // Activations and their slopes in 32 bits. The exponentials and quotients are the fast intrinsics, off by a few 2^-22 of

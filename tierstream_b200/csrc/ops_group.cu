@@ -46,45 +46,51 @@ struct Tile {
   int split, kb0, kb1;   // its slices of k, over all segments
 };
 
-// Tile L: groups in unit order, inside a group chunks of up to 8 tiles of its rows, inside a chunk the matrix' tiles, the
-// chunk's row tiles innermost: tiles running at the same time share a unit's matrix rows from L2.
+// The launch's tiles: groups in unit order, inside a group chunks of up to 8 tiles of its rows, inside a chunk the matrix'
+// tiles, the chunk's row tiles innermost, so that tiles running at the same time share a unit's matrix rows from L2. What
+// the plan says of a tile is read one tile ahead.
 template <int MODE>
-__device__ __forceinline__ bool tile_at(const Params& q, int L, Tile& t) {
-  constexpr int kChunk = 8;
-  const int all = (MODE == kDx ? 2 : 1) * q.k_blocks;
-  t.split = 0, t.kb0 = 0, t.kb1 = all;
-  if (MODE != kUp && MODE != kUpBack && q.splits > 1) {
-    t.split = L % q.splits;
-    L /= q.splits;
-    t.kb0 = all * t.split / q.splits;
-    t.kb1 = all * (t.split + 1) / q.splits;
+struct Tiles {
+  static constexpr bool dense = MODE == kLin || MODE == kLinDx;
+  static constexpr bool split = MODE != kUp && MODE != kUpBack;
+  int at, end;
+  int4 next;
+  __device__ __forceinline__ void fetch(const Params& q) {
+    if (at < end && !dense) next = q.plan.tiles[q.list][(split ? at / q.splits : at) / q.f_tiles];
   }
-  int cnt, local, first;
-  if constexpr (MODE == kLin || MODE == kLinDx) {
-    cnt = q.rows;
-    local = L;
-    first = t.slot = 0;
-  } else {
-    const int i = L / q.f_tiles;
-    if (i >= q.plan.head[2 * q.list]) return false;
-    const int unit = q.plan.tile_unit[q.list][i];
-    t.slot = q.plan.slot[unit];
-    cnt = (q.plan.cnt[unit] + int(q.plan.pad) - 1) / int(q.plan.pad) * int(q.plan.pad);  // padding rows too
-    local = L - (i - q.plan.tile_m0[q.list][i] / q.bm) * q.f_tiles;
-    first = q.plan.off[unit];
+  __device__ __forceinline__ Tiles(const Params& q) : at(blockIdx.x / 2), next(make_int4(0, 0, q.rows, 0)) {
+    end = (dense ? (q.rows + q.bm - 1) / q.bm : q.plan.head[2 * q.list]) * q.f_tiles * q.splits;
+    fetch(q);
   }
-  const int tiles = (cnt + q.bm - 1) / q.bm;
-  if ((MODE == kLin || MODE == kLinDx) && local >= tiles * q.f_tiles) return false;
-  const int size = ((cnt + tiles - 1) / tiles + 31) & ~31;
-  const int chunk = local / (kChunk * q.f_tiles), in = local - chunk * kChunk * q.f_tiles;
-  const int width = min(kChunk, tiles - chunk * kChunk);
-  const int f = in / width, m0 = (chunk * kChunk + in - f * width) * size;
-  t.f0 = f * 2 * kBM;
-  t.row0 = first + m0;
-  t.rows = min(size, cnt - m0);
-  t.cols = (t.rows + 31) & ~31;
-  return true;
-}
+  __device__ __forceinline__ bool take(const Params& q, Tile& t) {
+    constexpr int kChunk = 8;
+    if (at >= end) return false;
+    const int4 g = next;
+    int L = at;
+    at += gridDim.x / 2;
+    fetch(q);
+    const int all = (MODE == kDx ? 2 : 1) * q.k_blocks;
+    t.split = 0, t.kb0 = 0, t.kb1 = all;
+    if (split && q.splits > 1) {
+      t.split = L % q.splits;
+      L /= q.splits;
+      t.kb0 = all * t.split / q.splits;
+      t.kb1 = all * (t.split + 1) / q.splits;
+    }
+    const int cnt = dense ? g.z : (g.z + int(q.plan.pad) - 1) / int(q.plan.pad) * int(q.plan.pad);  // padding rows too
+    const int tiles = (cnt + q.bm - 1) / q.bm, local = L - g.w * q.f_tiles;
+    const int size = ((cnt + tiles - 1) / tiles + 31) & ~31;
+    const int chunk = local / (kChunk * q.f_tiles), in = local - chunk * kChunk * q.f_tiles;
+    const int width = min(kChunk, tiles - chunk * kChunk);
+    const int f = in / width, m0 = (chunk * kChunk + in - f * width) * size;
+    t.slot = g.x;
+    t.f0 = f * 2 * kBM;
+    t.row0 = g.y + m0;
+    t.rows = min(size, cnt - m0);
+    t.cols = (t.rows + 31) & ~31;
+    return true;
+  }
+};
 
 template <int MODE>
 struct Traits {
@@ -253,7 +259,6 @@ __global__ __launch_bounds__(kThreads, 1) void group_kernel(const __grid_constan
   volatile uint32_t* dead = words + 1;
   const int warp = __shfl_sync(0xffffffffu, int(threadIdx.x >> 5), 0);
   const uint32_t rank = cta_rank(), stages = uint32_t(q.stages), stage_bytes = uint32_t(q.stage_bytes);
-  const int first = blockIdx.x / 2, stride = gridDim.x / 2;
   if (threadIdx.x == 0) {
     for (uint32_t s = 0; s < stages; ++s) {
       bar_init(full + 8 * s, 1);
@@ -282,7 +287,7 @@ __global__ __launch_bounds__(kThreads, 1) void group_kernel(const __grid_constan
     bool ok = true;
     Tile t;
     const uint32_t ring = smem_u32(smem), arrive = in_cta(full, 0);
-    for (int L = first; ok && tile_at<MODE>(q, L, t); L += stride) {
+    for (Tiles<MODE> tiles(q); ok && tiles.take(q, t);) {
       const int boxes = t.cols / 32;  // of 16 rows
       const int r0 = t.row0 + int(rank) * (t.cols / 2), f0 = t.f0 + int(rank) * kBM;
 #pragma unroll
@@ -326,7 +331,7 @@ __global__ __launch_bounds__(kThreads, 1) void group_kernel(const __grid_constan
     Tile t;
     constexpr uint32_t type = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
     const uint32_t ring = smem_u32(smem);
-    for (int L = first; ok && tile_at<MODE>(q, L, t); L += stride, ++nt) {
+    for (Tiles<MODE> tiles(q); ok && tiles.take(q, t); ++nt) {
       const int buf = nt % X::bufs;
 #pragma unroll
       for (int s = 0; s < X::segs; ++s) {
@@ -372,7 +377,7 @@ __global__ __launch_bounds__(kThreads, 1) void group_kernel(const __grid_constan
     uint32_t nt = 0;
     Tile t;
     Out out{maps.out, store + (warp - 4) * kStoreBytes, 0, q.vec != 0};
-    for (int L = first; tile_at<MODE>(q, L, t); L += stride, ++nt) {
+    for (Tiles<MODE> tiles(q); tiles.take(q, t); ++nt) {
       const int buf = nt % X::bufs;
       if (!bar_wait(sums_full + 8 * buf, (nt / X::bufs) & 1, dead)) break;
       __syncwarp();

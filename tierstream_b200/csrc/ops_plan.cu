@@ -80,18 +80,10 @@ __global__ __launch_bounds__(kPlanThreads) void plan_fill_kernel(const __grid_co
       p.head[2] = twice + mine2;
     }
   }
-  for (int i = threadIdx.x; i < mine; i += kPlanThreads) {
-    p.tile_unit[0][tiles + i] = int32_t(e);
-    p.tile_m0[0][tiles + i] = i * int(p.bm);
-    p.tile_info[tiles + i] = make_int4(p.slot[e], rows + i * int(p.bm), min(int(p.bm), cnt - i * int(p.bm)), int32_t(e));
-  }
-  for (int i = threadIdx.x; i < mine2; i += kPlanThreads) {
-    p.tile_unit[1][twice + i] = int32_t(e);
-    p.tile_m0[1][twice + i] = i * 2 * int(p.bm);
-  }
+  for (int i = threadIdx.x; i < mine; i += kPlanThreads) p.tiles[0][tiles + i] = make_int4(p.slot[e], rows, cnt, tiles);
+  for (int i = threadIdx.x; i < mine2; i += kPlanThreads) p.tiles[1][twice + i] = make_int4(p.slot[e], rows, cnt, twice);
   if (e + 1 == p.units)
-    for (uint32_t i = tiles + mine + threadIdx.x; i < p.max_tiles; i += kPlanThreads)
-      p.tile_info[i] = make_int4(0, 0, 0, 0);
+    for (uint32_t i = tiles + mine + threadIdx.x; i < p.max_tiles; i += kPlanThreads) p.tiles[0][i] = make_int4(0, 0, 0, 0);
   for (int i = cnt + threadIdx.x; i < padded; i += kPlanThreads) p.pair_of_row[rows + i] = -1;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int done = 0;  // pairs of this unit before the current span of ids
@@ -135,7 +127,7 @@ __global__ __launch_bounds__(kSmallThreads) void plan_small_kernel(const __grid_
                                                                    const __grid_constant__ Units u,
                                                                    const int32_t* __restrict__ ids) {
   __shared__ int32_t id[kSmallPairs];
-  __shared__ int32_t cnt[kSmallUnits], rows[kSmallUnits], tiles[kSmallUnits];
+  __shared__ int32_t cnt[kSmallUnits], rows[kSmallUnits];
   __shared__ int32_t wr[32], wt[32], wd[32];
   const uint32_t t = threadIdx.x;
   const int lane = t & 31, warp = t >> 5;
@@ -171,28 +163,19 @@ __global__ __launch_bounds__(kSmallThreads) void plan_small_kernel(const __grid_
   __syncthreads();
   for (int w = 0; w < warp; ++w) r += wr[w], k += wt[w], d += wd[w];
   rows[t] = r - padded;
-  tiles[t] = k - nt;
   __syncthreads();
   if (t < p.units) {
     p.cnt[t] = c;
     p.off[t] = rows[t];
     p.slot[t] = my_slot;
     if (t + 1 == p.units) p.head[0] = k, p.head[1] = r, p.head[2] = d;
-    for (int i = 0; i < nt; ++i) {
-      p.tile_unit[0][tiles[t] + i] = int32_t(t);
-      p.tile_m0[0][tiles[t] + i] = i * int(p.bm);
-      p.tile_info[tiles[t] + i] =
-          make_int4(my_slot, rows[t] + i * int(p.bm), min(int(p.bm), c - i * int(p.bm)), int32_t(t));
-    }
-    for (int i = 0; i < nd; ++i) {
-      p.tile_unit[1][d - nd + i] = int32_t(t);
-      p.tile_m0[1][d - nd + i] = i * 2 * int(p.bm);
-    }
+    for (int i = 0; i < nt; ++i) p.tiles[0][k - nt + i] = make_int4(my_slot, rows[t], c, k - nt);
+    for (int i = 0; i < nd; ++i) p.tiles[1][d - nd + i] = make_int4(my_slot, rows[t], c, d - nd);
     for (int i = c; i < padded; ++i) p.pair_of_row[rows[t] + i] = -1;
   }
   int all = 0;
   for (int w = 0; w < 32; ++w) all += wt[w];
-  for (uint32_t i = uint32_t(all) + t; i < p.max_tiles; i += kSmallThreads) p.tile_info[i] = make_int4(0, 0, 0, 0);
+  for (uint32_t i = uint32_t(all) + t; i < p.max_tiles; i += kSmallThreads) p.tiles[0][i] = make_int4(0, 0, 0, 0);
   if (t < p.pairs) {
     int32_t row = -1;
     if (valid && cnt[mine]) {
@@ -510,17 +493,13 @@ Plan plan_at(void* ws, uint32_t units, uint64_t pairs, uint32_t pad, uint32_t bm
   p.slot = take(units);
   p.pair_of_row = take(p.max_rows);
   p.row_of_pair = take(pairs);
-  for (int i = 0; i < 2; ++i) {
-    p.tile_unit[i] = take(p.max_tiles);
-    p.tile_m0[i] = take(p.max_tiles);
-  }
-  p.tile_info = reinterpret_cast<int4*>(take(uint64_t(p.max_tiles) * 4));
+  for (int i = 0; i < 2; ++i) p.tiles[i] = reinterpret_cast<int4*>(take(uint64_t(p.max_tiles) * 4));
   return p;
 }
 uint64_t plan_bytes(uint32_t units, uint64_t pairs, uint32_t pad, uint32_t bm) {
   const uint64_t met = pairs < units ? pairs : units;
   return aligned(12) + 3 * aligned(uint64_t(units) * 4) + aligned((pairs + met * (pad - 1)) * 4) + aligned(pairs * 4) +
-         4 * aligned((pairs / bm + met) * 4) + aligned((pairs / bm + met) * 16);
+         2 * aligned((pairs / bm + met) * 16);
 }
 
 int launch_plan(const Plan& p, const Units& u, const int32_t* ids, cudaStream_t s) {

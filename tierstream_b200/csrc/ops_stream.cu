@@ -109,13 +109,13 @@ __global__ __launch_bounds__(kThreads) void stream_kernel(const __grid_constant_
     w0 = static_cast<const T*>(q.w);
     w1 = w0 + kHalf * ldw;
   } else {
-    const int4 info = q.plan.tile_info[blockIdx.y];  // slot, first row, rows, unit
-    rows = info.z;
-    if (rows <= 0) return;  // (every CTA of the cluster leaves)
-    row0 = info.y;
+    const int4 info = q.plan.tiles[0][blockIdx.y];
+    rows = min(kTok, info.z - (int(blockIdx.y) - info.w) * kTok);
+    if (!info.z) return;  // (every CTA of the cluster leaves)
+    row0 = info.y + (int(blockIdx.y) - info.w) * kTok;
     ldw = p.k;
-    w0 = reinterpret_cast<const T*>(unit_part(q.units, MODE == kUp ? 0 : 2, info.w, info.x));
-    w1 = MODE == kUp ? reinterpret_cast<const T*>(unit_part(q.units, 1, info.w, info.x)) : w0 + kHalf * ldw;
+    w0 = reinterpret_cast<const T*>(unit_part(q.units, MODE == kUp ? 0 : 2, info.x));
+    w1 = MODE == kUp ? reinterpret_cast<const T*>(unit_part(q.units, 1, info.x)) : w0 + kHalf * ldw;
   }
   w0 += (n0 + g) * ldw + 16 * t;
   w1 += (n0 + g) * ldw + 16 * t;

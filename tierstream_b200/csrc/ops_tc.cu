@@ -46,47 +46,58 @@ struct Tile {
   int m0, n, kb;
 };
 
-// Tile L of the launch: groups in unit order, inside a group chunks of up to 16 row tiles, inside a chunk the column
-// tiles, and the chunk's row tiles innermost, so that tiles running at the same time share a unit's columns from L2.
+// The launch's tiles: groups (or the units' matrices) in unit order, inside each chunks of 2048 rows, inside a chunk the
+// column tiles, and the chunk's row tiles innermost, so that tiles running at the same time share a unit's columns from
+// L2. What the plan says of a tile is read one tile ahead.
 template <int MODE, int CG>
-__device__ __forceinline__ bool tile_at(const Params& q, int L, Tile& t) {
-  constexpr int kRows = kBM * CG, kChunk = 16 / CG;
-  int local, mt;
-  if constexpr (MODE == kUp || MODE == kUpBack || MODE == kDown || MODE == kDx) {
-    const int i = L / q.n_tiles;
-    if (i >= q.plan.head[0]) return false;
-    t.unit = q.plan.tile_unit[0][i];
-    t.rows = q.plan.cnt[t.unit];
-    t.stored = (t.rows + int(q.plan.pad) - 1) / int(q.plan.pad) * int(q.plan.pad);
-    t.row0 = q.plan.off[t.unit];
-    t.slot = q.plan.slot[t.unit];
-    mt = (t.rows + kRows - 1) / kRows;
-    local = L - (i - q.plan.tile_m0[0][i] / kRows) * q.n_tiles;
-    t.kb = q.k_blocks;
-  } else if constexpr (MODE == kDw) {
-    const int per = q.m_tiles * q.n_tiles;
-    t.unit = L / per;
-    if (t.unit >= int(q.plan.units)) return false;
-    t.row0 = q.plan.off[t.unit];
-    t.slot = 0;
-    t.rows = t.stored = int(q.p.m);
-    t.kb = (q.plan.cnt[t.unit] + kBK - 1) / kBK;
-    mt = q.m_tiles;
-    local = L - t.unit * per;
-  } else {
-    if (L >= q.m_tiles * q.n_tiles) return false;
-    t.unit = t.slot = t.row0 = 0;
-    t.rows = t.stored = int(q.p.m);
-    mt = q.m_tiles;
-    local = L;
-    t.kb = q.k_blocks;
+struct Tiles {
+  static constexpr bool grouped = MODE == kUp || MODE == kUpBack || MODE == kDown || MODE == kDx;
+  int at, end;
+  int4 next;  // slot, first row, rows, first tile (of a unit's matrix: first row and rows of its group)
+  __device__ __forceinline__ void fetch(const Params& q) {
+    if (at >= end) return;
+    if (grouped) next = q.plan.tiles[0][at / q.n_tiles];
+    if (MODE == kDw) {
+      const int unit = at / (q.m_tiles * q.n_tiles);
+      next.y = q.plan.off[unit];
+      next.z = q.plan.cnt[unit];
+    }
   }
-  const int chunk = local / (kChunk * q.n_tiles), in = local - chunk * kChunk * q.n_tiles;
-  const int width = min(kChunk, mt - chunk * kChunk);
-  t.n = in / width;
-  t.m0 = (chunk * kChunk + in - t.n * width) * kRows;
-  return true;
-}
+  __device__ __forceinline__ Tiles(const Params& q) : at(blockIdx.x / CG), next(make_int4(0, 0, 0, 0)) {
+    end = grouped ? q.plan.head[0] * q.n_tiles : q.m_tiles * q.n_tiles * (MODE == kDw ? int(q.plan.units) : 1);
+    fetch(q);
+  }
+  __device__ __forceinline__ bool take(const Params& q, Tile& t) {
+    constexpr int kRows = kBM * CG, kChunk = 16 / CG;
+    if (at >= end) return false;
+    const int4 g = next;
+    int local = at, mt = q.m_tiles;
+    at += gridDim.x / CG;
+    fetch(q);
+    t.slot = g.x;
+    t.row0 = g.y;
+    t.unit = 0;
+    t.kb = q.k_blocks;
+    if constexpr (grouped) {
+      t.rows = g.z;
+      t.stored = (g.z + int(q.plan.pad) - 1) / int(q.plan.pad) * int(q.plan.pad);
+      mt = (g.z + kRows - 1) / kRows;
+      local -= g.w * q.n_tiles;
+    } else {
+      t.rows = t.stored = int(q.p.m);
+      if (MODE == kDw) {
+        t.unit = local / (mt * q.n_tiles);
+        t.kb = (g.z + kBK - 1) / kBK;
+        local -= t.unit * mt * q.n_tiles;
+      }
+    }
+    const int chunk = local / (kChunk * q.n_tiles), in = local - chunk * kChunk * q.n_tiles;
+    const int width = min(kChunk, mt - chunk * kChunk);
+    t.n = in / width;
+    t.m0 = (chunk * kChunk + in - t.n * width) * kRows;
+    return true;
+  }
+};
 
 template <int MODE>
 struct Traits {
@@ -300,7 +311,6 @@ __global__ __launch_bounds__(kThreads, 1) void tc_kernel(const __grid_constant__
   volatile uint32_t* dead = words + 1;
   const int warp = __shfl_sync(0xffffffffu, int(threadIdx.x >> 5), 0);
   const uint32_t rank = CG == 2 ? cta_rank() : 0;
-  const int first = blockIdx.x / CG, stride = gridDim.x / CG;
   if (threadIdx.x == 0) {
     for (uint32_t s = 0; s < stages; ++s) {
       bar_init(full + 8 * s, 1);
@@ -338,7 +348,7 @@ __global__ __launch_bounds__(kThreads, 1) void tc_kernel(const __grid_constant__
     bool ok = true;
     Tile t;
     const uint32_t ring = smem_u32(smem), arrive = CG == 2 ? in_cta(full, 0) : full;
-    for (int L = first; ok && tile_at<MODE, CG>(q, L, t); L += stride) {
+    for (Tiles<MODE, CG> tiles(q); ok && tiles.take(q, t);) {
       t.m0 += int(rank) * kBM;
 #pragma unroll
       for (int s = 0; s < X::segs; ++s) {
@@ -384,7 +394,7 @@ __global__ __launch_bounds__(kThreads, 1) void tc_kernel(const __grid_constant__
     Tile t;
     const uint64_t ring_a = desc(smem_u32(smem), X::a_mn);
     constexpr uint32_t type = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
-    for (int L = first; ok && tile_at<MODE, CG>(q, L, t); L += stride, ++nt) {
+    for (Tiles<MODE, CG> tiles(q); ok && tiles.take(q, t); ++nt) {
       const int buf = nt % X::bufs;
 #pragma unroll
       for (int s = 0; s < X::segs; ++s) {
@@ -428,7 +438,7 @@ __global__ __launch_bounds__(kThreads, 1) void tc_kernel(const __grid_constant__
     uint32_t nt = 0;
     Tile t;
     Out out{maps.out, 0, store + (warp - 4) * kStoreBytes, 0, q.vec != 0};
-    for (int L = first; tile_at<MODE, CG>(q, L, t); L += stride, ++nt) {
+    for (Tiles<MODE, CG> tiles(q); tiles.take(q, t); ++nt) {
       t.m0 += int(rank) * kBM;
       const int buf = nt % X::bufs;
       if (!bar_wait(sums_full + 8 * buf, (nt / X::bufs) & 1, dead)) break;

@@ -79,12 +79,12 @@ __global__ __launch_bounds__(kThreads) void tile_kernel(const __grid_constant__ 
   Group g{0, 0, 0, p.m};
   int64_t m0 = int64_t(blockIdx.x) * 64;
   if (p.grouped) {
-    if (int32_t(blockIdx.x) >= plan.head[0]) return;
-    g.unit = plan.tile_unit[0][blockIdx.x];
-    m0 = plan.tile_m0[0][blockIdx.x];
-    g.rows = plan.cnt[g.unit];
-    g.row0 = plan.off[g.unit];
-    g.slot = plan.slot[g.unit];
+    const int4 i = plan.tiles[0][blockIdx.x];
+    if (!i.z) return;
+    g.slot = i.x;
+    g.row0 = i.y;
+    g.rows = i.z;
+    m0 = int64_t(int(blockIdx.x) - i.w) * 64;
   } else if (p.per_unit) {
     g.unit = blockIdx.z;
     g.rows = plan.cnt[g.unit];
@@ -99,7 +99,7 @@ __global__ __launch_bounds__(kThreads) void tile_kernel(const __grid_constant__ 
   for (int s = 0; s < p.segs; ++s) {
     const Operand &oa = p.a[s], &ob = p.b[s];
     const T* pa = static_cast<const T*>(oa.p);
-    const T* pb = ob.part >= 0 ? reinterpret_cast<const T*>(unit_part(units, ob.part, g.unit, g.slot))
+    const T* pb = ob.part >= 0 ? reinterpret_cast<const T*>(unit_part(units, ob.part, g.slot))
                                : static_cast<const T*>(ob.p);
     const int which = p.acc[s];
     for (int64_t k0 = 0; k0 < n_k; k0 += kBK) {
