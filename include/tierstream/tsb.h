@@ -359,7 +359,7 @@ SS_API ss_status tsb_dg_peer_retier(ss_ctx* c, const tsb_peer_tier* peer);
  * logits, a streamed dense layer), each with its backward pass. All matrices are row-major, ld* in elements between
  * rows. Every call enqueues kernels on `stream` of the current device and returns; it allocates nothing, waits for
  * nothing, and may be captured into a graph. Scratch comes from the caller: *_workspace gives its bytes (0: none is
- * needed; on a refused argument 0 too, and the call itself names the refusal), a 256-byte aligned device area that
+ * needed; on a refused argument 0 too, and the call itself names the refusal; ask with the call's own arguments), a 256-byte aligned device area that
  * belongs to the call until the stream has passed it (two calls that may run at the same time, or two graphs, need one
  * each). No result depends on the order in which anything ran: the same inputs give the same bits. Outputs must not
  * overlap inputs, except that y may be the residual (of the feed-forward block even when that is x). On a device-gated
@@ -377,7 +377,7 @@ SS_API ss_status tsb_dg_peer_retier(ss_ctx* c, const tsb_peer_tier* peer);
 
 /* z = x w^T + bias, y = act(z) + residual: x [rows][k], w [n][k], bias [n], residual and y [rows][n], all of `dtype`
  * (TSB_BF16 or TSB_F16). pre: z, rounded to dtype, for the backward pass. bias, residual and pre may be NULL.
- * rows = 0 does nothing; n and k are at least 1. Rows that start on 16 bytes (x and w, so k and the lds multiples of 8)
+ * rows = 0 does nothing; rows is below 2^28, n and k in [1, 2^20]. Rows that start on 16 bytes (x and w, so k and the lds multiples of 8)
  * take the fast kernels; every other alignment is served too. */
 typedef struct tsb_linear_args {
   uint32_t struct_size, dtype, act, reserved0;
@@ -466,7 +466,7 @@ SS_API ss_status tsb_units_from_view(const ss_dg_device_view* v, uint32_t g, uin
  * Wd_e (act(Wg_e x[t]) * (Wu_e x[t])), e = ids[t][k]; x and y [rows][hidden], ids and weights [rows][top] (device
  * memory). An id outside [0, n_units) contributes nothing (a padded row's -1, which is not to be exported); a row with
  * none gives its residual, or zeros. The same unit twice in a row counts twice. act(..) * (..) is rounded to dtype between the products; the
- * choices' sums are added in 32 bits. residual may be NULL. top is at most 64, rows x top at most 2^28. */
+ * choices' sums are added in 32 bits. residual may be NULL. top is at most 64, rows x top at most 2^28, hidden and ffn at most 2^20. */
 typedef struct tsb_ffn_args {
   uint32_t struct_size, dtype, act, top;
   uint64_t rows, hidden, ffn;

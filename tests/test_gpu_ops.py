@@ -75,7 +75,8 @@ def wide(t, extra, shift=0):
 LINEAR = [(1, 8, 64), (1, 1, 1), (1, 128, 4096), (2, 24, 40), (3, 1000, 520), (5, 129, 264), (7, 16, 8), (8, 512, 1024),
           (9, 40, 2056), (15, 264, 512), (16, 72, 136), (17, 256, 64), (31, 136, 392), (33, 520, 200), (64, 128, 64),
           (65, 1, 513), (70, 257, 255), (127, 264, 264), (128, 256, 128), (129, 136, 72), (200, 33, 31),
-          (300, 776, 1032), (513, 512, 512)]
+          (300, 776, 1032), (513, 512, 512), (12, 1001, 4096), (40, 2055, 1024), (100, 129, 8192), (250, 1000, 2048),
+          (300, 333, 4096), (600, 1001, 512), (1100, 2056, 264)]
 
 
 @pytest.mark.parametrize("rows,n,k", LINEAR)
@@ -152,7 +153,7 @@ def test_linear_largest_and_no_rows():
     assert ops.linear(x[:0], w).shape == (0, 64)
 
 
-BACK = [(1, 8, 64), (2, 3, 5), (7, 129, 264), (16, 72, 136), (64, 128, 64), (100, 257, 255), (129, 136, 520),
+BACK = [(1, 8, 64), (2, 3, 5), (7, 129, 264), (9, 2048, 1024), (70, 4096, 264), (260, 1024, 2056), (1000, 512, 1032), (16, 72, 136), (64, 128, 64), (100, 257, 255), (129, 136, 520),
         (300, 776, 264), (513, 512, 256)]
 
 
@@ -333,7 +334,7 @@ def plain_ffn(x, ids, w, parts, act, res=None):
 FFN = [(1, 8, 8, 1, 1), (1, 64, 128, 4, 2), (1, 512, 1408, 8, 2), (2, 72, 40, 3, 3), (4, 128, 64, 16, 2),
        (5, 33, 17, 4, 2), (7, 264, 520, 8, 4), (16, 256, 136, 2, 2), (24, 128, 192, 64, 8), (33, 100, 60, 5, 2),
        (65, 512, 256, 4, 1), (130, 264, 392, 3, 2), (200, 128, 256, 2, 5), (300, 256, 512, 40, 6), (700, 136, 264, 7, 3),
-       (1500, 64, 72, 3, 2)]
+       (1500, 64, 72, 3, 2), (1200, 136, 264, 1, 1), (2100, 128, 72, 2, 1), (33, 72, 2056, 2, 1)]
 
 
 @pytest.mark.parametrize("rows,hidden,ffn,units,top", FFN)
@@ -532,6 +533,58 @@ def test_on_another_stream_and_captured():
                 assert torch.equal(out, layer(new))
 
 
+def test_captured_behind_copies_and_fills():
+    """A captured call right behind a fill and a copy of its inputs sees them; one in place on x as its own residual."""
+    t = torch.bfloat16
+    x, ids, w, un, parts = problem(4, 40, 128, 136, 5, 2, t)
+    src = x.clone()
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        want = ops.ffn(src, ids, w, un, residual=src)
+        lin = ops.linear(torch.zeros_like(src), parts[0][0])
+    s.synchronize()
+    g = torch.cuda.CUDAGraph()
+    y = torch.empty_like(x)
+    with torch.cuda.graph(g, stream=s):
+        y.zero_()
+        z = ops.linear(y, parts[0][0])
+        x.copy_(src)
+        ops.ffn(x, ids, w, un, residual=x, out=x)
+    for _ in range(3):
+        x.fill_(9.0)
+        y.fill_(9.0)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(s):
+            g.replay()
+        s.synchronize()
+        assert torch.equal(x, want) and torch.equal(z, lin)
+
+
+def test_ops_from_two_threads():
+    """Two threads on streams of their own, the same units and different inputs: each gets its own results."""
+    import threading
+    t = torch.bfloat16
+    jobs = []
+    for k, rows in enumerate((3, 170)):
+        x, ids, w, un, _ = problem(40 + k, rows, 256, 264, 6, 2, t)
+        jobs.append((x, ids, w, un, ops.ffn(x, ids, w, un, residual=x), []))
+    torch.cuda.synchronize()
+
+    def work(x, ids, w, un, want, bad):
+        s = torch.cuda.Stream()
+        with torch.cuda.stream(s):
+            got = [ops.ffn(x, ids, w, un, residual=x) for _ in range(40)]
+        s.synchronize()
+        bad += [i for i, y in enumerate(got) if not torch.equal(y, want)]
+    threads = [threading.Thread(target=work, args=j) for j in jobs]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join()
+    assert all(not j[-1] for j in jobs)
+
+
 def test_backward_captured():
     t = torch.bfloat16
     x, ids, w, un, parts = problem(5, 150, 128, 264, 6, 2, t)
@@ -611,7 +664,9 @@ def test_refusals_on_tensors():
                 lambda: ops.Units(un.keep[0], un.keep[1], un.keep[2], ids.float()), lambda: ops.route(x, 17),
                 lambda: ops.route(x, 0), lambda: ops.linear(x, torch.zeros((16, 16), dtype=t, device="cuda"), out=x),
                 lambda: ops.ffn(x, ids, p, un, out=x), lambda: ops.ffn(x, ids, p, un, residual=x, out=x[:2]),
-                lambda: ops.route_backward(p, x[:2], ids, p)):
+                lambda: ops.route_backward(p, x[:2], ids, p),
+                lambda: ops.linear(x[:, :8], w[:, :8], residual=w[:4, :8], out=w[1:5, :8]),
+                lambda: ops.ffn(x[:2], ids[:2], p[:2], un, residual=x[1:3], out=x[2:4])):
         with pytest.raises(ValueError):
             bad()
     with pytest.raises(abi.TsError):  # the library's own refusals

@@ -38,7 +38,7 @@ void ck(int e, const char* fn, const char* what) {
   tsb::fail(SS_E_BACKEND, std::string(fn) + ": " + what + ": " + cudaGetErrorString(cudaError_t(e)));
 }
 
-constexpr uint64_t kMaxDim = uint64_t(1) << 22, kMaxRows = uint64_t(1) << 28;
+constexpr uint64_t kMaxDim = uint64_t(1) << 20, kMaxRows = uint64_t(1) << 28;
 
 // The workspace handed out front to back, every piece on 256 bytes.
 struct Arena {
@@ -128,7 +128,7 @@ void check_linear(const tsb_linear_args* a) {
   need(a && a->struct_size >= sizeof *a, fn, "null or short argument struct");
   need(a->dtype == TSB_BF16 || a->dtype == TSB_F16, fn, "dtype must be TSB_BF16 or TSB_F16");
   need(a->act <= TSB_ACT_RELU, fn, "unknown activation");
-  need(a->n >= 1 && a->k >= 1 && a->n < kMaxDim && a->k < kMaxDim, fn, "n and k must be in [1, 2^22)");
+  need(a->n >= 1 && a->k >= 1 && a->n <= kMaxDim && a->k <= kMaxDim, fn, "n and k must be in [1, 2^20]");
   need(a->rows < kMaxRows, fn, "rows must be below 2^28");
   if (!a->rows) return;
   need(a->x && a->w && a->y, fn, "null argument");
@@ -167,7 +167,7 @@ void check_linear_back(const tsb_linear_grad_args* a) {
   need(a && a->struct_size >= sizeof *a, fn, "null or short argument struct");
   need(a->dtype == TSB_BF16 || a->dtype == TSB_F16, fn, "dtype must be TSB_BF16 or TSB_F16");
   need(a->act <= TSB_ACT_RELU, fn, "unknown activation");
-  need(a->n >= 1 && a->k >= 1 && a->n < kMaxDim && a->k < kMaxDim, fn, "n and k must be in [1, 2^22)");
+  need(a->n >= 1 && a->k >= 1 && a->n <= kMaxDim && a->k <= kMaxDim, fn, "n and k must be in [1, 2^20]");
   need(a->rows < kMaxRows, fn, "rows must be below 2^28");
   need(!a->dw || a->lddw >= a->k, fn, "a leading dimension is shorter than its row");
   if (!a->rows) return;
@@ -198,7 +198,7 @@ struct LinearBackSpace {
 LinearBackSpace linear_back_space(const tsb_linear_grad_args* a) {
   Arena w{static_cast<char*>(a->workspace)};
   LinearBackSpace r{a->dy, a->lddy, nullptr, nullptr, 0};
-  if (!a->rows) return r;
+  if (!a->rows || (!a->dx && !a->dw && !a->db)) return r;
   if (a->act != TSB_ACT_NONE) {
     r.ldz = (a->n + 7) / 8 * 8;
     r.dz = w.take(a->rows * r.ldz * 2);
@@ -218,6 +218,7 @@ void linear_back(const tsb_linear_grad_args* a) {
     if (a->db) ck(int(cudaMemsetAsync(a->db, 0, a->n * 2, s)), fn, "db");
     return;
   }
+  if (!a->dx && !a->dw && !a->db) return;
   const LinearBackSpace w = linear_back_space(a);
   need_workspace(fn, a->workspace, a->workspace_bytes, w.bytes);
   const bool slope = a->act != TSB_ACT_NONE;
@@ -263,8 +264,8 @@ void check_ffn_shape(const A* a, const char* fn) {
   need(a && a->struct_size >= sizeof *a, fn, "null or short argument struct");
   need(a->dtype == TSB_BF16 || a->dtype == TSB_F16, fn, "dtype must be TSB_BF16 or TSB_F16");
   need(a->act <= TSB_ACT_RELU, fn, "unknown activation");
-  need(a->hidden >= 1 && a->ffn >= 1 && a->hidden < kMaxDim && a->ffn < kMaxDim, fn,
-       "hidden and ffn must be in [1, 2^22)");
+  need(a->hidden >= 1 && a->ffn >= 1 && a->hidden <= kMaxDim && a->ffn <= kMaxDim, fn,
+       "hidden and ffn must be in [1, 2^20]");
   need(a->top >= 1 && a->top <= 64, fn, "top must be in [1, 64]");
   need(a->rows <= kMaxRows / a->top, fn, "rows x top must be at most 2^28");
   const tsb_units* u = a->units;

@@ -95,6 +95,10 @@ void apart(const char* name, const at::Tensor& out, const at::Tensor& in) {
   if (static_cast<char*>(out.data_ptr()) < end(in) && static_cast<char*>(in.data_ptr()) < end(out))
     refuse(name, ": overlaps an input");
 }
+// refuses an output that lies on its residual in any other way than element on element
+void on_residual(const at::Tensor& out, const at::Tensor& residual) {
+  if (out.data_ptr() != residual.data_ptr() || out.strides() != residual.strides()) apart("out", out, residual);
+}
 at::Tensor fresh(const at::Tensor& like, at::IntArrayRef shape) { return at::empty(shape, like.options().requires_grad(false)); }
 
 c10::Device cuda_of(const at::Tensor& t) {
@@ -166,6 +170,7 @@ PyObject* linear(PyObject*, PyObject* const* v, Py_ssize_t n) {
     m = mat("out", out, rows, cols, x);
     apart("out", out, x);
     apart("out", out, w);
+    if (there(v[3])) on_residual(out, tensor("residual", v[3]));
     if (there(v[5])) apart("out", out, tensor("pre", v[5]));
   } else {
     out = fresh(x, {rows, cols});
@@ -346,6 +351,7 @@ PyObject* ffn(PyObject*, PyObject* const* v, Py_ssize_t n) {
     out = tensor("out", v[7]);
     const Mat m = mat("out", out, rows, hidden, x);
     if (!on_x) apart("out", out, x);  // (in place on x as its own residual: x is read first)
+    if (there(v[6])) on_residual(out, tensor("residual", v[6]));
     a.y = m.p, a.ldy = m.ld;
   } else {
     out = fresh(x, {rows, hidden});
