@@ -980,9 +980,9 @@ def main():
                            "buffers); a miss from a pinned block at that copy rate; blended in the proportion of rank "
                            "0's timed tokens (%d file reads of %d units)" % (file_units, units_moved)})
         a.no_cpu_baseline = True  # the reference arm's sample is the pinned-RAM configuration
-    if not a.no_cpu_baseline and world == 1:
+    import oracle
+    if not a.no_cpu_baseline and world == 1 and oracle.ref_available():
         # the reference arm's own measurement (same trace, tokens and warm-up subtraction)
-        import oracle
         v_ref, dt_ref = reference_measure(ids, a)
         line["cpu_baseline"] = {"value": round(v_ref, 3), "unit": "GB/s",
                                 "cores": int(oracle.ref().oref_copy_threads()), "kind": "reference",
