@@ -156,7 +156,7 @@ __device__ __forceinline__ float from_f(float v) { return v; }
 
 // What a product writes. Sums are held in 32 bits up to here; each store below rounds once.
 enum Epi {
-  kEpiLinear,   // z = acc + bias; pre = z; out = act(z) + residual
+  kEpiLinear,   // z = acc + bias; pre = z; out = act(z) + residual (aligned operands only)
   kEpiStore,    // out = acc (a gradient), per unit at out + e x out_unit
   kEpiRows32,   // rows32[row][n] = acc in 32 bits (joined later)
   kEpiUp,       // out[row][n] = act(acc0) x acc1
@@ -218,14 +218,25 @@ int launch_route(int dtype, const void* logits, uint64_t ld, uint64_t rows, uint
 int launch_route_back(int dtype, int dw_dtype, const void* dw, const void* logits, uint64_t ld, const int32_t* ids,
                       const float* weights, uint64_t rows, uint32_t experts, uint32_t top, int norm, void* dlogits,
                       uint64_t ldd, cudaStream_t s);
+// Copies of matrices whose rows do not start on 16 bytes to rows that do, the columns up to ldd filled with zeros.
+struct Copy {
+  const void* src;
+  void* dst;
+  uint64_t ld, ldd, rows, cols;
+};
+struct Copies {
+  Copy c[2];
+  int n;
+};
+int launch_copies(const Copies& c, cudaStream_t s);
 // dz = dy x act'(pre) (act none: not written) and, with db, its column sums; part: [chunks][n] floats
 uint32_t dz_chunks(uint64_t rows, uint64_t n);
 int launch_dz(int dtype, int act, const void* dy, uint64_t ldy, const void* pre, uint64_t ldp, void* dz, uint64_t ldz,
               uint64_t rows, uint64_t n, void* db, float* part, cudaStream_t s);
 
-// ops_tile.cu: any product at any size, stride and alignment
+// ops_tile.cu: the feed-forward block's products at any size, stride and alignment
 constexpr uint32_t kTileM = 64, kTileN = 64;
-int launch_tile(int dtype, const Product& p, const Plan* plan, const Units* units, cudaStream_t s);
+int launch_tile(int dtype, const Product& p, const Plan& plan, const Units& units, cudaStream_t s);
 
 
 // ops_stream.cu: products of few rows, in tiles of 8 (the plan's bm). Rows of x and w start on 16 bytes and k

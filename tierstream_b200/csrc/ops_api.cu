@@ -72,16 +72,15 @@ constexpr uint64_t kStreamRows = kStreamTile, kStreamEach = 2;
 // 0.10 + 0.0012 columns for a pair of CTAs (0.254 measured at 128 columns, 0.405 at 256; 0.2 at least), 0.17 + 0.00098
 // columns for a single one, about 6 for a launch's start and end, 3 for the join's, which reads 32-bit rows at 6 TB/s.
 struct How {
-  enum Kind { kAny, kStream, kTc, kGroup } kind;
+  enum Kind { kStream, kTc, kGroup } kind;
   int splits;
 };
 constexpr int kSms = 148;
 double slice_us(double columns) { return columns < 84 ? 0.2 : 0.10 + 0.0012 * columns; }
 
 How how(const Product& p) {
-  if (!tc_fits(p.a[0], nullptr) || !tc_fits(p.b[0], nullptr)) return {How::kAny, 1};
   const bool forward = p.epi == kEpiLinear;
-  if (forward && uint64_t(p.m) <= kStreamRows && p.k % 8 == 0) return {How::kStream, 1};
+  if (forward && uint64_t(p.m) <= kStreamRows) return {How::kStream, 1};
   if (p.a[0].s_k != 1) return {How::kTc, 1};  // (dw: a sum over rows)
   const double kb = double(ceil_div(uint64_t(p.k), 64)), bytes = 2.0 * double(p.n) * double(p.k) / 6.5e6;
   // the matrix as columns, in the columns a tile that launch_tc would take
@@ -111,7 +110,6 @@ int product(int dtype, const Product& p, float* rows32, cudaStream_t s) {
   switch (h.kind) {
     case How::kStream: return launch_stream(dtype, p, 1, nullptr, nullptr, s);
     case How::kTc: return launch_tc(dtype, p, nullptr, nullptr, s);
-    case How::kAny: return launch_tile(dtype, p, nullptr, nullptr, s);
     case How::kGroup: break;
   }
   Product r = p;
@@ -120,6 +118,18 @@ int product(int dtype, const Product& p, float* rows32, cudaStream_t s) {
   if (const int e = launch_group(dtype, r, h.splits, nullptr, nullptr, s)) return e;
   return launch_join_linear(dtype, p.act, rows32, uint32_t(h.splits), uint64_t(p.m), uint64_t(p.n), p.bias, p.residual,
                             uint64_t(p.ldr), p.out, uint64_t(p.ldo), p.pre, uint64_t(p.ldp), s);
+}
+
+// An operand, [rows][cols] in memory, whose rows do not start on 16 bytes (or, `whole`, do not hold whole eights) is copied
+// into the workspace first: the fast kernels read it from there.
+void align(Operand& o, uint64_t rows, uint64_t cols, bool whole, Arena& w, Copies& copies) {
+  if (tc_fits(o, nullptr) && !(whole && cols % 8)) return;
+  const uint64_t ld = o.s_k == 1 ? uint64_t(o.s_i) : uint64_t(o.s_k), ldd = (cols + 7) / 8 * 8;
+  const bool k_inner = !o.map_k && o.s_k == 1;
+  void* dst = w.take(rows * ldd * 2);
+  copies.c[copies.n++] = {o.p, dst, ld, ldd, rows, cols};
+  o.p = dst;
+  (k_inner ? o.s_i : o.s_k) = int64_t(ldd);
 }
 
 // ---- linear ----
@@ -137,29 +147,44 @@ void check_linear(const tsb_linear_args* a) {
        fn, "a leading dimension is shorter than its row");
 }
 
-Product linear_product(const tsb_linear_args* a);
-void linear(const tsb_linear_args* a) {
-  const char* fn = "tsb_linear";
-  check_linear(a);
-  if (!a->rows) return;
-  const Product p = linear_product(a);
-  need_workspace(fn, a->workspace, a->workspace_bytes, product_bytes(p));
-  ck(product(int(a->dtype), p, static_cast<float*>(a->workspace), static_cast<cudaStream_t>(a->stream)), fn, "launch");
-}
-
-Product linear_product(const tsb_linear_args* a) {
-  Product p{};
+struct LinearSpace {
+  Product p;
+  Copies copies;
+  float* rows32;
+  uint64_t bytes;
+};
+LinearSpace linear_space(const tsb_linear_args* a) {
+  Arena w{static_cast<char*>(a->workspace)};
+  LinearSpace r{};
+  Product& p = r.p;
   p.segs = 1;
   p.a[0] = dense(a->x, int64_t(a->ldx), 1);
   p.b[0] = dense(a->w, int64_t(a->ldw), 1);
   p.m = int64_t(a->rows), p.n = int64_t(a->n), p.k = int64_t(a->k);
+  const bool few = a->rows <= kStreamRows;  // (streamed rows are read in whole eights)
+  align(p.a[0], a->rows, a->k, few, w, r.copies);
+  align(p.b[0], a->n, a->k, few, w, r.copies);
+  if (few) p.k = (p.k + 7) / 8 * 8;
   p.epi = kEpiLinear;
   p.act = int(a->act);
   p.out = a->y, p.ldo = int64_t(a->ldy);
   p.bias = a->bias;
   p.residual = a->residual, p.ldr = int64_t(a->ldr);
   p.pre = a->pre, p.ldp = int64_t(a->ldp);
-  return p;
+  r.rows32 = static_cast<float*>(w.take(product_bytes(p)));
+  r.bytes = w.used;
+  return r;
+}
+
+void linear(const tsb_linear_args* a) {
+  const char* fn = "tsb_linear";
+  check_linear(a);
+  if (!a->rows) return;
+  const LinearSpace w = linear_space(a);
+  need_workspace(fn, a->workspace, a->workspace_bytes, w.bytes);
+  cudaStream_t s = static_cast<cudaStream_t>(a->stream);
+  if (w.copies.n) ck(launch_copies(w.copies, s), fn, "aligned copies");
+  ck(product(int(a->dtype), w.p, w.rows32, s), fn, "launch");
 }
 
 void check_linear_back(const tsb_linear_grad_args* a) {
@@ -178,33 +203,47 @@ void check_linear_back(const tsb_linear_grad_args* a) {
        fn, "a leading dimension is shorter than its row");
 }
 
-Product dx_product(const tsb_linear_grad_args* a, const void* dz, uint64_t ldz) {
-  Product p{};
-  p.segs = 1;
-  p.a[0] = dense(dz, int64_t(ldz), 1);
-  p.b[0] = dense(a->w, 1, int64_t(a->ldw));
-  p.m = int64_t(a->rows), p.n = int64_t(a->k), p.k = int64_t(a->n);
-  p.epi = kEpiStore;
-  p.out = a->dx, p.ldo = int64_t(a->lddx);
-  return p;
-}
-
 struct LinearBackSpace {
-  const void* dz;  // dy itself without an activation
+  void* dz;  // NULL: dy itself
   uint64_t ldz;
+  Copies copies;
+  Product dx, dw;
   float *part, *rows32;
   uint64_t bytes;
 };
 LinearBackSpace linear_back_space(const tsb_linear_grad_args* a) {
   Arena w{static_cast<char*>(a->workspace)};
-  LinearBackSpace r{a->dy, a->lddy, nullptr, nullptr, 0};
+  LinearBackSpace r{};
   if (!a->rows || (!a->dx && !a->dw && !a->db)) return r;
-  if (a->act != TSB_ACT_NONE) {
+  const void* dz = a->dy;
+  r.ldz = a->lddy;
+  // dz: the slope times dy, or a copy of dy whose rows start on 16 bytes
+  if (a->act != TSB_ACT_NONE || ((a->dx || a->dw) && !tc_fits(dense(a->dy, int64_t(a->lddy), 1), nullptr))) {
     r.ldz = (a->n + 7) / 8 * 8;
-    r.dz = w.take(a->rows * r.ldz * 2);
+    dz = r.dz = w.take(a->rows * r.ldz * 2);
   }
   if (a->db) r.part = static_cast<float*>(w.take(uint64_t(dz_chunks(a->rows, a->n)) * a->n * 4));
-  if (a->dx) r.rows32 = static_cast<float*>(w.take(product_bytes(dx_product(a, r.dz, r.ldz))));
+  if (a->dx) {
+    Product& p = r.dx;
+    p.segs = 1;
+    p.a[0] = dense(dz, int64_t(r.ldz), 1);
+    p.b[0] = dense(a->w, 1, int64_t(a->ldw), 1);
+    align(p.b[0], a->n, a->k, false, w, r.copies);
+    p.m = int64_t(a->rows), p.n = int64_t(a->k), p.k = int64_t(a->n);
+    p.epi = kEpiStore;
+    p.out = a->dx, p.ldo = int64_t(a->lddx);
+    r.rows32 = static_cast<float*>(w.take(product_bytes(p)));
+  }
+  if (a->dw) {
+    Product& p = r.dw;
+    p.segs = 1;
+    p.a[0] = dense(dz, 1, int64_t(r.ldz), 1);
+    p.b[0] = dense(a->x, 1, int64_t(a->ldx), 1);
+    align(p.b[0], a->rows, a->k, false, w, r.copies);
+    p.m = int64_t(a->n), p.n = int64_t(a->k), p.k = int64_t(a->rows);
+    p.epi = kEpiStore;
+    p.out = a->dw, p.ldo = int64_t(a->lddw);
+  }
   r.bytes = w.used;
   return r;
 }
@@ -221,25 +260,12 @@ void linear_back(const tsb_linear_grad_args* a) {
   if (!a->dx && !a->dw && !a->db) return;
   const LinearBackSpace w = linear_back_space(a);
   need_workspace(fn, a->workspace, a->workspace_bytes, w.bytes);
-  const bool slope = a->act != TSB_ACT_NONE;
-  if (slope || a->db)
-    ck(launch_dz(int(a->dtype), int(a->act), a->dy, a->lddy, a->pre, a->ldp, slope ? const_cast<void*>(w.dz) : nullptr,
-                 w.ldz, a->rows, a->n, a->db, w.part, s),
+  if (w.copies.n) ck(launch_copies(w.copies, s), fn, "aligned copies");
+  if (w.dz || a->db)
+    ck(launch_dz(int(a->dtype), int(a->act), a->dy, a->lddy, a->pre, a->ldp, w.dz, w.ldz, a->rows, a->n, a->db, w.part, s),
        fn, "slope");
-  if (a->dx) {
-    Product p = dx_product(a, w.dz, w.ldz);
-    ck(product(int(a->dtype), p, w.rows32, s), fn, "dx");
-  }
-  if (a->dw) {
-    Product p{};
-    p.segs = 1;
-    p.a[0] = dense(w.dz, 1, int64_t(w.ldz), 1);
-    p.b[0] = dense(a->x, 1, int64_t(a->ldx), 1);
-    p.m = int64_t(a->n), p.n = int64_t(a->k), p.k = int64_t(a->rows);
-    p.epi = kEpiStore;
-    p.out = a->dw, p.ldo = int64_t(a->lddw);
-    ck(product(int(a->dtype), p, nullptr, s), fn, "dw");
-  }
+  if (a->dx) ck(product(int(a->dtype), w.dx, w.rows32, s), fn, "dx");
+  if (a->dw) ck(product(int(a->dtype), w.dw, nullptr, s), fn, "dw");
 }
 
 // ---- the gated feed-forward block ----
@@ -353,7 +379,7 @@ void ffn(const tsb_ffn_args* a) {
   const auto go = [&](const Product& pr) {
     return w.stream ? launch_stream(int(a->dtype), pr, a->top, &w.plan, &u, s)
            : w.tc   ? launch_grouped(int(a->dtype), pr, &w.plan, &u, s)
-                    : launch_tile(int(a->dtype), pr, &w.plan, &u, s);
+                    : launch_tile(int(a->dtype), pr, w.plan, u, s);
   };
   if (w.tc) {
     ck(launch_gather(w.plan, a->top, a->x, a->ldx, a->hidden, w.xs, s), fn, "gather");
@@ -433,7 +459,7 @@ void ffn_back(const tsb_ffn_grad_args* a) {
   const int dt = int(a->dtype);
   ck(launch_plan(w.plan, u, a->ids, s), fn, "plan");
   const auto go = [&](const Product& pr) {
-    return w.tc ? launch_grouped(dt, pr, &w.plan, &u, s) : launch_tile(dt, pr, &w.plan, &u, s);
+    return w.tc ? launch_grouped(dt, pr, &w.plan, &u, s) : launch_tile(dt, pr, w.plan, u, s);
   };
   Operand x_rows = gathered(a->x, int64_t(a->ldx), 1, w.plan, a->top),
           dy_rows = gathered(a->dy, int64_t(a->lddy), 1, w.plan, a->top),
@@ -519,12 +545,7 @@ uint64_t bytes_of(const A* a, void (*check)(const A*), F&& space) {
 extern "C" {
 
 uint64_t tsb_linear_workspace(const tsb_linear_args* a) {
-  return bytes_of(a, check_linear, [](const tsb_linear_args* b) {
-    struct {
-      uint64_t bytes;
-    } r{product_bytes(linear_product(b))};
-    return r;
-  });
+  return bytes_of(a, check_linear, linear_space);
 }
 ss_status tsb_linear(const tsb_linear_args* a) {
   return run([&] { linear(a); });

@@ -265,11 +265,30 @@ __global__ __launch_bounds__(256) void join_dw_kernel(const int32_t* __restrict_
   if (lane == 0) dw[i] = from_f<T>(s);
 }
 
+// A warp a row, two bytes a lane: what a matrix of odd rows costs before its product (30 MB in about 10 us).
+__global__ __launch_bounds__(256) void copies_kernel(const __grid_constant__ Copies j) {
+  begin_after();
+  const uint64_t stride = uint64_t(gridDim.x) * 8;
+  uint64_t r = uint64_t(blockIdx.x) * 8 + (threadIdx.x >> 5);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    if (i >= j.n) break;
+    const Copy& c = j.c[i];
+    for (; r < c.rows; r += stride) {
+      const uint16_t* s = static_cast<const uint16_t*>(c.src) + r * c.ld;
+      uint16_t* d = static_cast<uint16_t*>(c.dst) + r * c.ldd;
+#pragma unroll 4
+      for (uint64_t k = threadIdx.x & 31; k < c.ldd; k += 32) d[k] = k < c.cols ? s[k] : uint16_t(0);
+    }
+    r -= c.rows;  // (the second matrix' rows follow the first's)
+  }
+}
+
 // ---------------------------------------------------------------------------------------------------------------
-// dz = dy act'(pre), rounded once to the operands' type (the products take 16-bit operands), and db from the unrounded
+// dz = dy act'(pre) (or a copy of dy without an activation), rounded once to the operands' type (the products take 16-bit operands), and db from the unrounded
 // values: each CTA sums kDzRows rows of 32 V columns, then one thread per column adds the CTAs' sums in order.
 // ---------------------------------------------------------------------------------------------------------------
-constexpr uint32_t kDzRows = 128;
+constexpr uint32_t kDzRows = 64;
 
 template <class T, int V>
 __global__ __launch_bounds__(256) void dz_kernel(int act, const T* __restrict__ dy, uint64_t ldy,
@@ -285,14 +304,14 @@ __global__ __launch_bounds__(256) void dz_kernel(int act, const T* __restrict__ 
       T a[V], z[V];
       if constexpr (V == 8) {
         *reinterpret_cast<uint4*>(a) = *reinterpret_cast<const uint4*>(dy + r * ldy + c);
-        if (dz) *reinterpret_cast<uint4*>(z) = *reinterpret_cast<const uint4*>(pre + r * ldp + c);
+        if (pre) *reinterpret_cast<uint4*>(z) = *reinterpret_cast<const uint4*>(pre + r * ldp + c);
       } else {
         a[0] = dy[r * ldy + c];
-        if (dz) z[0] = pre[r * ldp + c];
+        if (pre) z[0] = pre[r * ldp + c];
       }
 #pragma unroll
       for (int v = 0; v < V; ++v) {
-        const float d = to_f(a[v]) * (dz ? slope_rt(act, to_f(z[v])) : 1.f);
+        const float d = to_f(a[v]) * (pre ? slope_rt(act, to_f(z[v])) : 1.f);
         sum[v] += d;
         a[v] = from_f<T>(d);
       }
@@ -539,6 +558,13 @@ int launch_join_linear(int dtype, int act, const float* rows32, uint32_t splits,
   return e;
 }
 
+int launch_copies(const Copies& c, cudaStream_t s) {
+  uint64_t rows = 0;
+  for (int i = 0; i < c.n; ++i) rows += c.c[i].rows;
+  const uint64_t blocks = ceil_div(rows, 8);
+  return launch(copies_kernel, unsigned(blocks < 1184 ? blocks : 1184), 256, 0, 1, s, c);
+}
+
 int launch_join_dw(int dtype, const Plan& p, const float* dwp, uint32_t tiles, void* dw, cudaStream_t s) {
   int e = 0;
   by_type(dtype, [&](auto v) {
@@ -553,12 +579,12 @@ uint32_t dz_chunks(uint64_t rows, uint64_t) { return uint32_t(ceil_div(rows, kDz
 
 int launch_dz(int dtype, int act, const void* dy, uint64_t ldy, const void* pre, uint64_t ldp, void* dz, uint64_t ldz,
               uint64_t rows, uint64_t n, void* db, float* part, cudaStream_t s) {
-  const bool wide = n % 8 == 0 && on16(dy) && ldy % 8 == 0 && (!dz || (on16(pre) && ldp % 8 == 0 && ldz % 8 == 0));
+  const bool wide = n % 8 == 0 && on16(dy) && ldy % 8 == 0 && (!pre || (on16(pre) && ldp % 8 == 0)) && (!dz || ldz % 8 == 0);
   const uint32_t chunks = dz_chunks(rows, n);
   int e = 0;
   by_type(dtype, [&](auto v) {
     using T = decltype(v);
-    const T *a = static_cast<const T*>(dy), *b = static_cast<const T*>(pre);
+    const T *a = static_cast<const T*>(dy), *b = act == TSB_ACT_NONE ? nullptr : static_cast<const T*>(pre);
     T* z = static_cast<T*>(dz);
     float* sums = db ? part : nullptr;
     const unsigned each = wide ? 8 : 1;

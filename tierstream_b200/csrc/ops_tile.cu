@@ -1,9 +1,9 @@
-// A matrix product for every size, stride and alignment: C[m][n] = sum_k A[m][k] B[n][k] with up to three operand
-// pairs and three accumulators, rows gathered through the plan, the matrices of a unit found through its slot, and the
-// epilogues of ops.hpp. One CTA of four warps computes a 64 x 64 tile from 32-wide slices of k staged in shared memory
-// by element loads along whichever index is contiguous; the products run on mma.sync with 32-bit sums. Element loads
-// bound it (11 TFLOP/s at 2047 x 7168 x 4096, fp16): the aligned shapes run on ops_stream.cu and ops_tc.cu instead, and this
-// kernel serves what those refuse (rows that do not start on 16 bytes, units found by address with many rows).
+// The feed-forward block's products for every size, stride and alignment: C[m][n] = sum_k A[m][k] B[n][k] with up to three
+// operand pairs and three accumulators, rows gathered through the plan, the matrices of a unit found through its slot, and
+// the epilogues of ops.hpp. One CTA of four warps computes a 64 x 64 tile from 32-wide slices of k staged in shared memory
+// by element loads along whichever index is contiguous; the products run on mma.sync with 32-bit sums. The element loads
+// bound it (8.6 TFLOP/s for a prompt of 2047 rows over 128 units): it serves what the other kernels refuse, units whose
+// rows do not start on 16 bytes and gradients of units found by address.
 #include "ops.hpp"
 
 namespace tsb {
@@ -76,7 +76,7 @@ __global__ __launch_bounds__(kThreads) void tile_kernel(const __grid_constant__ 
   __shared__ __align__(16) T sb[64 * kLd];
   __shared__ float red[2][64];
   begin_after();
-  Group g{0, 0, 0, p.m};
+  Group g{};
   int64_t m0 = int64_t(blockIdx.x) * 64;
   if (p.grouped) {
     const int4 i = plan.tiles[0][blockIdx.x];
@@ -85,14 +85,14 @@ __global__ __launch_bounds__(kThreads) void tile_kernel(const __grid_constant__ 
     g.row0 = i.y;
     g.rows = i.z;
     m0 = int64_t(int(blockIdx.x) - i.w) * 64;
-  } else if (p.per_unit) {
+  } else {  // a matrix per unit
     g.unit = blockIdx.z;
     g.rows = plan.cnt[g.unit];
     g.row0 = plan.off[g.unit];
     g.slot = plan.slot[g.unit];
   }
   const int64_t n0 = int64_t(blockIdx.y) * 64;
-  const int64_t n_m = p.grouped ? g.rows : p.m, n_k = p.k_rows ? (p.per_unit ? g.rows : p.k) : p.k;
+  const int64_t n_m = p.grouped ? g.rows : p.m, n_k = p.k_rows ? g.rows : p.k;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, q = lane >> 2, t = lane & 3;
   const int wm = (warp & 1) * 32, wn = (warp >> 1) * 32;
   float acc[NACC][2][4][4] = {};
@@ -105,7 +105,7 @@ __global__ __launch_bounds__(kThreads) void tile_kernel(const __grid_constant__ 
     for (int64_t k0 = 0; k0 < n_k; k0 += kBK) {
       T va[16], vb[16];
       fetch(oa, pa, m0, n_m, k0, n_k, g.row0, va);
-      fetch(ob, pb, n0, p.n, k0, n_k, p.per_unit ? g.row0 : 0, vb);
+      fetch(ob, pb, n0, p.n, k0, n_k, g.row0, vb);
       __syncthreads();
       put(oa, va, sa);
       put(ob, vb, sb);
@@ -151,13 +151,7 @@ __global__ __launch_bounds__(kThreads) void tile_kernel(const __grid_constant__ 
           const int64_t n = n0 + wn + j * 8 + 2 * t + c;
           const float a0 = acc[0][i][j][2 * h + c];
           if (!in || n >= p.n) continue;
-          if (p.epi == kEpiLinear) {
-            const float z = a0 + (p.bias ? to_f(static_cast<const T*>(p.bias)[n]) : 0.f);
-            if (p.pre) static_cast<T*>(p.pre)[m * p.ldp + n] = from_f<T>(z);
-            float y = act_rt(p.act, z);
-            if (p.residual) y += to_f(static_cast<const T*>(p.residual)[m * p.ldr + n]);
-            static_cast<T*>(p.out)[m * p.ldo + n] = from_f<T>(y);
-          } else if (p.epi == kEpiStore) {
+          if (p.epi == kEpiStore) {
             static_cast<T*>(p.out)[g.unit * p.out_unit + m * p.ldo + n] = from_f<T>(a0);
           } else if (p.epi == kEpiRows32) {
             p.rows32[(g.row0 + m) * p.n + n] = a0;
@@ -202,10 +196,8 @@ int go(const Product& p, const Plan& plan, const Units& u, cudaStream_t s) {
 
 }  // namespace
 
-int launch_tile(int dtype, const Product& p, const Plan* plan, const Units* units, cudaStream_t s) {
-  const Plan pl = plan ? *plan : Plan{};
-  const Units u = units ? *units : Units{};
-  return dtype == TSB_BF16 ? go<__nv_bfloat16>(p, pl, u, s) : go<__half>(p, pl, u, s);
+int launch_tile(int dtype, const Product& p, const Plan& plan, const Units& units, cudaStream_t s) {
+  return dtype == TSB_BF16 ? go<__nv_bfloat16>(p, plan, units, s) : go<__half>(p, plan, units, s);
 }
 
 }  // namespace ops
