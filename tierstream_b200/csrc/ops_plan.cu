@@ -265,22 +265,28 @@ __global__ __launch_bounds__(256) void join_dw_kernel(const int32_t* __restrict_
   if (lane == 0) dw[i] = from_f<T>(s);
 }
 
-// A warp a row, two bytes a lane: what a matrix of odd rows costs before its product (30 MB in about 10 us).
+// A warp takes 256 columns of a row, two bytes a lane and load, eight loads in flight: rows that start anywhere are read
+// and written in whole sectors all the same.
+constexpr uint32_t kCopyCols = 256;
 __global__ __launch_bounds__(256) void copies_kernel(const __grid_constant__ Copies j) {
   begin_after();
   const uint64_t stride = uint64_t(gridDim.x) * 8;
-  uint64_t r = uint64_t(blockIdx.x) * 8 + (threadIdx.x >> 5);
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    if (i >= j.n) break;
+  uint64_t at = uint64_t(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  for (int i = 0; i < j.n; ++i) {
     const Copy& c = j.c[i];
-    for (; r < c.rows; r += stride) {
+    const uint64_t spans = (c.ldd + kCopyCols - 1) / kCopyCols, all = c.rows * spans;
+    for (; at < all; at += stride) {
+      const uint64_t r = at / spans, k0 = (at - r * spans) * kCopyCols + (threadIdx.x & 31);
       const uint16_t* s = static_cast<const uint16_t*>(c.src) + r * c.ld;
       uint16_t* d = static_cast<uint16_t*>(c.dst) + r * c.ldd;
-#pragma unroll 4
-      for (uint64_t k = threadIdx.x & 31; k < c.ldd; k += 32) d[k] = k < c.cols ? s[k] : uint16_t(0);
+      uint16_t v[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) v[u] = k0 + 32 * u < c.cols ? s[k0 + 32 * u] : uint16_t(0);
+#pragma unroll
+      for (int u = 0; u < 8; ++u)
+        if (k0 + 32 * u < c.ldd) d[k0 + 32 * u] = v[u];
     }
-    r -= c.rows;  // (the second matrix' rows follow the first's)
+    at -= all;  // (the second matrix' spans follow the first's)
   }
 }
 
@@ -559,10 +565,10 @@ int launch_join_linear(int dtype, int act, const float* rows32, uint32_t splits,
 }
 
 int launch_copies(const Copies& c, cudaStream_t s) {
-  uint64_t rows = 0;
-  for (int i = 0; i < c.n; ++i) rows += c.c[i].rows;
-  const uint64_t blocks = ceil_div(rows, 8);
-  return launch(copies_kernel, unsigned(blocks < 1184 ? blocks : 1184), 256, 0, 1, s, c);
+  uint64_t spans = 0;
+  for (int i = 0; i < c.n; ++i) spans += c.c[i].rows * ceil_div(c.c[i].ldd, kCopyCols);
+  const uint64_t blocks = ceil_div(spans, 8);
+  return launch(copies_kernel, unsigned(blocks < 2368 ? blocks : 2368), 256, 0, 1, s, c);
 }
 
 int launch_join_dw(int dtype, const Plan& p, const float* dwp, uint32_t tiles, void* dw, cudaStream_t s) {
