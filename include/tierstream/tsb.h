@@ -465,8 +465,9 @@ SS_API ss_status tsb_units_from_view(const ss_dg_device_view* v, uint32_t g, uin
 /* The gated feed-forward block of the routed units: y[t] = residual[t] + sum over k of weights[t][k] x
  * Wd_e (act(Wg_e x[t]) * (Wu_e x[t])), e = ids[t][k]; x and y [rows][hidden], ids and weights [rows][top] (device
  * memory). An id outside [0, n_units) contributes nothing (a padded row's -1, which is not to be exported); a row with
- * none gives its residual, or zeros. The same unit twice in a row counts twice. act(..) * (..) is rounded to dtype between the products; the
- * choices' sums are added in 32 bits. residual may be NULL. top is at most 64, rows x top at most 2^28, hidden and ffn at most 2^20. */
+ * none gives its residual, or zeros. The same unit twice in a row counts twice. act(..) * (..) is rounded to dtype
+ * between the products (for at most two rows a unit on average it is kept to twice those bits); the choices' sums are added
+ * in 32 bits. residual may be NULL. top is at most 64, rows x top at most 2^28, hidden and ffn at most 2^20. */
 typedef struct tsb_ffn_args {
   uint32_t struct_size, dtype, act, top;
   uint64_t rows, hidden, ffn;

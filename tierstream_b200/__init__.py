@@ -2,7 +2,8 @@
 
 The runtime itself is native: C++ for the host control plane (descriptor, planner, slot cache, service thread) and
 CUDA for sm_100a for the data path (land / write-back / compaction / peer copies, device-gated control kernels,
-device xxh64). This package only locates and describes it; see abi.py for the ctypes view and runtime.py for handles.
+device xxh64). This package only locates and describes it; see abi.py for the ctypes view, runtime.py for handles and
+ops.py for the operators an engine runs beside the streamed units.
 """
 from . import abi  # noqa: F401
 

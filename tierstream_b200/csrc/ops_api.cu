@@ -325,6 +325,7 @@ struct FfnSpace {
   bool tc, stream;
   void* xs;
   void* h;
+  int64_t ldh;
   float* rows32;
   uint64_t bytes;
 };
@@ -340,7 +341,9 @@ FfnSpace ffn_space(const tsb_ffn_args* a) {
   const uint32_t bm = r.stream ? kStreamTile : r.tc ? tc_tile(each) : kTileM;
   r.plan = plan_at(w.take(plan_bytes(a->units->n_units, pairs, 1, bm)), a->units->n_units, pairs, 1, bm);
   if (r.tc) r.xs = w.take(uint64_t(r.plan.max_rows) * a->hidden * 2);
-  r.h = w.take(uint64_t(r.plan.max_rows) * a->ffn * 2);
+  // (streamed, the middle is two 16-bit values)
+  r.ldh = int64_t(a->ffn) * (r.stream ? 2 : 1);
+  r.h = w.take(uint64_t(r.plan.max_rows) * uint64_t(r.ldh) * 2);
   r.rows32 = static_cast<float*>(w.take(uint64_t(r.plan.max_rows) * a->hidden * 4));
   r.bytes = w.used;
   return r;
@@ -375,7 +378,7 @@ void ffn(const tsb_ffn_args* a) {
   p.n = f, p.k = d;
   p.epi = kEpiUp;
   p.act = int(a->act);
-  p.out = w.h, p.ldo = f;
+  p.out = w.h, p.ldo = w.ldh;
   const auto go = [&](const Product& pr) {
     return w.stream ? launch_stream(int(a->dtype), pr, a->top, &w.plan, &u, s)
            : w.tc   ? launch_grouped(int(a->dtype), pr, &w.plan, &u, s)
@@ -389,7 +392,7 @@ void ffn(const tsb_ffn_args* a) {
   Product q{};
   q.grouped = 1;
   q.segs = 1;
-  q.a[0] = dense(w.h, f, 1);
+  q.a[0] = dense(w.h, w.ldh, 1);
   q.b[0] = of_unit(2, f, 1);
   q.n = d, q.k = f;
   q.epi = kEpiRows32;

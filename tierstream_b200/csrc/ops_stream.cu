@@ -10,6 +10,9 @@
 // result end in the same CTA. (More rows of x a tile, with more rows of w a warp to pay for them, lost to the tensor
 // cores' own path at every size tried: 143 us against 35 us for 24 rows of 8192 x 8192.)
 //
+// Between the block's two products act(g) u is kept as two 16-bit values, its rounding and what that left out, which both
+// meet the down matrix' fragments: the weights' loads stay the bound, and the middle is as good as 32 bits.
+//
 // A CTA of four warps owns 16 rows of w (8 of gate and up) and splits k over its warps, a cluster of up to 8 CTAs splits
 // it further when there are few rows of w; the sums are added in a fixed order through (distributed) shared memory.
 #include "ops.hpp"
@@ -135,10 +138,14 @@ __global__ __launch_bounds__(kThreads) void stream_kernel(const __grid_constant_
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
       const int64_t k = k0 + u * kStep, left = p.k - k - 16 * t;
-      const Words x = load_x<WIDE>(xr + k, inx ? left : 0);
 #pragma unroll
-      for (int h = 0; h < 4; ++h)
-        mma16816<T>(acc, a[u].w[2 * h], b[u].w[2 * h], a[u].w[2 * h + 1], b[u].w[2 * h + 1], x.w[2 * h], x.w[2 * h + 1]);
+      for (int part = 0; part < (MODE == kDown ? 2 : 1); ++part) {
+        const Words x = load_x<WIDE>(xr + k + part * p.k, inx ? left : 0);
+#pragma unroll
+        for (int h = 0; h < 4; ++h)
+          mma16816<T>(acc, a[u].w[2 * h], b[u].w[2 * h], a[u].w[2 * h + 1], b[u].w[2 * h + 1], x.w[2 * h],
+                      x.w[2 * h + 1]);
+      }
     }
   }
 #pragma unroll
@@ -170,7 +177,12 @@ __global__ __launch_bounds__(kThreads) void stream_kernel(const __grid_constant_
     if (r >= rows || n >= p.n) continue;
     const float z0 = sum[c][r];
     if constexpr (MODE == kUp) {
-      static_cast<T*>(p.out)[(int64_t(row0) + r) * p.ldo + n] = from_f<T>(act_rt(p.act, z0) * sum[c + kHalf][r]);
+      T* out = static_cast<T*>(p.out) + (int64_t(row0) + r) * p.ldo + n;
+      const float h = act_rt(p.act, z0) * sum[c + kHalf][r];
+      const T hi = from_f<T>(h);
+      const float lo = h - to_f(hi);
+      out[0] = hi;
+      out[p.n] = from_f<T>(lo - lo == 0.f ? lo : 0.f);  // (nothing is left out of an infinity or a NaN)
     } else if constexpr (MODE == kDown) {
       p.rows32[(int64_t(row0) + r) * p.n + n] = z0;
     } else {

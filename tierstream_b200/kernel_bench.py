@@ -1,10 +1,12 @@
 """Per-kernel rates through the C ABI, each timed with CUDA events on the launching stream after warm-up, with inputs
 larger than L2: the land kernel (K1: one tsb_land launch per repetition) for pinned host -> HBM, HBM -> pinned host
 and HBM -> HBM, the move kernel (K4: one tsb_move launch, HBM -> HBM, `--kernel move`), and the device xxh64 (K3: tsb_xxh64_units) for one unit alone (its serial chain) and for many
-units at once (aggregate). Also the small cases the committed ncu summaries were captured on.
+units at once (aggregate). Also the small cases the committed ncu summaries were captured on. The operators of ops.py
+(linear, route, ffn; --back: their backward passes) are timed the same way, one call a repetition.
 
     python -m tierstream_b200.kernel_bench land --dir h2d --part-bytes 33030144 --parts 15
     python -m tierstream_b200.kernel_bench xxh64 --units 296 --part-bytes 12582912
+    python -m tierstream_b200.kernel_bench ffn --rows 24 --hidden 4096 --ffn 1536 --units 128 --top 8
 """
 import argparse
 import ctypes as C
