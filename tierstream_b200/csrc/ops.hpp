@@ -204,9 +204,9 @@ struct Product {
 uint64_t plan_bytes(uint32_t units, uint64_t pairs, uint32_t pad, uint32_t bm);
 Plan plan_at(void* ws, uint32_t units, uint64_t pairs, uint32_t pad, uint32_t bm);
 int launch_plan(const Plan& p, const Units& u, const int32_t* ids, cudaStream_t s);
-// y[t] = residual[t] + sum over k, then over the splits, of w[t][k] x rows32[split][row_of_pair[t top + k]]
-int launch_join(int dtype, const Plan& p, const float* rows32, uint32_t splits, const float* weights, uint32_t top,
-                uint64_t rows, uint64_t n, const void* residual, uint64_t ldr, void* y, uint64_t ldy, cudaStream_t s);
+// y[t] = residual[t] + sum over k of w[t][k] x rows32[row_of_pair[t top + k]]
+int launch_join(int dtype, const Plan& p, const float* rows32, const float* weights, uint32_t top, uint64_t rows,
+                uint64_t n, const void* residual, uint64_t ldr, void* y, uint64_t ldy, cudaStream_t s);
 // y = act(sum over the splits of rows32 + bias) + residual, pre the sum itself
 int launch_join_linear(int dtype, int act, const float* rows32, uint32_t splits, uint64_t rows, uint64_t n,
                        const void* bias, const void* residual, uint64_t ldr, void* y, uint64_t ldy, void* pre,

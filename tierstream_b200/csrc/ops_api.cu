@@ -398,7 +398,7 @@ void ffn(const tsb_ffn_args* a) {
   q.epi = kEpiRows32;
   q.rows32 = w.rows32;
   ck(go(q), fn, "down");
-  ck(launch_join(int(a->dtype), w.plan, w.rows32, 1, a->weights, a->top, a->rows, a->hidden, a->residual, a->ldr, a->y,
+  ck(launch_join(int(a->dtype), w.plan, w.rows32, a->weights, a->top, a->rows, a->hidden, a->residual, a->ldr, a->y,
                  a->ldy, s),
      fn, "join");
 }
@@ -507,7 +507,7 @@ void ffn_back(const tsb_ffn_grad_args* a) {
     p.epi = kEpiRows32;
     p.rows32 = w.rows32;
     ck(go(p), fn, "dx");
-    ck(launch_join(dt, w.plan, w.rows32, 1, nullptr, a->top, a->rows, a->hidden, nullptr, 0, a->dx, a->lddx, s), fn,
+    ck(launch_join(dt, w.plan, w.rows32, nullptr, a->top, a->rows, a->hidden, nullptr, 0, a->dx, a->lddx, s), fn,
        "join");
   }
   if (a->dgate) {

@@ -189,12 +189,11 @@ __global__ __launch_bounds__(kSmallThreads) void plan_small_kernel(const __grid_
 }
 
 // ---------------------------------------------------------------------------------------------------------------
-// Joins: a row's contributions from its choices (and from the splits of a long sum), added in order in 32 bits and
+// Joins: a row's contributions from its choices, added in order in 32 bits and
 // rounded once with the residual. V columns a thread; bound by the 32-bit rows' bytes.
 // ---------------------------------------------------------------------------------------------------------------
 template <class T, int V>
 __global__ __launch_bounds__(256) void join_kernel(const int32_t* __restrict__ row_of_pair, const float* __restrict__ src,
-                                                   uint32_t splits, uint64_t split_stride,
                                                    const float* __restrict__ weights, uint32_t top, uint64_t n,
                                                    const T* residual, uint64_t ldr, T* y, uint64_t ldy) {
   begin_after();
@@ -203,22 +202,33 @@ __global__ __launch_bounds__(256) void join_kernel(const int32_t* __restrict__ r
   float sum[V];
 #pragma unroll
   for (int v = 0; v < V; ++v) sum[v] = residual ? to_f(residual[t * ldr + c + v]) : 0.f;
-  for (uint32_t k = 0; k < top; ++k) {
-    const int32_t row = row_of_pair[t * top + k];
-    if (row < 0) continue;
-    const float w = weights ? weights[t * top + k] : 1.f;
-    float part[V] = {};
-    for (uint32_t s = 0; s < splits; ++s) {
-      const float* p = src + s * split_stride + uint64_t(row) * n + c;
-      if constexpr (V == 4) {
-        const float4 f = *reinterpret_cast<const float4*>(p);
-        part[0] += f.x, part[1] += f.y, part[2] += f.z, part[3] += f.w;
+  constexpr uint32_t kAt = 4;  // choices whose loads are in flight together
+  for (uint32_t k0 = 0; k0 < top; k0 += kAt) {
+    int32_t row[kAt];
+    float w[kAt], part[kAt][V];
+#pragma unroll
+    for (uint32_t j = 0; j < kAt; ++j) {
+      row[j] = k0 + j < top ? row_of_pair[t * top + k0 + j] : -1;
+      w[j] = weights && row[j] >= 0 ? weights[t * top + k0 + j] : 1.f;
+    }
+#pragma unroll
+    for (uint32_t j = 0; j < kAt; ++j) {
+      const float* p = src + uint64_t(row[j] < 0 ? 0 : row[j]) * n + c;
+      if (row[j] < 0) {
+#pragma unroll
+        for (int v = 0; v < V; ++v) part[j][v] = 0.f;
+      } else if constexpr (V == 4) {
+        const float4 f = __ldcs(reinterpret_cast<const float4*>(p));
+        part[j][0] = f.x, part[j][1] = f.y, part[j][2] = f.z, part[j][3] = f.w;
       } else {
-        part[0] += *p;
+        part[j][0] = *p;
       }
     }
 #pragma unroll
-    for (int v = 0; v < V; ++v) sum[v] += w * part[v];
+    for (uint32_t j = 0; j < kAt; ++j)
+      if (row[j] >= 0)
+#pragma unroll
+        for (int v = 0; v < V; ++v) sum[v] += w[j] * part[j][v];
   }
 #pragma unroll
   for (int v = 0; v < V; ++v) y[t * ldy + c + v] = from_f<T>(sum[v]);
@@ -535,16 +545,15 @@ int launch_plan(const Plan& p, const Units& u, const int32_t* ids, cudaStream_t 
   return launch(plan_fill_kernel, p.units, kPlanThreads, 0, 1, s, p, ids);
 }
 
-int launch_join(int dtype, const Plan& p, const float* rows32, uint32_t splits, const float* weights, uint32_t top,
-                uint64_t rows, uint64_t n, const void* residual, uint64_t ldr, void* y, uint64_t ldy, cudaStream_t s) {
+int launch_join(int dtype, const Plan& p, const float* rows32, const float* weights, uint32_t top, uint64_t rows,
+                uint64_t n, const void* residual, uint64_t ldr, void* y, uint64_t ldy, cudaStream_t s) {
   int e = 0;
   by_type(dtype, [&](auto v) {
     using T = decltype(v);
-    const uint64_t stride = uint64_t(p.max_rows) * n;
     const T* r = static_cast<const T*>(residual);
     const unsigned v4 = n % 4 == 0 ? 4 : 1;
     e = launch(v4 == 4 ? join_kernel<T, 4> : join_kernel<T, 1>, dim3(unsigned(rows), unsigned(ceil_div(n, 256 * v4))), 256, 0,
-               1, s, p.row_of_pair, rows32, splits, stride, weights, top, n, r, ldr, static_cast<T*>(y), ldy);
+               1, s, p.row_of_pair, rows32, weights, top, n, r, ldr, static_cast<T*>(y), ldy);
   });
   return e;
 }
