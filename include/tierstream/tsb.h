@@ -359,9 +359,9 @@ SS_API ss_status tsb_dg_peer_retier(ss_ctx* c, const tsb_peer_tier* peer);
  * logits, a streamed dense layer), each with its backward pass. All matrices are row-major, ld* in elements between
  * rows. Every call enqueues kernels on `stream` of the current device and returns; it allocates nothing, waits for
  * nothing, and may be captured into a graph. Scratch comes from the caller: *_workspace gives its bytes (0: none is
- * needed; on a refused argument 0 too, and the call itself names the refusal; ask with the call's own arguments), a 256-byte aligned device area that
- * belongs to the call until the stream has passed it (two calls that may run at the same time, or two graphs, need one
- * each). No result depends on the order in which anything ran: the same inputs give the same bits. Outputs must not
+ * needed; on a refused argument 0 too, and the call itself names the refusal; ask with the call's own arguments), a
+ * 256-byte aligned device area that belongs to the call until the stream has passed it (two calls that may run at the
+ * same time, or two graphs, need one each). Every pointer is on a whole element. No result depends on the order in which anything ran: the same inputs give the same bits. Outputs must not
  * overlap inputs, except that y may be the residual (of the feed-forward block even when that is x). On a device-gated
  * context, capture the calls, or make a first call of each before a token runs: a kernel's first call loads it, which a
  * token's waiting kernel holds up. Sums are held in 32 bits; what is 16 bits wide between two
@@ -377,8 +377,8 @@ SS_API ss_status tsb_dg_peer_retier(ss_ctx* c, const tsb_peer_tier* peer);
 
 /* z = x w^T + bias, y = act(z) + residual: x [rows][k], w [n][k], bias [n], residual and y [rows][n], all of `dtype`
  * (TSB_BF16 or TSB_F16). pre: z, rounded to dtype, for the backward pass. bias, residual and pre may be NULL.
- * rows = 0 does nothing; rows is below 2^28, n and k in [1, 2^20]. Rows that start on 16 bytes (x and w, so k and the lds multiples of 8)
- * take the fast kernels; every other alignment is served too. */
+ * rows = 0 does nothing; rows is below 2^28, n and k in [1, 2^20]. Rows of x and w that start on 16 bytes (the lds
+ * multiples of 8) are read in place; others cost a copy first where there are many rows. */
 typedef struct tsb_linear_args {
   uint32_t struct_size, dtype, act, reserved0;
   uint64_t rows, n, k;
@@ -445,8 +445,8 @@ SS_API ss_status tsb_route_backward(uint32_t dtype, uint32_t dw_dtype, const voi
  * part[p] + slot x stride[p] bytes, slot = slot_of[*unit_base + u] (device memory, read when the kernels run; slot_of
  * NULL: slot = u; unit_base NULL: 0), or, with `table` (device array of n_units addresses, a host-mode
  * ss_layer_view.table_dev), at table[u] + stride[p] bytes. A slot outside [0, n_slots), a zero address or one that is
- * not a multiple of 16 is a unit that is not there: its rows contribute nothing and *absent_err (may be NULL) is set to 1; while *abort (may be NULL) is
- * non-zero no unit is there. */
+ * not a multiple of 16 is a unit that is not there: its rows contribute nothing and *absent_err (may be NULL) is set to
+ * 1; while *abort (may be NULL) is non-zero no unit is there. */
 typedef struct tsb_units {
   uint32_t struct_size, n_units, n_slots, reserved0;
   const int32_t* slot_of;

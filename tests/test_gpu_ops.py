@@ -496,6 +496,33 @@ def test_ffn_gradient_by_differences():
             assert abs(float(g.sum()) - want) <= 16 * half(t) * float(g.norm()) + 1e-6 * abs(want), n
 
 
+@pytest.mark.parametrize("rows", [2, 40, 1100])
+def test_ffn_units_far_apart(rows):
+    """Slots more than 2^32 bytes apart, in one allocation: forward and backward find the unit in the last one."""
+    t, hidden, ffn = torch.bfloat16, 128, 72
+    g = gen(17)
+    size = hidden * ffn
+    apart = (1 << 31) + 256  # elements between slots: 4 GiB and 512 bytes
+    buf = torch.empty(apart * 2 + 3 * size, dtype=t, device="cuda")
+    gate, up = (torch.as_strided(buf, (3, ffn, hidden), (apart, hidden, 1), o) for o in (0, size))
+    down = torch.as_strided(buf, (3, hidden, ffn), (apart, ffn, 1), 2 * size)
+    for m, k in ((gate, hidden), (up, hidden), (down, ffn)):
+        m.copy_(rand(g, *m.shape, dtype=t, scale=k ** -0.5))
+    slot_of = torch.tensor([2, 0], dtype=torch.int32, device="cuda")
+    x, dy = rand(g, rows, hidden, dtype=t), rand(g, rows, hidden, dtype=t)
+    ids = torch.zeros((rows, 1), dtype=torch.int32, device="cuda")
+    ids[0] = 1
+    w = torch.rand((rows, 1), generator=g, device="cuda")
+    parts = (gate, up, down, slot_of)
+    un = ops.Units(*parts)
+    want, tol = plain_ffn(x, ids, w, parts, "silu")
+    close(ops.ffn(x, ids, w, un), want, tol)
+    got = ops.ffn_backward(dy, x, ids, w, un)
+    want, tol = plain_back(dy, x, ids, w, parts, "silu")
+    for n in want:
+        close(got[n], want[n], tol[n], n)
+
+
 # ---- streams, graphs, and the operators together ----
 def test_on_another_stream_and_captured():
     """A layer (logits, route, block with its residual) on a side stream, captured into two graphs that are replayed with

@@ -143,6 +143,20 @@ def test_route_refusals(lib, args, text):
     assert text.encode() in lib.ss_last_error()
 
 
+def test_pointers_on_whole_elements(lib):
+    refused(lib, "tsb_linear", linear(x=P + 1), "whole element")
+    refused(lib, "tsb_linear", linear(bias=P + 1), "whole element")
+    refused(lib, "tsb_linear_backward", linear_back(dy=P + 1), "whole element")
+    refused(lib, "tsb_ffn", ffn(x=P + 1), "whole element")
+    refused(lib, "tsb_ffn", ffn(ids=P + 2), "whole element")
+    refused(lib, "tsb_ffn_backward", ffn_back(dweights=P + 1), "whole element")
+    for kw in (dict(slot_of=P + 2), dict(table=P + 4), dict(absent_err=P + 1)):
+        refused(lib, "tsb_ffn", ffn(units(**kw)), "whole element")
+    assert lib.tsb_route(abi.TSB_F32, P + 2, 8, 1, 8, 2, 1, P, P, None) == abi.SS_E_INVALID
+    assert lib.tsb_route(abi.TSB_BF16, P, 8, 1, 8, 2, 1, P + 2, P, None) == abi.SS_E_INVALID
+    assert lib.tsb_route_backward(0, 2, P + 2, P, 8, P, P, 1, 8, 2, 1, P, 8, None) == abi.SS_E_INVALID
+
+
 def test_no_rows_is_no_work(lib):
     """rows = 0 needs no workspace, no pointers and no device."""
     a = linear(rows=0, x=None, w=None, y=None)

@@ -3,6 +3,7 @@
 #include <algorithm>
 #include <cmath>
 #include <cstring>
+#include <initializer_list>
 #include <string>
 
 #include "errors.hpp"
@@ -31,6 +32,12 @@ ss_status run(F&& f) {
 }
 void need(bool ok, const char* fn, const char* what) {
   if (!ok) tsb::fail(SS_E_INVALID, std::string(fn) + ": " + what);
+}
+// pointers on whole elements of `size` bytes (NULL is)
+void need_elements(const char* fn, std::initializer_list<const void*> pointers, uintptr_t size) {
+  uintptr_t all = 0;
+  for (const void* p : pointers) all |= reinterpret_cast<uintptr_t>(p);
+  need((all & (size - 1)) == 0, fn, "a pointer is not on a whole element");
 }
 void ck(int e, const char* fn, const char* what) {
   if (e == 0) return;
@@ -86,7 +93,8 @@ How how(const Product& p) {
   // the matrix as columns, in the columns a tile that launch_tc would take
   const int cg = p.m > 128 ? 2 : 1;
   const int bn = tc_columns(p.m, p.n, kSms);
-  const double waves = double(ceil_div(ceil_div(uint64_t(p.m), 128 * cg) * ceil_div(uint64_t(p.n), uint64_t(bn)), uint64_t(kSms / cg)));
+  const uint64_t tc_tiles = ceil_div(uint64_t(p.m), 128 * cg) * ceil_div(uint64_t(p.n), uint64_t(bn));
+  const double waves = double(ceil_div(tc_tiles, uint64_t(kSms / cg)));
   const double tc = 6 + std::max(bytes, waves * kb * (cg == 2 ? slice_us(bn) : 0.17 + 0.00098 * bn));
   // the matrix as rows, k split
   const uint64_t tiles = ceil_div(uint64_t(p.m), 2 * kGroupRows);
@@ -123,7 +131,7 @@ int product(int dtype, const Product& p, float* rows32, cudaStream_t s) {
 // An operand, [rows][cols] in memory, whose rows do not start on 16 bytes (or, `whole`, do not hold whole eights) is copied
 // into the workspace first: the fast kernels read it from there.
 void align(Operand& o, uint64_t rows, uint64_t cols, bool whole, Arena& w, Copies& copies) {
-  if (tc_fits(o, nullptr) && !(whole && cols % 8)) return;
+  if (tc_fits(o) && !(whole && cols % 8)) return;
   const uint64_t ld = o.s_k == 1 ? uint64_t(o.s_i) : uint64_t(o.s_k), ldd = (cols + 7) / 8 * 8;
   const bool k_inner = !o.map_k && o.s_k == 1;
   void* dst = w.take(rows * ldd * 2);
@@ -142,6 +150,7 @@ void check_linear(const tsb_linear_args* a) {
   need(a->rows < kMaxRows, fn, "rows must be below 2^28");
   if (!a->rows) return;
   need(a->x && a->w && a->y, fn, "null argument");
+  need_elements(fn, {a->x, a->w, a->bias, a->residual, a->y, a->pre}, 2);
   need(a->ldx >= a->k && a->ldw >= a->k && a->ldy >= a->n && (!a->residual || a->ldr >= a->n) &&
            (!a->pre || a->ldp >= a->n),
        fn, "a leading dimension is shorter than its row");
@@ -195,6 +204,7 @@ void check_linear_back(const tsb_linear_grad_args* a) {
   need(a->n >= 1 && a->k >= 1 && a->n <= kMaxDim && a->k <= kMaxDim, fn, "n and k must be in [1, 2^20]");
   need(a->rows < kMaxRows, fn, "rows must be below 2^28");
   need(!a->dw || a->lddw >= a->k, fn, "a leading dimension is shorter than its row");
+  need_elements(fn, {a->dy, a->x, a->w, a->act == TSB_ACT_NONE ? nullptr : a->pre, a->dx, a->dw, a->db}, 2);
   if (!a->rows) return;
   need(a->dy && (!a->dx || a->w) && (!a->dw || a->x), fn, "null argument");
   need(a->act == TSB_ACT_NONE || a->pre, fn, "an activation's slope needs pre");
@@ -218,7 +228,7 @@ LinearBackSpace linear_back_space(const tsb_linear_grad_args* a) {
   const void* dz = a->dy;
   r.ldz = a->lddy;
   // dz: the slope times dy, or a copy of dy whose rows start on 16 bytes
-  if (a->act != TSB_ACT_NONE || ((a->dx || a->dw) && !tc_fits(dense(a->dy, int64_t(a->lddy), 1), nullptr))) {
+  if (a->act != TSB_ACT_NONE || ((a->dx || a->dw) && !tc_fits(dense(a->dy, int64_t(a->lddy), 1)))) {
     r.ldz = (a->n + 7) / 8 * 8;
     dz = r.dz = w.take(a->rows * r.ldz * 2);
   }
@@ -298,6 +308,9 @@ void check_ffn_shape(const A* a, const char* fn) {
   need(u && u->struct_size >= sizeof *u, fn, "null or short units struct");
   need(u->n_units >= 1 && u->n_units <= 65535, fn, "n_units must be in [1, 65535]");
   need(u->table || (u->part[0] && u->part[1] && u->part[2] && u->n_slots >= 1), fn, "no parts and no table");
+  if (!u->table) need_elements(fn, {u->part[0], u->part[1], u->part[2]}, 2);
+  need_elements(fn, {u->slot_of, u->unit_base, u->abort, u->absent_err, a->ids, a->weights}, 4);
+  need_elements(fn, {u->table}, 8);
   need(u->stride[0] % 2 == 0 && u->stride[1] % 2 == 0 && u->stride[2] % 2 == 0, fn,
        "the parts' strides must be whole elements");
 }
@@ -354,6 +367,7 @@ void check_ffn(const tsb_ffn_args* a) {
   check_ffn_shape(a, fn);
   if (!a->rows) return;
   need(a->x && a->ids && a->weights && a->y, fn, "null argument");
+  need_elements(fn, {a->x, a->residual, a->y}, 2);
   need(a->ldx >= a->hidden && a->ldy >= a->hidden && (!a->residual || a->ldr >= a->hidden), fn,
        "a leading dimension is shorter than its row");
 }
@@ -427,7 +441,9 @@ FfnBackSpace ffn_back_space(const tsb_ffn_grad_args* a) {
   r.dg = w.take(uint64_t(r.plan.max_rows) * a->ffn * 2);
   r.du = w.take(uint64_t(r.plan.max_rows) * a->ffn * 2);
   if (a->dgate) r.hw = w.take(uint64_t(r.plan.max_rows) * a->ffn * 2);
-  r.dw_tiles = r.tc ? (bm == kGroupRows ? 8 * uint32_t(ceil_div(a->ffn, 256)) : 2 * uint32_t(ceil_div(a->ffn, 128))) : uint32_t(ceil_div(a->ffn, kTileN));
+  r.dw_tiles = !r.tc               ? uint32_t(ceil_div(a->ffn, kTileN))
+               : bm == kGroupRows ? 8 * uint32_t(ceil_div(a->ffn, 256))
+                                  : 2 * uint32_t(ceil_div(a->ffn, 128));
   if (a->dweights) r.dwp = static_cast<float*>(w.take(uint64_t(r.plan.max_rows) * r.dw_tiles * 4));
   if (a->dx) r.rows32 = static_cast<float*>(w.take(uint64_t(r.plan.max_rows) * a->hidden * 4));
   r.bytes = w.used;
@@ -441,6 +457,7 @@ void check_ffn_back(const tsb_ffn_grad_args* a) {
        "dgate, dup and ddown go together");
   if (!a->rows) return;
   need(a->dy && a->x && a->ids && a->weights, fn, "null argument");
+  need_elements(fn, {a->dy, a->x, a->dx, a->dweights, a->dgate, a->dup, a->ddown}, 2);
   need(a->ldx >= a->hidden && a->lddy >= a->hidden && (!a->dx || a->lddx >= a->hidden), fn,
        "a leading dimension is shorter than its row");
 }
@@ -570,6 +587,8 @@ ss_status tsb_route(uint32_t dtype, const void* logits, uint64_t ld, uint64_t ro
     need(rows < kMaxRows, fn, "rows must be below 2^28");
     if (!rows) return;
     need(logits && ids && weights, fn, "null argument");
+    need_elements(fn, {logits}, dtype == TSB_F32 ? 4 : 2);
+    need_elements(fn, {ids, weights}, 4);
     need(ld >= experts, fn, "a leading dimension is shorter than its row");
     ck(launch_route(int(dtype), logits, ld, rows, experts, top, norm, ids, weights, static_cast<cudaStream_t>(stream)),
        fn, "launch");
@@ -586,6 +605,9 @@ ss_status tsb_route_backward(uint32_t dtype, uint32_t dw_dtype, const void* dwei
     need(rows < kMaxRows, fn, "rows must be below 2^28");
     if (!rows) return;
     need(dweights && (norm || logits) && ids && weights && dlogits, fn, "null argument");
+    need_elements(fn, {norm ? nullptr : logits, dlogits}, dtype == TSB_F32 ? 4 : 2);
+    need_elements(fn, {dweights}, dw_dtype == TSB_F32 ? 4 : 2);
+    need_elements(fn, {ids, weights}, 4);
     need((norm || ld >= experts) && ldd >= experts, fn, "a leading dimension is shorter than its row");
     ck(launch_route_back(int(dtype), int(dw_dtype), dweights, logits, ld, ids, weights, rows, experts, top, norm,
                          dlogits, ldd, static_cast<cudaStream_t>(stream)),

@@ -301,8 +301,8 @@ __global__ __launch_bounds__(256) void copies_kernel(const __grid_constant__ Cop
 }
 
 // ---------------------------------------------------------------------------------------------------------------
-// dz = dy act'(pre) (or a copy of dy without an activation), rounded once to the operands' type (the products take 16-bit operands), and db from the unrounded
-// values: each CTA sums kDzRows rows of 32 V columns, then one thread per column adds the CTAs' sums in order.
+// dz = dy act'(pre) (or a copy of dy without an activation), rounded once to the operands' type (the products take
+// 16-bit operands), and db from the unrounded values: each CTA sums kDzRows rows of 32 V columns, then one thread per column adds the CTAs' sums in order.
 // ---------------------------------------------------------------------------------------------------------------
 constexpr uint32_t kDzRows = 64;
 
