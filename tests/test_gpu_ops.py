@@ -184,6 +184,41 @@ def test_linear_backward_without_rows():
     assert dx.shape == (0, 8) and not dw.any() and not db.any() and dw.shape == (5, 8)
 
 
+@pytest.mark.parametrize("act", ACTS)
+def test_slopes_far_out(act):
+    """Values whose squares pass 32 bits, where the slopes end at 0 or 1: linear's backward pass and ffn's. (At 50 the
+    exponential is off by 60 ulp at most, 2^-17 of it.)"""
+    t = torch.bfloat16
+    far = torch.tensor([50.0, 1e4, 1e13, 1e19, 1e25, 3e38], device="cuda")
+    z = torch.cat([far, -far, torch.zeros(2, device="cuda")]).to(t)[None]
+    dy = torch.ones_like(z)
+    x, w = torch.ones((1, 8), dtype=t, device="cuda"), torch.zeros((z.shape[1], 8), dtype=t, device="cuda")
+    db = ops.linear_backward(dy, x, w, act=act, pre=z)[2]
+    want = slope(z[0].double(), act)[1]
+    close(db, want, (half(t) + 2.0 ** -16) * want.abs())
+    hidden, ffn, rows = 64, 40, 3
+    g = gen(23)
+    x = torch.full((rows, hidden), 1e10, dtype=t, device="cuda")
+    gate = torch.full((1, ffn, hidden), 1e10, dtype=t, device="cuda")
+    gate[:, ::2] *= -1
+    up = torch.full((1, ffn, hidden), 1e-12, dtype=t, device="cuda")
+    down, dy = rand(g, 1, hidden, ffn, dtype=t), rand(g, rows, hidden, dtype=t)
+    ids, weights = torch.zeros((rows, 1), dtype=torch.int32, device="cuda"), torch.ones((rows, 1), device="cuda")
+    for d in (64, 60):  # (60: the path for rows off 16 bytes)
+        parts = gate[:, :, :d].contiguous(), up[:, :, :d].contiguous(), down[:, :d].contiguous()
+        got = ops.ffn_backward(dy[:, :d], x[:, :d], ids, weights, ops.Units(*parts), act=act, need=("x",))["dx"]
+        # g is +-6e21 or so: with slope s, dx = (dh u s) gate + (dh act(g)) up, both of moderate size next to 1e10
+        dh = dy[:, :d].double() @ parts[2][0].double()
+        gz, u = x[:, :d].double() @ parts[0][0].double().T, x[:, :d].double() @ parts[1][0].double().T
+        f, s = slope(gz, act)
+        terms = (dh * u * s, parts[0][0].double()), (dh * f, parts[1][0].double())
+        want = sum(a @ b for a, b in terms)
+        mag = sum(a.abs() @ b.abs() for a, b in terms)
+        dmag = dy[:, :d].double().abs() @ parts[2][0].double().abs()
+        dmag = sum((dmag * c.abs()) @ b.abs() for c, b in ((u * s, terms[0][1]), (f, terms[1][1])))
+        close(got, want, half(t) * (want.abs() + mag) + 3 * fp32(d + ffn) * (mag + dmag), act)
+
+
 def test_linear_gradient_by_differences():
     """The gradients of sum(dy * y) against central differences of the 64-bit form, along random directions."""
     g = gen(21)

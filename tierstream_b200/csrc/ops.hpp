@@ -112,7 +112,8 @@ __device__ __forceinline__ float slope_of(float z) {
   }
   if constexpr (ACT == TSB_ACT_GELU_TANH) {
     const float p = logistic(z * (kGelu1 + kGelu3 * z * z));
-    return p + z * p * (1.f - p) * (kGelu1 + 3.f * kGelu3 * z * z);
+    const float r = p * (1.f - p);  // (0 far out, where the factors beside it pass 32 bits)
+    return r > 0.f ? p + z * r * (kGelu1 + 3.f * kGelu3 * z * z) : p;
   }
   if constexpr (ACT == TSB_ACT_RELU) return z > 0.f ? 1.f : 0.f;
   return 1.f;
