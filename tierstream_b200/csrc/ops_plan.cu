@@ -302,7 +302,8 @@ __global__ __launch_bounds__(256) void copies_kernel(const __grid_constant__ Cop
 
 // ---------------------------------------------------------------------------------------------------------------
 // dz = dy act'(pre) (or a copy of dy without an activation), rounded once to the operands' type (the products take
-// 16-bit operands), and db from the unrounded values: each CTA sums kDzRows rows of 32 V columns, then one thread per column adds the CTAs' sums in order.
+// 16-bit operands), and db from the unrounded values: each CTA sums kDzRows rows of 32 V columns, then 32 threads per
+// column add the CTAs' sums, every 32nd in order, and their sums in order.
 // ---------------------------------------------------------------------------------------------------------------
 constexpr uint32_t kDzRows = 64;
 
@@ -350,12 +351,18 @@ __global__ __launch_bounds__(256) void dz_kernel(int act, const T* __restrict__ 
 }
 
 template <class T>
-__global__ void db_kernel(const float* __restrict__ part, uint32_t chunks, uint64_t n, T* __restrict__ db) {
+__global__ __launch_bounds__(1024) void db_kernel(const float* __restrict__ part, uint32_t chunks, uint64_t n,
+                                                  T* __restrict__ db) {
   begin_after();
-  const uint64_t c = uint64_t(blockIdx.x) * blockDim.x + threadIdx.x;
-  if (c >= n) return;
+  __shared__ float red[32][33];
+  const uint64_t c = uint64_t(blockIdx.x) * 32 + threadIdx.x;
   float s = 0.f;
-  for (uint32_t j = 0; j < chunks; ++j) s += part[j * n + c];
+  if (c < n)
+    for (uint32_t j = threadIdx.y; j < chunks; j += 32) s += part[j * n + c];
+  red[threadIdx.y][threadIdx.x] = s;
+  __syncthreads();
+  if (threadIdx.y || c >= n) return;
+  for (int w = 1; w < 32; ++w) s += red[w][threadIdx.x];
   db[c] = from_f<T>(s);
 }
 
@@ -606,7 +613,7 @@ int launch_dz(int dtype, int act, const void* dy, uint64_t ldy, const void* pre,
     e = launch(wide ? dz_kernel<T, 8> : dz_kernel<T, 1>, dim3(chunks, unsigned(ceil_div(n, 32 * each))), dim3(32, 8), 0, 1,
                s, act, a, ldy, b, ldp, z, ldz, rows, n, sums);
     if (!e && db)
-      e = launch(db_kernel<T>, unsigned(ceil_div(n, 128)), 128, 0, 1, s, part, chunks, n, static_cast<T*>(db));
+      e = launch(db_kernel<T>, unsigned(ceil_div(n, 32)), dim3(32, 32), 0, 1, s, part, chunks, n, static_cast<T*>(db));
   });
   return e;
 }
