@@ -178,6 +178,14 @@ def test_linear_backward(rows, n, k, dtype):
     assert a is None and c is None and torch.equal(b, dw)
 
 
+@pytest.mark.parametrize("rows,n,k", [(2049, 300, 136), (2500, 64, 64), (5000, 200, 136), (3001, 40, 1003),
+                                      (4100, 129, 261), (33000, 8, 8), (6007, 1, 3), (2113, 128, 1024)])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_linear_backward_in_parts(rows, n, k, dtype):
+    """A small matrix and many rows: dw's sum over the rows runs in parts."""
+    test_linear_backward(rows, n, k, dtype)
+
+
 def test_linear_backward_without_rows():
     w = torch.ones((5, 8), dtype=torch.float16, device="cuda")
     dx, dw, db = ops.linear_backward(w[:0, :5], w[:0], w)

@@ -80,15 +80,38 @@ constexpr uint64_t kStreamRows = kStreamTile, kStreamEach = 2;
 // columns for a single one, about 6 for a launch's start and end, 3 for the join's, which reads 32-bit rows at 6 TB/s.
 struct How {
   enum Kind { kStream, kTc, kGroup } kind;
-  int splits;
+  int splits, columns;
 };
 constexpr int kSms = 148;
 double slice_us(double columns) { return columns < 84 ? 0.2 : 0.10 + 0.0012 * columns; }
 
+// The gradient of a matrix, a sum over rows: with few tiles the rows are split so that the parts fill the GPU's CTAs
+// once to four times (200 x 1024 over 32768 rows: 142 us whole, 26 in parts).
+How how_rows(const Product& p) {
+  const int cg = p.m > 128 ? 2 : 1;
+  const uint64_t kb = ceil_div(uint64_t(p.k), 64), m_tiles = ceil_div(uint64_t(p.m), uint64_t(128 * cg));
+  const auto us = [&](int bn, uint64_t s) {
+    const uint64_t waves = ceil_div(m_tiles * ceil_div(uint64_t(p.n), uint64_t(bn)) * s, uint64_t(kSms / cg));
+    return double(waves * ceil_div(kb, s)) * (cg == 2 ? slice_us(bn) : 0.17 + 0.00098 * bn);
+  };
+  How best{How::kTc, 1, tc_columns(p.m, p.n, kSms)};
+  double least = us(best.columns, 1);
+  for (int bn = 64; bn <= 256; bn += 64) {
+    const uint64_t tiles = m_tiles * ceil_div(uint64_t(p.n), uint64_t(bn));
+    for (uint64_t w = 1; w <= 4; ++w) {
+      const uint64_t s = std::min<uint64_t>(w * uint64_t(kSms / cg) / tiles, 32);
+      if (s < 2 || s * 4 > kb) continue;
+      const double t = us(bn, s) + 3 + double(s) * double(p.m) * double(p.n) * 8 / 6e6;
+      if (t < least) least = t, best = {How::kTc, int(s), bn};
+    }
+  }
+  return best;
+}
+
 How how(const Product& p) {
   const bool forward = p.epi == kEpiLinear;
-  if (forward && uint64_t(p.m) <= kStreamRows) return {How::kStream, 1};
-  if (p.a[0].s_k != 1) return {How::kTc, 1};  // (dw: a sum over rows)
+  if (forward && uint64_t(p.m) <= kStreamRows) return {How::kStream, 1, 0};
+  if (p.a[0].s_k != 1) return how_rows(p);
   const double kb = double(ceil_div(uint64_t(p.k), 64)), bytes = 2.0 * double(p.n) * double(p.k) / 6.5e6;
   // the matrix as columns, in the columns a tile that launch_tc would take
   const int cg = p.m > 128 ? 2 : 1;
@@ -99,31 +122,30 @@ How how(const Product& p) {
   // the matrix as rows, k split
   const uint64_t tiles = ceil_div(uint64_t(p.m), 2 * kGroupRows);
   const double cols = double((ceil_div(uint64_t(p.m), tiles) + 31) / 32 * 32);
-  How best{How::kTc, 1};
+  How best{How::kTc, 1, bn};
   double least = tc;
   for (int s = 1; s <= 8 && s * 4 <= kb; ++s) {
     const double w = double(ceil_div(tiles * ceil_div(uint64_t(p.n), 256) * s, kSms / 2));
     const double us = 9 + std::max(bytes, w * std::ceil(kb / s) * slice_us(cols)) + s * double(p.m) * double(p.n) * 8 / 6e6;
-    if (us < least) least = us, best = {How::kGroup, s};
+    if (us < least) least = us, best = {How::kGroup, s, 0};
   }
   return best;
 }
 
 uint64_t product_bytes(const Product& p) {
   const How h = how(p);
-  return h.kind == How::kGroup ? uint64_t(h.splits) * uint64_t(p.m) * uint64_t(p.n) * 4 : 0;
+  return h.kind == How::kGroup || h.splits > 1 ? uint64_t(h.splits) * uint64_t(p.m) * uint64_t(p.n) * 4 : 0;
 }
 int product(int dtype, const Product& p, float* rows32, cudaStream_t s) {
   const How h = how(p);
-  switch (h.kind) {
-    case How::kStream: return launch_stream(dtype, p, 1, nullptr, nullptr, s);
-    case How::kTc: return launch_tc(dtype, p, nullptr, nullptr, s);
-    case How::kGroup: break;
-  }
+  if (h.kind == How::kStream) return launch_stream(dtype, p, 1, nullptr, nullptr, s);
+  if (h.kind == How::kTc && h.splits == 1) return launch_tc(dtype, p, 1, h.columns, nullptr, nullptr, s);
   Product r = p;
   r.epi = kEpiRows32;
   r.rows32 = rows32;
-  if (const int e = launch_group(dtype, r, h.splits, nullptr, nullptr, s)) return e;
+  if (const int e = h.kind == How::kTc ? launch_tc(dtype, r, h.splits, h.columns, nullptr, nullptr, s)
+                                       : launch_group(dtype, r, h.splits, nullptr, nullptr, s))
+    return e;
   return launch_join_linear(dtype, p.act, rows32, uint32_t(h.splits), uint64_t(p.m), uint64_t(p.n), p.bias, p.residual,
                             uint64_t(p.ldr), p.out, uint64_t(p.ldo), p.pre, uint64_t(p.ldp), s);
 }
@@ -218,7 +240,7 @@ struct LinearBackSpace {
   uint64_t ldz;
   Copies copies;
   Product dx, dw;
-  float *part, *rows32;
+  float *part, *rows32, *dw32;
   uint64_t bytes;
 };
 LinearBackSpace linear_back_space(const tsb_linear_grad_args* a) {
@@ -253,6 +275,7 @@ LinearBackSpace linear_back_space(const tsb_linear_grad_args* a) {
     p.m = int64_t(a->n), p.n = int64_t(a->k), p.k = int64_t(a->rows);
     p.epi = kEpiStore;
     p.out = a->dw, p.ldo = int64_t(a->lddw);
+    r.dw32 = static_cast<float*>(w.take(product_bytes(p)));
   }
   r.bytes = w.used;
   return r;
@@ -275,7 +298,7 @@ void linear_back(const tsb_linear_grad_args* a) {
     ck(launch_dz(int(a->dtype), int(a->act), a->dy, a->lddy, a->pre, a->ldp, w.dz, w.ldz, a->rows, a->n, a->db, w.part, s),
        fn, "slope");
   if (a->dx) ck(product(int(a->dtype), w.dx, w.rows32, s), fn, "dx");
-  if (a->dw) ck(product(int(a->dtype), w.dw, nullptr, s), fn, "dw");
+  if (a->dw) ck(product(int(a->dtype), w.dw, w.dw32, s), fn, "dw");
 }
 
 // ---- the gated feed-forward block ----
@@ -330,7 +353,7 @@ bool ffn_rows16(const tsb_units* u, uint64_t hidden, uint64_t ffn, const void* x
 // long that whole 256-row tiles waste little of them.
 uint32_t tc_tile(uint64_t each) { return each >= 4 * kTcRows ? kTcRows : kGroupRows; }
 int launch_grouped(int dtype, const Product& p, const Plan* plan, const Units* u, cudaStream_t s) {
-  return p.grouped && plan->bm == kGroupRows ? launch_group(dtype, p, 1, plan, u, s) : launch_tc(dtype, p, plan, u, s);
+  return p.grouped && plan->bm == kGroupRows ? launch_group(dtype, p, 1, plan, u, s) : launch_tc(dtype, p, 1, 0, plan, u, s);
 }
 
 struct FfnSpace {
@@ -496,7 +519,7 @@ void ffn_back(const tsb_ffn_grad_args* a) {
   {
     Product p{};
     p.grouped = 1;
-      p.segs = 3;
+    p.segs = 3;
     p.a[0] = p.a[1] = x_rows;
     p.a[2] = dy_rows;
     p.b[0] = of_unit(0, d, 1);
@@ -515,7 +538,7 @@ void ffn_back(const tsb_ffn_grad_args* a) {
   if (a->dx) {
     Product p{};
     p.grouped = 1;
-      p.segs = 2;
+    p.segs = 2;
     p.a[0] = dense(w.dg, f, 1);
     p.a[1] = dense(w.du, f, 1);
     p.b[0] = of_unit(0, 1, d);
@@ -530,7 +553,7 @@ void ffn_back(const tsb_ffn_grad_args* a) {
   if (a->dgate) {
     Product p{};
     p.per_unit = 1;
-      p.k_rows = 1;
+    p.k_rows = 1;
     p.segs = 1;
     p.epi = kEpiStore;
     p.out_unit = d * f;

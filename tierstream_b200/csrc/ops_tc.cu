@@ -26,7 +26,8 @@ constexpr int kRowBytes = 64;  // a store buffer: 32 rows x 64 bytes
 
 __device__ uint32_t g_ops_timeouts;
 
-enum Mode { kLin, kLinDx, kLinDw, kUp, kUpBack, kDown, kDx, kDw };
+// kLinDwPart: parts of kLinDw's sum over the rows, each with its own 32-bit rows
+enum Mode { kLin, kLinDx, kLinDw, kLinDwPart, kUp, kUpBack, kDown, kDx, kDw };
 
 struct Params {
   Plan plan;
@@ -38,13 +39,15 @@ struct Params {
   int32_t vec;       // 16-byte stores are possible: `out` maps are made
   int32_t stages, stage_bytes;
   int32_t pair;      // two CTAs to a tile of 256 rows
+  int32_t splits;    // kLinDwPart's parts
 };
 struct Maps {
   CUtensorMap a[2], b[3], out[3];
 };
 
 struct Tile {
-  int unit, slot, row0, rows, stored;  // row0: the group's first row; rows: m limit; stored: rows to store (padding too)
+  int unit, slot, row0, rows, stored;  // unit: or the part; row0: the group's (of k: the part's) first row; rows: m limit;
+                                       // stored: rows to store (padding too)
   int m0, n, kb;
 };
 
@@ -66,7 +69,8 @@ struct Tiles {
     }
   }
   __device__ __forceinline__ Tiles(const Params& q) : at(blockIdx.x / CG), next(make_int4(0, 0, 0, 0)) {
-    end = grouped ? q.plan.head[0] * q.n_tiles : q.m_tiles * q.n_tiles * (MODE == kDw ? int(q.plan.units) : 1);
+    end = grouped ? q.plan.head[0] * q.n_tiles
+                  : q.m_tiles * q.n_tiles * (MODE == kDw ? int(q.plan.units) : MODE == kLinDwPart ? q.splits : 1);
     fetch(q);
   }
   __device__ __forceinline__ bool take(const Params& q, Tile& t) {
@@ -87,10 +91,15 @@ struct Tiles {
       local -= g.w * q.n_tiles;
     } else {
       t.rows = t.stored = int(q.p.m);
-      if (MODE == kDw) {
+      if (MODE == kDw || MODE == kLinDwPart) {
         t.unit = local / (mt * q.n_tiles);
-        t.kb = (g.z + kBK - 1) / kBK;
         local -= t.unit * mt * q.n_tiles;
+      }
+      if (MODE == kDw) t.kb = (g.z + kBK - 1) / kBK;
+      if (MODE == kLinDwPart) {
+        const int first = int(int64_t(q.k_blocks) * t.unit / q.splits);
+        t.kb = int(int64_t(q.k_blocks) * (t.unit + 1) / q.splits) - first;
+        t.row0 = first * kBK;
       }
     }
     const int chunk = local / (kChunk * q.n_tiles), in = local - chunk * kChunk * q.n_tiles;
@@ -105,12 +114,13 @@ template <int MODE>
 struct Traits {
   static constexpr bool grouped = MODE == kUp || MODE == kUpBack || MODE == kDown || MODE == kDx;
   static constexpr int segs = MODE == kUpBack || MODE == kDx ? 2 : 1;
-  static constexpr bool a_mn = MODE == kLinDw || MODE == kDw;
+  static constexpr bool rows_k = MODE == kDw || MODE == kLinDwPart;  // k runs over rows from row0
+  static constexpr bool a_mn = MODE == kLinDw || rows_k;
   // the segment whose B is columns of gate, then of up (the last: in the backward pass dh comes first)
   __host__ __device__ static constexpr bool both(int s) { return (MODE == kUp && s == 0) || (MODE == kUpBack && s == 1); }
   // B of segment s with n contiguous
   __host__ __device__ static constexpr bool b_mn(int s) {
-    return MODE == kLinDx || MODE == kLinDw || MODE == kDx || MODE == kDw || (MODE == kUpBack && s == 0);
+    return MODE == kLinDx || MODE == kLinDw || rows_k || MODE == kDx || (MODE == kUpBack && s == 0);
   }
   static constexpr int bufs = MODE == kUpBack ? 1 : 2;
 };
@@ -207,8 +217,8 @@ __device__ __forceinline__ void epilogue(const Params& q, const Tile& t, uint32_
   const bool zero = MODE == kDw && t.kb == 0;          // a unit without rows: nothing was computed
   // TMA clips at the matrix' edges: a block is whole unless it crosses its group's rows or its tile's columns
   const bool whole_rows = rows == 32 || (!Traits<MODE>::grouped && rows > 0);
-  const int64_t y = int64_t(t.row0) + m;
-  o.z = MODE == kDw ? t.unit : 0;
+  const int64_t y = Traits<MODE>::rows_k ? m : int64_t(t.row0) + m;
+  o.z = Traits<MODE>::rows_k ? t.unit : 0;
   if constexpr (MODE == kUp || MODE == kUpBack) {
     float w = 0.f, dw = 0.f;
     if (MODE == kUpBack && lane < rows && m + lane < t.rows) w = p.weights[q.plan.pair_of_row[y + lane]];
@@ -246,7 +256,8 @@ __device__ __forceinline__ void epilogue(const Params& q, const Tile& t, uint32_
       }
     }
     if (MODE == kUpBack && p.dwp && lane < rows && m + lane < t.rows) p.dwp[(y + lane) * p.ld_dwp + 2 * t.n + half] = dw;
-  } else if constexpr (MODE == kDown || MODE == kDx) {
+  } else if constexpr (MODE == kDown || MODE == kDx || MODE == kLinDwPart) {
+    float* to = p.rows32 + (MODE == kLinDwPart ? t.unit * p.m + y : y) * p.n + n0;
     for (int c = half * 16; c < cols; c += 32) {
       float v[16];
       tmem_ld16(base + c, v);
@@ -254,7 +265,7 @@ __device__ __forceinline__ void epilogue(const Params& q, const Tile& t, uint32_
       uint32_t b[16];
 #pragma unroll
       for (int i = 0; i < 16; ++i) b[i] = __float_as_uint(v[i]);
-      store_rows<float>(o, 0, b, n0 + c, y, p.rows32 + y * p.n + n0 + c, p.n, rows, cols - c, whole_rows);
+      store_rows<float>(o, 0, b, n0 + c, y, to + c, p.n, rows, cols - c, whole_rows);
     }
   } else if constexpr (MODE == kLin) {
     const T *bias = static_cast<const T*>(p.bias), *res = static_cast<const T*>(p.residual) + (m + lane) * p.ldr;
@@ -293,7 +304,7 @@ __device__ __forceinline__ void epilogue(const Params& q, const Tile& t, uint32_
 #pragma unroll
           for (int i = 0; i < 16; i += 2) h[s * 8 + i / 2] = pack<T>(v[s][i], v[s][i + 1]);
       }
-      store_rows<T>(o, 0, h, n0 + c, MODE == kDw ? m : y, out + c, p.ldo, rows, cols - c, whole_rows && c + 32 <= q.bn);
+      store_rows<T>(o, 0, h, n0 + c, y, out + c, p.ldo, rows, cols - c, whole_rows && c + 32 <= q.bn);
     }
   }
 }
@@ -360,7 +371,7 @@ __global__ __launch_bounds__(kThreads, 1) void tc_kernel(const __grid_constant__
         const CUtensorMap* mb = &maps.b[MODE == kUpBack && s == 0 ? 2 : pair ? rank : s];
         const int z = X::grouped ? t.slot : 0, n0 = t.n * q.bn + (pair ? 0 : int(rank) * half_n);
         const int m0 = X::a_mn ? t.m0 : t.row0 + t.m0;
-        int k0 = 0, krow = MODE == kDw ? t.row0 : 0;
+        int k0 = 0, krow = X::rows_k ? t.row0 : 0;
         for (int kb = 0; kb < t.kb; ++kb, k0 += kBK, krow += kBK) {
           ok = bar_wait(empty + 8 * st, parity, dead);
           if (!ok) break;
@@ -547,7 +558,7 @@ int launch_gather(const Plan& plan, uint32_t top, const void* src, uint64_t ld, 
                 uint32_t(n / 8), static_cast<uint4*>(dst));
 }
 
-int launch_tc(int dtype, const Product& p, const Plan* plan, const Units* u, cudaStream_t s) {
+int launch_tc(int dtype, const Product& p, int splits, int columns, const Plan* plan, const Units* u, cudaStream_t s) {
   if (!encoder()) return int(cudaErrorNotSupported);
   const int sms = sm_count();
   if (!sms) return int(cudaErrorInvalidDevice);
@@ -559,7 +570,7 @@ int launch_tc(int dtype, const Product& p, const Plan* plan, const Units* u, cud
   if (p.epi == kEpiLinear) mode = kLin;
   else if (p.epi == kEpiUp) mode = kUp;
   else if (p.epi == kEpiUpBack) mode = kUpBack;
-  else if (p.epi == kEpiRows32) mode = p.segs == 2 ? kDx : kDown;
+  else if (p.epi == kEpiRows32) mode = !p.grouped ? kLinDwPart : p.segs == 2 ? kDx : kDown;
   else mode = p.per_unit ? kDw : (a_mn ? kLinDw : kLinDx);
   // Pairs of CTAs share a 256-row tile when there are rows for it: each stages half of B, so a tile's operands cross from
   // L2 once for 256 x 256 sums instead of 128 x 256 (the SM's 64 bytes a clock from L2 bound the single CTA).
@@ -567,17 +578,17 @@ int launch_tc(int dtype, const Product& p, const Plan* plan, const Units* u, cud
   const int cg = q.pair ? 2 : 1;
   q.k_blocks = int(ceil_div(uint64_t(p.k), kBK));
   q.m_tiles = p.grouped ? 0 : int(ceil_div(uint64_t(p.m), uint64_t(cg * kBM)));
-  const int64_t m_tiles = p.grouped ? plan->max_tiles : p.per_unit ? int64_t(q.m_tiles) * plan->units : q.m_tiles;
+  q.splits = splits;
+  const int64_t m_tiles = p.grouped ? plan->max_tiles : int64_t(q.m_tiles) * (p.per_unit ? int64_t(plan->units) : splits);
   const bool narrow = mode == kUp || mode == kUpBack;
-  q.bn = p.grouped || p.per_unit ? (narrow ? 128 : 256) : tc_columns(p.m, p.n, sms);
+  q.bn = p.grouped || p.per_unit ? (narrow ? 128 : 256) : columns;
   const int64_t step = 16 * cg;  // a product's columns: whole 16 for one CTA, 32 for a pair
   if (q.bn > (p.n + step - 1) / step * step) q.bn = int((p.n + step - 1) / step * step);
   q.n_tiles = int(ceil_div(uint64_t(p.n), uint64_t(q.bn)));
-  q.vec = (p.epi == kEpiRows32 && p.n % 4 == 0) ||
-          (p.epi == kEpiUpBack ? on16(p.dg) && on16(p.du) && on16(p.hw) && p.ldo % 8 == 0
-                               : on16(p.out) && p.ldo % 8 == 0 && p.out_unit % 8 == 0 &&
-                                     on16(p.bias) && on16(p.residual) && p.ldr % 8 == 0 && on16(p.pre) &&
-                                     p.ldp % 8 == 0);
+  q.vec = p.epi == kEpiRows32   ? p.n % 4 == 0
+          : p.epi == kEpiUpBack ? on16(p.dg) && on16(p.du) && on16(p.hw) && p.ldo % 8 == 0
+                                : on16(p.out) && p.ldo % 8 == 0 && p.out_unit % 8 == 0 && on16(p.bias) &&
+                                      on16(p.residual) && p.ldr % 8 == 0 && on16(p.pre) && p.ldp % 8 == 0;
   Maps maps;
   std::memset(&maps, 0, sizeof maps);
   auto shape = [&](const Operand& o, int64_t n_i, int64_t n_k) {
@@ -612,9 +623,11 @@ int launch_tc(int dtype, const Product& p, const Plan* plan, const Units* u, cud
                            p.epi == kEpiUpBack ? p.du : p.pre, p.hw};
     const uint64_t lds[3] = {uint64_t(p.epi == kEpiRows32 ? p.n : p.ldo), uint64_t(p.epi == kEpiUpBack ? p.ldo : p.ldp),
                              uint64_t(p.ldo)};
+    const uint64_t slots = p.per_unit ? plan->units : uint64_t(splits);
+    const uint64_t slot_bytes = p.per_unit ? uint64_t(p.out_unit) * 2 : rows * n * 4;
     for (int i = 0; i < 3; ++i)
-      if (outs[i] && !make_map(&maps.out[i], p.epi == kEpiRows32 ? TSB_F32 : dtype, outs[i], n, rows, lds[i],
-                               p.per_unit ? plan->units : 1, uint64_t(p.out_unit) * 2, 32, true))
+      if (outs[i] && !make_map(&maps.out[i], p.epi == kEpiRows32 ? TSB_F32 : dtype, outs[i], n, rows, lds[i], slots,
+                               slot_bytes, 32, true))
         return int(cudaErrorInvalidValue);
   }
   // as many stages as the ring holds: narrow tiles are bound by the loads' latency
@@ -628,6 +641,7 @@ int launch_tc(int dtype, const Product& p, const Plan* plan, const Units* u, cud
     case kLin: return go_type<kLin>(dtype, p.act, maps, q, grid, s);
     case kLinDx: return go_type<kLinDx>(dtype, 0, maps, q, grid, s);
     case kLinDw: return go_type<kLinDw>(dtype, 0, maps, q, grid, s);
+    case kLinDwPart: return go_type<kLinDwPart>(dtype, 0, maps, q, grid, s);
     case kUp: return go_type<kUp>(dtype, p.act, maps, q, grid, s);
     case kUpBack: return go_type<kUpBack>(dtype, p.act, maps, q, grid, s);
     case kDown: return go_type<kDown>(dtype, 0, maps, q, grid, s);
