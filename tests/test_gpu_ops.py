@@ -306,6 +306,24 @@ def test_route_masks_ties_and_odd_values():
     assert ops.route(z[:0], 3)[0].shape == (0, 3)
 
 
+@pytest.mark.parametrize("experts,apart", [(1024, 32), (1001, 32), (512, 32), (257, 16), (96, 32), (1024, 1)])
+def test_route_with_the_largest_far_apart(experts, apart):
+    """The largest logits at equal distances (one lane's, a few lanes'), among equal, rising, falling and negative ones."""
+    j = torch.arange(experts, device="cuda")
+    on = j % apart == 5 % apart
+    rows = [torch.where(on, 2.0, 1.0), torch.where(on, 3.0 + j / 64, 1.0), torch.where(on, 99.0 - j / 64, j / 1e4),
+            torch.where(on, -1.0 - j % 3, -8.0), torch.where(on, (j // apart % 2).float(), -0.0),
+            torch.where(on, 2.0, -math.inf), torch.zeros(experts, device="cuda")]
+    z = torch.stack([r.float() for r in rows])
+    top = min(32, experts)
+    for t in (torch.float32, torch.float16):
+        for norm in (True, False):
+            ids, w = ops.route(z.to(t), top, norm=norm)
+            want_ids, want = plain_route(z.to(t), top, norm)
+            assert torch.equal(ids, want_ids)
+            close(w, want, 2.0 ** -20 * want)
+
+
 @pytest.mark.parametrize("rows,experts,top", ROUTE)
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_route_backward(rows, experts, top, dtype):
