@@ -14,9 +14,10 @@ constexpr uint32_t kNone = 0xffffffffu;
 // ---------------------------------------------------------------------------------------------------------------
 // The plan. Counting first: CTA e counts unit e's pairs and resolves its slot. Then CTA e adds up the groups before its
 // own (padded rows, tiles) and writes its pairs in ascending order, found by scanning the ids: no atomics,
-// so the order never changes. The scan reads the ids once per unit from L2 (256 units x 16,384 pairs: 16 MB).
+// so the order never changes. The scan reads the ids once per unit from L2 (256 units x 16,384 pairs: 16 MB); a warp takes
+// 512 neighbouring ids a step, 32 a load, and ranks its hits by ballots.
 // ---------------------------------------------------------------------------------------------------------------
-constexpr int kPlanThreads = 1024, kPlanEach = 4;  // ids a thread and step
+constexpr int kPlanThreads = 1024, kPlanEach = 16;  // ids a thread and step
 
 __device__ __forceinline__ int32_t resolve(const Units& u, int32_t e) {
   if (u.abort && *reinterpret_cast<const volatile uint32_t*>(u.abort)) return -1;
@@ -43,8 +44,10 @@ __global__ __launch_bounds__(kPlanThreads) void plan_count_kernel(const __grid_c
   __shared__ int red[kPlanThreads / 32];
   const int32_t e = blockIdx.x;
   int n = 0;
-#pragma unroll 4
+#pragma unroll 8
   for (uint32_t i = threadIdx.x; i < p.pairs; i += kPlanThreads) n += ids[i] == e;
+  for (uint32_t i = blockIdx.x * kPlanThreads + threadIdx.x; i < p.pairs; i += gridDim.x * kPlanThreads)
+    p.row_of_pair[i] = -1;  // (until a group takes it)
   n = block_sum(n, red);
   if (threadIdx.x) return;
   const int32_t slot = n ? resolve(u, e) : -1;
@@ -87,55 +90,56 @@ __global__ __launch_bounds__(kPlanThreads) void plan_fill_kernel(const __grid_co
   for (int i = cnt + threadIdx.x; i < padded; i += kPlanThreads) p.pair_of_row[rows + i] = -1;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int done = 0;  // pairs of this unit before the current span of ids
-  for (uint32_t i0 = 0; i0 < p.pairs && (cnt || e == 0); i0 += kPlanThreads * kPlanEach) {
-    const uint32_t i = i0 + threadIdx.x * kPlanEach;
-    int hits = 0;
-    uint32_t hit = 0;
+  for (uint32_t i0 = 0; i0 < p.pairs && cnt; i0 += kPlanThreads * kPlanEach) {
+    const uint32_t i = i0 + warp * 32 * kPlanEach + lane;
+    uint32_t hit[kPlanEach] = {};
+    int hits = 0;  // of the warp
+    if (i - lane < p.pairs) {
 #pragma unroll
-    for (int j = 0; j < kPlanEach; ++j) {
-      const int32_t id = i + j < p.pairs ? ids[i + j] : -1;
-      if (e == 0 && i + j < p.pairs && (uint32_t(id) >= p.units || p.cnt[id] == 0)) p.row_of_pair[i + j] = -1;
-      if (cnt && i + j < p.pairs && id == int32_t(e)) hit |= 1u << j, ++hits;
-    }
-    int upto = hits;  // inclusive over the warp
-    for (int o = 1; o < 32; o <<= 1) {
-      const int v = __shfl_up_sync(0xffffffffu, upto, o);
-      if (lane >= o) upto += v;
+      for (int j = 0; j < kPlanEach; ++j) hit[j] = i + 32 * j < p.pairs && ids[i + 32 * j] == int32_t(e);
+#pragma unroll
+      for (int j = 0; j < kPlanEach; ++j) {
+        hit[j] = __ballot_sync(0xffffffffu, hit[j]);
+        hits += __popc(hit[j]);
+      }
     }
     __syncthreads();
-    if (lane == 31) warp_n[warp] = upto;
+    if (lane == 0) warp_n[warp] = hits;
     __syncthreads();
-    int r = rows + done + upto - hits;
+    int r = rows + done;
     for (int w = 0; w < kPlanThreads / 32; ++w) {
       if (w < warp) r += warp_n[w];
       done += warp_n[w];
     }
+    if (!hits) continue;
 #pragma unroll
-    for (int j = 0; j < kPlanEach; ++j)
-      if (hit >> j & 1) {
-        p.pair_of_row[r] = int32_t(i + j);
-        p.row_of_pair[i + j] = r++;
+    for (int j = 0; j < kPlanEach; ++j) {
+      if (!hit[j]) continue;
+      if (hit[j] >> lane & 1) {
+        const int at = r + __popc(hit[j] & ((1u << lane) - 1));
+        p.pair_of_row[at] = int32_t(i + 32 * j);
+        p.row_of_pair[i + 32 * j] = at;
       }
+      r += __popc(hit[j]);
+    }
   }
 }
 
-// The same for few pairs in one launch: one CTA, the ids in shared memory, unit after unit by warps.
+// The same for few pairs in one launch: one CTA, a pair and a unit to a thread.
 constexpr int kSmallThreads = 1024;
 constexpr uint32_t kSmallPairs = 1024, kSmallUnits = 1024;
 
 __global__ __launch_bounds__(kSmallThreads) void plan_small_kernel(const __grid_constant__ Plan p,
                                                                    const __grid_constant__ Units u,
                                                                    const int32_t* __restrict__ ids) {
-  __shared__ int32_t id[kSmallPairs];
   __shared__ int32_t cnt[kSmallUnits], rows[kSmallUnits];
   __shared__ int32_t wr[32], wt[32], wd[32];
   const uint32_t t = threadIdx.x;
   const int lane = t & 31, warp = t >> 5;
   begin_after();
   cnt[t] = 0;
-  if (t < p.pairs) id[t] = ids[t];
+  const int32_t mine = t < p.pairs ? ids[t] : -1;
   __syncthreads();
-  const int32_t mine = t < p.pairs ? id[t] : -1;
   const bool valid = uint32_t(mine) < p.units;
   int32_t my_slot = 0;
   if (valid) atomicAdd(&cnt[mine], 1);  // (counts only: their value does not depend on the order)
@@ -162,28 +166,36 @@ __global__ __launch_bounds__(kSmallThreads) void plan_small_kernel(const __grid_
   if (lane == 31) wr[warp] = r, wt[warp] = k, wd[warp] = d;
   __syncthreads();
   for (int w = 0; w < warp; ++w) r += wr[w], k += wt[w], d += wd[w];
-  rows[t] = r - padded;
+  const int first = r - padded;
+  rows[t] = first;
   __syncthreads();
   if (t < p.units) {
     p.cnt[t] = c;
-    p.off[t] = rows[t];
+    p.off[t] = first;
     p.slot[t] = my_slot;
     if (t + 1 == p.units) p.head[0] = k, p.head[1] = r, p.head[2] = d;
-    for (int i = 0; i < nt; ++i) p.tiles[0][k - nt + i] = make_int4(my_slot, rows[t], c, k - nt);
-    for (int i = 0; i < nd; ++i) p.tiles[1][d - nd + i] = make_int4(my_slot, rows[t], c, d - nd);
-    for (int i = c; i < padded; ++i) p.pair_of_row[rows[t] + i] = -1;
+    for (int i = 0; i < nt; ++i) p.tiles[0][k - nt + i] = make_int4(my_slot, first, c, k - nt);
+    for (int i = 0; i < nd; ++i) p.tiles[1][d - nd + i] = make_int4(my_slot, first, c, d - nd);
+    for (int i = c; i < padded; ++i) p.pair_of_row[first + i] = -1;
   }
   int all = 0;
   for (int w = 0; w < 32; ++w) all += wt[w];
   for (uint32_t i = uint32_t(all) + t; i < p.max_tiles; i += kSmallThreads) p.tiles[0][i] = make_int4(0, 0, 0, 0);
-  if (t < p.pairs) {
-    int32_t row = -1;
-    if (valid && cnt[mine]) {
-      int before = 0;
-      for (uint32_t j = 0; j < t; ++j) before += id[j] == mine;
-      row = rows[mine] + before;
-      p.pair_of_row[row] = int32_t(t);
+  // warp after warp, its pairs of a unit take the unit's next rows in the lanes' order
+  const uint32_t same = __match_any_sync(0xffffffffu, mine);
+  const int before = __popc(same & ((1u << lane) - 1));
+  const bool takes = valid && cnt[mine];
+  int32_t row = -1;
+  for (int w = 0; w * 32 < int(p.pairs); ++w) {
+    if (warp == w) {
+      if (takes) row = rows[mine] + before;
+      __syncwarp();
+      if (takes && before == 0) rows[mine] += __popc(same);
     }
+    __syncthreads();
+  }
+  if (t < p.pairs) {
+    if (row >= 0) p.pair_of_row[row] = int32_t(t);
     p.row_of_pair[t] = row;
   }
 }
