@@ -247,11 +247,12 @@ int launch_stream(int dtype, const Product& p, uint32_t top, const Plan* plan, c
 
 // ops_tc.cu: products of many rows on tcgen05; grouped ones take tiles of kTcRows rows (the plan's bm). tc_fits: TMA can
 // read the operand. Gathered operands are gathered first: launch_gather copies n columns of every grouped row (n a
-// multiple of 8).
+// multiple of 8), of a second source too unless src2 is NULL.
 constexpr uint32_t kTcRows = 256;
 bool tc_fits(const Operand& o);
 int tc_columns(int64_t m, int64_t n, int sms);
-int launch_gather(const Plan& plan, uint32_t top, const void* src, uint64_t ld, uint64_t n, void* dst, cudaStream_t s);
+int launch_gather(const Plan& plan, uint32_t top, uint64_t n, const void* src, uint64_t ld, void* dst, const void* src2,
+                  uint64_t ld2, void* dst2, cudaStream_t s);
 // columns: of a plain product's tiles. kEpiRows32 of a plain product whose k runs over rows: parts of the sum, as in
 // launch_group.
 int launch_tc(int dtype, const Product& p, int splits, int columns, const Plan* plan, const Units* units, cudaStream_t s);

@@ -422,7 +422,7 @@ void ffn(const tsb_ffn_args* a) {
                     : launch_tile(int(a->dtype), pr, w.plan, u, s);
   };
   if (w.tc) {
-    ck(launch_gather(w.plan, a->top, a->x, a->ldx, a->hidden, w.xs, s), fn, "gather");
+    ck(launch_gather(w.plan, a->top, a->hidden, a->x, a->ldx, w.xs, nullptr, 0, nullptr, s), fn, "gather");
     p.a[0] = p.a[1] = dense(w.xs, d, 1);
   }
   ck(go(p), fn, "gate and up");
@@ -509,8 +509,7 @@ void ffn_back(const tsb_ffn_grad_args* a) {
           x_sum = gathered(a->x, 1, int64_t(a->ldx), w.plan, a->top, 1),
           dy_sum = gathered(a->dy, 1, int64_t(a->lddy), w.plan, a->top, 1);
   if (w.tc) {
-    ck(launch_gather(w.plan, a->top, a->x, a->ldx, a->hidden, w.xs, s), fn, "gather");
-    ck(launch_gather(w.plan, a->top, a->dy, a->lddy, a->hidden, w.dys, s), fn, "gather");
+    ck(launch_gather(w.plan, a->top, a->hidden, a->x, a->ldx, w.xs, a->dy, a->lddy, w.dys, s), fn, "gather");
     x_rows = dense(w.xs, d, 1);
     dy_rows = dense(w.dys, d, 1);
     x_sum = dense(w.xs, 1, d, 1);

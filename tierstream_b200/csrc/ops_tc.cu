@@ -480,13 +480,20 @@ __global__ __launch_bounds__(kThreads, 1) void tc_kernel(const __grid_constant__
 }
 
 // rows of grouped buffers: row r is source row pair_of_row[r] / top, padding rows are zeros
-__global__ __launch_bounds__(256) void gather_kernel(const __grid_constant__ Plan plan, uint32_t top, const uint4* src,
-                                                     uint64_t ld16, uint32_t n16, uint4* dst) {
+struct Gather {
+  const uint4* src[2];
+  uint4* dst[2];
+  uint64_t ld16[2];
+};
+__global__ __launch_bounds__(256) void gather_kernel(const __grid_constant__ Plan plan, uint32_t top, uint32_t n16,
+                                                     const __grid_constant__ Gather g) {
   begin_after();
   const uint32_t r = blockIdx.x;
+  const uint4* src = g.src[blockIdx.y];
+  uint4* dst = g.dst[blockIdx.y];
   if (int32_t(r) >= plan.head[1]) return;
   const int32_t pair = plan.pair_of_row[r];
-  const uint4* s = src + uint64_t(pair < 0 ? 0 : uint32_t(pair) / top) * ld16;
+  const uint4* s = src + uint64_t(pair < 0 ? 0 : uint32_t(pair) / top) * g.ld16[blockIdx.y];
   for (uint32_t c = threadIdx.x; c < n16; c += 256)
     dst[uint64_t(r) * n16 + c] = pair < 0 ? make_uint4(0, 0, 0, 0) : s[c];
 }
@@ -533,8 +540,9 @@ bool fits(const Shape& s) {
 }  // namespace
 
 // Columns a tile: of the multiples of 16 (32 for a pair) up to 256, the one whose last wave of tiles wastes least. A tile
-// costs its columns plus about 32 (the narrower tile re-reads A for fewer products); 2047 x 7168 on 74 pairs takes 224
-// (four waves) over 256 (four waves).
+// costs its columns plus about 32 (the narrower tile re-reads A for fewer products). Under the power cap the widths lie
+// close: 2047 x 7168 x 4096 on 74 pairs takes 95 us at 160 (five waves, the choice), 94 at 224, 96 at 256 and 102 at 128;
+// 4096^3 102 at 192 (the choice), 107 at 160; 8192 x 8192 x 4096 366 at 256 (the choice), 406 at 160.
 int tc_columns(int64_t m, int64_t n, int sms) {
   const int cg = m > kBM ? 2 : 1, step = 16 * cg;
   const uint64_t m_tiles = ceil_div(uint64_t(m), uint64_t(kBM * cg));
@@ -553,9 +561,12 @@ bool tc_fits(const Operand& o) {
   return on16(o.p) && (o.s_i == 1 || o.s_k == 1) && (o.s_k == 1 ? o.s_i : o.s_k) % 8 == 0 && (o.s_i != 1 || o.s_k != 1);
 }
 
-int launch_gather(const Plan& plan, uint32_t top, const void* src, uint64_t ld, uint64_t n, void* dst, cudaStream_t s) {
-  return launch(gather_kernel, plan.max_rows, 256, 0, 1, s, plan, top, static_cast<const uint4*>(src), ld / 8,
-                uint32_t(n / 8), static_cast<uint4*>(dst));
+int launch_gather(const Plan& plan, uint32_t top, uint64_t n, const void* src, uint64_t ld, void* dst, const void* src2,
+                  uint64_t ld2, void* dst2, cudaStream_t s) {
+  const Gather g{{static_cast<const uint4*>(src), static_cast<const uint4*>(src2)},
+                 {static_cast<uint4*>(dst), static_cast<uint4*>(dst2)},
+                 {ld / 8, ld2 / 8}};
+  return launch(gather_kernel, dim3(plan.max_rows, src2 ? 2 : 1), 256, 0, 1, s, plan, top, uint32_t(n / 8), g);
 }
 
 int launch_tc(int dtype, const Product& p, int splits, int columns, const Plan* plan, const Units* u, cudaStream_t s) {
