@@ -731,6 +731,36 @@ def test_a_layer_forward_and_backward():
         assert abs(float((got * d).sum()) - want) <= 64 * half(t) * float((got * d).norm())
 
 
+@pytest.mark.parametrize("rows", [3, 40, 300])
+def test_outputs_beside_inputs(rows):
+    """Outputs in other columns of the inputs' buffer are served, outputs that share elements with an input refused."""
+    t, n, k = torch.bfloat16, 64, 72
+    g = gen(rows)
+    buf = rand(g, rows, 2 * n + k + 16, dtype=t)
+    x, out, pre = buf[:, 8:8 + k], buf[:, 8 + k:8 + k + n], buf[:, 8 + k + n:8 + k + 2 * n]
+    w, bias = rand(g, n, k, dtype=t), rand(g, n, dtype=t)
+    edges = buf[:, :8].clone(), buf[:, -8:].clone()
+    want_pre = torch.empty((rows, n), dtype=t, device="cuda")
+    want = ops.linear(x.clone(), w, bias=bias, act="gelu", pre=want_pre)
+    ops.linear(x, w, bias=bias, act="gelu", pre=pre, out=out)
+    assert torch.equal(out, want) and torch.equal(pre, want_pre)
+    assert torch.equal(buf[:, :8], edges[0]) and torch.equal(buf[:, -8:], edges[1])
+    res = rand(g, rows, n, dtype=t)
+    flat = rand(g, rows * n, dtype=t)
+    for bad in (lambda: ops.linear(x, w, out=buf[:, k:k + n]), lambda: ops.linear(x, w, pre=buf[:, k:k + n]),
+                lambda: ops.linear(x, w, out=out, pre=buf[:, 9 + k:9 + k + n]), lambda: ops.linear(x, w, residual=res, pre=res),
+                lambda: ops.linear(x, w, bias=flat[:n], out=flat.view(rows, n)),
+                lambda: ops.linear(x, w, bias=flat[-n:], pre=flat.view(rows, n))):
+        with pytest.raises(ValueError):
+            bad()
+    ids, p = torch.zeros((rows, 1), dtype=torch.int32, device="cuda"), torch.ones((rows, 1), device="cuda")
+    un = ops.Units(*(rand(g, 1, a, b, dtype=t) for a, b in ((24, k), (24, k), (k, 24))))
+    big = torch.zeros((rows, k), dtype=t, device="cuda")
+    with pytest.raises(ValueError):
+        ops.ffn(x, big.view(torch.int32).view(-1)[:rows].view(rows, 1), p, un, out=big)
+    assert torch.equal(ops.ffn(x, ids, p, un, out=big), ops.ffn(x.clone(), ids, p, un))
+
+
 def test_refusals_on_tensors():
     t = torch.bfloat16
     x = torch.zeros((4, 16), dtype=t, device="cuda")

@@ -85,6 +85,15 @@ void* flat(const char* name, const at::Tensor& t, at::IntArrayRef shape, at::Sca
            c10::toString(t.scalar_type()), " ", shape_of(t.sizes()), " on ", place_of(t));
   return t.data_ptr();
 }
+// whether two matrices are other columns of one buffer's rows
+bool beside(const at::Tensor& a, const at::Tensor& b) {
+  if (a.dim() != 2 || b.dim() != 2 || a.scalar_type() != b.scalar_type() || a.stride(0) != b.stride(0)) return false;
+  const int64_t ld = a.stride(0), size = a.element_size();
+  const int64_t bytes = static_cast<char*>(a.data_ptr()) - static_cast<char*>(b.data_ptr());
+  if (ld <= 0 || a.stride(1) != 1 || b.stride(1) != 1 || bytes % size) return false;
+  const int64_t first = (bytes / size % ld + ld) % ld;  // a's first column, b's being 0
+  return first >= b.size(1) && first + a.size(1) <= ld;
+}
 // refuses an output that shares memory with an input
 void apart(const char* name, const at::Tensor& out, const at::Tensor& in) {
   auto end = [](const at::Tensor& t) {
@@ -92,7 +101,7 @@ void apart(const char* name, const at::Tensor& out, const at::Tensor& in) {
     for (int64_t d = 0; d < t.dim() && n; ++d) n += (t.size(d) - 1) * t.stride(d);
     return static_cast<char*>(t.data_ptr()) + n * t.element_size();
   };
-  if (static_cast<char*>(out.data_ptr()) < end(in) && static_cast<char*>(in.data_ptr()) < end(out))
+  if (static_cast<char*>(out.data_ptr()) < end(in) && static_cast<char*>(in.data_ptr()) < end(out) && !beside(out, in))
     refuse(name, ": overlaps an input");
 }
 // refuses an output that lies on its residual in any other way than element on element
@@ -159,8 +168,8 @@ PyObject* linear(PyObject*, PyObject* const* v, Py_ssize_t n) {
   if (there(v[5])) {
     const at::Tensor& pre = tensor("pre", v[5]);
     m = mat("pre", pre, rows, cols, x);
-    apart("pre", pre, x);
-    apart("pre", pre, w);
+    for (int i : {0, 1, 2, 3})
+      if (there(v[i])) apart("pre", pre, tensor("pre", v[i]));
     a.pre = m.p, a.ldp = m.ld;
   }
   const On on(x);
@@ -168,10 +177,9 @@ PyObject* linear(PyObject*, PyObject* const* v, Py_ssize_t n) {
   if (there(v[6])) {
     out = tensor("out", v[6]);
     m = mat("out", out, rows, cols, x);
-    apart("out", out, x);
-    apart("out", out, w);
+    for (int i : {0, 1, 2, 5})
+      if (there(v[i])) apart("out", out, tensor("out", v[i]));
     if (there(v[3])) on_residual(out, tensor("residual", v[3]));
-    if (there(v[5])) apart("out", out, tensor("pre", v[5]));
   } else {
     out = fresh(x, {rows, cols});
     m = {out.data_ptr(), uint64_t(cols)};
@@ -351,6 +359,8 @@ PyObject* ffn(PyObject*, PyObject* const* v, Py_ssize_t n) {
     out = tensor("out", v[7]);
     const Mat m = mat("out", out, rows, hidden, x);
     if (!on_x) apart("out", out, x);  // (in place on x as its own residual: x is read first)
+    apart("out", out, tensor("ids", v[1]));
+    apart("out", out, tensor("weights", v[2]));
     if (there(v[6])) on_residual(out, tensor("residual", v[6]));
     a.y = m.p, a.ldy = m.ld;
   } else {
