@@ -411,6 +411,15 @@ def test_ffn(rows, hidden, ffn, units, top, dtype):
     assert torch.equal(ops.ffn(x, ids, w, un, act=act, residual=res), y)
 
 
+@pytest.mark.parametrize("rows,hidden,ffn,units,top", [
+    (65, 1024, 1032, 4, 1), (130, 1032, 264, 3, 2), (200, 1288, 264, 2, 5), (333, 520, 264, 9, 2), (515, 392, 520, 5, 1),
+    (1500, 72, 328, 3, 2), (1201, 136, 520, 1, 1), (2100, 264, 136, 2, 1), (90, 2056, 72, 1, 6)])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_ffn_long(rows, hidden, ffn, units, top, dtype):
+    """More rows by units than are worth streaming."""
+    test_ffn(rows, hidden, ffn, units, top, dtype)
+
+
 @pytest.mark.parametrize("rows,hidden,ffn", [(3, 64, 136), (40, 128, 264), (400, 256, 264)])
 def test_ffn_uneven_groups_and_empty_rows(rows, hidden, ffn):
     """Most rows in one unit, some units without rows, rows whose every id is outside, strided x, residual and y."""
@@ -459,6 +468,11 @@ def test_ffn_units_that_are_not_there(rows):
                          device="cuda")
     t = ops.Units.of_table(table.data_ptr(), 6, 128, 136, dtype=torch.float16)
     close(ops.ffn(x, ids, w, t), want, tol)
+
+
+@pytest.mark.parametrize("rows", [2500, 4000])
+def test_ffn_units_that_are_not_there_in_long_groups(rows):
+    test_ffn_units_that_are_not_there(rows)
 
 
 def plain_back(dy, x, ids, w, parts, act):

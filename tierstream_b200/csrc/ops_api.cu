@@ -72,8 +72,12 @@ Operand of_unit(int part, int64_t s_i, int64_t s_k) { return {nullptr, s_i, s_k,
 // mostly empty then: a plain product of at most 8 rows (32 us against 58 at 6 x 8192 x 8192, 34 against 48 at 8 x 4096 x
 // 14336, where the other's 128 column tiles cannot keep enough bytes in flight), and the feed-forward block with at most
 // two rows for each unit that may be met (730 us against 767 at two of 64 units of 88 MB, 327 against 362 at one of 8 of
-// 352 MB, 663 against 644 at two of 128 of 38 MB; at four 800 against 750 there).
+// 352 MB, 663 against 644 at two of 128 of 38 MB; at four 800 against 750 there). A small block too, whose units are read
+// again for every 8 rows, from L2: it saves the tensor cores' path its gathered copy and the start of its kernels (11 us
+// against 18 at 37 rows for each of 3 units of 0.2 MB, 14 against 21 at 12 of 2 of 2.2 MB, 23 against 36 at 11 of 6 of
+// 5.1 MB, 43 MB read again; 30 against 24 at 142 of 7 of 0.6 MB, 76 MB; 36 against 25 at 32 of 16 of 3.1 MB, 200 MB).
 constexpr uint64_t kStreamRows = kStreamTile, kStreamEach = 2;
+constexpr double kStreamAgain = 48e6;
 
 // How a plain product runs. The times are fits, in us, to what the kernels took a 64-wide slice of k on this GPU (148 SMs):
 // 0.10 + 0.0012 columns for a pair of CTAs (0.254 measured at 128 columns, 0.405 at 256; 0.2 at least), 0.17 + 0.00098
@@ -371,7 +375,9 @@ FfnSpace ffn_space(const tsb_ffn_args* a) {
   const uint64_t pairs = a->rows * a->top;
   // few rows for each unit that may be met, or units by address, which TMA cannot find: the weights are streamed
   const uint64_t each = ceil_div(pairs, pairs < a->units->n_units ? pairs : a->units->n_units);
-  r.stream = (each <= kStreamEach || a->units->table) && pairs / kStreamTile + a->units->n_units <= 65535 &&  // (a grid's y)
+  const double again = double(pairs) / kStreamTile * 6 * double(a->hidden) * double(a->ffn);
+  r.stream = (each <= kStreamEach || again <= kStreamAgain || a->units->table) &&
+             pairs / kStreamTile + a->units->n_units <= 65535 &&  // (a grid's y)
              ffn_rows16(a->units, a->hidden, a->ffn, a->x, a->ldx, nullptr, 0);
   r.tc = !r.stream && !a->units->table && ffn_rows16(a->units, a->hidden, a->ffn, a->x, a->ldx, nullptr, 0);
   const uint32_t bm = r.stream ? kStreamTile : r.tc ? tc_tile(each) : kTileM;
